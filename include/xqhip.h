@@ -456,6 +456,152 @@ XQHIP_API int xqhip_linear_attn_scan_ws(const float* mixed, const float* a, cons
                                         int ksize, int tokens, float* out, int out_stride, void* workspace,
                                         void* stream);
 
+/* ---- drafted tokens: one decode step over a tree of them ----------------- */
+/* Checks several drafted tokens in one forward pass; no counterpart in the
+ * reference, which decodes one token at a time (CustomModel::decodeOne,
+ * custom_model.cpp:1340-1356).  A step's rows are the token sampled last (row
+ * 0, the root) and drafted continuations of it: row i continues row parent[i]
+ * < i and stands at position *pos0 + depth[i]; its key and value go to cache
+ * slot *pos0 + i.  Full-attention layers run xqhip_attn_prep_kv and
+ * xqhip_tree_attention, linear-attention layers xqhip_linear_attn_tree (the
+ * state stays as it is), the lm_head's logits go to xqhip_spec_verify, and
+ * xqhip_tree_keep moves the rows on the accepted path together: cache slots
+ * *pos0 .. *pos0 + count - 1, and the rows over which xqhip_linear_attn_scan
+ * then advances each linear-attention state. */
+#define XQHIP_TREE_MAX 64
+typedef struct xqhip_tree {
+    int32_t nodes;                   /* rows, 1 .. XQHIP_TREE_MAX                  */
+    int32_t parent[XQHIP_TREE_MAX];  /* -1: continues the cached context           */
+    int32_t depth[XQHIP_TREE_MAX];   /* rows above it on its path                  */
+    uint64_t mask[XQHIP_TREE_MAX];   /* bit j: row i's attention reads row j       */
+} xqhip_tree;
+/* Host helper: the tree with `nodes` rows and these parents (parent[0] = -1,
+ * -1 <= parent[i] < i): depths, and masks of each row's path with the row
+ * itself.  A caller may set other masks afterwards (only
+ * xqhip_tree_attention reads them: a padding row with mask 0, say).  Calls
+ * that take a tree copy it: it may be changed as soon as they return, and a
+ * captured graph keeps the one it was captured with. */
+XQHIP_API int xqhip_tree_init(const int32_t* parent, int nodes, xqhip_tree* out);
+
+/* Key/value cache of one full-attention layer, [position][kv head][head_dim]
+ * as appendKv keeps it (custom_model.cpp:673-733).
+ * KV_F16: fp16 values, the caches of the entry points above.
+ * KV_I8: signed 8-bit codes and one fp32 scale per position and kv head
+ * ([position][kv head]): scale = max |x| / 127 over the head's values, code =
+ * x / scale rounded to the nearest (ties to even), value = code * scale; half
+ * the bytes.  A head with a value that is not finite gets the scale NaN and
+ * reads back as NaN. */
+enum { XQHIP_KV_F16 = 0, XQHIP_KV_I8 = 1 };
+typedef struct xqhip_kv {
+    int32_t type;
+    int32_t nkv, head_dim;
+    int32_t capacity;  /* positions, <= 2^20 */
+    void* k;           /* device */
+    void* v;
+    float* k_scale;    /* KV_I8 only */
+    float* v_scale;
+} xqhip_kv;
+
+/* xqhip_attn_prep_batch for a cache of either type and rows of a tree: per
+ * query head (q, gate) split, q and k RMSNorm, partial RoPE at position *pos0 +
+ * depth (tree == NULL: *pos0 + t, and any number of tokens), k and v written
+ * to slot *pos0 + t of `kv` (custom_model.cpp:301-370, 673-753).  tokens: the
+ * tree's nodes.  rope_cs: `kv->capacity` positions of xqhip_rope_table.
+ * gate_out may be NULL when gated == 0.  A token whose slot or position lies
+ * outside the cache's capacity writes no cache row, and NaN as its q. */
+XQHIP_API int xqhip_attn_prep_kv(const float* q_src, const float* k_src, const float* v_src, int gated, int nq,
+                                 int rotary_dim, const float* q_norm, const float* k_norm, float eps,
+                                 const float* rope_cs, const int32_t* pos0, const xqhip_tree* tree, int tokens,
+                                 int src_stride, int out_stride, float* q_out, float* gate_out, const xqhip_kv* kv,
+                                 void* stream);
+/* Positions first .. first + count - 1 of a KV_I8 cache as values of out_type
+ * (XQHIP_F32 or XQHIP_F16: code * scale in fp32, then rounded once), for the
+ * kernels that take fp16 caches.  k_out, v_out: [count][nkv][head_dim], either
+ * may be NULL. */
+XQHIP_API int xqhip_kv_read(const xqhip_kv* kv, int first, int count, int out_type, void* k_out, void* v_out,
+                            void* stream);
+
+/* Attention of the rows over a cache of either type:
+ *   out[t] = softmax_s(q[t] k[s] / sqrt(head_dim)) v[s] * sigmoid(gate[t])
+ * over s in [0, *pos0) and the rows of the tree's mask (slot *pos0 + j for bit
+ * j; tree == NULL: the rows 0 .. t, any number of tokens: a prompt chunk).  A
+ * row that sees nothing, or scores of minus infinity only, gives 0; what a row
+ * does not see never reaches it, infinities and NaN included.  q, gate:
+ * [tokens][q_stride], gate may be NULL (no gate); out: [tokens][out_stride].
+ * Scores, weights and sums are held to fp32 accuracy.  The cache must hold the
+ * rows: slots past its capacity are not read.  workspace: 16-byte aligned, of
+ * workspace_bytes >= xqhip_tree_attention_workspace_bytes(...), no
+ * initialisation; calls that can overlap need one each.  nq / nkv <= 8. */
+XQHIP_API size_t xqhip_tree_attention_workspace_bytes(int nq, int nkv, int head_dim, int tokens);
+XQHIP_API int xqhip_tree_attention(const float* q, const float* gate, const xqhip_kv* kv, int nq,
+                                   const xqhip_tree* tree, int tokens, int q_stride, const int32_t* pos0, float* out,
+                                   int out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The linear-attention step (xqhip_linear_attn_step) for every row of a tree,
+ * each from its parent's state and convolution window, without changing
+ * either: conv_state ([2][conv_dim][ksize - 1], copy *pos0 & 1 is read) and
+ * state ([lv_n][lk_hd][lv_hd]) are read only.  mixed, a, b: rows at i * stride;
+ * out: rows at i * out_stride, lv_n * lv_hd values (custom_model.cpp:961-1096
+ * per row).  The same mathematics as a scan down each path, in another fp32
+ * summation order; decays are summed in 64 bits.  workspace: 16-byte aligned,
+ * of workspace_bytes >= xqhip_linear_attn_tree_workspace_bytes(...), no
+ * initialisation; calls that can overlap need one each. */
+XQHIP_API size_t xqhip_linear_attn_tree_workspace_bytes(int nodes, int lk_n, int lk_hd, int lv_n, int lv_hd);
+XQHIP_API int xqhip_linear_attn_tree(const float* mixed, const float* a, const float* b, int stride,
+                                     const float* conv_state, const int32_t* pos0, const float* conv_w,
+                                     const float* a_log, const float* dt_bias, const float* state, int lk_n,
+                                     int lk_hd, int lv_n, int lv_hd, int ksize, const xqhip_tree* tree, float* out,
+                                     int out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Verification of the drafts: walks from row 0 to the rows the target model
+ * accepts and samples the token after the last of them.
+ *   logits    [nodes][ld_logits]: row i's `vocab` logits (the token after row i)
+ *   tokens    [nodes]: the rows' token ids (row 0's is not read)
+ *   draft     [nodes][ld_draft]: the distribution that row i's children were
+ *             drawn from (sums to 1), or NULL: drafts taken without chance
+ *             (looked up, greedy), as if drawn from a point mass
+ *   inv_temperature  1 / T; 0: greedy (draft, u_accept, u_sample not read)
+ *   u_accept  [nodes], u_sample [1]: uniform numbers in [0, 1)
+ * With p = softmax(logits / T) of the current row and q its draft row, its
+ * children are tried in order: child j with token x is accepted when
+ * u_accept[j] * q(x) < p(x) (q(x) = 1 for a point mass); a rejection replaces p
+ * by the normalised max(p - q, 0) (point mass: p without x).  When no child is
+ * left the token comes from p by inverse CDF in index order: the first i with
+ * p(0) + .. + p(i) > u_sample * sum.  (Should a rejection leave nothing, p
+ * itself is sampled.)  Greedy: the child whose token is the row's argmax (ties
+ * to the lowest index) is accepted, the last token is that argmax.  The
+ * outcome is distributed as sampling from the target alone.  NaN logits count
+ * as minus infinity; a row with no finite or plus-infinite logit accepts
+ * nothing and samples -1.  Tokens outside [0, vocab) are never accepted.  Sums
+ * and probabilities are held in 64 bits.
+ * out_count: rows kept, row 0 included = new tokens, 1 .. nodes.  out_path
+ * [nodes]: the kept rows, then -1.  out_tokens [nodes]: the new tokens (the
+ * kept drafts', then the sampled one), then -1.  The tree has one root.
+ * workspace: 16-byte aligned, of workspace_bytes >=
+ * xqhip_spec_verify_workspace_bytes(...), no initialisation; calls that can
+ * overlap need one each. */
+XQHIP_API size_t xqhip_spec_verify_workspace_bytes(int nodes, int vocab);
+XQHIP_API int xqhip_spec_verify(const float* logits, int ld_logits, int vocab, const xqhip_tree* tree,
+                                const int32_t* tokens, const float* draft, int ld_draft, float inv_temperature,
+                                const float* u_accept, const float* u_sample, int32_t* out_count, int32_t* out_path,
+                                int32_t* out_tokens, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Moves kept rows together in n_sets buffers: in each, row
+ * first + path[j] replaces row first + j for j < *count (path: strictly
+ * increasing, path[j] >= j, as xqhip_spec_verify leaves it; path, count:
+ * device; at most max_rows <= XQHIP_TREE_MAX rows).  first: *sets[i].first
+ * (device), or 0 when that is NULL.  The buffers do not overlap.  Rows outside
+ * [0, sets[i].rows) and paths that do not increase are left alone from there
+ * on. */
+typedef struct xqhip_rows {
+    void* base;            /* device */
+    uint64_t row_bytes;
+    int64_t rows;
+    const int32_t* first;  /* device, or NULL */
+} xqhip_rows;
+XQHIP_API int xqhip_tree_keep(const xqhip_rows* sets, int n_sets, const int32_t* path, const int32_t* count,
+                              int max_rows, void* stream);
+
 /* One kernel of one thread that stores the device's 100 MHz realtime counter
  * (s_memrealtime) to *slot with a system-scope store; slot may be device or
  * coherent host memory (xqhip_host_alloc_coherent).  Between two kernels on a

@@ -234,4 +234,123 @@ size_t linear_scan_workspace_bytes(int tokens, int lk_n, int lk_hd, int lv_n, in
 bool linear_scan_supported(int lk_n, int lk_hd, int lv_n, int lv_hd, int ksize);
 hipError_t launch_linear_scan(const LinearScanLaunch& p, hipStream_t s);
 
+// ---- a decode step over a tree of drafted tokens -------------------------------
+constexpr int kTreeMax = 64;  // rows of a tree (one mask word each)
+struct TreeMasks {
+    uint64_t m[kTreeMax];
+};
+struct TreeLinks {
+    int8_t parent[kTreeMax];  // -1: continues the context
+};
+
+// A key/value cache of either type (include/xqhip.h, xqhip_kv).
+struct KvCache {
+    void* k;
+    void* v;
+    float* k_scale;  // 8-bit caches: [position][kv head]
+    float* v_scale;
+    int i8, nkv, head_dim, capacity;
+};
+
+// kv_cache.hip
+struct KvPrepLaunch {
+    const float* q_src;
+    const float* k_src;
+    const float* v_src;
+    int gated, nq, rope_pairs;
+    const float* q_norm;
+    const float* k_norm;
+    float eps;
+    const float* rope_cs;  // [capacity][rope_pairs] (cos, sin)
+    const int32_t* pos0;
+    int tokens, src_stride, out_stride;
+    float* q_out;
+    float* gate_out;
+    KvCache kv;
+    int has_tree;
+    int8_t depth[kTreeMax];  // has_tree: position of row t is *pos0 + depth[t]
+};
+hipError_t launch_kv_prep(const KvPrepLaunch& p, hipStream_t s);
+
+struct KvReadLaunch {
+    KvCache kv;
+    int first, count, f16;
+    void* k_out;
+    void* v_out;
+};
+hipError_t launch_kv_read(const KvReadLaunch& p, hipStream_t s);
+
+constexpr int kKeepSets = 64;  // row buffers of one launch
+struct KeepSet {
+    uint8_t* base;
+    uint64_t row_bytes;
+    int64_t rows;
+    const int32_t* first;
+};
+struct KeepLaunch {
+    KeepSet sets[kKeepSets];
+    const int32_t* path;
+    const int32_t* count;
+    int max_rows;
+};
+hipError_t launch_tree_keep(const KeepLaunch& p, int n_sets, hipStream_t s);
+
+// tree_attn.hip
+struct TreeAttnLaunch {
+    const float* q;     // [tokens][q_stride], heads [nq][hd]
+    const float* gate;  // same layout, or nullptr
+    KvCache kv;
+    int nq, tokens, q_stride, out_stride;
+    const int32_t* pos0;
+    float* out;
+    float* ws;     // tree_attn_workspace_bytes
+    int has_tree;  // 0: row t sees the rows 0 .. t
+    TreeMasks masks;
+};
+bool tree_attn_supported(int nq, int nkv, int head_dim);
+size_t tree_attn_workspace_bytes(int nq, int nkv, int head_dim, int tokens);
+hipError_t launch_tree_attn(const TreeAttnLaunch& p, hipStream_t s);
+
+// tree_linear.hip
+struct TreeLinearLaunch {
+    const float* mixed;
+    const float* a;
+    const float* b;
+    int stride;
+    const float* conv_state;  // [2][conv_dim][ksize - 1]
+    const int32_t* pos0;
+    const float* conv_w;
+    const float* a_log;
+    const float* dt_bias;
+    const float* state;  // [lv_n][lk_hd][lv_hd]
+    int lk_n, lk_hd, lv_n, lv_hd, ksize, nodes;
+    float* out;
+    int out_stride;
+    float* ws;  // tree_linear_workspace_bytes
+    TreeLinks links;
+};
+bool tree_linear_supported(int lk_n, int lk_hd, int lv_n, int lv_hd, int ksize);
+size_t tree_linear_workspace_bytes(int nodes, int lk_n, int lk_hd, int lv_n, int lv_hd);
+hipError_t launch_tree_linear(const TreeLinearLaunch& p, hipStream_t s);
+
+// spec_verify.hip
+struct VerifyLaunch {
+    const float* logits;
+    int64_t ld;
+    int vocab, nodes, max_children;
+    const int32_t* tokens;
+    const float* draft;  // nullptr: point masses
+    int64_t ld_draft;
+    float inv_t;  // 0: greedy
+    const float* u_accept;
+    const float* u_sample;
+    int32_t* out_count;
+    int32_t* out_path;
+    int32_t* out_tokens;
+    void* ws;  // verify_workspace_bytes
+    TreeLinks links;
+};
+size_t verify_workspace_bytes(int nodes, int vocab);
+hipError_t launch_verify(const VerifyLaunch& p, hipStream_t s);
+
 }  // namespace xqhip

@@ -50,6 +50,28 @@ class ChainOp(ctypes.Structure):
                 ("res", ChainSrc), ("y_plain", c_void_p)]
 
 
+KV_F16, KV_I8 = 0, 1
+TREE_MAX = 64
+
+
+class Tree(ctypes.Structure):
+    """Mirror of xqhip_tree (include/xqhip.h)."""
+    _fields_ = [("nodes", ctypes.c_int32), ("parent", ctypes.c_int32 * TREE_MAX), ("depth", ctypes.c_int32 * TREE_MAX),
+                ("mask", c_uint64 * TREE_MAX)]
+
+
+class Kv(ctypes.Structure):
+    """Mirror of xqhip_kv (include/xqhip.h)."""
+    _fields_ = [("type", ctypes.c_int32), ("nkv", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("capacity", ctypes.c_int32), ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p),
+                ("v_scale", c_void_p)]
+
+
+class Rows(ctypes.Structure):
+    """Mirror of xqhip_rows (include/xqhip.h)."""
+    _fields_ = [("base", c_void_p), ("row_bytes", c_uint64), ("rows", ctypes.c_int64), ("first", c_void_p)]
+
+
 _P = ctypes.POINTER
 
 _HIP_SIGS = {
@@ -138,6 +160,22 @@ _HIP_SIGS = {
     "xqhip_linear_attn_scan_ws": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                           c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
                                           c_int, c_void_p, c_void_p]),
+    "xqhip_tree_init": (c_int, [c_void_p, c_int, _P(Tree)]),
+    "xqhip_attn_prep_kv": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_float,
+                                   c_void_p, c_void_p, _P(Tree), c_int, c_int, c_int, c_void_p, c_void_p, _P(Kv),
+                                   c_void_p]),
+    "xqhip_kv_read": (c_int, [_P(Kv), c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "xqhip_tree_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "xqhip_tree_attention": (c_int, [c_void_p, c_void_p, _P(Kv), c_int, _P(Tree), c_int, c_int, c_void_p, c_void_p,
+                                     c_int, c_void_p, c_size_t, c_void_p]),
+    "xqhip_linear_attn_tree_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "xqhip_linear_attn_tree": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, _P(Tree), c_void_p,
+                                       c_int, c_void_p, c_size_t, c_void_p]),
+    "xqhip_spec_verify_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "xqhip_spec_verify": (c_int, [c_void_p, c_int, c_int, _P(Tree), c_void_p, c_void_p, c_int, c_float, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "xqhip_tree_keep": (c_int, [_P(Rows), c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "xqhip_rmsnorm": (c_int, [c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p]),
     "xqhip_lds_fill": (c_int, [c_float, c_void_p]),
     "xqhip_timestamp": (c_int, [c_void_p, c_void_p]),
@@ -197,6 +235,19 @@ def ck(rc):
     if rc != 0:
         raise HipError(f"xqhip error {rc}: {hip().xqhip_last_error().decode(errors='replace')}")
     return rc
+
+
+def tree(parents):
+    """The xqhip_tree of a list of parents (xqhip_tree_init)."""
+    t = Tree()
+    a = (ctypes.c_int32 * max(1, len(parents)))(*parents)
+    ck(hip().xqhip_tree_init(a, len(parents), ctypes.byref(t)))
+    return t
+
+
+def rows(sets):
+    """An array of xqhip_rows from (base, row_bytes, rows, first) tuples."""
+    return (Rows * len(sets))(*[Rows(*s) for s in sets])
 
 
 def ptr(a):
