@@ -61,7 +61,7 @@ xqhip::KvCache cache_of(const xqhip_kv* kv) {
 
 xqhip::TreeLinks links_of(const xqhip_tree* t) {
     xqhip::TreeLinks l{};
-    for (int i = 0; i < t->nodes; ++i) l.parent[i] = static_cast<int8_t>(t->parent[i]);
+    for (int i = 0; i < t->nodes; ++i) l.words[i / 4] |= static_cast<uint32_t>(t->parent[i] & 0xff) << 8 * (i % 4);
     return l;
 }
 
@@ -230,9 +230,10 @@ int xqhip_spec_verify(const float* logits, int ld_logits, int vocab, const xqhip
     const size_t need = xqhip::verify_workspace_bytes(tree->nodes, vocab);
     if (!workspace_ok(workspace, workspace_bytes, need))
         return refuse("xqhip_spec_verify: a 16-byte aligned workspace of %zu bytes (%zu given)", need, workspace_bytes);
-    const xqhip::VerifyLaunch p{logits, ld_logits, vocab, tree->nodes, most, tokens, sampled ? draft : nullptr, ld_draft,
-                                inv_temperature, u_accept, u_sample, out_count, out_path, out_tokens, workspace,
-                                links_of(tree)};
+    xqhip::VerifyLaunch p{logits, ld_logits, vocab, tree->nodes, most, tokens, sampled ? draft : nullptr, ld_draft,
+                          inv_temperature, u_accept, u_sample, out_count, out_path, out_tokens, workspace,
+                          links_of(tree), {}};
+    for (int i = 1; i < tree->nodes; ++i) p.kids[tree->parent[i]] |= uint64_t(1) << i;
     return check(xqhip::launch_verify(p, as_stream(stream)), "verify launch");
 }
 

@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kWave) tree_conv_kernel(TreeLinearLaunch p) {
         float tap[kTreeLinMaxTaps];
         for (int t = hist; t >= 0; --t) {
             tap[t] = row >= 0 ? p.mixed[static_cast<size_t>(row) * p.stride + c] : hs[static_cast<size_t>(c) * hist + hist - 1 - back++];
-            if (row >= 0) row = p.links.parent[row];
+            if (row >= 0) row = static_cast<int8_t>(p.links.words[row / 4] >> 8 * (row % 4));
         }
         for (int t = 0; t <= hist; ++t) acc += tap[t] * p.conv_w[static_cast<size_t>(c) * p.ksize + t];
         y[e] = silu_dev(acc);
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(256) tree_delta_kernel(TreeLinearLaunch p) {
     double sum = 0.0;
     uint64_t above = 0;
     if (tid < n)
-        for (int r = tid; r >= 0; r = p.links.parent[r]) {
+        for (int r = tid; r >= 0; r = static_cast<int8_t>(p.links.words[r / 4] >> 8 * (r % 4))) {
             sum += L[r];
             if (r != tid) above |= uint64_t(1) << r;
         }

@@ -240,7 +240,7 @@ struct TreeMasks {
     uint64_t m[kTreeMax];
 };
 struct TreeLinks {
-    int8_t parent[kTreeMax];  // -1: continues the context
+    uint32_t words[kTreeMax / 4];  // byte i: the parent of row i (signed; -1: continues the context)
 };
 
 // A key/value cache of either type (include/xqhip.h, xqhip_kv).
@@ -349,6 +349,7 @@ struct VerifyLaunch {
     int32_t* out_tokens;
     void* ws;  // verify_workspace_bytes
     TreeLinks links;
+    uint64_t kids[kTreeMax];  // bit j: row j continues this row
 };
 size_t verify_workspace_bytes(int nodes, int vocab);
 hipError_t launch_verify(const VerifyLaunch& p, hipStream_t s);
