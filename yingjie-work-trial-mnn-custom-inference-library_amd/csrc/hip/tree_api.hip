@@ -198,9 +198,14 @@ int xqhip_linear_attn_tree(const float* mixed, const float* a, const float* b, i
     if (!workspace_ok(workspace, workspace_bytes, need))
         return refuse("xqhip_linear_attn_tree: a 16-byte aligned workspace of %zu bytes (%zu given)", need,
                       workspace_bytes);
-    const xqhip::TreeLinearLaunch p{mixed, a, b, stride, conv_state, pos0, conv_w, a_log, dt_bias, state, lk_n, lk_hd,
-                                    lv_n, lv_hd, ksize, tree->nodes, out, out_stride, static_cast<float*>(workspace),
-                                    links_of(tree)};
+    xqhip::TreeLinearLaunch p{mixed, a, b, stride, conv_state, pos0, conv_w, a_log, dt_bias, state, lk_n, lk_hd,
+                              lv_n, lv_hd, ksize, tree->nodes, out, out_stride, static_cast<float*>(workspace),
+                              links_of(tree), {}, 0};
+    for (int i = 0; i < tree->nodes; ++i)
+        if (const int up = tree->parent[i]; up >= 0) {
+            p.above.m[i] = p.above.m[up] | uint64_t(1) << up;
+            p.inner |= uint64_t(1) << up;
+        }
     return check(xqhip::launch_tree_linear(p, as_stream(stream)), "linear attention tree launch");
 }
 

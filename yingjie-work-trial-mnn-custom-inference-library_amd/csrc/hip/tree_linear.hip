@@ -147,16 +147,304 @@ __global__ void __launch_bounds__(256) tree_delta_kernel(TreeLinearLaunch p) {
         }
 }
 
+// ---------------------------------------------------------------------------
+// Heads of 128 dims and four taps, two launches.
+//
+// tree_linear_prep_kernel: one wave per (row, head): the convolution over the
+//   row's path, SiLU and L2 norm; q and k go out as fp16 hi + lo of 2^10 times
+//   their values (22 bits: a unit vector's entries), the operands of what
+//   follows.  One wave per value head, a row a lane: beta and L (in powers of 2).
+// tree_linear_rows_kernel: one block per value head and 16 columns.  The products
+//   with the state (k_i S0, q_i S0) and among the rows (k_i.k_j, q_i.k_j) on
+//   fp16 MFMA, hi hi + hi lo + lo hi, S0 scaled per column by a power of two and
+//   split likewise.  Then a wave has two columns and a lane a row: for each row j
+//   that others continue, in order, delta_j goes to all lanes as a scalar and the
+//   rows below j add its part: steps as many as inner rows, each a dozen
+//   dependent instructions, no barrier.
+//
+// What bounds it: latency (a launch, one round of loads, the steps); the bytes (the
+// state, 2 MB for 32 heads, and 128 KB a row) are 1 us.
+// ---------------------------------------------------------------------------
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+constexpr int kTL = 128;          // head dims
+constexpr int kTLCols = 16;       // columns of a block
+constexpr int kTLWaves = 8;       // of a block, kTLCols / kTLWaves columns each
+constexpr int kTLPitch = kTreeMax + 4;
+constexpr float kTLRaise = 1024.0f;
+
+namespace {
+struct FastWs {
+    _Float16 *q, *k;  // [lk_n][2 (hi, lo)][rows][128], rows to a multiple of 16
+    float* v;         // [lv_n][rows][128]
+    double* L;        // [lv_n][64]: log2 of the decay from the state to each row
+    float* beta;      // [lv_n][64]
+};
+__host__ __device__ inline int fast_rows(int nodes) { return (nodes + 15) / 16 * 16; }
+__host__ __device__ inline size_t fast_bytes(int nodes, int lk_n, int lv_n) {
+    const size_t rows = fast_rows(nodes);
+    return 2 * (static_cast<size_t>(lk_n) * 2 * rows * kTL * 2) + static_cast<size_t>(lv_n) * rows * kTL * 4 +
+           static_cast<size_t>(lv_n) * kTreeMax * 12;
+}
+__device__ inline FastWs fast_ws(const TreeLinearLaunch& p) {
+    const size_t rows = fast_rows(p.nodes), half = static_cast<size_t>(p.lk_n) * 2 * rows * kTL;
+    FastWs w;
+    w.q = reinterpret_cast<_Float16*>(p.ws);
+    w.k = w.q + half;
+    w.v = reinterpret_cast<float*>(w.k + half);
+    w.L = reinterpret_cast<double*>(w.v + static_cast<size_t>(p.lv_n) * rows * kTL);
+    w.beta = reinterpret_cast<float*>(w.L + static_cast<size_t>(p.lv_n) * kTreeMax);
+    return w;
+}
+}  // namespace
+
+constexpr int kTLPrepWaves = 4;
+__global__ void __launch_bounds__(kWave* kTLPrepWaves) tree_linear_prep_kernel(TreeLinearLaunch p, int row_blocks) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const FastWs ws = fast_ws(p);
+    if (static_cast<int>(blockIdx.x) >= row_blocks) {  // the gates: lane = row
+        const int vh = (static_cast<int>(blockIdx.x) - row_blocks) * kTLPrepWaves + threadIdx.x / kWave;
+        if (vh >= p.lv_n) return;
+        const bool on = lane < p.nodes;
+        const size_t at = static_cast<size_t>(on ? lane : 0) * p.stride + vh;
+        const float a = p.a[at], b = p.b[at];
+        const float log_gate = fmaxf(-expf(p.a_log[vh]) * softplus_dev(a + p.dt_bias[vh]), -1000.0f);
+        const double mine = on ? static_cast<double>(log_gate) * 1.44269504088896340736 : 0.0;
+        // path sums by doubling: after step s a lane has the sum of the last 2^s rows of its path
+        int up = on ? static_cast<int8_t>(p.links.words[lane / 4] >> 8 * (lane % 4)) : -1;
+        double sum = mine;
+#pragma unroll
+        for (int s = 0; s < 6; ++s) {
+            const double add = __shfl(sum, up < 0 ? lane : up, kWave);
+            const int next = __shfl(up, up < 0 ? lane : up, kWave);
+            if (up >= 0) {
+                sum += add;
+                up = next;
+            }
+        }
+        ws.L[vh * kTreeMax + lane] = sum;
+        ws.beta[vh * kTreeMax + lane] = sigmoid_dev(b);
+        return;
+    }
+    const int units = 2 * p.lk_n + p.lv_n, rows = fast_rows(p.nodes);
+    const int id = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * kTLPrepWaves + static_cast<int>(threadIdx.x) / kWave);
+    const int i = id / units, u = id % units;
+    if (i >= p.nodes) return;
+    const bool is_q = u < p.lk_n, is_k = !is_q && u < 2 * p.lk_n;
+    const int h = is_q ? u : (is_k ? u - p.lk_n : u - 2 * p.lk_n);
+    const int c = (is_q ? 0 : (is_k ? p.lk_n : 2 * p.lk_n)) * kTL + h * kTL + 2 * lane;
+    const int conv_dim = (2 * p.lk_n + p.lv_n) * kTL;
+    // the window, newest first: rows of the path, then the history's newest entries
+    float2 x[4];
+    int r = i, back = 0;
+    const float* hs = p.conv_state + static_cast<size_t>(*p.pos0 & 1) * conv_dim * 3 + static_cast<size_t>(c) * 3;
+    const float w[8] = {p.conv_w[4 * c], p.conv_w[4 * c + 1], p.conv_w[4 * c + 2], p.conv_w[4 * c + 3],
+                        p.conv_w[4 * c + 4], p.conv_w[4 * c + 5], p.conv_w[4 * c + 6], p.conv_w[4 * c + 7]};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (r >= 0) {  // wave-uniform
+            const float* row = p.mixed + static_cast<size_t>(r) * p.stride + c;
+            x[t] = make_float2(row[0], row[1]);
+            r = static_cast<int8_t>(p.links.words[r / 4] >> 8 * (r % 4));
+        } else {
+            x[t] = make_float2(hs[2 - back], hs[5 - back]);
+            ++back;
+        }
+    }
+    float y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        y0 += x[3 - t].x * w[t];
+        y1 += x[3 - t].y * w[4 + t];
+    }
+    y0 = silu_dev(y0);
+    y1 = silu_dev(y1);
+    if (!is_q && !is_k) {
+        *reinterpret_cast<float2*>(ws.v + (static_cast<size_t>(h) * rows + i) * kTL + 2 * lane) = make_float2(y0, y1);
+        return;
+    }
+    const float inv = 1.0f / sqrtf(wave_sum(y0 * y0 + y1 * y1) + 1.0e-6f);
+    float z[2] = {y0 * inv * kTLRaise, y1 * inv * kTLRaise};
+    h2 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        asm("" : "+v"(z[e]));  // (one rounding for hi and for what lo is taken from)
+        hi[e] = static_cast<_Float16>(z[e]);
+        lo[e] = static_cast<_Float16>(z[e] - static_cast<float>(hi[e]));
+    }
+    _Float16* out = (is_q ? ws.q : ws.k) + (static_cast<size_t>(h) * 2 * rows + i) * kTL + 2 * lane;
+    *reinterpret_cast<h2*>(out) = hi;
+    *reinterpret_cast<h2*>(out + static_cast<size_t>(rows) * kTL) = lo;
+}
+
+constexpr int kTLLd = kTL + 8;  // halves per operand row: 16-byte rows shifted by 4 banks
+struct RowsSmem {
+    float kk[kTreeMax][kTLPitch], qk[kTreeMax][kTLPitch];  // [j][i]: k_i.k_j, q_i.k_j
+    float kS[kTLCols][kTLPitch], qS[kTLCols][kTLPitch];    // [column][i]
+};
+// behind it the operands: [q, k][hi, lo][rows][kTLLd]
+inline size_t rows_lds(int nodes) { return sizeof(RowsSmem) + static_cast<size_t>(4) * fast_rows(nodes) * kTLLd * 2; }
+
+__global__ void __launch_bounds__(kWave* kTLWaves, 2) tree_linear_rows_kernel(TreeLinearLaunch p) {
+    extern __shared__ uint4 tree_lds[];
+    RowsSmem& sm = *reinterpret_cast<RowsSmem*>(tree_lds);
+    _Float16* ops = reinterpret_cast<_Float16*>(&sm + 1);
+    const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int vh = blockIdx.x, j0 = blockIdx.y * kTLCols, kh = vh / (p.lv_n / p.lk_n);
+    const int n = p.nodes, rows = fast_rows(n), tiles = rows / 16;
+    const FastWs ws = fast_ws(p);
+    const int g = lane / 16, cl = lane % 16;
+    // every load first: the state's columns, the operands, the wave's two columns of v and its rows' gates
+    float s0[4][8];
+    const bool has_tile = wid < 2 * tiles;  // (q or k, row tile) of this wave
+    {
+        const float* S = p.state + (static_cast<size_t>(vh) * kTL + 8 * g) * kTL + j0 + cl;
+        if (has_tile)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s0[s][e] = S[(32 * s + e) * kTL];
+    }
+    const int row = lane < n ? lane : n - 1, col = j0 + 2 * wid;
+    const float2 v = *reinterpret_cast<const float2*>(ws.v + (static_cast<size_t>(vh) * rows + row) * kTL + col);
+    const double L = ws.L[vh * kTreeMax + lane];
+    const float beta = ws.beta[vh * kTreeMax + lane];
+    const uint64_t above = p.above.m[lane];
+    // a quarter of the operands is rows * 16 pieces of 16 bytes: q hi, q lo, k hi, k lo
+    const int quarter = rows * (kTL / 8);
+    u32x4 piece[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int at = threadIdx.x + u * kWave * kTLWaves, part = at / quarter, in = at % quarter;
+        const _Float16* src = (part < 2 ? ws.q : ws.k) + (static_cast<size_t>(kh) * 2 + (part & 1)) * rows * kTL;
+        if (part < 4) piece[u] = *reinterpret_cast<const u32x4*>(src + 8 * in);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int at = threadIdx.x + u * kWave * kTLWaves, part = at / quarter, in = at % quarter;
+        if (part < 4)
+            *reinterpret_cast<u32x4*>(ops + (static_cast<size_t>(part) * rows + in / (kTL / 8)) * kTLLd + 8 * (in % (kTL / 8))) = piece[u];
+    }
+    __syncthreads();
+    // operand fragments of 16 rows: lane holds row cl, dims 32 s + 8 g .. + 7
+    auto frag = [&](bool of_k, int t, half8 (&hi)[4], half8 (&lo)[4]) {
+        const _Float16* at = ops + (static_cast<size_t>(of_k ? 2 : 0) * rows + 16 * t + cl) * kTLLd + 8 * g;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            hi[s] = *reinterpret_cast<const half8*>(at + 32 * s);
+            lo[s] = *reinterpret_cast<const half8*>(at + rows * kTLLd + 32 * s);
+        }
+    };
+    auto product = [&](const half8 (&ah)[4], const half8 (&al)[4], const half8 (&bh)[4], const half8 (&bl)[4]) {
+        floatx4 c = {0.0f, 0.0f, 0.0f, 0.0f}, d = c, e = c;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], bh[s], c, 0, 0, 0);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], bl[s], d, 0, 0, 0);
+            e = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], bh[s], e, 0, 0, 0);
+        }
+        return c + d + e;
+    };
+    if (has_tile) {
+        const bool of_k = wid < tiles;
+        const int a = wid % tiles;
+        half8 ah[4], al[4], bh[4], bl[4];
+        frag(of_k, a, ah, al);
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(s0[s][e]));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+        int ex = 13;  // a power of two brings the column's largest magnitude into [2^12, 2^13)
+        if (mx > 0.0f && mx < INFINITY) frexpf(mx, &ex);
+        ex = max(ex, -100);
+        const float up = ldexpf(1.0f, 13 - ex), down = ldexpf(1.0f / kTLRaise, ex - 13);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = s0[s][e] * up;
+                bh[s][e] = static_cast<_Float16>(x);
+                bl[s][e] = static_cast<_Float16>(x - static_cast<float>(bh[s][e]));
+            }
+        *reinterpret_cast<floatx4*>(&(of_k ? sm.kS : sm.qS)[cl][16 * a + 4 * g]) = product(ah, al, bh, bl) * down;
+        // among the rows: with the k rows of every tile that holds a row above one of this tile's, or the rows themselves
+        for (int b = 0; b <= a; ++b) {
+            if (b < a && !__builtin_amdgcn_ballot_w64(lane / 16 == a && (above >> 16 * b & 0xffff))) continue;
+            frag(true, b, bh, bl);
+            *reinterpret_cast<floatx4*>(&(of_k ? sm.kk : sm.qk)[16 * b + cl][16 * a + 4 * g]) =
+                product(ah, al, bh, bl) * (1.0f / (kTLRaise * kTLRaise));
+        }
+    }
+    __syncthreads();
+    // lane: a row; two columns
+    const float from0 = __builtin_amdgcn_exp2f(static_cast<float>(L));
+    float pred[2], o[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        pred[e] = from0 * sm.kS[2 * wid + e][row];
+        o[e] = from0 * sm.qS[2 * wid + e][row];
+    }
+    const float self = sm.qk[row][row];
+    const long long lb = __double_as_longlong(L);
+    uint64_t left = p.inner;
+    int j = left ? __builtin_ctzll(left) : 0;
+    float a = sm.kk[j][row], b = sm.qk[j][row];
+    while (left) {
+        const int at = j;
+        const float ka = a, qa = b;
+        left &= left - 1;
+        j = left ? __builtin_ctzll(left) : 0;
+        a = sm.kk[j][row];  // the next step's
+        b = sm.qk[j][row];
+        const double Lj = __hiloint2double(__builtin_amdgcn_readlane(static_cast<int>(lb >> 32), at),
+                                           __builtin_amdgcn_readlane(static_cast<int>(lb), at));
+        const float decay = __builtin_amdgcn_exp2f(static_cast<float>(L - Lj));
+        const bool below = above >> at & 1;  // (rows elsewhere may hold anything)
+        const float ck = decay * ka, cq = decay * qa;
+        const float d0 = readlane_f32(beta * (v.x - pred[0]), at), d1 = readlane_f32(beta * (v.y - pred[1]), at);
+        if (below) {
+            pred[0] += ck * d0;
+            pred[1] += ck * d1;
+            o[0] += cq * d0;
+            o[1] += cq * d1;
+        }
+    }
+    if (lane >= n) return;
+    const float rs = 0.08838834764831845f;  // 1 / sqrt(128)
+    float* out = p.out + static_cast<size_t>(lane) * p.out_stride + vh * kTL + col;
+    out[0] = (o[0] + self * (beta * (v.x - pred[0]))) * rs;
+    out[1] = (o[1] + self * (beta * (v.y - pred[1]))) * rs;
+}
+
+static bool linear_fast(int lk_hd, int lv_hd) { return lk_hd == kTL && lv_hd == kTL; }
+
 bool tree_linear_supported(int lk_n, int lk_hd, int lv_n, int lv_hd, int ksize) {
     return lk_n > 0 && lv_n > 0 && lk_n <= 4096 && lv_n <= 4096 && lv_n % lk_n == 0 && lk_hd > 0 && lv_hd > 0 &&
            lk_hd <= kTreeLinMaxDim && lv_hd <= kTreeLinMaxDim && ksize > 0 && ksize <= kTreeLinMaxTaps;
 }
 
 size_t tree_linear_workspace_bytes(int nodes, int lk_n, int lk_hd, int lv_n, int lv_hd) {
+    if (linear_fast(lk_hd, lv_hd)) return fast_bytes(nodes, lk_n, lv_n);  // (more than the general form takes)
     return static_cast<size_t>(nodes) * (2 * lk_n * lk_hd + lv_n * lv_hd) * sizeof(float);
 }
 
 hipError_t launch_tree_linear(const TreeLinearLaunch& p, hipStream_t s) {
+    if (linear_fast(p.lk_hd, p.lv_hd) && p.ksize == 4) {
+        const int row_blocks = ((2 * p.lk_n + p.lv_n) * p.nodes + kTLPrepWaves - 1) / kTLPrepWaves;
+        hipLaunchKernelGGL(tree_linear_prep_kernel, dim3(row_blocks + (p.lv_n + kTLPrepWaves - 1) / kTLPrepWaves),
+                           dim3(kWave * kTLPrepWaves), 0, s, p, row_blocks);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        const size_t lds = rows_lds(p.nodes);
+        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_linear_rows_kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(rows_lds(kTreeMax)));
+            e != hipSuccess)
+            return e;
+        hipLaunchKernelGGL(tree_linear_rows_kernel, dim3(p.lv_n, kTL / kTLCols), dim3(kWave * kTLWaves), lds, s, p);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL(tree_conv_kernel, dim3(2 * p.lk_n + p.lv_n, p.nodes), dim3(kWave), 0, s, p);
     hipLaunchKernelGGL(tree_delta_kernel, dim3(p.lv_n, (p.lv_hd + kTreeLinCols - 1) / kTreeLinCols), dim3(256), 0, s, p);
     return hipGetLastError();

@@ -328,6 +328,8 @@ struct TreeLinearLaunch {
     int out_stride;
     float* ws;  // tree_linear_workspace_bytes
     TreeLinks links;
+    TreeMasks above;  // bit j: row j is on the row's path, above it
+    uint64_t inner;   // rows that another row continues
 };
 bool tree_linear_supported(int lk_n, int lk_hd, int lv_n, int lv_hd, int ksize);
 size_t tree_linear_workspace_bytes(int nodes, int lk_n, int lk_hd, int lv_n, int lv_hd);
