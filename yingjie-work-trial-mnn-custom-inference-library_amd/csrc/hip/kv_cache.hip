@@ -52,13 +52,27 @@ __global__ void __launch_bounds__(kWave* kPrepWaves) kv_prep_kernel(KvPrepLaunch
             for (int e = 0; e < E; ++e) x[e] = in(e) ? s[dim(e)] : 0.0f;
         }
     };
-    float x[E], w[E], gate[E];
+    auto put = [&](auto* row, const auto (&v)[E]) {
+        if constexpr (VEC) {
+            typedef std::remove_pointer_t<decltype(row)> T;
+            struct alignas(E * sizeof(T)) Piece {
+                T v[E];
+            };
+            Piece piece;
+#pragma unroll
+            for (int e = 0; e < E; ++e) piece.v[e] = v[e];
+            *reinterpret_cast<Piece*>(row + lane * E) = piece;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (in(e)) row[dim(e)] = v[e];
+        }
+    };
+    float x[E], w[E], gate[E] = {};
     load(src, x);
     if (is_q && p.gated) load(src + hd, gate);
     const float* norm = is_q ? p.q_norm : p.k_norm;
-    if (is_q || is_k)
-#pragma unroll
-        for (int e = 0; e < E; ++e) w[e] = in(e) ? norm[dim(e)] : 0.0f;
+    if (is_q || is_k) load(norm, w);
     // (64 bits: *pos0 is the caller's)
     const int64_t slot = static_cast<int64_t>(*p.pos0) + t;
     const int64_t pos = static_cast<int64_t>(*p.pos0) + (p.has_tree ? p.depth[t] : t);
@@ -92,19 +106,20 @@ __global__ void __launch_bounds__(kWave* kPrepWaves) kv_prep_kernel(KvPrepLaunch
         const size_t o = static_cast<size_t>(t) * p.out_stride + static_cast<size_t>(h) * hd;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if (!in(e)) continue;
-            p.q_out[o + dim(e)] = held ? x[e] : __builtin_nanf("");
-            if (p.gate_out) p.gate_out[o + dim(e)] = p.gated ? gate[e] : 0.0f;
+            x[e] = held ? x[e] : __builtin_nanf("");
+            gate[e] = p.gated ? gate[e] : 0.0f;
         }
+        put(p.q_out + o, x);
+        if (p.gate_out) put(p.gate_out + o, gate);
         return;
     }
     if (!held) return;
     const size_t head = static_cast<size_t>(slot) * nkv + h;
     if (!p.kv.i8) {
-        _Float16* row = static_cast<_Float16*>(is_k ? p.kv.k : p.kv.v) + head * hd;
+        _Float16 v[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (in(e)) row[dim(e)] = static_cast<_Float16>(x[e]);
+        for (int e = 0; e < E; ++e) v[e] = static_cast<_Float16>(x[e]);
+        put(static_cast<_Float16*>(is_k ? p.kv.k : p.kv.v) + head * hd, v);
         return;
     }
     float mx = 0.0f;
@@ -117,13 +132,11 @@ __global__ void __launch_bounds__(kWave* kPrepWaves) kv_prep_kernel(KvPrepLaunch
     mx = wave_max(mx);
     fine = __builtin_amdgcn_ballot_w64(!fine) == 0;
     const float scale = fine ? mx / 127.0f : __builtin_nanf("");
-    int8_t* row = static_cast<int8_t*>(is_k ? p.kv.k : p.kv.v) + head * hd;
+    int8_t code[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        // (a scale this small is a denormal with few bits: the quotient can pass 127)
-        const float c = fine && scale > 0.0f ? fminf(fmaxf(rintf(x[e] / scale), -127.0f), 127.0f) : 0.0f;
-        if (in(e)) row[dim(e)] = static_cast<int8_t>(c);
-    }
+    for (int e = 0; e < E; ++e)  // (a tiny scale is a denormal with few bits: the quotient can pass 127)
+        code[e] = static_cast<int8_t>(fine && scale > 0.0f ? fminf(fmaxf(rintf(x[e] / scale), -127.0f), 127.0f) : 0.0f);
+    put(static_cast<int8_t*>(is_k ? p.kv.k : p.kv.v) + head * hd, code);
     if (lane == 0) (is_k ? p.kv.k_scale : p.kv.v_scale)[head] = scale;
 }
 
@@ -131,8 +144,11 @@ hipError_t launch_kv_prep(const KvPrepLaunch& p, hipStream_t s) {
     const int hd = p.kv.head_dim, units = p.nq + 2 * p.kv.nkv;
     const dim3 grid((units + kPrepWaves - 1) / kPrepWaves, p.tokens), block(kWave * kPrepWaves);
     const uintptr_t ptrs = reinterpret_cast<uintptr_t>(p.q_src) | reinterpret_cast<uintptr_t>(p.k_src) |
-                           reinterpret_cast<uintptr_t>(p.v_src);
-    const bool al = (ptrs & 15u) == 0 && p.src_stride % 4 == 0;
+                           reinterpret_cast<uintptr_t>(p.v_src) | reinterpret_cast<uintptr_t>(p.q_norm) |
+                           reinterpret_cast<uintptr_t>(p.k_norm) | reinterpret_cast<uintptr_t>(p.q_out) |
+                           reinterpret_cast<uintptr_t>(p.gate_out) | reinterpret_cast<uintptr_t>(p.kv.k) |
+                           reinterpret_cast<uintptr_t>(p.kv.v);
+    const bool al = (ptrs & 15u) == 0 && p.src_stride % 4 == 0 && p.out_stride % 4 == 0;
     if (hd == 128 && al)
         hipLaunchKernelGGL((kv_prep_kernel<2, false, true>), grid, block, 0, s, p);
     else if (hd == 256 && al)
@@ -144,8 +160,17 @@ hipError_t launch_kv_prep(const KvPrepLaunch& p, hipStream_t s) {
 
 // ---------------------------------------------------------------------------
 // 8-bit rows read back: value = code * scale, in fp32, rounded once for fp16.
-// Memory-bound: 1 byte in, 2 or 4 out per value.
+// Memory-bound: 1 byte in, 2 or 4 out per value.  A thread takes the codes of one
+// 16-byte piece of the output at a time (a wave then writes 1 KiB in a row), four
+// pieces in flight.  General form: value by value.
 // ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ T read_value(int code, float scale) {
+    float x = static_cast<float>(code) * scale;
+    asm("" : "+v"(x));  // the fp32 product is a value of its own (else it is rounded to fp16 without it)
+    return static_cast<T>(x);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvReadLaunch p) {
     const int hd = p.kv.head_dim;
@@ -156,20 +181,67 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvReadLaunch p) {
     T* out = static_cast<T*>(v ? p.v_out : p.k_out);
     if (!out) return;
     for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < heads * hd;
-         i += static_cast<size_t>(gridDim.x) * 256) {
-        float x = static_cast<float>(code[i]) * scale[i / hd];
-        asm("" : "+v"(x));  // the fp32 product is a value of its own (else it is rounded to fp16 without it)
-        out[i] = static_cast<T>(x);
+         i += static_cast<size_t>(gridDim.x) * 256)
+        out[i] = read_value<T>(code[i], scale[i / hd]);
+}
+
+constexpr int kReadPieces = 4;  // pieces of a thread
+template <typename T>
+__global__ void __launch_bounds__(256) kv_read_pieces_kernel(KvReadLaunch p, uint32_t pieces, uint32_t per_head, int shift) {
+    constexpr int N = 16 / sizeof(T);
+    typedef T out_t __attribute__((ext_vector_type(N)));
+    typedef signed char code_t __attribute__((ext_vector_type(N)));
+    const size_t first = static_cast<size_t>(p.first) * p.kv.nkv;
+    const bool v = blockIdx.y != 0;
+    const code_t* code = reinterpret_cast<const code_t*>(static_cast<const int8_t*>(v ? p.kv.v : p.kv.k) + first * p.kv.head_dim);
+    const float* scale = (v ? p.kv.v_scale : p.kv.k_scale) + first;
+    out_t* out = static_cast<out_t*>(v ? p.v_out : p.k_out);
+    if (!out) return;
+    const uint32_t i0 = blockIdx.x * (256u * kReadPieces) + threadIdx.x;
+    code_t c[kReadPieces];
+    float f[kReadPieces];
+#pragma unroll
+    for (int u = 0; u < kReadPieces; ++u) {
+        const uint32_t i = i0 + 256u * u;
+        if (i < pieces) {
+            c[u] = code[i];
+            f[u] = scale[shift >= 0 ? i >> shift : i / per_head];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kReadPieces; ++u) {
+        const uint32_t i = i0 + 256u * u;
+        if (i >= pieces) return;
+        out_t o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = read_value<T>(c[u][e], f[u]);
+        out[i] = o;
     }
 }
 
+template <typename T>
+static void launch_read(const KvReadLaunch& p, hipStream_t s) {
+    constexpr int N = 16 / sizeof(T);
+    const int hd = p.kv.head_dim;
+    const size_t n = static_cast<size_t>(p.count) * p.kv.nkv * hd;
+    const uintptr_t outs = reinterpret_cast<uintptr_t>(p.k_out) | reinterpret_cast<uintptr_t>(p.v_out);
+    const uintptr_t codes = reinterpret_cast<uintptr_t>(p.kv.k) | reinterpret_cast<uintptr_t>(p.kv.v);
+    if (hd % N == 0 && (outs & 15u) == 0 && codes % N == 0 && n / N < (size_t(1) << 31)) {
+        const uint32_t pieces = static_cast<uint32_t>(n / N), per = hd / N;
+        const int shift = (per & (per - 1)) == 0 ? __builtin_ctz(per) : -1;
+        hipLaunchKernelGGL(kv_read_pieces_kernel<T>, dim3((pieces + 256 * kReadPieces - 1) / (256 * kReadPieces), 2), dim3(256),
+                           0, s, p, pieces, per, shift);
+        return;
+    }
+    hipLaunchKernelGGL(kv_read_kernel<T>, dim3(static_cast<unsigned>(std::min<size_t>((n + 255) / 256, 16384)), 2), dim3(256),
+                       0, s, p);
+}
+
 hipError_t launch_kv_read(const KvReadLaunch& p, hipStream_t s) {
-    const size_t n = static_cast<size_t>(p.count) * p.kv.nkv * p.kv.head_dim;
-    const dim3 grid(static_cast<unsigned>(std::min<size_t>((n + 255) / 256, 16384)), 2);
     if (p.f16)
-        hipLaunchKernelGGL((kv_read_kernel<_Float16>), grid, dim3(256), 0, s, p);
+        launch_read<_Float16>(p, s);
     else
-        hipLaunchKernelGGL((kv_read_kernel<float>), grid, dim3(256), 0, s, p);
+        launch_read<float>(p, s);
     return hipGetLastError();
 }
 
@@ -180,14 +252,15 @@ hipError_t launch_kv_read(const KvReadLaunch& p, hipStream_t s) {
 // waits for another.
 // ---------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ void keep_column(const KeepLaunch& p, const KeepSet& s, int count, int64_t first, size_t at) {
+__device__ __forceinline__ void keep_column(const KeepSet& s, int path, int from, int count, int64_t first, size_t at) {
     constexpr int kBatch = 8;  // rows in flight
     uint8_t* col = s.base + static_cast<size_t>(first) * s.row_bytes + at * sizeof(T);
-    for (int j0 = 0; j0 < count; j0 += kBatch) {
-        T v[kBatch];
+    for (int j0 = from; j0 < count; j0 += kBatch) {
+        T v[kBatch] = {};
 #pragma unroll
         for (int u = 0; u < kBatch; ++u)
-            if (j0 + u < count) v[u] = *reinterpret_cast<const T*>(col + static_cast<size_t>(p.path[j0 + u]) * s.row_bytes);
+            if (j0 + u < count)
+                v[u] = *reinterpret_cast<const T*>(col + static_cast<size_t>(__builtin_amdgcn_readlane(path, j0 + u)) * s.row_bytes);
 #pragma unroll
         for (int u = 0; u < kBatch; ++u)
             if (j0 + u < count) *reinterpret_cast<T*>(col + static_cast<size_t>(j0 + u) * s.row_bytes) = v[u];
@@ -199,18 +272,24 @@ __global__ void __launch_bounds__(256) tree_keep_kernel(KeepLaunch p) {
     const bool wide = ((reinterpret_cast<uintptr_t>(s.base) | s.row_bytes) & 15u) == 0;
     const size_t pieces = wide ? s.row_bytes / 16 : s.row_bytes;
     if (static_cast<size_t>(blockIdx.x) * 256 >= pieces) return;
+    // lane j holds path[j]; the moves go up to the first that is none: a row outside the buffer, a path that does not
+    // increase (read one after the other they would be a memory round trip each)
+    const int lane = threadIdx.x & (kWave - 1);
     const int64_t first = s.first ? *s.first : 0;
-    // the moves up to the first that is none: a row outside the buffer, a path that does not increase
     const int want = min(*p.count, p.max_rows);
-    int count = 0, last = -1;
-    if (first >= 0)
-        while (count < want && p.path[count] > last && first + p.path[count] < s.rows) last = p.path[count++];
+    const int path = lane < p.max_rows ? p.path[lane] : -1;
+    int before = __shfl_up(path, 1, kWave);
+    if (lane == 0) before = -1;
+    const uint64_t good = __builtin_amdgcn_ballot_w64(lane < want && path > before && first >= 0 && first + path < s.rows);
+    const int count = ~good ? __builtin_ctzll(~good) : kWave;
+    const uint64_t moved = __builtin_amdgcn_ballot_w64(path != lane);  // the rows before the first such one are in place
+    const int from = moved ? __builtin_ctzll(moved) : kWave;
     for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < pieces;
          i += static_cast<size_t>(gridDim.x) * 256) {
         if (wide)
-            keep_column<uint4>(p, s, count, first, i);
+            keep_column<u32x4>(s, path, from, count, first, i);
         else
-            keep_column<uint8_t>(p, s, count, first, i);
+            keep_column<uint8_t>(s, path, from, count, first, i);
     }
 }
 
