@@ -47,9 +47,10 @@ HIP_FLAGS = [
     "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
     "-I", INCLUDE, "-I", HIP_SRC,
 ]
-# per-source additions: the prefill GEMM scales every MFMA result with VALU ops, so its
-# MFMAs write VGPRs directly instead of accumulation registers that need copying out
-HIP_FILE_FLAGS = {"prefill_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# per-source additions: the prefill GEMM and the tree attention work on every MFMA result with VALU
+# ops, so their MFMAs write VGPRs directly instead of accumulation registers that need copying out
+HIP_FILE_FLAGS = {"prefill_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                  "tree_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-parameter",
               "-fvisibility=hidden", "-I", INCLUDE, "-I", HOST_SRC, "-DXQWEN35_BUILD=1"]
 
