@@ -158,33 +158,19 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 constexpr int kTTile = 32;  // keys and columns of an MFMA tile
 constexpr int kTreeMaxSplits = 64;
 
-template <int HD, bool I8, int CT, int KS, int BUFS = 1>
-struct TreeTile {
+// Columns, waves and output rows of a block: CT column tiles x KS key waves.
+template <int HD, int CT, int KS, int COLS>
+struct TreeBlock {
     static constexpr int kThreads = kWave * CT * KS;
-    static constexpr int kCols = kTTile * CT, kKeys = kTTile * KS;
-    static constexpr int kLdk = HD + 8;   // halves per K row: 16-byte rows shifted by 4 banks
-    static constexpr int kLdv = HD + 16;  // halves per V row: the 4 rows of a transposed read in distinct banks
-    static constexpr int kLdo = HD + 4;   // floats per column of a wave's output
-    static constexpr int kPieceDims = I8 ? 16 : 8;  // values of a 16-byte piece
-    static constexpr int kRowPieces = HD / kPieceDims;
-    static constexpr int kPieces = kKeys * kRowPieces / kThreads;  // pieces of K (or V) per thread and chunk
-    static constexpr int kKeyStep = kThreads / kRowPieces;
+    static constexpr int kCols = COLS, kKeys = kTTile * KS;
+    static constexpr int kLdo = HD + 4;                   // floats per column of a wave's output
     static constexpr int kQuads = HD / 4;                 // float4 of an output row
     static constexpr int kMergeCols = kThreads / kQuads;  // columns per pass of the merge
     static constexpr int kPasses = kCols / kMergeCols;
-    // scales of K and V, then each wave's V scales over its R
-    static constexpr size_t kScaleBytes = !I8 ? 0 : BUFS == 1 ? static_cast<size_t>(kKeys) * 2 * 4 + static_cast<size_t>(CT * KS) * kTTile * 4
-                                                              : static_cast<size_t>(BUFS) * (2 * kKeys + KS) * 4;
-    static constexpr size_t kKvBytes = static_cast<size_t>(BUFS) * kKeys * (kLdk + kLdv) * 2 + kScaleBytes;
-    static constexpr size_t kOutBytes = static_cast<size_t>(CT * KS) * kTTile * (kLdo + 2) * 4;
-    static constexpr size_t kLds = kKvBytes > kOutBytes ? kKvBytes : kOutBytes;
-    static_assert(kPieces * kThreads == kKeys * kRowPieces && kPieces > 0, "K / V staging");
+    static constexpr size_t kOutBytes = static_cast<size_t>(kCols) * KS * (kLdo + 2) * 4;
+    static constexpr int kLdv = HD + 16;  // halves per V row: the 4 rows of a transposed read in distinct banks
     static_assert(kPasses * kThreads == kCols * kQuads, "merge");
-    static_assert(!I8 || 2 * kKeys <= kThreads, "one scale per thread");
-    static_assert(kLds + 64 <= 160 * 1024, "LDS");
-    static_assert(BUFS > 1 || static_cast<size_t>(kKeys) * kLdk * 2 + static_cast<size_t>(kCols) * kLdo * 4 <= kLds, "q fits behind K");
-    static_assert(static_cast<size_t>(kCols) * kLdo * 4 <= kLds, "q fits");
-    static_assert(kLds >= tree_row_lds(kTreeMaxGroup, HD) * 4, "the general form runs in it");
+    static_assert(kOutBytes >= tree_row_lds(kTreeMaxGroup, HD) * 4, "the general form runs in it");
 };
 
 __device__ __forceinline__ float pair32_max(float v) {  // of v[l] and v[l ^ 32]
@@ -192,6 +178,18 @@ __device__ __forceinline__ float pair32_max(float v) {  // of v[l] and v[l ^ 32]
     const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])),
                  __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+
+__device__ __forceinline__ float xor16_max(float v) {  // of v[l] and v[l ^ 16]
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])),
+                 __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+// even rows of 16 lanes: a[l] + a[l ^ 16]; odd rows: b[l] + b[l ^ 16]
+__device__ __forceinline__ float rows_sum(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
 }
 
 // fp32 -> fp16 hi + fp16 lo (x - hi) of 8 values
@@ -231,392 +229,448 @@ struct TreeGrid {
 };
 
 // key chunks [begin, end) of split s of `chunks`: the first min(splits, chunks) splits have some
-__device__ __forceinline__ void split_range(int chunks, int splits, int s, int& begin, int& end) {
+// (returned)
+__device__ __forceinline__ int split_range(int chunks, int splits, int s, int& begin, int& end) {
     const int n = min(splits, chunks), per = chunks / n, more = chunks - per * n;
     begin = s * per + min(s, more);
     end = s < n ? begin + per + (s < more ? 1 : 0) : begin;
+    return n;
 }
 
-template <int HD, bool I8, int CT, int KS>
-__global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_mfma_kernel(TreeAttnLaunch p, TreeGrid grid) {
-    using F = TreeTile<HD, I8, CT, KS>;
-    constexpr int kSteps = HD / 16, kDimTiles = HD / 32;
-    constexpr float kLog2e = 1.44269504088896340736f;
-    constexpr float kRaise = 6.0f;  // weights are held times 2^kRaise
-    constexpr float kSlack = 6.0f;  // the max may outgrow the reference by 2^kSlack before it is moved
-    constexpr float kScaleSlack = 8.0f;
-    extern __shared__ uint4 flash_lds[];
-    __shared__ int redo;
-    _Float16* Kl = reinterpret_cast<_Float16*>(flash_lds);  // [kKeys][kLdk]
-    _Float16* Vl = Kl + F::kKeys * F::kLdk;                 // [kKeys][kLdv]
-    float* Sl = reinterpret_cast<float*>(Vl + F::kKeys * F::kLdv);  // [2][kKeys] scales of K, V
-    // the kv heads of a tile are neighbours in launch order (8 heads: an XCD each), then the row tiles of the
-    // same keys, so that a head's blocks read its K / V from one L2
-    const int nkv = p.kv.nkv, kh = blockIdx.x % nkv;
-    const int rest = static_cast<int>(blockIdx.x) / nkv, tile = grid.tiles - 1 - rest % grid.tiles, sp = rest / grid.tiles;
-    const int group = p.nq / nkv, T = F::kCols / group;
-    const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int ct = wid % CT, ks = wid / CT;
-    const int cl = lane & 31, g = lane >> 5;
-    const int pos0 = __builtin_amdgcn_readfirstlane(clamp_pos0(p));
-    const uint32_t inv_t = (65535u + T) / T;  // c / T = c inv_t >> 16 for c < 128, T <= 128
-    const int t0 = tile * T, ntok = min(T, p.tokens - t0);
-    const int col = ct * kTTile + cl, ch = static_cast<int>(col * inv_t >> 16), ctok = col - ch * T;
-    const bool live = ch < group && ctok < ntok;
-    const int last = min(pos0 + (p.has_tree ? p.tokens : t0 + ntok), p.kv.capacity) - 1;  // any column's last key
-    const int sure = p.has_tree ? pos0 - 1 : pos0 + t0;  // every column sees the keys up to here
-    const int qpos = live ? pos0 + t0 + ctok : -1;
-    const uint64_t mask = live && p.has_tree ? p.masks.m[t0 + ctok] : 0;
-    int begin, end;
-    split_range(last / F::kKeys + 1, grid.splits, sp, begin, end);
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    end = __builtin_amdgcn_readfirstlane(end);
-    if (begin >= end) return;  // fewer chunks than splits (or no key at all: the merge sees to it)
+// exponent of a V scale, for the reference of its key's weights
+__device__ __forceinline__ float scale_exponent(float s) {
+    return fabsf(s) > 0.0f ? fminf(fmaxf(static_cast<float>(__builtin_amdgcn_frexp_expf(s)), -80.0f), 100.0f) : -80.0f;
+}
 
-    const uint32_t es = I8 ? 1u : 2u, krow = static_cast<uint32_t>(nkv) * HD * es;  // bytes per cache position
-    const int pk = threadIdx.x / F::kRowPieces, pd = threadIdx.x % F::kRowPieces;
-    u32x4 kr[F::kPieces], vr[F::kPieces];
-    auto load = [&](const void* cache, int c0, u32x4 (&r)[F::kPieces]) {  // keys past `last` read 0
-        const int n = __builtin_amdgcn_readfirstlane(max(0, min(F::kKeys, last - c0 + 1)));
-        const uint8_t* base = static_cast<const uint8_t*>(cache) +
-                              static_cast<size_t>(__builtin_amdgcn_readfirstlane(max(0, min(c0, last)))) * krow +
-                              static_cast<uint32_t>(kh) * HD * es;
-        const __amdgpu_buffer_rsrc_t rs = buf_rsrc(base, static_cast<uint32_t>(n) * krow);
-#pragma unroll
-        for (int u = 0; u < F::kPieces; ++u)
-            r[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, static_cast<uint32_t>(pk + u * F::kKeyStep) * krow + pd * 16u,
-                                                         0, 0);
-    };
-    auto store = [&](_Float16* d, int ld, const u32x4 (&r)[F::kPieces]) {
-#pragma unroll
-        for (int u = 0; u < F::kPieces; ++u) {
-            _Float16* at = d + (pk + u * F::kKeyStep) * ld + F::kPieceDims * pd;
-            if constexpr (I8) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const u32x2 a = codes_to_half(r[u][2 * h]), b = codes_to_half(r[u][2 * h + 1]);
-                    *reinterpret_cast<u32x4*>(at + 8 * h) = u32x4{a.x, a.y, b.x, b.y};
-                }
-            } else {
-                *reinterpret_cast<u32x4*>(at) = r[u];
-            }
-        }
-    };
-    // scales: thread i < kKeys holds K's of key i, the next kKeys threads V's
-    const bool k_half = threadIdx.x < F::kKeys;
-    float sr = 0.0f;
-    auto load_scale = [&](int c0) {
-        if constexpr (I8) {
-            const int key = threadIdx.x % F::kKeys;
-            if (threadIdx.x < 2 * F::kKeys)
-                sr = c0 + key <= last ? (k_half ? p.kv.k_scale : p.kv.v_scale)[static_cast<size_t>(c0 + key) * nkv + kh] : 0.0f;
-        }
-    };
-    auto store_scale = [&](bool k) {
-        if constexpr (I8)
-            if (threadIdx.x < 2 * F::kKeys && k_half == k) Sl[threadIdx.x] = sr;
-    };
-    // rows of q, the gate and the output: thread i takes float4 i % kQuads of columns i / kQuads, + kMergeCols, ...
-    auto place = [&](int tid, int u, int stride) {  // float offset of the pass's column from row t0, or -1
-        const int c = tid / F::kQuads + u * F::kMergeCols;
-        const int hc = static_cast<int>(c * inv_t >> 16), tc = c - hc * T;
-        return hc < group && tc < ntok ? tc * stride + (kh * group + hc) * HD + 4 * (tid % F::kQuads) : -1;
-    };
-    u32x4 qr[F::kPasses];
-    {
+// The block's columns of q as fp16 hi + lo in LDS, each scaled by a power of two into [2^12, 2^13), and the factor of
+// each column's scores in the exponent of 2.
+template <typename F, int HD>
+struct QueryStage {
+    static constexpr int kLanes = HD / 8, kStep = F::kThreads / kLanes;  // eight dims a thread
+    static constexpr int kPasses = (F::kCols + kStep - 1) / kStep;
+    static constexpr int kLd = HD + 8;  // halves per column: 16-byte rows shifted by 4 banks
+    static constexpr size_t kBytes = static_cast<size_t>(F::kCols) * (2 * kLd * 2 + 4);
+    u32x4 r[kPasses][2];
+
+    __device__ __forceinline__ void load(const TreeAttnLaunch& p, int kh, int t0, int ntok, int group, int T, uint32_t inv_t) {
         const __amdgpu_buffer_rsrc_t rq =
             buf_rsrc(p.q + static_cast<size_t>(t0) * p.q_stride, static_cast<uint32_t>(ntok) * p.q_stride * 4u);
 #pragma unroll
-        for (int u = 0; u < F::kPasses; ++u) {  // columns without a row read 0
-            const int at = place(threadIdx.x, u, p.q_stride);
-            qr[u] = __builtin_amdgcn_raw_buffer_load_b128(rq, at >= 0 ? static_cast<uint32_t>(at) * 4u : kBufOOB, 0, 0);
+        for (int u = 0; u < kPasses; ++u) {  // columns without a row read 0
+            const int c = threadIdx.x / kLanes + u * kStep, hc = static_cast<int>(c * inv_t >> 16), tc = c - hc * T;
+            const uint32_t at = tc * p.q_stride + (kh * group + hc) * HD + 8 * (threadIdx.x % kLanes);
+            const bool on = c < F::kCols && hc < group && tc < ntok;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                r[u][i] = __builtin_amdgcn_raw_buffer_load_b128(rq, on ? at * 4u + 16u * i : kBufOOB, 0, 0);
         }
     }
-    load(p.kv.k, begin * F::kKeys, kr);
-    load_scale(begin * F::kKeys);
-    float* Ql = reinterpret_cast<float*>(Vl);  // [kCols][kLdo]
+    __device__ __forceinline__ void store(void* lds) const {
+        constexpr float kLog2e = 1.44269504088896340736f;
+        _Float16* Q = static_cast<_Float16*>(lds);  // [2][kCols][kLd]
+        float* S = reinterpret_cast<float*>(Q + 2 * F::kCols * kLd);
 #pragma unroll
-    for (int u = 0; u < F::kPasses; ++u)
-        *reinterpret_cast<u32x4*>(Ql + (threadIdx.x / F::kQuads + u * F::kMergeCols) * F::kLdo +
-                                  4 * (threadIdx.x % F::kQuads)) = qr[u];
-    store(Kl, F::kLdk, kr);
-    if (threadIdx.x == 0) redo = 0;
-    __syncthreads();
-    half8 qhi[kSteps], qlo[kSteps];  // lane supplies dims 16 s + 8 g .. + 7 of its column
-    float sscale;                    // score scale in the exponent of 2
-    {
-        float x[kSteps][8], mx = 0.0f;
+        for (int u = 0; u < kPasses; ++u) {
+            const int c = threadIdx.x / kLanes + u * kStep;
+            if (c >= F::kCols) break;  // wave-uniform
+            float x[8], mx = 0.0f;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(Ql + col * F::kLdo + 16 * s + 8 * g + e);
-                x[s][e] = v.x;
-                x[s][e + 1] = v.y;
-                x[s][e + 2] = v.z;
-                x[s][e + 3] = v.w;
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __uint_as_float(r[u][e / 4][e % 4]);
+                mx = fmaxf(mx, fabsf(x[e]));
             }
+            mx = lanes_max<16>(mx);
+            if constexpr (kLanes == 32) mx = xor16_max(mx);
+            int ex = 13;  // an infinity or 0 stays
+            if (mx > 0.0f && mx < INFINITY) frexpf(mx, &ex);
+            ex = max(ex, -100);  // 2^(13 - ex) stays finite
+            const float down = ldexpf(1.0f, 13 - ex);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[s][e]));
-        mx = pair32_max(mx);
-        // a power of two brings the column's largest magnitude into [2^12, 2^13); an infinity or 0 stays
-        int ex = 13;
-        if (mx > 0.0f && mx < INFINITY) frexpf(mx, &ex);
-        ex = max(ex, -100);  // 2^(13 - ex) stays finite
-        const float down = ldexpf(1.0f, 13 - ex);
-        sscale = ldexpf(kLog2e / sqrtf(static_cast<float>(HD)), ex - 13);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[s][e] *= down;
-            split8(x[s], qhi[s], qlo[s]);
+            for (int e = 0; e < 8; ++e) x[e] *= down;
+            half8 hi, lo;
+            split8(x, hi, lo);
+            _Float16* at = Q + c * kLd + 8 * (threadIdx.x % kLanes);
+            *reinterpret_cast<half8*>(at) = hi;
+            *reinterpret_cast<half8*>(at + F::kCols * kLd) = lo;
+            if (threadIdx.x % kLanes == 0) S[c] = ldexpf(kLog2e / sqrtf(static_cast<float>(HD)), ex - 13);
         }
     }
-    __syncthreads();  // every wave has its q: V (and the scales behind it) may take its place
-    store_scale(true);
-    store_scale(false);
-    __syncthreads();
-    float m = -1.0e30f, l = 0.0f;  // reference of the exponents, this lane's part of the sum
-    float R = 0.0f;                // 8-bit V: the weights' scales are held over R (a power of two)
-    floatx16 o[kDimTiles];
-#pragma unroll
-    for (int j = 0; j < kDimTiles; ++j) o[j] = floatx16{};
-    for (int c = begin; c < end; ++c) {  // block-uniform
-        const int c0 = c * F::kKeys;
-        load(p.kv.v, c0, vr);
-        const int key0 = c0 + ks * kTTile;
-        const bool any = key0 <= last;  // wave-uniform: this wave's tile holds a key
-        half8 phi[2], plo[2];
-        if (any) {
-            floatx16 st = floatx16{};
-            const _Float16* krow_l = Kl + (ks * kTTile + cl) * F::kLdk + 8 * g;
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                const half8 a = *reinterpret_cast<const half8*>(krow_l + 16 * s);
-                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qlo[s], st, 0, 0, 0);
-                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qhi[s], st, 0, 0, 0);
-            }
-            float sc[16], vs[16], mc = -INFINITY;
-            if constexpr (I8) {
-                // V's scales of the tile over R; R moves (rarely after the first tile) when one outgrows it
-                const float mine = Sl[F::kKeys + ks * kTTile + cl];
-                const float top = wave_max(mine);
-                if (top > R * kScaleSlack) {
-                    int ex;
-                    frexpf(top, &ex);
-                    const float to = top < INFINITY ? ldexpf(1.0f, min(ex, 127)) : R;
-                    const float f = R > 0.0f ? R / to : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < kDimTiles; ++j) o[j] *= f;
-                    R = to;
-                }
-                float* over = Sl + 2 * F::kKeys + wid * kTTile;
-                over[cl] = R > 0.0f ? mine / R : mine;
-#pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    typedef float f32x4 __attribute__((ext_vector_type(4)));
-                    const f32x4 k4 = *reinterpret_cast<const f32x4*>(Sl + ks * kTTile + 8 * a + 4 * g);
-                    const f32x4 v4 = *reinterpret_cast<const f32x4*>(over + 8 * a + 4 * g);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sc[4 * a + e] = st[4 * a + e] * k4[e];
-                        vs[4 * a + e] = v4[e];
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) sc[v] = st[v];
-            }
-            if (key0 + kTTile - 1 > sure || key0 + kTTile - 1 > last) {  // wave-uniform: keys that some column does not see
-                uint32_t see;
-                if (p.has_tree) {
-                    see = mask_window(mask, key0 + 4 * g - pos0);
-                } else {
-                    const int b = qpos - (key0 + 4 * g);
-                    see = b < 0 ? 0u : (b >= 31 ? ~0u : (2u << b) - 1u);
-                }
-                const int left = last - (key0 + 4 * g);  // (tree rows and positions past the capacity)
-                see &= left < 0 ? 0u : (left >= 31 ? ~0u : (2u << left) - 1u);
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    if (!(see >> (8 * (v >> 2) + (v & 3)) & 1u)) {
-                        sc[v] = -INFINITY;
-                        if constexpr (I8) vs[v] = 0.0f;  // (its scale may be NaN)
-                    }
-            }
-#pragma unroll
-            for (int v = 0; v < 16; ++v) mc = fmaxf(mc, sc[v]);
-            mc = pair32_max(mc) * sscale;
-            // the reference moves only when a column's max has outgrown it (rarely after the first tiles)
-            const bool up = mc > m + kSlack;
-            if (__builtin_amdgcn_ballot_w64(up)) {
-                const float to = up ? mc : m, f = exp2f(m - to);
-                m = to;
-                l *= f;
-#pragma unroll
-                for (int j = 0; j < kDimTiles; ++j) o[j] *= f;
-            }
-            const float off = kRaise - m;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(fmaf(sc[8 * h + e], sscale, off));
-                    l += x[e];
-                    if constexpr (I8) {
-                        x[e] *= vs[8 * h + e];
-                        // the rounded product: hi and lo would else be taken from two roundings of it
-                        asm("" : "+v"(x[e]));
-                    }
-                }
-                split8(x, phi[h], plo[h]);
-            }
-        }
-        store(Vl, F::kLdv, vr);
-        const bool more = c + 1 < end;  // block-uniform
-        if (more) {
-            load(p.kv.k, c0 + F::kKeys, kr);
-            load_scale(c0 + F::kKeys);
-        }
-        __syncthreads();  // V is staged; every wave has read K and the scales
-        if (any) {
-            // transposed reads: 16 lanes cover four keys x 16 dims, lane i gets dim i of the four
-            const _Float16* vb = Vl + (ks * kTTile + 4 * g + ((lane & 15) >> 2)) * F::kLdv + (lane & 16) + 4 * (lane & 3);
-#pragma unroll
-            for (int j = 0; j < kDimTiles; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    typedef __attribute__((address_space(3))) short4_t lds_s4;
-                    const _Float16* q0 = vb + 16 * h * F::kLdv + 32 * j;
-                    const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(q0));
-                    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(q0 + 8 * F::kLdv));
-                    const half8 a = __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, phi[h], o[j], 0, 0, 0);
-                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, plo[h], o[j], 0, 0, 0);
-                }
-        }
-        if (more) {
-            store(Kl, F::kLdk, kr);
-            store_scale(true);
-            store_scale(false);
-        }
-        __syncthreads();  // the next K is staged; every wave has read V
+    // dims d .. d + 7 of column c
+    static __device__ __forceinline__ half8 part(const void* lds, int low, int c, int d) {
+        return *reinterpret_cast<const half8*>(static_cast<const _Float16*>(lds) + (low * F::kCols + c) * kLd + d);
     }
-    // merge the key waves of each column tile that had a key: outputs, then (reference, sum)
-    const int key_waves = min(KS, (last - begin * F::kKeys) / kTTile + 1);
-    float* Ol = reinterpret_cast<float*>(flash_lds);  // [waves][32][kLdo]
-    float* Ml = Ol + CT * KS * kTTile * F::kLdo;      // [waves][32][2]
-    l = xor_pair_sum<32>(l);
-    const float back = I8 ? R : 1.0f;
-    if (ks < key_waves) {
-        float* oc = Ol + (wid * kTTile + cl) * F::kLdo + 4 * g;
-#pragma unroll
-        for (int j = 0; j < kDimTiles; ++j)
-#pragma unroll
-            for (int a = 0; a < 4; ++a)
-                *reinterpret_cast<float4*>(oc + 32 * j + 8 * a) =
-                    make_float4(o[j][4 * a] * back, o[j][4 * a + 1] * back, o[j][4 * a + 2] * back, o[j][4 * a + 3] * back);
-        if (g == 0) *reinterpret_cast<float2*>(Ml + (wid * kTTile + cl) * 2) = make_float2(m, l);
+    static __device__ __forceinline__ float scale(const void* lds, int c) {
+        return reinterpret_cast<const float*>(static_cast<const _Float16*>(lds) + 2 * F::kCols * kLd)[c];
     }
-    __syncthreads();
-    const bool whole = grid.splits == 1;  // this block has all the keys of its rows
+};
+
+template <int HD, bool I8, int CT, int KS>
+struct WideTile : TreeBlock<HD, CT, KS, kTTile * CT> {
+    using B = TreeBlock<HD, CT, KS, kTTile * CT>;
+    static constexpr int kLdk = HD + 8;             // halves per K row: 16-byte rows shifted by 4 banks
+    static constexpr int kPieceDims = I8 ? 16 : 8;  // values of a 16-byte piece
+    static constexpr int kRowPieces = HD / kPieceDims;
+    static constexpr int kPieces = B::kKeys * kRowPieces / B::kThreads;  // pieces of K (or V) per thread and chunk
+    static constexpr int kKeyStep = B::kThreads / kRowPieces;
+    static constexpr int kScales = I8 ? 3 * B::kKeys : 0;
+    static constexpr size_t kKvBytes = 2 * (static_cast<size_t>(B::kKeys) * (kLdk + B::kLdv) * 2 + kScales * 4);
+    static constexpr size_t kLds = kKvBytes > B::kOutBytes ? kKvBytes : B::kOutBytes;
+    static_assert(kPieces * B::kThreads == B::kKeys * kRowPieces && kPieces > 0, "K / V staging");
+    static_assert(!I8 || 2 * B::kKeys <= B::kThreads, "one scale per thread");
+    static_assert(kLds + 64 <= 160 * 1024, "LDS");
+    static_assert(QueryStage<B, HD>::kBytes <= kLds, "q fits");
+};
+
+template <int HD, bool I8, int KS, int COLS>
+struct NarrowTile : TreeBlock<HD, 1, KS, COLS> {
+    using B = TreeBlock<HD, 1, KS, COLS>;
+    static constexpr int kPieces = HD / (I8 ? 32 : 16);     // 16-byte pieces of K (or V) per lane and tile
+    static constexpr int kRowPieces = HD / (I8 ? 16 : 8);   // ... of a row
+    static constexpr int kScales = I8 ? 3 * kTTile : 0;     // floats per wave
+    static constexpr size_t kWaveBytes = static_cast<size_t>(kTTile) * B::kLdv * 2 + kScales * 4;
+    static constexpr size_t kKvBytes = KS * kWaveBytes + QueryStage<B, HD>::kBytes;
+    static constexpr size_t kLds = kKvBytes > B::kOutBytes ? kKvBytes : B::kOutBytes;
+    static_assert(kWave % kRowPieces == 0 && kWaveBytes % 16 == 0, "V staging");
+    static_assert(kLds + 64 <= 160 * 1024, "LDS");
+};
+
+constexpr float kRaise = 6.0f;  // weights are held times 2^kRaise
+constexpr float kSlack = 6.0f;  // the max may outgrow the reference by 2^kSlack before it is moved
+
+// The key waves of a block's columns joined, then written: the partial output of one split of several, or the output.
+template <typename F, bool I8, int CT, int KS, bool HALF, int N>
+__device__ __forceinline__ void finish_columns(const TreeAttnLaunch& p, const TreeGrid& grid, bool whole, int sp, int kh, int t0,
+                                               int ntok, int T, uint32_t inv_t, bool live, const floatx16 (&o)[N], float m, float l,
+                                               void* lds, int* redo) {
+    constexpr int HD = 32 * N;
+    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, cl = lane & 31, g = lane >> 5;
+    const int group = p.nq / p.kv.nkv;
+    float* Ol = static_cast<float*>(lds);          // [waves][columns][kLdo]: column c of key wave s is s kCols + c
+    float* Ml = Ol + KS * F::kCols * F::kLdo;      // [waves][columns][2]
     const __amdgpu_buffer_rsrc_t rg = buf_rsrc(p.gate ? p.gate + static_cast<size_t>(t0) * p.q_stride : p.q,
                                                p.gate ? static_cast<uint32_t>(ntok) * p.q_stride * 4u : 0u);
+    u32x4 gt[F::kPasses];
+    if (whole)
+#pragma unroll
+        for (int u = 0; u < F::kPasses; ++u) {
+            const int c = threadIdx.x / F::kQuads + u * F::kMergeCols, hc = static_cast<int>(c * inv_t >> 16), tc = c - hc * T;
+            const uint32_t at = tc * p.q_stride + (kh * group + hc) * HD + 4 * (threadIdx.x % F::kQuads);
+            gt[u] = __builtin_amdgcn_raw_buffer_load_b128(rg, hc < group && tc < ntok ? at * 4u : kBufOOB, 0, 0);
+        }
+    l = xor_pair_sum<32>(l);
+    if constexpr (HALF) l = xor_pair_sum<16>(l);
+    const int cw = HALF ? cl & 15 : cl, part = HALF ? cl >> 4 : 0;
+    if (live) {
+        const int at = wid * (F::kCols / CT) + cw;
+        float* oc = Ol + at * F::kLdo + 4 * g + 16 * part;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int a = 0; a < (HALF ? 2 : 4); ++a) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = HALF ? rows_sum(o[j][4 * a + e], o[j][(8 + 4 * a + e) % 16]) : o[j][4 * a + e];
+                *reinterpret_cast<float4*>(oc + 32 * j + 8 * a) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        if (g == 0 && part == 0) *reinterpret_cast<float2*>(Ml + at * 2) = make_float2(m, l);
+    }
+    __syncthreads();
     float* po = p.ws + static_cast<size_t>(sp) * p.tokens * p.nq * HD;
     float2* pm = reinterpret_cast<float2*>(p.ws + static_cast<size_t>(grid.splits) * p.tokens * p.nq * HD) +
                  static_cast<size_t>(sp) * p.tokens * p.nq;
     bool bad = false;
 #pragma unroll
     for (int u = 0; u < F::kPasses; ++u) {
-        const int c = threadIdx.x / F::kQuads + u * F::kMergeCols;
+        const int c = threadIdx.x / F::kQuads + u * F::kMergeCols, d = 4 * (threadIdx.x % F::kQuads);
         const int hc = static_cast<int>(c * inv_t >> 16), tc = c - hc * T;
         if (hc >= group || tc >= ntok) continue;
-        const int at = tc * p.out_stride + (kh * group + hc) * HD + 4 * (threadIdx.x % F::kQuads);
-        const int gat = tc * p.q_stride + (kh * group + hc) * HD + 4 * (threadIdx.x % F::kQuads);
-        const int w0 = (c / kTTile) * kTTile + (c % kTTile);  // column c of wave (ct, ks): w0 + ks CT 32
+        const int at = tc * p.out_stride + (kh * group + hc) * HD + d;
         float ml[KS], ll[KS], M = -INFINITY;
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-            if (s < key_waves) {
-                const float2 v = *reinterpret_cast<const float2*>(Ml + (w0 + s * F::kCols) * 2);
-                ml[s] = v.x;
-                ll[s] = v.y;
-                M = fmaxf(M, v.x);
-            }
+        for (int s = 0; s < KS; ++s) {
+            const float2 v = *reinterpret_cast<const float2*>(Ml + (c + s * F::kCols) * 2);
+            ml[s] = v.x;
+            ll[s] = v.y;
+            M = fmaxf(M, v.x);
+        }
         float L = 0.0f;
         float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-            if (s < key_waves) {
-                const float f = exp2f(ml[s] - M);
-                const float4 v = *reinterpret_cast<const float4*>(Ol + (w0 + s * F::kCols) * F::kLdo + 4 * (threadIdx.x % F::kQuads));
-                L += f * ll[s];
-                r.x += f * v.x;
-                r.y += f * v.y;
-                r.z += f * v.z;
-                r.w += f * v.w;
-            }
+        for (int s = 0; s < KS; ++s) {
+            const float f = __builtin_amdgcn_exp2f(ml[s] - M);
+            const float4 v = *reinterpret_cast<const float4*>(Ol + (c + s * F::kCols) * F::kLdo + d);
+            L += f * ll[s];
+            r.x += f * v.x;
+            r.y += f * v.y;
+            r.z += f * v.z;
+            r.w += f * v.w;
+        }
         if (!whole) {
             const size_t row = static_cast<size_t>(t0 + tc) * p.nq + kh * group + hc;
-            *reinterpret_cast<float4*>(po + row * HD + 4 * (threadIdx.x % F::kQuads)) = r;
-            if (threadIdx.x % F::kQuads == 0) pm[row] = make_float2(M, L);
+            *reinterpret_cast<float4*>(po + row * HD + d) = r;
+            if (d == 0) pm[row] = make_float2(M, L);
             continue;
         }
-        const u32x4 gt = __builtin_amdgcn_raw_buffer_load_b128(rg, static_cast<uint32_t>(gat) * 4u, 0, 0);
         const float inv = L > 0.0f ? 1.0f / L : 0.0f;
         bad |= !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
         float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
         if (p.gate) {
-            y.x *= sigmoid_dev(__uint_as_float(gt[0]));
-            y.y *= sigmoid_dev(__uint_as_float(gt[1]));
-            y.z *= sigmoid_dev(__uint_as_float(gt[2]));
-            y.w *= sigmoid_dev(__uint_as_float(gt[3]));
+            y.x *= sigmoid_dev(__uint_as_float(gt[u][0]));
+            y.y *= sigmoid_dev(__uint_as_float(gt[u][1]));
+            y.z *= sigmoid_dev(__uint_as_float(gt[u][2]));
+            y.w *= sigmoid_dev(__uint_as_float(gt[u][3]));
         }
         *reinterpret_cast<float4*>(p.out + static_cast<size_t>(t0) * p.out_stride + at) = y;
     }
     if (!whole) return;
-    if (bad) redo = 1;
+    if (bad) *redo = 1;
     __syncthreads();
-    if (__builtin_expect(!redo, 1)) return;  // block-uniform
+    if (__builtin_expect(!*redo, 1)) return;  // block-uniform
     for (int t = t0; t < t0 + ntok; ++t) {
         __syncthreads();
-        attend_row<F::kThreads, I8>(p, t, kh, reinterpret_cast<float*>(flash_lds));
+        attend_row<F::kThreads, I8>(p, t, kh, static_cast<float*>(lds));
     }
 }
 
-// max over aligned groups of 32 lanes
-__device__ __forceinline__ float half_max(float v) {
-    v = lanes_max<16>(v);
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+// Up to 32 columns (a decode step's few rows): one column tile, and no barrier before the waves join.  Each wave takes
+// its own 32-key tiles: K straight into registers as the A operand (16-byte pieces; the order of the dims within a
+// step is free as long as q's is the same), V through the wave's own LDS, the next tile's K and V on their way meanwhile.
+template <int HD, bool I8, int KS, bool HALF>
+__global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kernel(TreeAttnLaunch p, TreeGrid grid) {
+    using F = NarrowTile<HD, I8, KS, HALF ? 16 : 32>;
+    using Q = QueryStage<typename F::B, HD>;
+    constexpr int kSteps = HD / 16, kDimTiles = HD / 32, kSlots = HALF ? 8 : 16;
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    extern __shared__ uint4 flash_lds[];
+    __shared__ int redo;
+    const int nkv = p.kv.nkv, kh = blockIdx.x % nkv, sp = static_cast<int>(blockIdx.x) / nkv;
+    const int group = p.nq / nkv, T = F::kCols / group, ntok = p.tokens;
+    const int lane = threadIdx.x & (kWave - 1), ks = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int cl = lane & 31, g = lane >> 5;
+    const uint32_t inv_t = (65535u + T) / T;
+    const int col = HALF ? cl & 15 : cl, part = HALF ? cl >> 4 : 0;
+    const int ch = static_cast<int>(col * inv_t >> 16), ctok = col - ch * T;
+    const bool live = ch < group && ctok < ntok;
+    if (threadIdx.x == 0) redo = 0;
+    Q query;
+    query.load(p, kh, 0, ntok, group, T, inv_t);
+    const int pos0 = __builtin_amdgcn_readfirstlane(clamp_pos0(p));
+    const int last = min(pos0 + ntok, p.kv.capacity) - 1;
+    const int sure = min(p.has_tree ? pos0 - 1 : pos0, last);  // every column sees the keys up to here
+    const int qpos = live ? pos0 + ctok : -1;
+    const uint64_t mask = live && p.has_tree ? p.masks.m[ctok] : 0;
+    int begin, end;
+    const int splits = split_range(last / F::kKeys + 1, grid.splits, sp, begin, end);
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+    if (begin >= end) return;  // fewer chunks than splits
+
+    const uint32_t es = I8 ? 1u : 2u, krow = static_cast<uint32_t>(nkv) * HD * es;  // bytes per cache position
+    u32x4 kr[F::kPieces], vr[F::kPieces];
+    const float *k_scale = p.kv.k_scale, *v_scale = p.kv.v_scale;
+    asm("" : "+s"(k_scale), "+s"(v_scale));  // (else each lane fetches its pointer from the arguments, chunk by chunk)
+    const uint32_t kat = cl * krow + 16u * g, vat = lane / F::kRowPieces * krow + lane % F::kRowPieces * 16u;
+    auto rows_of = [&](const void* cache, int c) {  // of the wave's tile of chunk c; keys past `last` (or `end`) read 0
+        const int key0 = c * F::kKeys + ks * kTTile;
+        const int n = __builtin_amdgcn_readfirstlane(c < end ? max(0, min(kTTile, last - key0 + 1)) : 0);
+        const uint8_t* base = static_cast<const uint8_t*>(cache) +
+                              static_cast<size_t>(__builtin_amdgcn_readfirstlane(min(key0, last))) * krow +
+                              static_cast<uint32_t>(kh) * HD * es;
+        return buf_rsrc(base, static_cast<uint32_t>(n) * krow);
+    };
+    const float* scales = I8 && g ? v_scale : k_scale;  // lanes 0 - 31 hold K's of key cl, 32 - 63 V's
+    float sr = 0.0f;
+    auto load_k = [&](int c) {
+        const __amdgpu_buffer_rsrc_t rs = rows_of(p.kv.k, c);
+#pragma unroll
+        for (int u = 0; u < F::kPieces; ++u) kr[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, kat + 32u * u, 0, 0);
+        if constexpr (I8) {
+            const int key = c * F::kKeys + ks * kTTile + cl;
+            sr = c < end && key <= last ? scales[static_cast<size_t>(key) * nkv + kh] : 0.0f;
+        }
+    };
+    auto load_v = [&](int c) {
+        const __amdgpu_buffer_rsrc_t rs = rows_of(p.kv.v, c);
+#pragma unroll
+        for (int u = 0; u < F::kPieces; ++u)
+            vr[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, vat + static_cast<uint32_t>(u * (kWave / F::kRowPieces)) * krow, 0, 0);
+    };
+    load_k(begin);
+    load_v(begin);
+    uint8_t* Ql = reinterpret_cast<uint8_t*>(flash_lds) + KS * F::kWaveBytes;
+    query.store(Ql);
+    __syncthreads();
+    half8 qhi[HALF ? 1 : kSteps], qlo[kSteps];  // (HALF: qlo is the lane's own part, hi or lo)
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int d = I8 ? 32 * (s / 2) + 16 * g + 8 * (s % 2) : 16 * s + 8 * g;
+        if constexpr (!HALF) qhi[s] = Q::part(Ql, 0, col, d);
+        qlo[s] = Q::part(Ql, HALF ? part : 1, col, d);
+    }
+    const float sscale = Q::scale(Ql, col);
+    _Float16* Vl = reinterpret_cast<_Float16*>(reinterpret_cast<uint8_t*>(flash_lds) + ks * F::kWaveBytes);  // [32][kLdv]
+    float* Sl = reinterpret_cast<float*>(Vl + kTTile * F::kLdv);  // [3][32]: scales of K, of V, exponents of V's
+    float m = -1.0e30f, l = 0.0f;  // reference of the exponents, this lane's part of the sum
+    floatx16 o[kDimTiles];
+#pragma unroll
+    for (int j = 0; j < kDimTiles; ++j) o[j] = floatx16{};
+    for (int c = begin; c < end; ++c) {
+        const int key0 = c * F::kKeys + ks * kTTile;
+        floatx16 st = floatx16{};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            half8 a;
+            if constexpr (I8) {
+                const u32x2 w0 = codes_to_half(kr[s / 2][2 * (s % 2)]), w1 = codes_to_half(kr[s / 2][2 * (s % 2) + 1]);
+                a = __builtin_bit_cast(half8, u32x4{w0.x, w0.y, w1.x, w1.y});
+            } else {
+                a = __builtin_bit_cast(half8, kr[s]);
+            }
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qlo[s], st, 0, 0, 0);
+            if constexpr (!HALF) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qhi[s], st, 0, 0, 0);
+        }
+        if constexpr (I8) {
+            Sl[lane] = sr;
+            if (g) Sl[kTTile + lane] = scale_exponent(sr);
+        }
+        load_k(c + 1);
+#pragma unroll
+        for (int u = 0; u < F::kPieces; ++u) {
+            _Float16* at = Vl + (lane / F::kRowPieces + u * (kWave / F::kRowPieces)) * F::kLdv + lane % F::kRowPieces * (I8 ? 16 : 8);
+            if constexpr (I8) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x2 a = codes_to_half(vr[u][2 * h]), b = codes_to_half(vr[u][2 * h + 1]);
+                    *reinterpret_cast<u32x4*>(at + 8 * h) = u32x4{a.x, a.y, b.x, b.y};
+                }
+            } else {
+                *reinterpret_cast<u32x4*>(at) = vr[u];
+            }
+        }
+        load_v(c + 1);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // LDS takes a wave's accesses in their order
+        __builtin_amdgcn_wave_barrier();
+        float sc[kSlots], vs[kSlots], lv[kSlots], mc = -INFINITY;  // of keys 16 part + 8 (v / 4) + 4 g + v % 4
+#pragma unroll
+        for (int v = 0; v < kSlots; ++v) sc[v] = HALF ? rows_sum(st[v], st[(v + 8) % 16]) : st[v];
+        if constexpr (I8) {
+#pragma unroll
+            for (int a = 0; a < kSlots / 4; ++a) {
+                const float* at = Sl + 16 * part + 8 * a + 4 * g;
+                const f32x4 k4 = *reinterpret_cast<const f32x4*>(at);
+                const f32x4 v4 = *reinterpret_cast<const f32x4*>(at + kTTile);
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(at + 2 * kTTile);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[4 * a + e] *= k4[e];
+                    vs[4 * a + e] = v4[e];
+                    lv[4 * a + e] = l4[e];
+                }
+            }
+        }
+        if (key0 + kTTile - 1 > sure) {  // wave-uniform: keys that some column does not see
+            uint32_t see;
+            const int from = key0 + 16 * part + 4 * g;
+            if (p.has_tree) {
+                see = mask_window(mask, from - pos0);
+            } else {
+                const int b = qpos - from;
+                see = b < 0 ? 0u : (b >= 31 ? ~0u : (2u << b) - 1u);
+            }
+            const int left = last - from;  // (rows and positions past the capacity)
+            see &= left < 0 ? 0u : (left >= 31 ? ~0u : (2u << left) - 1u);
+#pragma unroll
+            for (int v = 0; v < kSlots; ++v)
+                if (!(see >> (8 * (v >> 2) + (v & 3)) & 1u)) {
+                    sc[v] = -INFINITY;
+                    if constexpr (I8) vs[v] = 0.0f;  // (its scale may be NaN)
+                }
+        }
+#pragma unroll
+        for (int v = 0; v < kSlots; ++v) mc = fmaxf(mc, I8 ? fmaf(sc[v], sscale, lv[v]) : sc[v]);
+        if constexpr (HALF) mc = xor16_max(mc);
+        mc = pair32_max(mc) * (I8 ? 1.0f : sscale);
+        // the reference moves only when a column's max has outgrown it (rarely after the first tiles)
+        const bool up = mc > m + kSlack;
+        if (__builtin_amdgcn_ballot_w64(up)) {
+            const float to = up ? mc : m, f = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < kDimTiles; ++j) o[j] *= f;
+        }
+        const float off = kRaise - m;
+        half8 phi[2], plo[2];  // (HALF: plo is the lane's own part)
+#pragma unroll
+        for (int h = 0; h < kSlots / 8; ++h) {
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e] = __builtin_amdgcn_exp2f(fmaf(sc[8 * h + e], sscale, off));
+                l += w[e];
+                if constexpr (I8) {
+                    w[e] *= vs[8 * h + e];
+                    // the rounded product: hi and lo would else be taken from two roundings of it
+                    asm("" : "+v"(w[e]));
+                }
+            }
+            split8(w, phi[h], plo[h]);
+        }
+        if constexpr (HALF) {  // lanes of the hi columns give their lo for the other 8 keys' hi
+            const u32x4 hi = __builtin_bit_cast(u32x4, phi[0]), lo = __builtin_bit_cast(u32x4, plo[0]);
+            u32x4 w[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const auto r = __builtin_amdgcn_permlane16_swap(hi[i], lo[i], false, false);
+                w[0][i] = r[0];
+                w[1][i] = r[1];
+            }
+            plo[0] = __builtin_bit_cast(half8, w[0]);
+            plo[1] = __builtin_bit_cast(half8, w[1]);
+        }
+        // transposed reads: 16 lanes cover four keys x 16 dims, lane i gets dim i of the four
+        const _Float16* vb = Vl + (4 * g + ((lane & 15) >> 2)) * F::kLdv + (lane & 16) + 4 * (lane & 3);
+#pragma unroll
+        for (int j = 0; j < kDimTiles; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                typedef __attribute__((address_space(3))) short4_t lds_s4;
+                const _Float16* q0 = vb + 16 * h * F::kLdv + 32 * j;
+                const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(q0));
+                const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(q0 + 8 * F::kLdv));
+                const half8 a = __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, plo[h], o[j], 0, 0, 0);
+                if constexpr (!HALF) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, phi[h], o[j], 0, 0, 0);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();  // every wave is done with its V
+    finish_columns<F, I8, 1, KS, HALF>(p, grid, splits == 1, sp, kh, 0, ntok, T, inv_t, live, o, m, l, flash_lds, &redo);
 }
 
 template <int HD, bool I8, int CT, int KS>
 __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wide_kernel(TreeAttnLaunch p, TreeGrid grid) {
-    using F = TreeTile<HD, I8, CT, KS, 2>;
+    using F = WideTile<HD, I8, CT, KS>;
+    using Q = QueryStage<typename F::B, HD>;
     constexpr int kSteps = HD / 16, kDimTiles = HD / 32;
-    constexpr float kLog2e = 1.44269504088896340736f;
-    constexpr float kRaise = 6.0f;  // weights are held times 2^kRaise
-    constexpr float kSlack = 6.0f;  // the max may outgrow the reference by 2^kSlack before it is moved
     extern __shared__ uint4 flash_lds[];
     __shared__ int redo;
-    constexpr int kKBuf = F::kKeys * F::kLdk, kVBuf = F::kKeys * F::kLdv, kSBuf = 2 * F::kKeys + KS;
+    constexpr int kKBuf = F::kKeys * F::kLdk, kVBuf = F::kKeys * F::kLdv, kSBuf = F::kScales;
     _Float16* Kl = reinterpret_cast<_Float16*>(flash_lds);       // [2][kKeys][kLdk]
     _Float16* Vl = Kl + 2 * kKBuf;                               // [2][kKeys][kLdv]
-    float* Sl = reinterpret_cast<float*>(Vl + 2 * kVBuf);        // [2]: scales of K, of V, exponent of V's per key tile
+    float* Sl = reinterpret_cast<float*>(Vl + 2 * kVBuf);        // [2][3][kKeys]: scales of K, of V, exponents of V's
     const int nkv = p.kv.nkv, kh = blockIdx.x % nkv;
     const int rest = static_cast<int>(blockIdx.x) / nkv, tile = grid.tiles - 1 - rest % grid.tiles, sp = rest / grid.tiles;
     const int group = p.nq / nkv, T = F::kCols / group;
     const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int ct = wid % CT, ks = wid / CT;
     const int cl = lane & 31, g = lane >> 5;
-    const int pos0 = __builtin_amdgcn_readfirstlane(clamp_pos0(p));
     const uint32_t inv_t = (65535u + T) / T;  // c / T = c inv_t >> 16 for c < 128, T <= 128
     const int t0 = tile * T, ntok = min(T, p.tokens - t0);
+    Q query;
+    query.load(p, kh, t0, ntok, group, T, inv_t);
+    const int pos0 = __builtin_amdgcn_readfirstlane(clamp_pos0(p));
     const int col = ct * kTTile + cl, ch = static_cast<int>(col * inv_t >> 16), ctok = col - ch * T;
     const bool live = ch < group && ctok < ntok;
     const int last = min(pos0 + (p.has_tree ? p.tokens : t0 + ntok), p.kv.capacity) - 1;  // any column's last key
@@ -624,7 +678,7 @@ __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wi
     const int qpos = live ? pos0 + t0 + ctok : -1;
     const uint64_t mask = live && p.has_tree ? p.masks.m[t0 + ctok] : 0;
     int begin, end;
-    split_range(last / F::kKeys + 1, grid.splits, sp, begin, end);
+    const int splits = split_range(last / F::kKeys + 1, grid.splits, sp, begin, end);
     begin = __builtin_amdgcn_readfirstlane(begin);
     end = __builtin_amdgcn_readfirstlane(end);
     if (begin >= end) return;
@@ -659,14 +713,15 @@ __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wi
             }
         }
     };
-    // scales: thread i < kKeys holds K's of key i, the next kKeys threads V's, of which each 32-key tile's exponent
-    // goes along (0 for a tile of zeros)
+    // scales: thread i < kKeys holds K's of key i, the next kKeys threads V's
+    const float *k_scale = p.kv.k_scale, *v_scale = p.kv.v_scale;
+    asm("" : "+s"(k_scale), "+s"(v_scale));  // (else each lane fetches its pointer from the arguments, chunk by chunk)
+    const float* scales = threadIdx.x < F::kKeys ? k_scale : v_scale;
     float sr = 0.0f;
     auto load_scale = [&](int c) {
         if constexpr (I8) {
             const int key = c * F::kKeys + static_cast<int>(threadIdx.x) % F::kKeys;
-            const float* from = threadIdx.x < F::kKeys ? p.kv.k_scale : p.kv.v_scale;
-            sr = threadIdx.x < 2 * F::kKeys && key <= last ? from[static_cast<size_t>(key) * nkv + kh] : 0.0f;
+            sr = threadIdx.x < 2 * F::kKeys && key <= last ? scales[static_cast<size_t>(key) * nkv + kh] : 0.0f;
         }
     };
     auto store_scale = [&](int buf) {
@@ -674,69 +729,23 @@ __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wi
             if (threadIdx.x >= 2 * F::kKeys) return;  // wave-uniform
             float* at = Sl + buf * kSBuf;
             at[threadIdx.x] = sr;
-            if (threadIdx.x < F::kKeys) return;
-            const float top = half_max(sr);
-            int ex = 0;
-            if (top > 0.0f) frexpf(top, &ex);
-            if (lane % kTTile == 0) at[2 * F::kKeys + (threadIdx.x - F::kKeys) / kTTile] = fminf(fmaxf(ex, -100.0f), 100.0f);
+            if (threadIdx.x >= F::kKeys) at[F::kKeys + threadIdx.x] = scale_exponent(sr);
         }
-    };
-    auto place = [&](int tid, int u, int stride) {  // float offset of the pass's column from row t0, or -1
-        const int c = tid / F::kQuads + u * F::kMergeCols;
-        const int hc = static_cast<int>(c * inv_t >> 16), tc = c - hc * T;
-        return hc < group && tc < ntok ? tc * stride + (kh * group + hc) * HD + 4 * (tid % F::kQuads) : -1;
     };
     load(p.kv.k, begin, kr);
     load_scale(begin);
     load(p.kv.v, begin, vr);
     half8 qhi[kSteps], qlo[kSteps];  // lane supplies dims 16 s + 8 g .. + 7 of its column
-    float sscale;                    // score scale in the exponent of 2
-    {
-        float* Ql = reinterpret_cast<float*>(flash_lds);  // [kCols][kLdo]
-        const __amdgpu_buffer_rsrc_t rq =
-            buf_rsrc(p.q + static_cast<size_t>(t0) * p.q_stride, static_cast<uint32_t>(ntok) * p.q_stride * 4u);
-        u32x4 qr[F::kPasses];
+    query.store(flash_lds);
+    if (threadIdx.x == 0) redo = 0;
+    __syncthreads();
 #pragma unroll
-        for (int u = 0; u < F::kPasses; ++u) {  // columns without a row read 0
-            const int at = place(threadIdx.x, u, p.q_stride);
-            qr[u] = __builtin_amdgcn_raw_buffer_load_b128(rq, at >= 0 ? static_cast<uint32_t>(at) * 4u : kBufOOB, 0, 0);
-        }
-#pragma unroll
-        for (int u = 0; u < F::kPasses; ++u)
-            *reinterpret_cast<u32x4*>(Ql + (threadIdx.x / F::kQuads + u * F::kMergeCols) * F::kLdo +
-                                      4 * (threadIdx.x % F::kQuads)) = qr[u];
-        if (threadIdx.x == 0) redo = 0;
-        __syncthreads();
-        float x[kSteps][8], mx = 0.0f;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(Ql + col * F::kLdo + 16 * s + 8 * g + e);
-                x[s][e] = v.x;
-                x[s][e + 1] = v.y;
-                x[s][e + 2] = v.z;
-                x[s][e + 3] = v.w;
-            }
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[s][e]));
-        mx = pair32_max(mx);
-        // a power of two brings the column's largest magnitude into [2^12, 2^13); an infinity or 0 stays
-        int ex = 13;
-        if (mx > 0.0f && mx < INFINITY) frexpf(mx, &ex);
-        ex = max(ex, -100);  // 2^(13 - ex) stays finite
-        const float down = ldexpf(1.0f, 13 - ex);
-        sscale = ldexpf(kLog2e / sqrtf(static_cast<float>(HD)), ex - 13);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[s][e] *= down;
-            split8(x[s], qhi[s], qlo[s]);
-        }
-        __syncthreads();  // every wave has its q: K and V may take its place
+    for (int s = 0; s < kSteps; ++s) {
+        qhi[s] = Q::part(flash_lds, 0, col, 16 * s + 8 * g);
+        qlo[s] = Q::part(flash_lds, 1, col, 16 * s + 8 * g);
     }
+    const float sscale = Q::scale(flash_lds, col);
+    __syncthreads();  // every wave has its q: K and V may take its place
     store(Kl + (begin & 1) * kKBuf, F::kLdk, kr);
     store_scale(begin & 1);
     __syncthreads();
@@ -784,19 +793,20 @@ __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wi
         load(p.kv.k, c + 2, kr);
         load_scale(c + 2);
         if constexpr (!FIRST) add_values(c - 1);
-        float sc[16], vs[16], mc = -INFINITY, ev = 0.0f;
+        float sc[16], vs[16], lv[16], mc = -INFINITY;
         if constexpr (I8) {
             typedef float f32x4 __attribute__((ext_vector_type(4)));
             const float* at = Sl + (c & 1) * kSBuf;
-            ev = at[2 * F::kKeys + ks];
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 const f32x4 k4 = *reinterpret_cast<const f32x4*>(at + ks * kTTile + 8 * a + 4 * g);
                 const f32x4 v4 = *reinterpret_cast<const f32x4*>(at + F::kKeys + ks * kTTile + 8 * a + 4 * g);
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(at + 2 * F::kKeys + ks * kTTile + 8 * a + 4 * g);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     sc[4 * a + e] = st[4 * a + e] * k4[e];
                     vs[4 * a + e] = v4[e];
+                    lv[4 * a + e] = l4[e];
                 }
             }
         } else {
@@ -821,8 +831,8 @@ __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wi
                 }
         }
 #pragma unroll
-        for (int v = 0; v < 16; ++v) mc = fmaxf(mc, sc[v]);
-        mc = pair32_max(mc) * sscale + ev;
+        for (int v = 0; v < 16; ++v) mc = fmaxf(mc, I8 ? fmaf(sc[v], sscale, lv[v]) : sc[v]);
+        mc = pair32_max(mc) * (I8 ? 1.0f : sscale);
         // the reference moves only when a column's max has outgrown it (rarely after the first chunks)
         const bool up = mc > m + kSlack;
         const float to = up ? mc : m, f = __builtin_amdgcn_exp2f(m - to);
@@ -860,131 +870,155 @@ __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wi
     for (; c < end; ++c) chunk(c, std::false_type{}, std::true_type{});
     add_values(end - 1);
     __syncthreads();
-    // merge the key waves of each column tile: outputs, then (reference, sum)
-    float* Ol = reinterpret_cast<float*>(flash_lds);  // [waves][32][kLdo]
-    float* Ml = Ol + CT * KS * kTTile * F::kLdo;      // [waves][32][2]
-    l = xor_pair_sum<32>(l);
-    {
-        float* oc = Ol + (wid * kTTile + cl) * F::kLdo + 4 * g;
-#pragma unroll
-        for (int j = 0; j < kDimTiles; ++j)
-#pragma unroll
-            for (int a = 0; a < 4; ++a)
-                *reinterpret_cast<float4*>(oc + 32 * j + 8 * a) =
-                    make_float4(o[j][4 * a], o[j][4 * a + 1], o[j][4 * a + 2], o[j][4 * a + 3]);
-        if (g == 0) *reinterpret_cast<float2*>(Ml + (wid * kTTile + cl) * 2) = make_float2(m, l);
-    }
-    __syncthreads();
-    const bool whole = grid.splits == 1;  // this block has all the keys of its rows
-    const __amdgpu_buffer_rsrc_t rg = buf_rsrc(p.gate ? p.gate + static_cast<size_t>(t0) * p.q_stride : p.q,
-                                               p.gate ? static_cast<uint32_t>(ntok) * p.q_stride * 4u : 0u);
-    float* po = p.ws + static_cast<size_t>(sp) * p.tokens * p.nq * HD;
-    float2* pm = reinterpret_cast<float2*>(p.ws + static_cast<size_t>(grid.splits) * p.tokens * p.nq * HD) +
-                 static_cast<size_t>(sp) * p.tokens * p.nq;
-    bool bad = false;
-#pragma unroll
-    for (int u = 0; u < F::kPasses; ++u) {
-        const int cc = threadIdx.x / F::kQuads + u * F::kMergeCols;
-        const int hc = static_cast<int>(cc * inv_t >> 16), tc = cc - hc * T;
-        if (hc >= group || tc >= ntok) continue;
-        const int at = tc * p.out_stride + (kh * group + hc) * HD + 4 * (threadIdx.x % F::kQuads);
-        const int gat = tc * p.q_stride + (kh * group + hc) * HD + 4 * (threadIdx.x % F::kQuads);
-        const int w0 = (cc / kTTile) * kTTile + (cc % kTTile);  // column cc of wave (ct, ks): w0 + ks CT 32
-        float ml[KS], ll[KS], M = -INFINITY;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const float2 v = *reinterpret_cast<const float2*>(Ml + (w0 + s * F::kCols) * 2);
-            ml[s] = v.x;
-            ll[s] = v.y;
-            M = fmaxf(M, v.x);
-        }
-        float L = 0.0f;
-        float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const float f = exp2f(ml[s] - M);
-            const float4 v = *reinterpret_cast<const float4*>(Ol + (w0 + s * F::kCols) * F::kLdo + 4 * (threadIdx.x % F::kQuads));
-            L += f * ll[s];
-            r.x += f * v.x;
-            r.y += f * v.y;
-            r.z += f * v.z;
-            r.w += f * v.w;
-        }
-        if (!whole) {
-            const size_t row = static_cast<size_t>(t0 + tc) * p.nq + kh * group + hc;
-            *reinterpret_cast<float4*>(po + row * HD + 4 * (threadIdx.x % F::kQuads)) = r;
-            if (threadIdx.x % F::kQuads == 0) pm[row] = make_float2(M, L);
-            continue;
-        }
-        const u32x4 gt = __builtin_amdgcn_raw_buffer_load_b128(rg, static_cast<uint32_t>(gat) * 4u, 0, 0);
-        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-        bad |= !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
-        float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
-        if (p.gate) {
-            y.x *= sigmoid_dev(__uint_as_float(gt[0]));
-            y.y *= sigmoid_dev(__uint_as_float(gt[1]));
-            y.z *= sigmoid_dev(__uint_as_float(gt[2]));
-            y.w *= sigmoid_dev(__uint_as_float(gt[3]));
-        }
-        *reinterpret_cast<float4*>(p.out + static_cast<size_t>(t0) * p.out_stride + at) = y;
-    }
-    if (!whole) return;
-    if (bad) redo = 1;
-    __syncthreads();
-    if (__builtin_expect(!redo, 1)) return;  // block-uniform
-    for (int t = t0; t < t0 + ntok; ++t) {
-        __syncthreads();
-        attend_row<F::kThreads, I8>(p, t, kh, reinterpret_cast<float*>(flash_lds));
-    }
+    finish_columns<F, I8, CT, KS, false>(p, grid, splits == 1, sp, kh, t0, ntok, T, inv_t, live, o, m, l, flash_lds, &redo);
 }
 
-// The splits' partial outputs of one row and kv head joined, normalised and gated.
-template <int HD, bool I8, int KEYS>
-__global__ void __launch_bounds__(256) tree_attn_merge_kernel(TreeAttnLaunch p, TreeGrid grid, int T) {
-    extern __shared__ float smem[];  // attend_row's
-    __shared__ float2 stat[kTreeMaxSplits * kTreeMaxGroup];
-    __shared__ int redo;
-    const int t = blockIdx.x, kh = blockIdx.y, group = p.nq / p.kv.nkv, t0 = t / T * T;
-    const int pos0 = clamp_pos0(p);
+// What the merge kernels share: the keys' splits of row t, and an output quad from its sums.
+constexpr int kMergeThreads = 512;
+constexpr int kFewSplits = 4;
+template <int KEYS>
+__device__ __forceinline__ int used_splits(const TreeAttnLaunch& p, const TreeGrid& grid, int t, int T) {
+    const int pos0 = clamp_pos0(p), t0 = t / T * T;
     const int last = min(pos0 + (p.has_tree ? p.tokens : min(t0 + T, p.tokens)), p.kv.capacity) - 1;
-    const int splits = last < 0 ? 0 : min(grid.splits, last / KEYS + 1);
-    const size_t rows = static_cast<size_t>(p.tokens) * p.nq, row0 = static_cast<size_t>(t) * p.nq + kh * group;
-    const float2* pm = reinterpret_cast<const float2*>(p.ws + grid.splits * rows * HD);
-    for (int i = threadIdx.x; i < splits * group; i += 256) stat[i] = pm[(i / group) * rows + row0 + i % group];
+    return min(grid.splits, last / KEYS + 1);
+}
+struct TreeParts {
+    __amdgpu_buffer_rsrc_t o, st;
+    uint32_t rows;  // of a split's
+};
+__device__ __forceinline__ TreeParts tree_parts(const TreeAttnLaunch& p, const TreeGrid& grid, int hd) {
+    const uint32_t rows = static_cast<uint32_t>(p.tokens) * p.nq, all = grid.splits * rows;
+    return TreeParts{buf_rsrc(p.ws, all * hd * 4u), buf_rsrc(p.ws + static_cast<size_t>(all) * hd, all * 8u), rows};
+}
+__device__ __forceinline__ float4 as_float4(u32x4 v) {
+    return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+}
+// writes the quad at `out`; whether its row has to be computed again
+__device__ __forceinline__ bool write_quad(float4 r, float L, bool gated, float4 gt, float* out) {
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
+    if (gated) {
+        y.x *= sigmoid_dev(gt.x);
+        y.y *= sigmoid_dev(gt.y);
+        y.z *= sigmoid_dev(gt.z);
+        y.w *= sigmoid_dev(gt.w);
+    }
+    *reinterpret_cast<float4*>(out) = y;
+    return !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
+}
+__device__ __forceinline__ void add_scaled(float4& r, float f, float4 v) {
+    r.x += f * v.x;
+    r.y += f * v.y;
+    r.z += f * v.z;
+    r.w += f * v.w;
+}
+
+// The splits' partial outputs of one row and kv head joined, normalised and gated (nothing to do where one split held
+// every key).  `slices` threads share an output's splits; their first loads go out before the position has come.
+template <int HD, bool I8, int KEYS>
+__global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_kernel(TreeAttnLaunch p, TreeGrid grid, int T) {
+    extern __shared__ float smem[];  // attend_row's
+    __shared__ float factor[kTreeMaxGroup][kTreeMaxSplits], total[kTreeMaxGroup];
+    __shared__ float4 partial[kMergeThreads];
+    __shared__ int redo;
+    constexpr int kBatch = 8;
+    const int t = blockIdx.x, kh = blockIdx.y, group = p.nq / p.kv.nkv;
+    const int items = group * (HD / 4), slices = kMergeThreads / items;  // items <= 8 * 64
+    const int slice = threadIdx.x / items, item = threadIdx.x - slice * items, h = item / (HD / 4), d = 4 * (item % (HD / 4));
+    const TreeParts in = tree_parts(p, grid, HD);
+    const uint32_t row0 = static_cast<uint32_t>(t) * p.nq + kh * group;
+    u32x4 v[kBatch];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int s = s0 + i * slices;
+            v[i] = __builtin_amdgcn_raw_buffer_load_b128(in.o, slice < slices && s < grid.splits ? ((s * in.rows + row0 + h) * HD + d) * 4u : kBufOOB, 0, 0);
+        }
+    };
+    load(slice);  // (a split without keys holds anything)
+    const int wid = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const u32x2 st = __builtin_amdgcn_raw_buffer_load_b64(in.st, wid < group && lane < grid.splits ? (lane * in.rows + row0 + wid) * 8u : kBufOOB, 0, 0);
+    const size_t at = static_cast<size_t>(kh * group + h) * HD + d;
+    const float4 gt = p.gate ? *reinterpret_cast<const float4*>(p.gate + static_cast<size_t>(t) * p.q_stride + at) : float4{};
+    const int splits = used_splits<KEYS>(p, grid, t, T);
+    if (splits == 1) return;
+    if (wid < group) {
+        const float M = wave_max(lane < splits ? __uint_as_float(st.x) : -INFINITY);
+        const float f = lane < splits ? __builtin_amdgcn_exp2f(__uint_as_float(st.x) - M) : 0.0f;
+        const float L = wave_sum(lane < splits ? f * __uint_as_float(st.y) : 0.0f);
+        factor[wid][lane] = f;
+        if (lane == 0) total[wid] = L;
+    }
     if (threadIdx.x == 0) redo = 0;
     __syncthreads();
-    bool bad = false;
-    for (int i = threadIdx.x; i < group * HD / 4; i += 256) {
-        const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
-        float M = -INFINITY, L = 0.0f;
-        for (int s = 0; s < splits; ++s) M = fmaxf(M, stat[s * group + h].x);
-        float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float* po = p.ws + (row0 + h) * HD + d;
-        for (int s = 0; s < splits; ++s) {
-            const float2 st = stat[s * group + h];
-            const float f = exp2f(st.x - M);
-            const float4 v = *reinterpret_cast<const float4*>(po + s * rows * HD);
-            L += f * st.y;
-            r.x += f * v.x;
-            r.y += f * v.y;
-            r.z += f * v.z;
-            r.w += f * v.w;
+    float4 r = float4{};
+    if (slice < slices)
+        for (int s0 = slice;;) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int s = s0 + i * slices;
+                if (s < splits) add_scaled(r, factor[h][s], as_float4(v[i]));
+            }
+            s0 += kBatch * slices;
+            if (s0 >= splits) break;
+            load(s0);
         }
-        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-        bad |= !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
-        float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
-        if (p.gate) {
-            const float4 gt = *reinterpret_cast<const float4*>(p.gate + static_cast<size_t>(t) * p.q_stride + (kh * group + h) * HD + d);
-            y.x *= sigmoid_dev(gt.x);
-            y.y *= sigmoid_dev(gt.y);
-            y.z *= sigmoid_dev(gt.z);
-            y.w *= sigmoid_dev(gt.w);
-        }
-        *reinterpret_cast<float4*>(p.out + static_cast<size_t>(t) * p.out_stride + (kh * group + h) * HD + d) = y;
-    }
-    if (bad) redo = 1;
+    partial[threadIdx.x] = r;
     __syncthreads();
-    if (redo) attend_row<256, I8>(p, t, kh, smem);  // block-uniform
+    if (slice == 0) {
+        for (int i = 1; i < slices; ++i) add_scaled(r, 1.0f, partial[i * items + item]);
+        if (write_quad(r, total[h], p.gate, gt, p.out + static_cast<size_t>(t) * p.out_stride + at)) redo = 1;
+    }
+    __syncthreads();
+    if (redo) attend_row<kMergeThreads, I8>(p, t, kh, smem);  // block-uniform
+}
+
+// ... of up to kFewSplits splits (calls of many rows): each thread has an output's partials by itself, a block several
+// kv heads of a row.
+template <int HD, bool I8, int KEYS>
+__global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_few_kernel(TreeAttnLaunch p, TreeGrid grid, int T) {
+    extern __shared__ float smem[];  // attend_row's
+    __shared__ uint32_t redo;        // a bit per kv head of the block
+    const int t = blockIdx.x, group = p.nq / p.kv.nkv;
+    const int items = group * (HD / 4), heads = kMergeThreads / items, k0 = blockIdx.y * heads;
+    const int kl = threadIdx.x / items, item = threadIdx.x - kl * items, h = item / (HD / 4), d = 4 * (item % (HD / 4));
+    const bool on = kl < heads && k0 + kl < p.kv.nkv;
+    const TreeParts in = tree_parts(p, grid, HD);
+    const uint32_t head = (k0 + kl) * group + h, row = static_cast<uint32_t>(t) * p.nq + head;
+    u32x4 v[kFewSplits];
+    u32x2 st[kFewSplits];
+#pragma unroll
+    for (int s = 0; s < kFewSplits; ++s) {
+        const bool has = on && s < grid.splits;
+        v[s] = __builtin_amdgcn_raw_buffer_load_b128(in.o, has ? ((s * in.rows + row) * HD + d) * 4u : kBufOOB, 0, 0);
+        st[s] = __builtin_amdgcn_raw_buffer_load_b64(in.st, has ? (s * in.rows + row) * 8u : kBufOOB, 0, 0);
+    }
+    const size_t at = static_cast<size_t>(head) * HD + d;
+    const float4 gt = p.gate && on ? *reinterpret_cast<const float4*>(p.gate + static_cast<size_t>(t) * p.q_stride + at) : float4{};
+    const int splits = used_splits<KEYS>(p, grid, t, T);
+    if (splits == 1) return;
+    if (threadIdx.x == 0) redo = 0;
+    __syncthreads();
+    if (on) {
+        float M = -INFINITY, L = 0.0f;
+        float4 r = float4{};
+#pragma unroll
+        for (int s = 0; s < kFewSplits; ++s)
+            if (s < splits) M = fmaxf(M, __uint_as_float(st[s].x));
+#pragma unroll
+        for (int s = 0; s < kFewSplits; ++s)
+            if (s < splits) {
+                const float f = __builtin_amdgcn_exp2f(__uint_as_float(st[s].x) - M);
+                L += f * __uint_as_float(st[s].y);
+                add_scaled(r, f, as_float4(v[s]));
+            }
+        if (write_quad(r, L, p.gate, gt, p.out + static_cast<size_t>(t) * p.out_stride + at)) atomicOr(&redo, 1u << kl);
+    }
+    __syncthreads();
+    for (uint32_t again = redo; again; again &= again - 1) {  // block-uniform
+        attend_row<kMergeThreads, I8>(p, t, k0 + __builtin_ctz(again), smem);
+        __syncthreads();
+    }
 }
 
 bool tree_attn_supported(int nq, int nkv, int head_dim) {
@@ -992,18 +1026,14 @@ bool tree_attn_supported(int nq, int nkv, int head_dim) {
            sizeof(float) * tree_row_lds(nq / nkv, head_dim) <= 64 * 1024;
 }
 
-// The kernel of a call: column tiles of a block and key waves.
-struct TreeShape {
-    int ct, ks, keys;
-};
-static TreeShape tree_shape(int group, int hd, int tokens) {
+// The columns of a call's blocks.
+static int tree_cols(int group, int tokens) {
     const int cols = tokens * group;
-    if (cols <= kTTile) return hd == 128 ? TreeShape{1, 8, 256} : TreeShape{1, 4, 128};
-    return hd == 128 ? TreeShape{2, 4, 128} : TreeShape{2, 2, 64};
+    return cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
 }
 // Row tiles, and key splits that give every CU a block.
-static TreeGrid tree_grid(int nq, int nkv, int hd, int tokens) {
-    const int T = kTTile * tree_shape(nq / nkv, hd, tokens).ct / (nq / nkv);
+static TreeGrid tree_grid(int nq, int nkv, int tokens) {
+    const int T = tree_cols(nq / nkv, tokens) / (nq / nkv);
     const int tiles = (tokens + T - 1) / T;
     const int64_t blocks = static_cast<int64_t>(tiles) * nkv;
     return TreeGrid{tiles, static_cast<int>(std::min<int64_t>(kTreeMaxSplits, std::max<int64_t>(1, 256 / blocks)))};
@@ -1011,37 +1041,47 @@ static TreeGrid tree_grid(int nq, int nkv, int hd, int tokens) {
 
 size_t tree_attn_workspace_bytes(int nq, int nkv, int head_dim, int tokens) {
     if (head_dim != 128 && head_dim != 256) return 16;
-    const TreeGrid g = tree_grid(nq, nkv, head_dim, tokens);
+    const TreeGrid g = tree_grid(nq, nkv, tokens);
     return g.splits == 1 ? 16 : static_cast<size_t>(g.splits) * tokens * nq * (head_dim + 2) * sizeof(float);
 }
 
 template <typename F, int HD, bool I8, typename Kernel>
 static hipError_t launch_tree(const TreeAttnLaunch& p, Kernel kernel, hipStream_t s) {
-    const TreeGrid g = tree_grid(p.nq, p.kv.nkv, HD, p.tokens);
+    const TreeGrid g = tree_grid(p.nq, p.kv.nkv, p.tokens);
     if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                            static_cast<int>(F::kLds));
         e != hipSuccess)
         return e;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(g.tiles * g.splits) * p.kv.nkv), dim3(F::kThreads), F::kLds, s, p, g);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || g.splits == 1) return e;
-    const int group = p.nq / p.kv.nkv;
-    hipLaunchKernelGGL((tree_attn_merge_kernel<HD, I8, F::kKeys>), dim3(p.tokens, p.kv.nkv), dim3(256),
-                       sizeof(float) * tree_row_lds(group, HD), s, p, g, F::kCols / group);
+    const int group = p.nq / p.kv.nkv, T = F::kCols / group;
+    const size_t lds = sizeof(float) * tree_row_lds(group, HD);  // attend_row's
+    if (g.splits <= kFewSplits) {
+        const int heads = kMergeThreads / (group * (HD / 4));
+        hipLaunchKernelGGL((tree_attn_merge_few_kernel<HD, I8, F::kKeys>), dim3(p.tokens, (p.kv.nkv + heads - 1) / heads),
+                           dim3(kMergeThreads), lds, s, p, g, T);
+    } else {
+        hipLaunchKernelGGL((tree_attn_merge_kernel<HD, I8, F::kKeys>), dim3(p.tokens, p.kv.nkv), dim3(kMergeThreads), lds, s, p,
+                           g, T);
+    }
     return hipGetLastError();
 }
-template <int HD, bool I8, int CT, int KS, bool WIDE>
-static hipError_t launch_tree_mfma(const TreeAttnLaunch& p, hipStream_t s) {
-    if constexpr (WIDE)
-        return launch_tree<TreeTile<HD, I8, CT, KS, 2>, HD, I8>(p, &tree_attn_wide_kernel<HD, I8, CT, KS>, s);
-    else
-        return launch_tree<TreeTile<HD, I8, CT, KS>, HD, I8>(p, &tree_attn_mfma_kernel<HD, I8, CT, KS>, s);
+template <int HD, bool I8, int CT, int KS>
+static hipError_t launch_wide(const TreeAttnLaunch& p, hipStream_t s) {
+    return launch_tree<WideTile<HD, I8, CT, KS>, HD, I8>(p, &tree_attn_wide_kernel<HD, I8, CT, KS>, s);
 }
-template <bool I8>
+template <int HD, bool I8, int KS, bool HALF>
+static hipError_t launch_narrow(const TreeAttnLaunch& p, hipStream_t s) {
+    return launch_tree<NarrowTile<HD, I8, KS, HALF ? 16 : 32>, HD, I8>(p, &tree_attn_narrow_kernel<HD, I8, KS, HALF>, s);
+}
+template <int HD, bool I8>
 static hipError_t launch_tree_heads(const TreeAttnLaunch& p, hipStream_t s) {
-    const TreeShape t = tree_shape(p.nq / p.kv.nkv, p.kv.head_dim, p.tokens);
-    if (p.kv.head_dim == 256) return t.ct == 1 ? launch_tree_mfma<256, I8, 1, 4, false>(p, s) : launch_tree_mfma<256, I8, 2, 2, true>(p, s);
-    if (t.ct == 1) return launch_tree_mfma<128, I8, 1, 8, false>(p, s);
-    return launch_tree_mfma<128, I8, 2, 4, true>(p, s);
+    constexpr int KS = HD == 128 ? 8 : 4;
+    switch (tree_cols(p.nq / p.kv.nkv, p.tokens)) {
+        case 16: return launch_narrow<HD, I8, KS, true>(p, s);
+        case 32: return launch_narrow<HD, I8, KS, false>(p, s);
+        default: return launch_wide<HD, I8, 2, KS / 2>(p, s);
+    }
 }
 
 hipError_t launch_tree_attn(const TreeAttnLaunch& p, hipStream_t s) {
@@ -1052,7 +1092,8 @@ hipError_t launch_tree_attn(const TreeAttnLaunch& p, hipStream_t s) {
                     ((reinterpret_cast<uintptr_t>(p.kv.k) | reinterpret_cast<uintptr_t>(p.kv.v)) & 3u) == 0;
     const bool in32 = p.q_stride < 1 << 22 && p.out_stride < 1 << 22;  // offsets within a block's (at most 64) rows
     const bool kv32 = static_cast<int64_t>(p.kv.nkv) * hd * 2 * 256 < int64_t(1) << 31;  // ... and its keys
-    if (al && in32 && kv32 && (hd == 128 || hd == 256)) return p.kv.i8 ? launch_tree_heads<true>(p, s) : launch_tree_heads<false>(p, s);
+    if (al && in32 && kv32 && hd == 128) return p.kv.i8 ? launch_tree_heads<128, true>(p, s) : launch_tree_heads<128, false>(p, s);
+    if (al && in32 && kv32 && hd == 256) return p.kv.i8 ? launch_tree_heads<256, true>(p, s) : launch_tree_heads<256, false>(p, s);
     const size_t lds = sizeof(float) * tree_row_lds(p.nq / p.kv.nkv, hd);
     const dim3 grid(p.tokens, p.kv.nkv);
     if (p.kv.i8)
