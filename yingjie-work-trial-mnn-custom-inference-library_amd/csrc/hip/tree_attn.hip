@@ -157,6 +157,7 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 constexpr int kTTile = 32;  // keys and columns of an MFMA tile
 constexpr int kTreeMaxSplits = 64;
+constexpr int kMinTiles = 2;
 
 // Columns, waves and output rows of a block: CT column tiles x KS key waves.
 template <int HD, int CT, int KS, int COLS>
@@ -228,13 +229,11 @@ struct TreeGrid {
     int tiles, splits;  // row tiles, key splits
 };
 
-// key chunks [begin, end) of split s of `chunks`: the first min(splits, chunks) splits have some
-// (returned)
-__device__ __forceinline__ int split_range(int chunks, int splits, int s, int& begin, int& end) {
-    const int n = min(splits, chunks), per = chunks / n, more = chunks - per * n;
+// pieces [begin, end) of split s of n
+__device__ __forceinline__ void split_range(int pieces, int n, int s, int& begin, int& end) {
+    const int per = pieces / n, more = pieces - per * n;
     begin = s * per + min(s, more);
     end = s < n ? begin + per + (s < more ? 1 : 0) : begin;
-    return n;
 }
 
 // exponent of a V scale, for the reference of its key's weights
@@ -319,6 +318,10 @@ struct WideTile : TreeBlock<HD, CT, KS, kTTile * CT> {
     static_assert(!I8 || 2 * B::kKeys <= B::kThreads, "one scale per thread");
     static_assert(kLds + 64 <= 160 * 1024, "LDS");
     static_assert(QueryStage<B, HD>::kBytes <= kLds, "q fits");
+    // splits that hold keys, of `splits`: whole chunks
+    static __host__ __device__ __forceinline__ int used_splits(int last, int splits) {
+        return last / B::kKeys + 1 < splits ? last / B::kKeys + 1 : splits;
+    }
 };
 
 template <int HD, bool I8, int KS, int COLS>
@@ -331,15 +334,27 @@ struct NarrowTile : TreeBlock<HD, 1, KS, COLS> {
     static constexpr size_t kKvBytes = KS * kWaveBytes + QueryStage<B, HD>::kBytes;
     static constexpr size_t kLds = kKvBytes > B::kOutBytes ? kKvBytes : B::kOutBytes;
     static_assert(kWave % kRowPieces == 0 && kWaveBytes % 16 == 0, "V staging");
+    // splits that hold keys, of `splits`: one while each of its waves has one tile at most
+    static __host__ __device__ __forceinline__ int used_splits(int last, int splits) {
+        const int tiles = last / kTTile + 1, n = (tiles + kMinTiles - 1) / kMinTiles;
+        return tiles <= KS ? 1 : n < splits ? n : splits;
+    }
     static_assert(kLds + 64 <= 160 * 1024, "LDS");
 };
+
+__device__ __forceinline__ void add_scaled(float4& r, float f, float4 v) {
+    r.x += f * v.x;
+    r.y += f * v.y;
+    r.z += f * v.z;
+    r.w += f * v.w;
+}
 
 constexpr float kRaise = 6.0f;  // weights are held times 2^kRaise
 constexpr float kSlack = 6.0f;  // the max may outgrow the reference by 2^kSlack before it is moved
 
 // The key waves of a block's columns joined, then written: the partial output of one split of several, or the output.
 template <typename F, bool I8, int CT, int KS, bool HALF, int N>
-__device__ __forceinline__ void finish_columns(const TreeAttnLaunch& p, const TreeGrid& grid, bool whole, int sp, int kh, int t0,
+__device__ __forceinline__ void finish_columns(const TreeAttnLaunch& p, const TreeGrid& grid, bool whole, int waves, int sp, int kh, int t0,
                                                int ntok, int T, uint32_t inv_t, bool live, const floatx16 (&o)[N], float m, float l,
                                                void* lds, int* redo) {
     constexpr int HD = 32 * N;
@@ -360,7 +375,7 @@ __device__ __forceinline__ void finish_columns(const TreeAttnLaunch& p, const Tr
     l = xor_pair_sum<32>(l);
     if constexpr (HALF) l = xor_pair_sum<16>(l);
     const int cw = HALF ? cl & 15 : cl, part = HALF ? cl >> 4 : 0;
-    if (live) {
+    if (live && wid / CT < waves) {
         const int at = wid * (F::kCols / CT) + cw;
         float* oc = Ol + at * F::kLdo + 4 * g + 16 * part;
 #pragma unroll
@@ -385,26 +400,21 @@ __device__ __forceinline__ void finish_columns(const TreeAttnLaunch& p, const Tr
         const int hc = static_cast<int>(c * inv_t >> 16), tc = c - hc * T;
         if (hc >= group || tc >= ntok) continue;
         const int at = tc * p.out_stride + (kh * group + hc) * HD + d;
-        float ml[KS], ll[KS], M = -INFINITY;
+        float ml[KS], M = -INFINITY, L = 0.0f;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const float2 v = *reinterpret_cast<const float2*>(Ml + (c + s * F::kCols) * 2);
-            ml[s] = v.x;
-            ll[s] = v.y;
-            M = fmaxf(M, v.x);
-        }
-        float L = 0.0f;
-        float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int s = 0; s < KS; ++s)
+            if (s < waves) {  // block-uniform
+                ml[s] = Ml[(c + s * F::kCols) * 2];
+                M = fmaxf(M, ml[s]);
+            }
+        float4 r = float4{};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const float f = __builtin_amdgcn_exp2f(ml[s] - M);
-            const float4 v = *reinterpret_cast<const float4*>(Ol + (c + s * F::kCols) * F::kLdo + d);
-            L += f * ll[s];
-            r.x += f * v.x;
-            r.y += f * v.y;
-            r.z += f * v.z;
-            r.w += f * v.w;
-        }
+        for (int s = 0; s < KS; ++s)
+            if (s < waves) {
+                const float f = __builtin_amdgcn_exp2f(ml[s] - M);
+                L += f * Ml[(c + s * F::kCols) * 2 + 1];
+                add_scaled(r, f, *reinterpret_cast<const float4*>(Ol + (c + s * F::kCols) * F::kLdo + d));
+            }
         if (!whole) {
             const size_t row = static_cast<size_t>(t0 + tc) * p.nq + kh * group + hc;
             *reinterpret_cast<float4*>(po + row * HD + d) = r;
@@ -460,19 +470,21 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kern
     const int qpos = live ? pos0 + ctok : -1;
     const uint64_t mask = live && p.has_tree ? p.masks.m[ctok] : 0;
     int begin, end;
-    const int splits = split_range(last / F::kKeys + 1, grid.splits, sp, begin, end);
+    const int splits = F::used_splits(last, grid.splits);
+    split_range(last / kTTile + 1, splits, sp, begin, end);  // tiles
     begin = __builtin_amdgcn_readfirstlane(begin);
     end = __builtin_amdgcn_readfirstlane(end);
-    if (begin >= end) return;  // fewer chunks than splits
+    if (begin >= end) return;  // fewer tiles than splits
+    const int waves = min(KS, end - begin), first = begin + ks;
 
     const uint32_t es = I8 ? 1u : 2u, krow = static_cast<uint32_t>(nkv) * HD * es;  // bytes per cache position
     u32x4 kr[F::kPieces], vr[F::kPieces];
     const float *k_scale = p.kv.k_scale, *v_scale = p.kv.v_scale;
     asm("" : "+s"(k_scale), "+s"(v_scale));  // (else each lane fetches its pointer from the arguments, chunk by chunk)
     const uint32_t kat = cl * krow + 16u * g, vat = lane / F::kRowPieces * krow + lane % F::kRowPieces * 16u;
-    auto rows_of = [&](const void* cache, int c) {  // of the wave's tile of chunk c; keys past `last` (or `end`) read 0
-        const int key0 = c * F::kKeys + ks * kTTile;
-        const int n = __builtin_amdgcn_readfirstlane(c < end ? max(0, min(kTTile, last - key0 + 1)) : 0);
+    auto rows_of = [&](const void* cache, int tile) {  // keys past `last`, tiles past `end` read 0
+        const int key0 = tile * kTTile;
+        const int n = __builtin_amdgcn_readfirstlane(tile < end ? max(0, min(kTTile, last - key0 + 1)) : 0);
         const uint8_t* base = static_cast<const uint8_t*>(cache) +
                               static_cast<size_t>(__builtin_amdgcn_readfirstlane(min(key0, last))) * krow +
                               static_cast<uint32_t>(kh) * HD * es;
@@ -480,23 +492,23 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kern
     };
     const float* scales = I8 && g ? v_scale : k_scale;  // lanes 0 - 31 hold K's of key cl, 32 - 63 V's
     float sr = 0.0f;
-    auto load_k = [&](int c) {
-        const __amdgpu_buffer_rsrc_t rs = rows_of(p.kv.k, c);
+    auto load_k = [&](int tile) {
+        const __amdgpu_buffer_rsrc_t rs = rows_of(p.kv.k, tile);
 #pragma unroll
         for (int u = 0; u < F::kPieces; ++u) kr[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, kat + 32u * u, 0, 0);
         if constexpr (I8) {
-            const int key = c * F::kKeys + ks * kTTile + cl;
-            sr = c < end && key <= last ? scales[static_cast<size_t>(key) * nkv + kh] : 0.0f;
+            const int key = tile * kTTile + cl;
+            sr = tile < end && key <= last ? scales[static_cast<size_t>(key) * nkv + kh] : 0.0f;
         }
     };
-    auto load_v = [&](int c) {
-        const __amdgpu_buffer_rsrc_t rs = rows_of(p.kv.v, c);
+    auto load_v = [&](int tile) {
+        const __amdgpu_buffer_rsrc_t rs = rows_of(p.kv.v, tile);
 #pragma unroll
         for (int u = 0; u < F::kPieces; ++u)
             vr[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, vat + static_cast<uint32_t>(u * (kWave / F::kRowPieces)) * krow, 0, 0);
     };
-    load_k(begin);
-    load_v(begin);
+    load_k(first);
+    load_v(first);
     uint8_t* Ql = reinterpret_cast<uint8_t*>(flash_lds) + KS * F::kWaveBytes;
     query.store(Ql);
     __syncthreads();
@@ -514,8 +526,8 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kern
     floatx16 o[kDimTiles];
 #pragma unroll
     for (int j = 0; j < kDimTiles; ++j) o[j] = floatx16{};
-    for (int c = begin; c < end; ++c) {
-        const int key0 = c * F::kKeys + ks * kTTile;
+    for (int tile = first; tile < end; tile += KS) {
+        const int key0 = tile * kTTile;
         floatx16 st = floatx16{};
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
@@ -533,7 +545,7 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kern
             Sl[lane] = sr;
             if (g) Sl[kTTile + lane] = scale_exponent(sr);
         }
-        load_k(c + 1);
+        load_k(tile + KS);
 #pragma unroll
         for (int u = 0; u < F::kPieces; ++u) {
             _Float16* at = Vl + (lane / F::kRowPieces + u * (kWave / F::kRowPieces)) * F::kLdv + lane % F::kRowPieces * (I8 ? 16 : 8);
@@ -547,7 +559,7 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kern
                 *reinterpret_cast<u32x4*>(at) = vr[u];
             }
         }
-        load_v(c + 1);
+        load_v(tile + KS);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // LDS takes a wave's accesses in their order
         __builtin_amdgcn_wave_barrier();
         float sc[kSlots], vs[kSlots], lv[kSlots], mc = -INFINITY;  // of keys 16 part + 8 (v / 4) + 4 g + v % 4
@@ -646,7 +658,7 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kern
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();  // every wave is done with its V
-    finish_columns<F, I8, 1, KS, HALF>(p, grid, splits == 1, sp, kh, 0, ntok, T, inv_t, live, o, m, l, flash_lds, &redo);
+    finish_columns<F, I8, 1, KS, HALF>(p, grid, splits == 1, waves, sp, kh, 0, ntok, T, inv_t, live, o, m, l, flash_lds, &redo);
 }
 
 template <int HD, bool I8, int CT, int KS>
@@ -678,7 +690,8 @@ __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wi
     const int qpos = live ? pos0 + t0 + ctok : -1;
     const uint64_t mask = live && p.has_tree ? p.masks.m[t0 + ctok] : 0;
     int begin, end;
-    const int splits = split_range(last / F::kKeys + 1, grid.splits, sp, begin, end);
+    const int splits = F::used_splits(last, grid.splits);
+    split_range(last / F::kKeys + 1, splits, sp, begin, end);
     begin = __builtin_amdgcn_readfirstlane(begin);
     end = __builtin_amdgcn_readfirstlane(end);
     if (begin >= end) return;
@@ -870,17 +883,16 @@ __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wi
     for (; c < end; ++c) chunk(c, std::false_type{}, std::true_type{});
     add_values(end - 1);
     __syncthreads();
-    finish_columns<F, I8, CT, KS, false>(p, grid, splits == 1, sp, kh, t0, ntok, T, inv_t, live, o, m, l, flash_lds, &redo);
+    finish_columns<F, I8, CT, KS, false>(p, grid, splits == 1, KS, sp, kh, t0, ntok, T, inv_t, live, o, m, l, flash_lds, &redo);
 }
 
 // What the merge kernels share: the keys' splits of row t, and an output quad from its sums.
 constexpr int kMergeThreads = 512;
 constexpr int kFewSplits = 4;
-template <int KEYS>
+template <typename F>
 __device__ __forceinline__ int used_splits(const TreeAttnLaunch& p, const TreeGrid& grid, int t, int T) {
     const int pos0 = clamp_pos0(p), t0 = t / T * T;
-    const int last = min(pos0 + (p.has_tree ? p.tokens : min(t0 + T, p.tokens)), p.kv.capacity) - 1;
-    return min(grid.splits, last / KEYS + 1);
+    return F::used_splits(min(pos0 + (p.has_tree ? p.tokens : min(t0 + T, p.tokens)), p.kv.capacity) - 1, grid.splits);
 }
 struct TreeParts {
     __amdgpu_buffer_rsrc_t o, st;
@@ -906,16 +918,10 @@ __device__ __forceinline__ bool write_quad(float4 r, float L, bool gated, float4
     *reinterpret_cast<float4*>(out) = y;
     return !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
 }
-__device__ __forceinline__ void add_scaled(float4& r, float f, float4 v) {
-    r.x += f * v.x;
-    r.y += f * v.y;
-    r.z += f * v.z;
-    r.w += f * v.w;
-}
 
 // The splits' partial outputs of one row and kv head joined, normalised and gated (nothing to do where one split held
 // every key).  `slices` threads share an output's splits; their first loads go out before the position has come.
-template <int HD, bool I8, int KEYS>
+template <typename F, int HD, bool I8>
 __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_kernel(TreeAttnLaunch p, TreeGrid grid, int T) {
     extern __shared__ float smem[];  // attend_row's
     __shared__ float factor[kTreeMaxGroup][kTreeMaxSplits], total[kTreeMaxGroup];
@@ -940,7 +946,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_kernel(TreeAttn
     const u32x2 st = __builtin_amdgcn_raw_buffer_load_b64(in.st, wid < group && lane < grid.splits ? (lane * in.rows + row0 + wid) * 8u : kBufOOB, 0, 0);
     const size_t at = static_cast<size_t>(kh * group + h) * HD + d;
     const float4 gt = p.gate ? *reinterpret_cast<const float4*>(p.gate + static_cast<size_t>(t) * p.q_stride + at) : float4{};
-    const int splits = used_splits<KEYS>(p, grid, t, T);
+    const int splits = used_splits<F>(p, grid, t, T);
     if (splits == 1) return;
     if (wid < group) {
         const float M = wave_max(lane < splits ? __uint_as_float(st.x) : -INFINITY);
@@ -975,7 +981,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_kernel(TreeAttn
 
 // ... of up to kFewSplits splits (calls of many rows): each thread has an output's partials by itself, a block several
 // kv heads of a row.
-template <int HD, bool I8, int KEYS>
+template <typename F, int HD, bool I8>
 __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_few_kernel(TreeAttnLaunch p, TreeGrid grid, int T) {
     extern __shared__ float smem[];  // attend_row's
     __shared__ uint32_t redo;        // a bit per kv head of the block
@@ -995,7 +1001,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_few_kernel(Tree
     }
     const size_t at = static_cast<size_t>(head) * HD + d;
     const float4 gt = p.gate && on ? *reinterpret_cast<const float4*>(p.gate + static_cast<size_t>(t) * p.q_stride + at) : float4{};
-    const int splits = used_splits<KEYS>(p, grid, t, T);
+    const int splits = used_splits<F>(p, grid, t, T);
     if (splits == 1) return;
     if (threadIdx.x == 0) redo = 0;
     __syncthreads();
@@ -1058,10 +1064,10 @@ static hipError_t launch_tree(const TreeAttnLaunch& p, Kernel kernel, hipStream_
     const size_t lds = sizeof(float) * tree_row_lds(group, HD);  // attend_row's
     if (g.splits <= kFewSplits) {
         const int heads = kMergeThreads / (group * (HD / 4));
-        hipLaunchKernelGGL((tree_attn_merge_few_kernel<HD, I8, F::kKeys>), dim3(p.tokens, (p.kv.nkv + heads - 1) / heads),
+        hipLaunchKernelGGL((tree_attn_merge_few_kernel<F, HD, I8>), dim3(p.tokens, (p.kv.nkv + heads - 1) / heads),
                            dim3(kMergeThreads), lds, s, p, g, T);
     } else {
-        hipLaunchKernelGGL((tree_attn_merge_kernel<HD, I8, F::kKeys>), dim3(p.tokens, p.kv.nkv), dim3(kMergeThreads), lds, s, p,
+        hipLaunchKernelGGL((tree_attn_merge_kernel<F, HD, I8>), dim3(p.tokens, p.kv.nkv), dim3(kMergeThreads), lds, s, p,
                            g, T);
     }
     return hipGetLastError();
