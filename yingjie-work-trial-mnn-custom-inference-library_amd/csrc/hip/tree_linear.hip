@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(256) tree_delta_kernel(TreeLinearLaunch p) {
 }
 
 // ---------------------------------------------------------------------------
-// Heads of 128 dims and four taps, two launches.
+// Heads of 128 dims and four taps: two launches, or one (below) for up to 16 rows.
 //
 // tree_linear_prep_kernel: one wave per (row, head): the convolution over the
 //   row's path, SiLU and L2 norm; q and k go out as fp16 hi + lo of 2^10 times
@@ -162,8 +162,9 @@ __global__ void __launch_bounds__(256) tree_delta_kernel(TreeLinearLaunch p) {
 //   rows below j add its part: steps as many as inner rows, each a dozen
 //   dependent instructions, no barrier.
 //
-// What bounds it: latency (a launch, one round of loads, the steps); the bytes (the
-// state, 2 MB for 32 heads, and 128 KB a row) are 1 us.
+// What bounds it: latency (a launch, rounds of loads, the steps); the bytes (the
+// state, 2 MB for 32 heads, and 128 KB a row) are 1 us.  With 16 / 32 heads: 6 rows
+// 6.6 us, a tree of 64 rows (three children a row) 14.1, a chain of 64 19.8.
 // ---------------------------------------------------------------------------
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -198,32 +199,85 @@ __device__ inline FastWs fast_ws(const TreeLinearLaunch& p) {
 }
 }  // namespace
 
+// beta and L of every row (a lane each) of value head vh, by one wave
+__device__ __forceinline__ void row_gates(const TreeLinearLaunch& p, int vh, double* L, float* beta) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const bool on = lane < p.nodes;
+    const size_t at = static_cast<size_t>(on ? lane : 0) * p.stride + vh;
+    const float a = p.a[at], b = p.b[at];
+    const float log_gate = fmaxf(-expf(p.a_log[vh]) * softplus_dev(a + p.dt_bias[vh]), -1000.0f);
+    const double mine = on ? static_cast<double>(log_gate) * 1.44269504088896340736 : 0.0;
+    // path sums by doubling: after step s a lane has the sum of the last 2^s rows of its path
+    int up = on ? static_cast<int8_t>(p.links.words[lane / 4] >> 8 * (lane % 4)) : -1;
+    double sum = mine;
+#pragma unroll
+    for (int s = 0; s < 6; ++s) {
+        const double add = __shfl(sum, up < 0 ? lane : up, kWave);
+        const int next = __shfl(up, up < 0 ? lane : up, kWave);
+        if (up >= 0) {
+            sum += add;
+            up = next;
+        }
+    }
+    L[lane] = sum;
+    beta[lane] = sigmoid_dev(b);
+}
+
+__device__ __forceinline__ int conv_channels(const TreeLinearLaunch& p) { return (2 * p.lk_n + p.lv_n) * kTL; }
+__device__ __forceinline__ const float* conv_history(const TreeLinearLaunch& p) {
+    return p.conv_state + static_cast<size_t>(*p.pos0 & 1) * conv_channels(p) * 3;
+}
+// The window of row i in channels c and c + 1, newest first: rows of its path (`parent`), then the history's newest
+// entries; and its convolution.
+template <typename Parent>
+__device__ __forceinline__ void conv_window(const TreeLinearLaunch& p, const float* history, int i, int c, Parent parent,
+                                            float2 (&x)[4]) {
+    const float* hs = history + static_cast<size_t>(c) * 3;
+    int r = i, back = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (r >= 0) {
+            const float* row = p.mixed + static_cast<size_t>(r) * p.stride + c;
+            x[t] = make_float2(row[0], row[1]);
+            r = parent(r);
+        } else {
+            x[t] = make_float2(hs[2 - back], hs[5 - back]);
+            ++back;
+        }
+    }
+}
+__device__ __forceinline__ void conv_weights(const TreeLinearLaunch& p, int c, float (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = p.conv_w[4 * c + i];
+}
+__device__ __forceinline__ float2 conv_silu(const float2 (&x)[4], const float (&w)[8]) {
+    float2 y = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        y.x += x[3 - t].x * w[t];
+        y.y += x[3 - t].y * w[4 + t];
+    }
+    return make_float2(silu_dev(y.x), silu_dev(y.y));
+}
+// y over its norm (a wave has the row, two dims a lane), times kTLRaise, as hi + lo
+__device__ __forceinline__ void unit_split(float2 y, h2& hi, h2& lo) {
+    const float inv = 1.0f / sqrtf(wave_sum(y.x * y.x + y.y * y.y) + 1.0e-6f);
+    float z[2] = {y.x * inv * kTLRaise, y.y * inv * kTLRaise};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        asm("" : "+v"(z[e]));  // (one rounding for hi and for what lo is taken from)
+        hi[e] = static_cast<_Float16>(z[e]);
+        lo[e] = static_cast<_Float16>(z[e] - static_cast<float>(hi[e]));
+    }
+}
+
 constexpr int kTLPrepWaves = 4;
 __global__ void __launch_bounds__(kWave* kTLPrepWaves) tree_linear_prep_kernel(TreeLinearLaunch p, int row_blocks) {
     const int lane = threadIdx.x & (kWave - 1);
     const FastWs ws = fast_ws(p);
-    if (static_cast<int>(blockIdx.x) >= row_blocks) {  // the gates: lane = row
+    if (static_cast<int>(blockIdx.x) >= row_blocks) {
         const int vh = (static_cast<int>(blockIdx.x) - row_blocks) * kTLPrepWaves + threadIdx.x / kWave;
-        if (vh >= p.lv_n) return;
-        const bool on = lane < p.nodes;
-        const size_t at = static_cast<size_t>(on ? lane : 0) * p.stride + vh;
-        const float a = p.a[at], b = p.b[at];
-        const float log_gate = fmaxf(-expf(p.a_log[vh]) * softplus_dev(a + p.dt_bias[vh]), -1000.0f);
-        const double mine = on ? static_cast<double>(log_gate) * 1.44269504088896340736 : 0.0;
-        // path sums by doubling: after step s a lane has the sum of the last 2^s rows of its path
-        int up = on ? static_cast<int8_t>(p.links.words[lane / 4] >> 8 * (lane % 4)) : -1;
-        double sum = mine;
-#pragma unroll
-        for (int s = 0; s < 6; ++s) {
-            const double add = __shfl(sum, up < 0 ? lane : up, kWave);
-            const int next = __shfl(up, up < 0 ? lane : up, kWave);
-            if (up >= 0) {
-                sum += add;
-                up = next;
-            }
-        }
-        ws.L[vh * kTreeMax + lane] = sum;
-        ws.beta[vh * kTreeMax + lane] = sigmoid_dev(b);
+        if (vh < p.lv_n) row_gates(p, vh, ws.L + vh * kTreeMax, ws.beta + vh * kTreeMax);
         return;
     }
     const int units = 2 * p.lk_n + p.lv_n, rows = fast_rows(p.nodes);
@@ -232,46 +286,18 @@ __global__ void __launch_bounds__(kWave* kTLPrepWaves) tree_linear_prep_kernel(T
     if (i >= p.nodes) return;
     const bool is_q = u < p.lk_n, is_k = !is_q && u < 2 * p.lk_n;
     const int h = is_q ? u : (is_k ? u - p.lk_n : u - 2 * p.lk_n);
-    const int c = (is_q ? 0 : (is_k ? p.lk_n : 2 * p.lk_n)) * kTL + h * kTL + 2 * lane;
-    const int conv_dim = (2 * p.lk_n + p.lv_n) * kTL;
-    // the window, newest first: rows of the path, then the history's newest entries
+    const int c = u * kTL + 2 * lane;
+    float w[8];
     float2 x[4];
-    int r = i, back = 0;
-    const float* hs = p.conv_state + static_cast<size_t>(*p.pos0 & 1) * conv_dim * 3 + static_cast<size_t>(c) * 3;
-    const float w[8] = {p.conv_w[4 * c], p.conv_w[4 * c + 1], p.conv_w[4 * c + 2], p.conv_w[4 * c + 3],
-                        p.conv_w[4 * c + 4], p.conv_w[4 * c + 5], p.conv_w[4 * c + 6], p.conv_w[4 * c + 7]};
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        if (r >= 0) {  // wave-uniform
-            const float* row = p.mixed + static_cast<size_t>(r) * p.stride + c;
-            x[t] = make_float2(row[0], row[1]);
-            r = static_cast<int8_t>(p.links.words[r / 4] >> 8 * (r % 4));
-        } else {
-            x[t] = make_float2(hs[2 - back], hs[5 - back]);
-            ++back;
-        }
-    }
-    float y0 = 0.0f, y1 = 0.0f;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        y0 += x[3 - t].x * w[t];
-        y1 += x[3 - t].y * w[4 + t];
-    }
-    y0 = silu_dev(y0);
-    y1 = silu_dev(y1);
+    conv_weights(p, c, w);
+    conv_window(p, conv_history(p), i, c, [&](int r) { return static_cast<int>(static_cast<int8_t>(p.links.words[r / 4] >> 8 * (r % 4))); }, x);
+    const float2 y = conv_silu(x, w);
     if (!is_q && !is_k) {
-        *reinterpret_cast<float2*>(ws.v + (static_cast<size_t>(h) * rows + i) * kTL + 2 * lane) = make_float2(y0, y1);
+        *reinterpret_cast<float2*>(ws.v + (static_cast<size_t>(h) * rows + i) * kTL + 2 * lane) = y;
         return;
     }
-    const float inv = 1.0f / sqrtf(wave_sum(y0 * y0 + y1 * y1) + 1.0e-6f);
-    float z[2] = {y0 * inv * kTLRaise, y1 * inv * kTLRaise};
     h2 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        asm("" : "+v"(z[e]));  // (one rounding for hi and for what lo is taken from)
-        hi[e] = static_cast<_Float16>(z[e]);
-        lo[e] = static_cast<_Float16>(z[e] - static_cast<float>(hi[e]));
-    }
+    unit_split(y, hi, lo);
     _Float16* out = (is_q ? ws.q : ws.k) + (static_cast<size_t>(h) * 2 * rows + i) * kTL + 2 * lane;
     *reinterpret_cast<h2*>(out) = hi;
     *reinterpret_cast<h2*>(out + static_cast<size_t>(rows) * kTL) = lo;
@@ -285,14 +311,20 @@ struct RowsSmem {
 // behind it the operands: [q, k][hi, lo][rows][kTLLd]
 inline size_t rows_lds(int nodes) { return sizeof(RowsSmem) + static_cast<size_t>(4) * fast_rows(nodes) * kTLLd * 2; }
 
+// ALONE: up to 16 rows, without the first launch: each block convolves its own key head's rows and its own columns of v,
+// 16 times over in all, which costs less than a launch and its round trip: with 16 / 32 heads 1 row 5.0 us (two launches
+// 7.6), 6 rows 6.6 (8.3), a chain of 16 9.3 (9.8).
+constexpr int kTLAlone = 16;
+template <bool ALONE>
 __global__ void __launch_bounds__(kWave* kTLWaves, 2) tree_linear_rows_kernel(TreeLinearLaunch p) {
     extern __shared__ uint4 tree_lds[];
+    __shared__ float v_own[ALONE ? kTLAlone : 1][kTLCols + 2], beta_own[ALONE ? kTreeMax : 1];
+    __shared__ double L_own[ALONE ? kTreeMax : 1];
     RowsSmem& sm = *reinterpret_cast<RowsSmem*>(tree_lds);
     _Float16* ops = reinterpret_cast<_Float16*>(&sm + 1);
     const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int vh = blockIdx.x, j0 = blockIdx.y * kTLCols, kh = vh / (p.lv_n / p.lk_n);
     const int n = p.nodes, rows = fast_rows(n), tiles = rows / 16;
-    const FastWs ws = fast_ws(p);
     const int g = lane / 16, cl = lane % 16;
     // every load first: the state's columns, the operands, the wave's two columns of v and its rows' gates
     float s0[4][8];
@@ -306,26 +338,71 @@ __global__ void __launch_bounds__(kWave* kTLWaves, 2) tree_linear_rows_kernel(Tr
                 for (int e = 0; e < 8; ++e) s0[s][e] = S[(32 * s + e) * kTL];
     }
     const int row = lane < n ? lane : n - 1, col = j0 + 2 * wid;
-    const float2 v = *reinterpret_cast<const float2*>(ws.v + (static_cast<size_t>(vh) * rows + row) * kTL + col);
-    const double L = ws.L[vh * kTreeMax + lane];
-    const float beta = ws.beta[vh * kTreeMax + lane];
     const uint64_t above = p.above.m[lane];
-    // a quarter of the operands is rows * 16 pieces of 16 bytes: q hi, q lo, k hi, k lo
-    const int quarter = rows * (kTL / 8);
-    u32x4 piece[8];
+    float2 v;
+    double L;
+    float beta;
+    if constexpr (ALONE) {
+        const float* history = conv_history(p);
+        // this wave's rows of q (even waves) or k, 4 apart; v eight rows a wave and the gates by the last ones
+        constexpr int kRounds = kTLAlone / (kTLWaves / 2);
+        const int c = ((wid & 1) * p.lk_n + kh) * kTL + 2 * lane;
+        float2 x[kRounds][4];
+        float w[8];
+        conv_weights(p, c, w);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-        const int at = threadIdx.x + u * kWave * kTLWaves, part = at / quarter, in = at % quarter;
-        const _Float16* src = (part < 2 ? ws.q : ws.k) + (static_cast<size_t>(kh) * 2 + (part & 1)) * rows * kTL;
-        if (part < 4) piece[u] = *reinterpret_cast<const u32x4*>(src + 8 * in);
-    }
+        for (int u = 0; u < kRounds; ++u)
+            if (const int i = wid / 2 + u * (kTLWaves / 2); i < n)
+                conv_window(p, history, i, c, [&](int r) { return static_cast<int>(static_cast<int8_t>(p.links.words[r / 4] >> 8 * (r % 4))); }, x[u]);
+        if (const int t = kTLWaves - 1 - wid; 8 * t < n) {
+            const int i = min(8 * t + lane / 8, n - 1), at = 2 * (lane % 8), vc = (2 * p.lk_n + vh) * kTL + j0 + at;
+            float2 xv[4];
+            float wv[8];
+            conv_weights(p, vc, wv);
+            conv_window(p, history, i, vc, [&](int r) {  // (a row of its own per lane: the words as scalars)
+                uint32_t word = p.links.words[0];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-        const int at = threadIdx.x + u * kWave * kTLWaves, part = at / quarter, in = at % quarter;
-        if (part < 4)
-            *reinterpret_cast<u32x4*>(ops + (static_cast<size_t>(part) * rows + in / (kTL / 8)) * kTLLd + 8 * (in % (kTL / 8))) = piece[u];
+                for (int b = 1; b < kTLAlone / 4; ++b) word = r / 4 == b ? p.links.words[b] : word;
+                return static_cast<int>(static_cast<int8_t>(word >> 8 * (r % 4)));
+            }, xv);
+            *reinterpret_cast<float2*>(&v_own[i][at]) = conv_silu(xv, wv);
+        }
+        if (wid == kTLWaves - 3) row_gates(p, vh, L_own, beta_own);
+#pragma unroll
+        for (int u = 0; u < kRounds; ++u)
+            if (const int i = wid / 2 + u * (kTLWaves / 2); i < n) {
+                h2 hi, lo;
+                unit_split(conv_silu(x[u], w), hi, lo);
+                _Float16* out = ops + (static_cast<size_t>(wid & 1) * 2 * rows + i) * kTLLd + 2 * lane;
+                *reinterpret_cast<h2*>(out) = hi;
+                *reinterpret_cast<h2*>(out + rows * kTLLd) = lo;
+            }
+        __syncthreads();
+        v = *reinterpret_cast<const float2*>(&v_own[row][2 * wid]);
+        L = L_own[lane];
+        beta = beta_own[lane];
+    } else {
+        const FastWs ws = fast_ws(p);
+        v = *reinterpret_cast<const float2*>(ws.v + (static_cast<size_t>(vh) * rows + row) * kTL + col);
+        L = ws.L[vh * kTreeMax + lane];
+        beta = ws.beta[vh * kTreeMax + lane];
+        // a quarter of the operands is rows * 16 pieces of 16 bytes: q hi, q lo, k hi, k lo
+        const int quarter = rows * (kTL / 8);
+        u32x4 piece[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int at = threadIdx.x + u * kWave * kTLWaves, part = at / quarter, in = at % quarter;
+            const _Float16* src = (part < 2 ? ws.q : ws.k) + (static_cast<size_t>(kh) * 2 + (part & 1)) * rows * kTL;
+            if (part < 4) piece[u] = *reinterpret_cast<const u32x4*>(src + 8 * in);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int at = threadIdx.x + u * kWave * kTLWaves, part = at / quarter, in = at % quarter;
+            if (part < 4)
+                *reinterpret_cast<u32x4*>(ops + (static_cast<size_t>(part) * rows + in / (kTL / 8)) * kTLLd + 8 * (in % (kTL / 8))) = piece[u];
+        }
+        __syncthreads();
     }
-    __syncthreads();
     // operand fragments of 16 rows: lane holds row cl, dims 32 s + 8 g .. + 7
     auto frag = [&](bool of_k, int t, half8 (&hi)[4], half8 (&lo)[4]) {
         const _Float16* at = ops + (static_cast<size_t>(of_k ? 2 : 0) * rows + 16 * t + cl) * kTLLd + 8 * g;
@@ -433,16 +510,20 @@ size_t tree_linear_workspace_bytes(int nodes, int lk_n, int lk_hd, int lv_n, int
 
 hipError_t launch_tree_linear(const TreeLinearLaunch& p, hipStream_t s) {
     if (linear_fast(p.lk_hd, p.lv_hd) && p.ksize == 4) {
+        const dim3 grid(p.lv_n, kTL / kTLCols), block(kWave * kTLWaves);
+        if (p.nodes <= kTLAlone) {
+            hipLaunchKernelGGL(tree_linear_rows_kernel<true>, grid, block, rows_lds(p.nodes), s, p);
+            return hipGetLastError();
+        }
         const int row_blocks = ((2 * p.lk_n + p.lv_n) * p.nodes + kTLPrepWaves - 1) / kTLPrepWaves;
         hipLaunchKernelGGL(tree_linear_prep_kernel, dim3(row_blocks + (p.lv_n + kTLPrepWaves - 1) / kTLPrepWaves),
                            dim3(kWave * kTLPrepWaves), 0, s, p, row_blocks);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-        const size_t lds = rows_lds(p.nodes);
-        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_linear_rows_kernel),
+        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_linear_rows_kernel<false>),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(rows_lds(kTreeMax)));
             e != hipSuccess)
             return e;
-        hipLaunchKernelGGL(tree_linear_rows_kernel, dim3(p.lv_n, kTL / kTLCols), dim3(kWave * kTLWaves), lds, s, p);
+        hipLaunchKernelGGL(tree_linear_rows_kernel<false>, grid, block, rows_lds(p.nodes), s, p);
         return hipGetLastError();
     }
     hipLaunchKernelGGL(tree_conv_kernel, dim3(2 * p.lk_n + p.lv_n, p.nodes), dim3(kWave), 0, s, p);
