@@ -529,7 +529,8 @@ XQHIP_API int xqhip_kv_read(const xqhip_kv* kv, int first, int count, int out_ty
  * does not see never reaches it, infinities and NaN included.  q, gate:
  * [tokens][q_stride], gate may be NULL (no gate); out: [tokens][out_stride].
  * Scores, weights and sums are held to fp32 accuracy.  The cache must hold the
- * rows: slots past its capacity are not read.  workspace: 16-byte aligned, of
+ * rows: slots past its capacity are not read.  out overlaps no input (rows that
+ * meet infinities are computed a second time).  workspace: 16-byte aligned, of
  * workspace_bytes >= xqhip_tree_attention_workspace_bytes(...), no
  * initialisation; calls that can overlap need one each.  nq / nkv <= 8. */
 XQHIP_API size_t xqhip_tree_attention_workspace_bytes(int nq, int nkv, int head_dim, int tokens);
@@ -590,9 +591,9 @@ XQHIP_API int xqhip_spec_verify(const float* logits, int ld_logits, int vocab, c
  * first + path[j] replaces row first + j for j < *count (path: strictly
  * increasing, path[j] >= j, as xqhip_spec_verify leaves it; path, count:
  * device; at most max_rows <= XQHIP_TREE_MAX rows).  first: *sets[i].first
- * (device), or 0 when that is NULL.  The buffers do not overlap.  Rows outside
- * [0, sets[i].rows) and paths that do not increase are left alone from there
- * on. */
+ * (device), or 0 when that is NULL.  Buffers of one call that overlap are
+ * refused.  Rows outside [0, sets[i].rows) and paths that do not increase are
+ * left alone from there on. */
 typedef struct xqhip_rows {
     void* base;            /* device */
     uint64_t row_bytes;

@@ -151,6 +151,9 @@ def test_keep_refuses():
         refused(L.xqhip_tree_keep(xb.rows([good]), 1, P, P, n, None), "tree_keep")
     for bad in ((None, 16, 4, None), (P, 0, 4, None), (P, 16, -1, None), (P, 1 << 31, 4, None)):
         refused(L.xqhip_tree_keep(xb.rows([good, bad]), 2, P, P, 4, None), "buffer 1")
+    at = lambda f: ctypes.c_void_p(P.value + f)  # noqa: E731
+    for other in ((P, 16, 4, None), (at(63), 16, 4, None), (at(16), 8, 1, None)):
+        refused(L.xqhip_tree_keep(xb.rows([(P, 16, 4, None), (at(4096), 16, 4, None), other]), 3, P, P, 4, None), "0 and 2 overlap")
     assert L.xqhip_tree_keep(None, 0, P, P, 4, None) == 0
 
 

@@ -378,6 +378,89 @@ def test_attention_without_a_gate_and_unaligned_rows(kind):
 
 
 @KINDS
+@pytest.mark.parametrize("nq,nkv,hd,T,pos0", [
+    (8, 8, 128, 16, 20000), (8, 8, 128, 20, 20001), (8, 8, 128, 40, 20031), (4, 4, 256, 3, 20000), (4, 4, 256, 17, 19999),
+    (4, 4, 256, 64, 9000), (8, 1, 128, 2, 70000)])
+def test_attention_of_several_chunks_per_wave(kind, nq, nkv, hd, T, pos0):
+    """Every wave of a split takes several tiles: the loads ahead, the moves of the running maximum."""
+    rng = np.random.default_rng(T + hd)
+    cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, pos0, spare=3)
+    par = to.random_tree(rng, T)
+    k, v = cache.values()
+    want = to.attention(q, gate, k, v, pos0, to.path_masks(par))
+    got = attend(cache, q, gate, pos0, par)
+    assert np.abs(got - want).max() <= 3e-5, np.abs(got - want).max()
+    assert np.linalg.norm(got - want) <= 5e-6 * np.linalg.norm(want)
+
+
+@KINDS
+@pytest.mark.parametrize("hd,nkv,edge", [(128, 8, 256), (256, 4, 128)])
+@pytest.mark.parametrize("T", [1, 4, 6])
+def test_attention_around_a_split_of_its_own(kind, hd, nkv, edge, T):
+    """The lengths at which a call's keys go from one split to several, and their neighbours."""
+    rng = np.random.default_rng(edge + T)
+    for n in (edge - 1, edge, edge + 1, edge + 31, edge + 32, edge + 33, 2 * edge + 1):
+        cache, q, gate = attention_case(rng, kind, 4 * nkv, nkv, hd, T, n - T, spare=0)
+        par = to.random_tree(rng, T)
+        want = to.attention(q, gate, *cache.values(), n - T, to.path_masks(par))
+        assert np.abs(attend(cache, q, gate, n - T, par) - want).max() <= 3e-5, n
+
+
+@pytest.mark.parametrize("T", [1000, 5000])
+def test_attention_of_a_long_chunk(T):
+    """Many row tiles, so that few splits are left, and a row of infinities in the middle of them."""
+    rng = np.random.default_rng(T)
+    nq, nkv, hd = 1, 1, 128
+    k, v = (rng.normal(0, 1, (T, nkv, hd)) for _ in range(2))
+    q, gate = (rng.normal(0, 1, (T, nq, hd)).astype(np.float32) for _ in range(2))
+    see = np.tril(np.ones((T, T), bool))
+    clean = Cache(xb.KV_F16, nkv, hd, T, k, v)
+    want = to.attention(q, gate, *clean.values(), 0, see)
+    assert np.abs(attend(clean, q, gate, 0) - want).max() <= 3e-5
+    bad = T - 30
+    v[bad, :, 7] = np.inf
+    got = attend(Cache(xb.KV_F16, nkv, hd, T, k, v), q, gate, 0)
+    assert np.abs(got[:bad] - want[:bad]).max() <= 3e-5 and not np.isfinite(got[bad:, 0, 7]).any()
+    others = np.arange(hd) != 7
+    assert np.abs(got[bad:][..., others] - want[bad:][..., others]).max() <= 3e-5
+
+
+@KINDS
+@pytest.mark.parametrize("nq,nkv,hd,T", [(8, 2, 128, 3), (8, 2, 128, 8), (8, 2, 128, 20), (8, 2, 256, 4), (8, 2, 256, 8),
+                                         (8, 2, 256, 30)])
+def test_values_of_every_size(kind, nq, nkv, hd, T):
+    """A value row that is far larger than the others, in a row that is not seen and under a weight so small that it
+    adds as much as they do.  A weight and its value's scale together are off by 2^-22 of the largest such product, so
+    the bound is that of ordinary values for each of the two parts; and values that are all tiny."""
+    rng = np.random.default_rng(T + hd)
+    pos0, far = 100, 2.0**(15 if kind == xb.KV_F16 else 20)
+    k, v = (rng.normal(0, 1, (pos0 + T, nkv, hd)) for _ in range(2))
+    q, gate = (rng.normal(0, 1, (T, nq, hd)).astype(np.float32) for _ in range(2))
+    q[..., 0] = 8
+    weight = 4 - math.log(far)  # the key's score
+    k[41], k[41, :, 0] = 0, weight * math.sqrt(hd) / 8
+    v[41] *= far / 6
+    par = [-1] + [0] * (T - 1)  # siblings: row 1's values do not reach the others
+    v[pos0 + 1] *= (1 if kind == xb.KV_F16 else 2.0**30) * far / 6
+    see = to.path_masks(par)
+    cache = Cache(kind, nkv, hd, pos0 + T, k, v)
+    ck, cv = cache.values()
+    want = to.attention(q, gate, ck, cv, pos0, see)
+    plain = cv.copy()
+    plain[41] = 0
+    other = np.arange(T) != 1
+    part = np.abs(want - to.attention(q, gate, ck, plain, pos0, see))[other].max()
+    got = attend(cache, q, gate, pos0, par)
+    assert part > 0.01 and np.abs(got - want)[other].max() <= 3e-5 * (1 + part)
+    reach = np.abs(want[1]).max()
+    assert np.abs(got - want)[1].max() <= 3e-5 * reach
+    if kind == xb.KV_I8:
+        tiny = Cache(kind, nkv, hd, pos0 + T, k, rng.normal(0, 1, v.shape) * 2.0**-80)
+        want = to.attention(q, gate, *tiny.values(), pos0, see)
+        assert np.abs(attend(tiny, q, gate, pos0, par) - want).max() <= 3e-5 * 2.0**-80
+
+
+@KINDS
 def test_attention_past_the_capacity(kind):
     """Slots past the cache's end are not read: the rows see what lies before it."""
     rng = np.random.default_rng(12)
@@ -558,7 +641,7 @@ def run_verify(logits, par, tokens, draft, inv_t, ua, us, ld=None, stream=None):
 @pytest.mark.parametrize("inv_t", [0.0, 1.0, 0.75, 4.0])
 @pytest.mark.parametrize("mode", ["point", "probs"])
 @pytest.mark.parametrize("vocab,n,reach,ld", [(1, 1, 1, 0), (5, 4, 2, 0), (1000, 17, 3, 0), (8192, 9, 1, 0), (8193, 64, 4, 8195),
-                                             (248320, 6, 1, 0), (50001, 40, 5, 50004), (20000, 64, 64, 0)])
+                                             (248320, 6, 1, 0), (300001, 5, 2, 0), (50001, 40, 5, 50004), (20000, 64, 64, 0)])
 def test_verify(vocab, n, reach, ld, mode, inv_t):
     """Equal, token by token: all decisions are taken in 64 bits."""
     rng = np.random.default_rng(vocab + n)
@@ -736,3 +819,82 @@ def test_a_step_over_a_tree(kind):
                                   norms[0].ptr, norms[1].ptr, EPS, cs.ptr, i32(pos0).ptr, other.buf[0].ptr,
                                   other.buf[1].ptr, cap, out.ptr, ws.ptr, None))
         assert np.abs(out.download(np.float32, nq * hd) - tree_out[0]).max() <= 3e-5
+
+
+@KINDS
+def test_a_step_in_graphs_that_share_a_workspace(kind):
+    """The step's calls captured twice, over trees of 5 and 40 rows with one workspace between them, and replayed in turn
+    with eager work in between: each replay leaves what the eager calls leave."""
+    L = xb.hip()
+    rng = np.random.default_rng(21)
+    nq, nkv, hd, rotary, lk, lv, ks, pos0, vocab, cap = 8, 2, 128, 32, 2, 4, 4, 600, 9000, 700
+    cd, n = 128 * (2 * lk + lv), 40
+    row, lrow = 2 * nq * hd + 2 * nkv * hd, cd + 2 * lv
+    k, v = (rng.normal(0, 1, (pos0, nkv, hd)) for _ in range(2))
+    fresh = Cache(kind, nkv, hd, cap, k, v)
+    held = [b.download(np.uint8, b.nbytes) for b in fresh.buf]
+    norms = [dev(rng.normal(1, 0.1, hd).astype(np.float32)) for _ in range(2)]
+    cs, pos, proj = dev(rope(rotary, cap)), i32(pos0), dev(rng.normal(0, 1, (n, row)).astype(np.float32))
+    c = {m: np.ascontiguousarray(x, np.float32) for m, x in linear_case(rng, lk, 128, lv, 128, ks, n).items()}
+    lin, hist, S = dev(np.concatenate([c["mixed"], c["a"], c["b"]], 1)), dev(c["hist"]), dev(c["S"])
+    keep = [dev(c[m]) for m in ("w", "a_log", "dt")]
+    logits, us = dev(rng.normal(0, 2, (n, vocab)).astype(np.float32)), dev(np.array([0.6], np.float32))
+    tokens, ua = dev(rng.integers(0, vocab, n).astype(np.int32)), dev(np.full(n, 1e-6, np.float32))
+    sizes = [f(n) for f in (lambda t: L.xqhip_tree_attention_workspace_bytes(nq, nkv, hd, t),
+                            lambda t: L.xqhip_linear_attn_tree_workspace_bytes(t, lk, 128, lv, 128),
+                            lambda t: L.xqhip_spec_verify_workspace_bytes(t, vocab))]
+    size = max([*sizes, L.xqhip_tree_attention_workspace_bytes(nq, nkv, hd, 5)])
+    ws = dev(np.full(size, 0xff, np.uint8))
+    q, gate, out = (xb.DeviceBuffer(n * nq * hd * 4) for _ in range(3))
+    lout, count, path, new = xb.DeviceBuffer(n * lv * 128 * 4), i32(0), dev(np.zeros(n, np.int32)), dev(np.zeros(n, np.int32))
+    at = lambda b, f: ctypes.c_void_p(b.ptr.value + 4 * f)  # noqa: E731
+    widths = 2 * [nkv * hd * (1 if kind == xb.KV_I8 else 2)] + (2 * [nkv * 4] if kind == xb.KV_I8 else [])
+    sets = xb.rows([(b.ptr, w, cap, pos.ptr) for b, w in zip(fresh.buf, widths)])
+
+    def step(par, s):
+        T, tr = len(par), ctypes.byref(xb.tree(par))
+        xb.ck(L.xqhip_attn_prep_kv(proj.ptr, at(proj, 2 * nq * hd), at(proj, (2 * nq + nkv) * hd), 1, nq, rotary,
+                                   norms[0].ptr, norms[1].ptr, EPS, cs.ptr, pos.ptr, tr, T, row, nq * hd, q.ptr, gate.ptr,
+                                   fresh.ref, s))
+        xb.ck(L.xqhip_tree_attention(q.ptr, gate.ptr, fresh.ref, nq, tr, T, nq * hd, pos.ptr, out.ptr, nq * hd, ws.ptr,
+                                     size, s))
+        xb.ck(L.xqhip_linear_attn_tree(lin.ptr, at(lin, cd), at(lin, cd + lv), lrow, hist.ptr, pos.ptr, keep[0].ptr,
+                                       keep[1].ptr, keep[2].ptr, S.ptr, lk, 128, lv, 128, ks, tr, lout.ptr, lv * 128,
+                                       ws.ptr, size, s))
+        xb.ck(L.xqhip_spec_verify(logits.ptr, vocab, vocab, tr, tokens.ptr, None, 0, 1.0, ua.ptr, us.ptr, count.ptr,
+                                  path.ptr, new.ptr, ws.ptr, size, s))
+        xb.ck(L.xqhip_tree_keep(sets, len(sets), path.ptr, count.ptr, T, s))
+
+    def reset():
+        for b, x in zip(fresh.buf, held):
+            b.upload(x)
+        for b in (out, lout, path, new):
+            b.zero()
+        xb.ck(L.xqhip_device_synchronize())
+
+    def left(s):
+        xb.ck(L.xqhip_stream_synchronize(s) if s else L.xqhip_device_synchronize())
+        return [b.download(np.uint8, b.nbytes) for b in (*fresh.buf[:len(widths)], out, lout, count, path, new)]
+
+    trees = [to.random_tree(rng, 5), to.random_tree(rng, 40)]
+    want = []
+    for par in trees:
+        reset()
+        step(par, None)
+        want.append(left(None))
+    s, graphs = ctypes.c_void_p(), [ctypes.c_void_p(), ctypes.c_void_p()]
+    xb.ck(L.xqhip_stream_create(ctypes.byref(s)))
+    for par, g in zip(trees, graphs):
+        xb.ck(L.xqhip_graph_begin(s))
+        step(par, s)
+        xb.ck(L.xqhip_graph_end(s, ctypes.byref(g)))
+    for i in (0, 1, 1, 0, 1):
+        reset()
+        step(trees[1 - i], None)  # eager work of the other tree
+        reset()
+        xb.ck(L.xqhip_graph_launch(graphs[i], s))
+        for a, b in zip(left(s), want[i]):
+            assert np.array_equal(a, b)
+    for g in graphs:
+        xb.ck(L.xqhip_graph_destroy(g))
+    xb.ck(L.xqhip_stream_destroy(s))

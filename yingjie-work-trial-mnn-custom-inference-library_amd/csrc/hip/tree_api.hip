@@ -246,9 +246,15 @@ int xqhip_tree_keep(const xqhip_rows* sets, int n_sets, const int32_t* path, con
                     void* stream) {
     if (n_sets < 0 || (n_sets > 0 && !sets) || !path || !count || max_rows < 1 || max_rows > XQHIP_TREE_MAX)
         return refuse("xqhip_tree_keep: bad args");
-    for (int i = 0; i < n_sets; ++i)
-        if (!sets[i].base || sets[i].row_bytes == 0 || sets[i].row_bytes > uint64_t(1) << 30 || sets[i].rows < 0)
+    for (int i = 0; i < n_sets; ++i) {
+        if (!sets[i].base || sets[i].row_bytes == 0 || sets[i].row_bytes > uint64_t(1) << 30 || sets[i].rows < 0 ||
+            sets[i].rows > int64_t(1) << 32)
             return refuse("xqhip_tree_keep: buffer %d", i);
+        const auto begin = [&](int j) { return reinterpret_cast<uintptr_t>(sets[j].base); };
+        const auto end = [&](int j) { return begin(j) + sets[j].row_bytes * static_cast<uint64_t>(sets[j].rows); };
+        for (int j = 0; j < i; ++j)
+            if (begin(i) < end(j) && begin(j) < end(i)) return refuse("xqhip_tree_keep: buffers %d and %d overlap", j, i);
+    }
     for (int i0 = 0; i0 < n_sets; i0 += xqhip::kKeepSets) {
         const int n = std::min(n_sets - i0, xqhip::kKeepSets);
         xqhip::KeepLaunch p{};

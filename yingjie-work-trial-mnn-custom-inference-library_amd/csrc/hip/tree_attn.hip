@@ -238,7 +238,7 @@ __device__ __forceinline__ void split_range(int pieces, int n, int s, int& begin
 
 // exponent of a V scale, for the reference of its key's weights
 __device__ __forceinline__ float scale_exponent(float s) {
-    return fabsf(s) > 0.0f ? fminf(fmaxf(static_cast<float>(__builtin_amdgcn_frexp_expf(s)), -80.0f), 100.0f) : -80.0f;
+    return fabsf(s) > 0.0f ? fminf(fmaxf(static_cast<float>(__builtin_amdgcn_frexp_expf(s)), -90.0f), 100.0f) : -90.0f;
 }
 
 // The block's columns of q as fp16 hi + lo in LDS, each scaled by a power of two into [2^12, 2^13), and the factor of
