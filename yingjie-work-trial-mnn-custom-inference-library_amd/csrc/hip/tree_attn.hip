@@ -124,15 +124,13 @@ __global__ void __launch_bounds__(256) tree_attn_row_kernel(TreeAttnLaunch p) {
 }
 
 // ---------------------------------------------------------------------------
-// Matrix-core form, heads of 128 and 256 dims.  A block takes 32 CT columns of
+// Matrix-core forms, heads of 128 and 256 dims.  A block takes some columns of
 // one kv head and one split of its keys, a column being one (row, query head)
-// pair: column c is head c / T of the kv head's `group` and row t0 + c % T, T =
-// 32 CT / group.  CT x KS waves: wave (ct, ks) owns the 32 columns of tile ct
-// and every KS-th 32-key tile, with its own running max, sum and output, merged
-// through LDS at the end.  K and V are staged chunk by chunk (32 KS keys, shared
-// by all column tiles) as fp16 in LDS; an 8-bit cache's codes become fp16
-// integers there, exactly, and the scales enter as factors of the scores and
-// of the weights.
+// pair: column c of C is head c / T of the kv head's `group` and row t0 + c % T,
+// T = C / group.  Its waves share the keys in 32-key tiles, each with its own
+// running max, sum and output, joined through LDS at the end.  An 8-bit cache's
+// codes become fp16 integers, exactly, and its scales enter as factors of the
+// scores and of the weights.
 //
 // Scores are formed transposed, S^T = K Q^T (keys are the MFMA rows): lane l
 // holds column l & 31 and the keys 8 (v / 4) + 4 (l >> 5) + v % 4 of its tile,
@@ -140,23 +138,36 @@ __global__ void __launch_bounds__(256) tree_attn_row_kernel(TreeAttnLaunch p) {
 // [key][dim]; ds_read_tr16_b64 hands each lane four keys of its dim.
 //
 // Precision: q (scaled per column by a power of two to [2^12, 2^13)) and the
-// weights (times 2^6, within 2^6 of the column's running max) are split into
-// fp16 hi + lo, 22 bits together; fp32 accumulation.  One fp16 each would leave
-// errors of 2^-12 of the weights, where the caches' own values are exact.  An
-// 8-bit V's weights carry its scale over a power of two R at or above the
-// split's largest scale (moved when one outgrows it), so they stay in fp16's
-// range: the output is off by 2^-31 sqrt(keys) of the largest |v| at most.
+// weights (times 2^6) are split into fp16 hi + lo, 22 bits together; fp32
+// accumulation.  One fp16 each would leave errors of 2^-12 of the weights, where
+// the caches' own values are exact.  The exponents' reference m is a column's
+// largest score so far, or up to 2^6 less; over an 8-bit cache the largest of
+// score + log2 of V's scale, since the weights carry V's scales and must stay in
+// fp16's range: the output is off by 2^-22 of the largest weight times |v|.
 //
 // A masked key has weight 0, but 0 times an infinity is not 0, and neither hi +
 // lo nor the finite start of the running max can carry infinities.  Where that
 // happens a sum is not finite or the weights sum to 0: the block that writes
 // such an output computes its rows again by attend_row.
+//
+// tree_attn_narrow_kernel: calls of up to 16 or 32 columns (a decode step's few
+//   rows).  What bounds it: the cache's bytes in long contexts (one row after
+//   120000 positions of an 8-bit cache, 8 heads: 246 MB in 56 us, 4.4 TB/s), a
+//   chain of a launch's latencies in short ones (4 rows at position 0: 8 us).
+// tree_attn_wide_kernel: 64 columns.  What bounds it: the two products' two
+//   passes each and, beside them, the weights' exponentials and splits, which
+//   issue in turn with the MFMAs (64 rows after 131000 positions of an 8-bit
+//   cache, 32 / 8 heads: 2.75e11 operations in 320 us, 0.86 PFLOP/s).  500 rows
+//   after 3584: 82 us.  A wave with two column tiles read K and V half as often
+//   and was slower below 100000 positions: twice the registers, half the waves.
 // ---------------------------------------------------------------------------
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 constexpr int kTTile = 32;  // keys and columns of an MFMA tile
 constexpr int kTreeMaxSplits = 64;
+// A narrow call's splits hold two tiles or more: 8 rows of 256 dims after 2000 positions 16.4 us (one tile 18.3, four
+// 17.3), after 540 14.2 (14.7, 16.4); a wave each of one block, where that is all, needs no join.
 constexpr int kMinTiles = 2;
 
 // Columns, waves and output rows of a block: CT column tiles x KS key waves.
@@ -442,9 +453,12 @@ __device__ __forceinline__ void finish_columns(const TreeAttnLaunch& p, const Tr
     }
 }
 
-// Up to 32 columns (a decode step's few rows): one column tile, and no barrier before the waves join.  Each wave takes
-// its own 32-key tiles: K straight into registers as the A operand (16-byte pieces; the order of the dims within a
-// step is free as long as q's is the same), V through the wave's own LDS, the next tile's K and V on their way meanwhile.
+// One column tile, and no barrier before the waves join.  Each wave takes its own 32-key tiles: K straight into registers
+// as the A operand (16-byte pieces; the order of the dims within a step is free as long as q's is the same), V through
+// the wave's own LDS, the next tile's K and V on their way meanwhile.
+// HALF: up to 16 columns, q's hi parts in the tile's first 16 columns and its lo parts in the others.  One MFMA then does
+// what two do, a lane and its neighbour 16 lanes on add their scores and take eight keys each, and the weights' hi and lo
+// parts go back into the two halves.  One row after 8100 positions 11.8 us, in 32 columns 14.0.
 template <int HD, bool I8, int KS, bool HALF>
 __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kernel(TreeAttnLaunch p, TreeGrid grid) {
     using F = NarrowTile<HD, I8, KS, HALF ? 16 : 32>;
@@ -661,6 +675,9 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kern
     finish_columns<F, I8, 1, KS, HALF>(p, grid, splits == 1, waves, sp, kh, 0, ntok, T, inv_t, live, o, m, l, flash_lds, &redo);
 }
 
+// CT column tiles x KS key waves.  K and V are staged chunk by chunk (32 KS keys, shared by the column tiles) in LDS,
+// twice each: one barrier a chunk, the next chunk's loads over a whole chunk ahead, and a chunk's products with V beside
+// the next one's softmax.
 template <int HD, bool I8, int CT, int KS>
 __global__ void __launch_bounds__(kWave* CT* KS, (CT * KS + 3) / 4) tree_attn_wide_kernel(TreeAttnLaunch p, TreeGrid grid) {
     using F = WideTile<HD, I8, CT, KS>;
@@ -920,7 +937,7 @@ __device__ __forceinline__ bool write_quad(float4 r, float L, bool gated, float4
 }
 
 // The splits' partial outputs of one row and kv head joined, normalised and gated (nothing to do where one split held
-// every key).  `slices` threads share an output's splits; their first loads go out before the position has come.
+// every key): 4 us, a launch and two round trips.  `slices` threads share an output's splits; their first loads go out before the position has come.
 template <typename F, int HD, bool I8>
 __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_kernel(TreeAttnLaunch p, TreeGrid grid, int T) {
     extern __shared__ float smem[];  // attend_row's
@@ -980,7 +997,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_kernel(TreeAttn
 }
 
 // ... of up to kFewSplits splits (calls of many rows): each thread has an output's partials by itself, a block several
-// kv heads of a row.
+// kv heads of a row.  256 rows, two splits: 16.5 us in all, with the kernel above 22.7.
 template <typename F, int HD, bool I8>
 __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_few_kernel(TreeAttnLaunch p, TreeGrid grid, int T) {
     extern __shared__ float smem[];  // attend_row's
@@ -1032,12 +1049,16 @@ bool tree_attn_supported(int nq, int nkv, int head_dim) {
            sizeof(float) * tree_row_lds(nq / nkv, head_dim) <= 64 * 1024;
 }
 
-// The columns of a call's blocks.
+// The columns of a call's blocks.  Few rows are bound by latency and bytes, where the narrow kernel's waves run apart:
+// 4 rows of 4 heads after 8100 positions 12.7 us in 16 columns, 14.7 in 32, 16.4 in the wide kernel's 64; 8 rows 15.7
+// in 32, 17.4 in 64.
 static int tree_cols(int group, int tokens) {
     const int cols = tokens * group;
     return cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
 }
-// Row tiles, and key splits that give every CU a block.
+// Row tiles, and key splits that give every CU a block.  Twice or half as many blocks: one row after 8100 positions 11.8 us
+// (16.0, 13.0), 64 rows after 131000 319 (325, 517), 128 rows after 2000 24.8 (34.6, 29.5); half as many is better only
+// where there is next to no context (256 rows at position 0 16.5, 13.5).
 static TreeGrid tree_grid(int nq, int nkv, int tokens) {
     const int T = tree_cols(nq / nkv, tokens) / (nq / nkv);
     const int tiles = (tokens + T - 1) / T;
