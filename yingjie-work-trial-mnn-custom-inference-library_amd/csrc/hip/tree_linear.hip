@@ -207,11 +207,10 @@ __device__ __forceinline__ void row_gates(const TreeLinearLaunch& p, int vh, dou
     const float a = p.a[at], b = p.b[at];
     const float log_gate = fmaxf(-expf(p.a_log[vh]) * softplus_dev(a + p.dt_bias[vh]), -1000.0f);
     const double mine = on ? static_cast<double>(log_gate) * 1.44269504088896340736 : 0.0;
-    // path sums by doubling: after step s a lane has the sum of the last 2^s rows of its path
+    // path sums by doubling: before step s a lane has the sum of the last s rows of its path
     int up = on ? static_cast<int8_t>(p.links.words[lane / 4] >> 8 * (lane % 4)) : -1;
     double sum = mine;
-#pragma unroll
-    for (int s = 0; s < 6; ++s) {
+    for (int s = 1; s < p.nodes; s *= 2) {
         const double add = __shfl(sum, up < 0 ? lane : up, kWave);
         const int next = __shfl(up, up < 0 ? lane : up, kWave);
         if (up >= 0) {
@@ -329,6 +328,7 @@ __global__ void __launch_bounds__(kWave* kTLWaves, 2) tree_linear_rows_kernel(Tr
     // every load first: the state's columns, the operands, the wave's two columns of v and its rows' gates
     float s0[4][8];
     const bool has_tile = wid < 2 * tiles;  // (q or k, row tile) of this wave
+    const bool has_rows = ALONE ? wid / 2 == 1 : has_tile;  // ... of which it does the products among the rows
     {
         const float* S = p.state + (static_cast<size_t>(vh) * kTL + 8 * g) * kTL + j0 + cl;
         if (has_tile)
@@ -422,11 +422,11 @@ __global__ void __launch_bounds__(kWave* kTLWaves, 2) tree_linear_rows_kernel(Tr
         }
         return c + d + e;
     };
+    const bool of_k = ALONE ? wid % 2 == 0 : wid < tiles;
+    const int ta = wid % tiles;
+    half8 ah[4], al[4], bh[4], bl[4];
+    if (has_tile || has_rows) frag(of_k, ta, ah, al);
     if (has_tile) {
-        const bool of_k = wid < tiles;
-        const int a = wid % tiles;
-        half8 ah[4], al[4], bh[4], bl[4];
-        frag(of_k, a, ah, al);
         float mx = 0.0f;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
@@ -446,12 +446,13 @@ __global__ void __launch_bounds__(kWave* kTLWaves, 2) tree_linear_rows_kernel(Tr
                 bh[s][e] = static_cast<_Float16>(x);
                 bl[s][e] = static_cast<_Float16>(x - static_cast<float>(bh[s][e]));
             }
-        *reinterpret_cast<floatx4*>(&(of_k ? sm.kS : sm.qS)[cl][16 * a + 4 * g]) = product(ah, al, bh, bl) * down;
-        // among the rows: with the k rows of every tile that holds a row above one of this tile's, or the rows themselves
-        for (int b = 0; b <= a; ++b) {
-            if (b < a && !__builtin_amdgcn_ballot_w64(lane / 16 == a && (above >> 16 * b & 0xffff))) continue;
+        *reinterpret_cast<floatx4*>(&(of_k ? sm.kS : sm.qS)[cl][16 * ta + 4 * g]) = product(ah, al, bh, bl) * down;
+    }
+    if (has_rows) {  // with the k rows of every tile that holds a row above one of this tile's, or the rows themselves
+        for (int b = 0; b <= ta; ++b) {
+            if (b < ta && !__builtin_amdgcn_ballot_w64(lane / 16 == ta && (above >> 16 * b & 0xffff))) continue;
             frag(true, b, bh, bl);
-            *reinterpret_cast<floatx4*>(&(of_k ? sm.kk : sm.qk)[16 * b + cl][16 * a + 4 * g]) =
+            *reinterpret_cast<floatx4*>(&(of_k ? sm.kk : sm.qk)[16 * b + cl][16 * ta + 4 * g]) =
                 product(ah, al, bh, bl) * (1.0f / (kTLRaise * kTLRaise));
         }
     }
