@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(256) tree_delta_kernel(TreeLinearLaunch p) {
 //
 // What bounds it: latency (a launch, rounds of loads, the steps); the bytes (the
 // state, 2 MB for 32 heads, and 128 KB a row) are 1 us.  With 16 / 32 heads: 6 rows
-// 6.6 us, a tree of 64 rows (three children a row) 14.1, a chain of 64 19.8.
+// 5.9 us, a tree of 64 rows (three children a row) 14.4, a chain of 64 19.7.  Weights
+// with decay and mask applied beforehand left the chain's step as long.
 // ---------------------------------------------------------------------------
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -199,6 +200,16 @@ __device__ inline FastWs fast_ws(const TreeLinearLaunch& p) {
 }
 }  // namespace
 
+// Row r's parent, r < 4 WORDS, each lane for its own r: the words as scalars.  (Indexed by lane, each step up a path would
+// be a memory round trip.)
+template <int WORDS>
+__device__ __forceinline__ int parent_in(const TreeLinks& links, int r) {
+    uint32_t w = links.words[0];
+#pragma unroll
+    for (int i = 1; i < WORDS; ++i) w = r / 4 == i ? links.words[i] : w;
+    return static_cast<int8_t>(w >> 8 * (r % 4));
+}
+
 // beta and L of every row (a lane each) of value head vh, by one wave
 __device__ __forceinline__ void row_gates(const TreeLinearLaunch& p, int vh, double* L, float* beta) {
     const int lane = threadIdx.x & (kWave - 1);
@@ -223,44 +234,64 @@ __device__ __forceinline__ void row_gates(const TreeLinearLaunch& p, int vh, dou
 }
 
 __device__ __forceinline__ int conv_channels(const TreeLinearLaunch& p) { return (2 * p.lk_n + p.lv_n) * kTL; }
-__device__ __forceinline__ const float* conv_history(const TreeLinearLaunch& p) {
-    return p.conv_state + static_cast<size_t>(*p.pos0 & 1) * conv_channels(p) * 3;
-}
-// The window of row i in channels c and c + 1, newest first: rows of its path (`parent`), then the history's newest
-// entries; and its convolution.
+// What the convolution of channels c and c + 1 takes besides rows: the weights, and the history's three newest steps
+// (oldest first) in both copies.  Which copy counts is known when the position has come; no load waits for it.
+struct ConvTaps {
+    float w[8], past[2][6] = {};
+    __device__ __forceinline__ void load_weights(const TreeLinearLaunch& p, int c) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = p.conv_w[4 * c + i];
+    }
+    __device__ __forceinline__ void load_past(const TreeLinearLaunch& p, int c) {
+        const float* h = p.conv_state + static_cast<size_t>(c) * 3;
+#pragma unroll
+        for (int i = 0; i < 6; ++i) {
+            past[0][i] = h[i];
+            past[1][i] = h[static_cast<size_t>(conv_channels(p)) * 3 + i];
+        }
+    }
+};
+// Row i's newest four rows of its path, itself first, in channels c and c + 1; how many there are
 template <typename Parent>
-__device__ __forceinline__ void conv_window(const TreeLinearLaunch& p, const float* history, int i, int c, Parent parent,
-                                            float2 (&x)[4]) {
-    const float* hs = history + static_cast<size_t>(c) * 3;
-    int r = i, back = 0;
+__device__ __forceinline__ int path_window(const TreeLinearLaunch& p, int i, int c, Parent parent, float2 (&x)[4]) {
+    int r = i, have = 0;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
+        x[t] = make_float2(0.0f, 0.0f);
         if (r >= 0) {
             const float* row = p.mixed + static_cast<size_t>(r) * p.stride + c;
             x[t] = make_float2(row[0], row[1]);
             r = parent(r);
-        } else {
-            x[t] = make_float2(hs[2 - back], hs[5 - back]);
-            ++back;
+            ++have;
         }
     }
+    return have;
 }
-__device__ __forceinline__ void conv_weights(const TreeLinearLaunch& p, int c, float (&w)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = p.conv_w[4 * c + i];
+// x / (1 + e^-x) by the hardware's exponential and reciprocal, an ulp each: off by |x| 2^-24 of itself at most where it
+// is small, by 2^-22 elsewhere.  (The exact division and exponential were half of what few rows take.)
+__device__ __forceinline__ float silu_fast(float x) {
+    return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x));
 }
-__device__ __forceinline__ float2 conv_silu(const float2 (&x)[4], const float (&w)[8]) {
-    float2 y = make_float2(0.0f, 0.0f);
+__device__ __forceinline__ float2 conv_silu(const float2 (&x)[4], int have, const ConvTaps& taps, bool odd) {
+    float y[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        y.x += x[3 - t].x * w[t];
-        y.y += x[3 - t].y * w[4 + t];
+    for (int e = 0; e < 2; ++e) {
+        float past[3];  // newest first
+#pragma unroll
+        for (int i = 0; i < 3; ++i) past[i] = odd ? taps.past[1][3 * e + 2 - i] : taps.past[0][3 * e + 2 - i];
+#pragma unroll
+        for (int t = 3; t >= 0; --t) {
+            float v = e ? x[t].y : x[t].x;
+#pragma unroll
+            for (int i = 0; i < t; ++i) v = have == t - i ? past[i] : v;
+            y[e] += v * taps.w[4 * e + 3 - t];
+        }
     }
-    return make_float2(silu_dev(y.x), silu_dev(y.y));
+    return make_float2(silu_fast(y[0]), silu_fast(y[1]));
 }
 // y over its norm (a wave has the row, two dims a lane), times kTLRaise, as hi + lo
 __device__ __forceinline__ void unit_split(float2 y, h2& hi, h2& lo) {
-    const float inv = 1.0f / sqrtf(wave_sum(y.x * y.x + y.y * y.y) + 1.0e-6f);
+    const float inv = __builtin_amdgcn_rsqf(wave_sum(y.x * y.x + y.y * y.y) + 1.0e-6f);
     float z[2] = {y.x * inv * kTLRaise, y.y * inv * kTLRaise};
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -286,11 +317,13 @@ __global__ void __launch_bounds__(kWave* kTLPrepWaves) tree_linear_prep_kernel(T
     const bool is_q = u < p.lk_n, is_k = !is_q && u < 2 * p.lk_n;
     const int h = is_q ? u : (is_k ? u - p.lk_n : u - 2 * p.lk_n);
     const int c = u * kTL + 2 * lane;
-    float w[8];
+    ConvTaps taps;
     float2 x[4];
-    conv_weights(p, c, w);
-    conv_window(p, conv_history(p), i, c, [&](int r) { return static_cast<int>(static_cast<int8_t>(p.links.words[r / 4] >> 8 * (r % 4))); }, x);
-    const float2 y = conv_silu(x, w);
+    taps.load_weights(p, c);
+    const int have = path_window(
+        p, i, c, [&](int r) { return static_cast<int>(static_cast<int8_t>(p.links.words[r / 4] >> 8 * (r % 4))); }, x);
+    if (have < 4) taps.load_past(p, c);
+    const float2 y = conv_silu(x, have, taps, *p.pos0 & 1);
     if (!is_q && !is_k) {
         *reinterpret_cast<float2*>(ws.v + (static_cast<size_t>(h) * rows + i) * kTL + 2 * lane) = y;
         return;
@@ -311,8 +344,8 @@ struct RowsSmem {
 inline size_t rows_lds(int nodes) { return sizeof(RowsSmem) + static_cast<size_t>(4) * fast_rows(nodes) * kTLLd * 2; }
 
 // ALONE: up to 16 rows, without the first launch: each block convolves its own key head's rows and its own columns of v,
-// 16 times over in all, which costs less than a launch and its round trip: with 16 / 32 heads 1 row 5.0 us (two launches
-// 7.6), 6 rows 6.6 (8.3), a chain of 16 9.3 (9.8).
+// 16 times over in all, which costs less than a launch and its round trip: with 16 / 32 heads 1 row 4.7 us (two launches
+// 7.6), 6 rows 5.9 (8.3), a chain of 16 8.5 (9.8).
 constexpr int kTLAlone = 16;
 template <bool ALONE>
 __global__ void __launch_bounds__(kWave* kTLWaves, 2) tree_linear_rows_kernel(TreeLinearLaunch p) {
@@ -343,36 +376,35 @@ __global__ void __launch_bounds__(kWave* kTLWaves, 2) tree_linear_rows_kernel(Tr
     double L;
     float beta;
     if constexpr (ALONE) {
-        const float* history = conv_history(p);
         // this wave's rows of q (even waves) or k, 4 apart; v eight rows a wave and the gates by the last ones
         constexpr int kRounds = kTLAlone / (kTLWaves / 2);
         const int c = ((wid & 1) * p.lk_n + kh) * kTL + 2 * lane;
+        ConvTaps taps;
         float2 x[kRounds][4];
-        float w[8];
-        conv_weights(p, c, w);
+        int have[kRounds] = {};
+        taps.load_weights(p, c);
+        taps.load_past(p, c);
+        const int up = parent_in<kTLAlone / 4>(p.links, lane);  // (of the first 16 lanes' rows)
 #pragma unroll
         for (int u = 0; u < kRounds; ++u)
             if (const int i = wid / 2 + u * (kTLWaves / 2); i < n)
-                conv_window(p, history, i, c, [&](int r) { return static_cast<int>(static_cast<int8_t>(p.links.words[r / 4] >> 8 * (r % 4))); }, x[u]);
+                have[u] = path_window(p, i, c, [&](int r) { return __builtin_amdgcn_readlane(up, r); }, x[u]);
+        const bool odd = *p.pos0 & 1;
         if (const int t = kTLWaves - 1 - wid; 8 * t < n) {
             const int i = min(8 * t + lane / 8, n - 1), at = 2 * (lane % 8), vc = (2 * p.lk_n + vh) * kTL + j0 + at;
+            ConvTaps vtaps;
             float2 xv[4];
-            float wv[8];
-            conv_weights(p, vc, wv);
-            conv_window(p, history, i, vc, [&](int r) {  // (a row of its own per lane: the words as scalars)
-                uint32_t word = p.links.words[0];
-#pragma unroll
-                for (int b = 1; b < kTLAlone / 4; ++b) word = r / 4 == b ? p.links.words[b] : word;
-                return static_cast<int>(static_cast<int8_t>(word >> 8 * (r % 4)));
-            }, xv);
-            *reinterpret_cast<float2*>(&v_own[i][at]) = conv_silu(xv, wv);
+            vtaps.load_weights(p, vc);
+            vtaps.load_past(p, vc);
+            const int vhave = path_window(p, i, vc, [&](int r) { return parent_in<kTLAlone / 4>(p.links, r); }, xv);
+            *reinterpret_cast<float2*>(&v_own[i][at]) = conv_silu(xv, vhave, vtaps, odd);
         }
         if (wid == kTLWaves - 3) row_gates(p, vh, L_own, beta_own);
 #pragma unroll
         for (int u = 0; u < kRounds; ++u)
             if (const int i = wid / 2 + u * (kTLWaves / 2); i < n) {
                 h2 hi, lo;
-                unit_split(conv_silu(x[u], w), hi, lo);
+                unit_split(conv_silu(x[u], have[u], taps, odd), hi, lo);
                 _Float16* out = ops + (static_cast<size_t>(wid & 1) * 2 * rows + i) * kTLLd + 2 * lane;
                 *reinterpret_cast<h2*>(out) = hi;
                 *reinterpret_cast<h2*>(out + rows * kTLLd) = lo;
