@@ -467,7 +467,8 @@ XQHIP_API int xqhip_linear_attn_scan_ws(const float* mixed, const float* a, cons
  * state stays as it is), the lm_head's logits go to xqhip_spec_verify, and
  * xqhip_tree_keep moves the rows on the accepted path together: cache slots
  * *pos0 .. *pos0 + count - 1, and the rows over which xqhip_linear_attn_scan
- * then advances each linear-attention state. */
+ * then advances each linear-attention state.  No call's outputs may overlap
+ * its inputs. */
 #define XQHIP_TREE_MAX 64
 typedef struct xqhip_tree {
     int32_t nodes;                   /* rows, 1 .. XQHIP_TREE_MAX                  */
@@ -529,8 +530,7 @@ XQHIP_API int xqhip_kv_read(const xqhip_kv* kv, int first, int count, int out_ty
  * does not see never reaches it, infinities and NaN included.  q, gate:
  * [tokens][q_stride], gate may be NULL (no gate); out: [tokens][out_stride].
  * Scores, weights and sums are held to fp32 accuracy.  The cache must hold the
- * rows: slots past its capacity are not read.  out overlaps no input (rows that
- * meet infinities are computed a second time).  workspace: 16-byte aligned, of
+ * rows: slots past its capacity are not read.  workspace: 16-byte aligned, of
  * workspace_bytes >= xqhip_tree_attention_workspace_bytes(...), no
  * initialisation; calls that can overlap need one each.  nq / nkv <= 8. */
 XQHIP_API size_t xqhip_tree_attention_workspace_bytes(int nq, int nkv, int head_dim, int tokens);

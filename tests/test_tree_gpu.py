@@ -287,7 +287,8 @@ def test_tree_attention(kind, nq, nkv, hd, T, pos0):
 
 
 @KINDS
-@pytest.mark.parametrize("nq,nkv,hd,T,pos0", [(32, 8, 128, 1, 5), (32, 8, 128, 65, 0), (32, 8, 128, 130, 70),
+@pytest.mark.parametrize("nq,nkv,hd,T,pos0", [(32, 8, 128, 1, 5), (32, 8, 128, 3, 40), (32, 8, 128, 8, 300), (16, 4, 256, 2, 31),
+                                              (32, 8, 128, 65, 0), (32, 8, 128, 130, 70),
                                               (16, 4, 256, 100, 3), (16, 4, 256, 300, 513), (6, 3, 64, 70, 9)])
 def test_chunk_attention(kind, nq, nkv, hd, T, pos0):
     rng = np.random.default_rng(T + pos0)
@@ -510,6 +511,58 @@ def test_attention_offsets_past_32_bits():
             assert np.abs(got[t, h] - want).max() <= 1e-4  # scores up to 8 times those of the other tests
     for b in bufs:
         b.free()
+
+
+def test_cache_offsets_past_32_bits():
+    """The last rows of an 8-bit cache of 5.4 GB a side: written, read back, moved together."""
+    L, nq, nkv, hd, cap = xb.hip(), 20, 20, 256, 1 << 20
+    rng = np.random.default_rng(15)
+    bufs = [xb.DeviceBuffer(cap * nkv * hd) for _ in range(2)] + [xb.DeviceBuffer(cap * nkv * 4) for _ in range(2)]
+    kv = xb.Kv(xb.KV_I8, nkv, hd, cap, *(b.ptr for b in bufs))
+    x = rng.normal(0, 1, (3, (nq + 2 * nkv) * hd)).astype(np.float32)
+    src, q, norm = dev(x), xb.DeviceBuffer(3 * nq * hd * 4), dev(np.ones(hd, np.float32))
+    at = lambda f: ctypes.c_void_p(src.ptr.value + 4 * f)  # noqa: E731
+    pos = i32(cap - 3)
+    xb.ck(L.xqhip_attn_prep_kv(at(0), at(nq * hd), at((nq + nkv) * hd), 0, nq, 0, norm.ptr, norm.ptr, EPS, None, pos.ptr,
+                               ctypes.byref(xb.tree([-1, 0, 0])), 3, x.shape[1], nq * hd, q.ptr, None, ctypes.byref(kv), None))
+    codes, scales = to.quantise(x[:, (nq + nkv) * hd:].reshape(3, nkv, hd))
+    want = codes.astype(np.float32) * scales[..., None]
+
+    def back():
+        out = dev(np.zeros((3, nkv, hd), np.float32))
+        xb.ck(L.xqhip_kv_read(ctypes.byref(kv), cap - 3, 3, xb.F32, None, out.ptr, None))
+        return out.download(np.float32, want.size).reshape(want.shape)
+
+    assert np.array_equal(back(), want)
+    sets = xb.rows([(b.ptr, w, cap, pos.ptr) for b, w in zip(bufs, (nkv * hd, nkv * hd, nkv * 4, nkv * 4))])
+    xb.ck(L.xqhip_tree_keep(sets, 4, i32(0, 2).ptr, i32(2).ptr, 2, None))
+    assert np.array_equal(back(), want[[0, 2, 2]])
+    for b in bufs:
+        b.free()
+
+
+@KINDS
+def test_attention_on_two_streams_at_once(kind):
+    """Calls in flight together, each with its own workspace: the outputs of calls one after the other."""
+    L, rng = xb.hip(), np.random.default_rng(16)
+    nq, nkv, hd, n = 32, 8, 128, 32 * 128
+    cases = []
+    for T, pos0 in ((1, 9000), (64, 5000)):
+        cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, pos0)
+        par = to.random_tree(rng, T)
+        want = attend(cache, q, gate, pos0, par, pad=0)
+        size, s = L.xqhip_tree_attention_workspace_bytes(nq, nkv, hd, T), ctypes.c_void_p()
+        xb.ck(L.xqhip_stream_create(ctypes.byref(s)))
+        cases.append((cache, dev(q), dev(gate), xb.tree(par), T, i32(pos0), dev(np.zeros((T, n), np.float32)), dev(np.zeros(size, np.uint8)),
+                      size, s, want))
+    xb.ck(L.xqhip_device_synchronize())
+    for _ in range(20):
+        for cache, q, gate, tree, T, pos, out, ws, size, s, _want in cases:
+            xb.ck(L.xqhip_tree_attention(q.ptr, gate.ptr, cache.ref, nq, ctypes.byref(tree), T, n, pos.ptr, out.ptr, n, ws.ptr, size, s))
+    for _cache, _q, _gate, _tree, T, _pos, out, _ws, _size, s, want in cases:
+        xb.ck(L.xqhip_stream_synchronize(s))
+        assert np.array_equal(out.download(np.float32, T * n).reshape(want.shape), want)
+        xb.ck(L.xqhip_stream_destroy(s))
 
 
 @KINDS
