@@ -395,6 +395,25 @@ def test_attention_of_several_chunks_per_wave(kind, nq, nkv, hd, T, pos0):
 
 
 @KINDS
+@pytest.mark.parametrize("nq,nkv,T,pos0,tree", [(8, 2, 64, 3000, True), (8, 2, 33, 4097, True), (16, 2, 16, 900, True),
+                                                (2, 2, 130, 50, False), (32, 8, 600, 65, False), (3, 1, 50, 6000, True)])
+def test_attention_over_a_cache_that_can_get_long(kind, nq, nkv, T, pos0, tree):
+    """Caches of 40000 positions; the last of the rows' values infinite in one dim, for those that see it."""
+    rng = np.random.default_rng(T + pos0)
+    k, v = (rng.normal(0, 1, (pos0 + T, nkv, 128)) for _ in range(2))
+    q, gate = (rng.normal(0, 1, (T, nq, 128)).astype(np.float32) for _ in range(2))
+    par = to.random_tree(rng, T) if tree else None
+    see = to.path_masks(par) if tree else np.tril(np.ones((T, T), bool))
+    cache = Cache(kind, nkv, 128, 40000, k, v)
+    want = to.attention(q, gate, *(x[:pos0 + T] for x in cache.values()), pos0, see)
+    assert np.abs(attend(cache, q, gate, pos0, par) - want).max() <= 3e-5
+    if kind == xb.KV_F16:
+        v[pos0 + T - 1, :, 9] = np.inf
+        got = attend(Cache(kind, nkv, 128, 40000, k, v), q, gate, pos0, par)
+        assert np.abs(got[:-1] - want[:-1]).max() <= 3e-5 and not np.isfinite(got[-1, :, 9]).any()
+
+
+@KINDS
 @pytest.mark.parametrize("hd,nkv,edge", [(128, 8, 256), (256, 4, 128)])
 @pytest.mark.parametrize("T", [1, 4, 6])
 def test_attention_around_a_split_of_its_own(kind, hd, nkv, edge, T):

@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(256) tree_attn_row_kernel(TreeAttnLaunch p) {
 //   rows).  What bounds it: the cache's bytes in long contexts (one row after
 //   120000 positions of an 8-bit cache, 8 heads: 246 MB in 56 us, 4.4 TB/s), a
 //   chain of a launch's latencies in short ones (4 rows at position 0: 8 us).
-// tree_attn_wide_kernel: 64 columns.  What bounds it: the two products' two
+// tree_attn_wide_kernel: 64 columns, or 128.  What bounds it: the two products' two
 //   passes each and, beside them, the weights' exponentials and splits, which
 //   issue in turn with the MFMAs (64 rows after 131000 positions of an 8-bit
 //   cache, 32 / 8 heads: 2.75e11 operations in 320 us, 0.86 PFLOP/s).  500 rows
@@ -1052,15 +1052,21 @@ bool tree_attn_supported(int nq, int nkv, int head_dim) {
 // The columns of a call's blocks.  Few rows are bound by latency and bytes, where the narrow kernel's waves run apart:
 // 4 rows of 4 heads after 8100 positions 12.7 us in 16 columns, 14.7 in 32, 16.4 in the wide kernel's 64; 8 rows 15.7
 // in 32, 17.4 in 64.
-static int tree_cols(int group, int tokens) {
+// With 128 columns each key and value is staged (8-bit codes converted) for four column tiles instead of two, but there
+// are half as many row tiles, and so twice the splits to join: 64 rows after 131000 positions of an 8-bit cache 320 us
+// (64 columns 352 on the same card), 512 rows after 16000 318 (345), 64 rows after 8000 36.3 (34.7), 500 rows after 3584
+// of an fp16 cache 81.4 (79.9).  How long the context is only the device knows; a cache that can hold kFar positions is
+// taken for one that does.
+constexpr int kFar = 1 << 15;
+static int tree_cols(int group, int hd, int tokens, bool far) {
     const int cols = tokens * group;
-    return cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
+    return cols <= 16 ? 16 : cols <= 32 ? 32 : far && cols >= 128 && hd == 128 ? 128 : 64;
 }
 // Row tiles, and key splits that give every CU a block.  Twice or half as many blocks: one row after 8100 positions 11.8 us
 // (16.0, 13.0), 64 rows after 131000 319 (325, 517), 128 rows after 2000 24.8 (34.6, 29.5); half as many is better only
 // where there is next to no context (256 rows at position 0 16.5, 13.5).
-static TreeGrid tree_grid(int nq, int nkv, int tokens) {
-    const int T = tree_cols(nq / nkv, tokens) / (nq / nkv);
+static TreeGrid tree_grid(int nq, int nkv, int hd, int tokens, bool far) {
+    const int T = tree_cols(nq / nkv, hd, tokens, far) / (nq / nkv);
     const int tiles = (tokens + T - 1) / T;
     const int64_t blocks = static_cast<int64_t>(tiles) * nkv;
     return TreeGrid{tiles, static_cast<int>(std::min<int64_t>(kTreeMaxSplits, std::max<int64_t>(1, 256 / blocks)))};
@@ -1068,13 +1074,13 @@ static TreeGrid tree_grid(int nq, int nkv, int tokens) {
 
 size_t tree_attn_workspace_bytes(int nq, int nkv, int head_dim, int tokens) {
     if (head_dim != 128 && head_dim != 256) return 16;
-    const TreeGrid g = tree_grid(nq, nkv, tokens);
-    return g.splits == 1 ? 16 : static_cast<size_t>(g.splits) * tokens * nq * (head_dim + 2) * sizeof(float);
+    const int splits = std::max(tree_grid(nq, nkv, head_dim, tokens, false).splits, tree_grid(nq, nkv, head_dim, tokens, true).splits);
+    return splits == 1 ? 16 : static_cast<size_t>(splits) * tokens * nq * (head_dim + 2) * sizeof(float);
 }
 
 template <typename F, int HD, bool I8, typename Kernel>
 static hipError_t launch_tree(const TreeAttnLaunch& p, Kernel kernel, hipStream_t s) {
-    const TreeGrid g = tree_grid(p.nq, p.kv.nkv, p.tokens);
+    const TreeGrid g = tree_grid(p.nq, p.kv.nkv, HD, p.tokens, p.kv.capacity >= kFar);
     if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                            static_cast<int>(F::kLds));
         e != hipSuccess)
@@ -1104,10 +1110,13 @@ static hipError_t launch_narrow(const TreeAttnLaunch& p, hipStream_t s) {
 template <int HD, bool I8>
 static hipError_t launch_tree_heads(const TreeAttnLaunch& p, hipStream_t s) {
     constexpr int KS = HD == 128 ? 8 : 4;
-    switch (tree_cols(p.nq / p.kv.nkv, p.tokens)) {
+    switch (tree_cols(p.nq / p.kv.nkv, HD, p.tokens, p.kv.capacity >= kFar)) {
         case 16: return launch_narrow<HD, I8, KS, true>(p, s);
         case 32: return launch_narrow<HD, I8, KS, false>(p, s);
-        default: return launch_wide<HD, I8, 2, KS / 2>(p, s);
+        case 64: return launch_wide<HD, I8, 2, KS / 2>(p, s);
+        default:
+            if constexpr (HD == 128) return launch_wide<HD, I8, 4, KS / 4>(p, s);
+            return hipErrorInvalidValue;  // (128 columns are for 128 dims)
     }
 }
 
@@ -1117,7 +1126,7 @@ hipError_t launch_tree_attn(const TreeAttnLaunch& p, hipStream_t s) {
     const bool al = ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.gate) |
                       reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0 && p.q_stride % 4 == 0 && p.out_stride % 4 == 0 &&
                     ((reinterpret_cast<uintptr_t>(p.kv.k) | reinterpret_cast<uintptr_t>(p.kv.v)) & 3u) == 0;
-    const bool in32 = p.q_stride < 1 << 22 && p.out_stride < 1 << 22;  // offsets within a block's (at most 64) rows
+    const bool in32 = p.q_stride < 1 << 21 && p.out_stride < 1 << 21;  // offsets within a block's (at most 128) rows
     const bool kv32 = static_cast<int64_t>(p.kv.nkv) * hd * 2 * 256 < int64_t(1) << 31;  // ... and its keys
     if (al && in32 && kv32 && hd == 128) return p.kv.i8 ? launch_tree_heads<128, true>(p, s) : launch_tree_heads<128, false>(p, s);
     if (al && in32 && kv32 && hd == 256) return p.kv.i8 ? launch_tree_heads<256, true>(p, s) : launch_tree_heads<256, false>(p, s);
