@@ -289,7 +289,7 @@ def test_tree_attention(kind, nq, nkv, hd, T, pos0):
 @KINDS
 @pytest.mark.parametrize("nq,nkv,hd,T,pos0", [(32, 8, 128, 1, 5), (32, 8, 128, 3, 40), (32, 8, 128, 8, 300), (16, 4, 256, 2, 31),
                                               (32, 8, 128, 65, 0), (32, 8, 128, 130, 70),
-                                              (16, 4, 256, 100, 3), (16, 4, 256, 300, 513), (6, 3, 64, 70, 9)])
+                                              (32, 8, 128, 1030, 21), (16, 4, 256, 100, 3), (16, 4, 256, 300, 513), (6, 3, 64, 70, 9)])
 def test_chunk_attention(kind, nq, nkv, hd, T, pos0):
     rng = np.random.default_rng(T + pos0)
     cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, pos0)

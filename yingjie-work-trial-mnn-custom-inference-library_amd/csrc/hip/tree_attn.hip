@@ -1053,20 +1053,23 @@ bool tree_attn_supported(int nq, int nkv, int head_dim) {
 // 4 rows of 4 heads after 8100 positions 12.7 us in 16 columns, 14.7 in 32, 16.4 in the wide kernel's 64; 8 rows 15.7
 // in 32, 17.4 in 64.
 // With 128 columns each key and value is staged (8-bit codes converted) for four column tiles instead of two, but there
-// are half as many row tiles, and so twice the splits to join: 64 rows after 131000 positions of an 8-bit cache 320 us
-// (64 columns 352 on the same card), 512 rows after 16000 318 (345), 64 rows after 8000 36.3 (34.7), 500 rows after 3584
-// of an fp16 cache 81.4 (79.9).  How long the context is only the device knows; a cache that can hold kFar positions is
-// taken for one that does.
+// are half as many row tiles.  Where those still give every CU a block: 2048 rows after 2000 positions 229 us (64 columns
+// 262), 1024 after 4000 177 (189), after none 45.5 (43.3).  Where they take splits that have to be joined it depends on the
+// context: 64 rows after 131000 positions of an 8-bit cache 320 us (352 on the same card), 512 after 16000 318 (345), 64
+// after 8000 36.3 (34.7), 512 after none 27 (18).  How long it is only the device knows; a cache that can hold kFar
+// positions is taken for one that does.
 constexpr int kFar = 1 << 15;
-static int tree_cols(int group, int hd, int tokens, bool far) {
-    const int cols = tokens * group;
-    return cols <= 16 ? 16 : cols <= 32 ? 32 : far && cols >= 128 && hd == 128 ? 128 : 64;
+static int tree_cols(int nq, int nkv, int hd, int tokens, bool far) {
+    const int group = nq / nkv, cols = tokens * group, T = 128 / group;
+    if (cols <= kTTile) return cols <= 16 ? 16 : 32;
+    const bool full = static_cast<int64_t>((tokens + T - 1) / T) * nkv >= 256;
+    return (far || full) && cols >= 128 && hd == 128 ? 128 : 64;
 }
 // Row tiles, and key splits that give every CU a block.  Twice or half as many blocks: one row after 8100 positions 11.8 us
 // (16.0, 13.0), 64 rows after 131000 319 (325, 517), 128 rows after 2000 24.8 (34.6, 29.5); half as many is better only
 // where there is next to no context (256 rows at position 0 16.5, 13.5).
 static TreeGrid tree_grid(int nq, int nkv, int hd, int tokens, bool far) {
-    const int T = tree_cols(nq / nkv, hd, tokens, far) / (nq / nkv);
+    const int T = tree_cols(nq, nkv, hd, tokens, far) / (nq / nkv);
     const int tiles = (tokens + T - 1) / T;
     const int64_t blocks = static_cast<int64_t>(tiles) * nkv;
     return TreeGrid{tiles, static_cast<int>(std::min<int64_t>(kTreeMaxSplits, std::max<int64_t>(1, 256 / blocks)))};
@@ -1110,7 +1113,7 @@ static hipError_t launch_narrow(const TreeAttnLaunch& p, hipStream_t s) {
 template <int HD, bool I8>
 static hipError_t launch_tree_heads(const TreeAttnLaunch& p, hipStream_t s) {
     constexpr int KS = HD == 128 ? 8 : 4;
-    switch (tree_cols(p.nq / p.kv.nkv, HD, p.tokens, p.kv.capacity >= kFar)) {
+    switch (tree_cols(p.nq, p.kv.nkv, HD, p.tokens, p.kv.capacity >= kFar)) {
         case 16: return launch_narrow<HD, I8, KS, true>(p, s);
         case 32: return launch_narrow<HD, I8, KS, false>(p, s);
         case 64: return launch_wide<HD, I8, 2, KS / 2>(p, s);
