@@ -25,8 +25,8 @@
 // distribution over 2^18 tokens is 2^-18, and the sampled token is the one
 // whose share the random number falls into.  What bounds it: the logits are read
 // once; the exponentials' fp64 work (15 operations a logit) takes about as long
-// as the memory and half hides behind it (40 rows of 248320 logits: 14.7 us for
-// 39.7 MB, 2.7 TB/s); the walk is a chain of a dozen steps that wait for each
+// as the memory and half hides behind it (40 rows of 248320 logits: 15 us for
+// 39.7 MB, 2.6 TB/s); the walk is a chain of a dozen steps that wait for each
 // other (11 to 13 us for 6 as for 40 rows).
 #include <algorithm>
 
@@ -180,75 +180,68 @@ __device__ __forceinline__ bool aligned_rows(const float* base, int64_t ld) {
     return (reinterpret_cast<uintptr_t>(base) & 15u) == 0 && ld % 4 == 0;
 }
 
-// One row's pieces NP blockIdx.x + 0 .. NP - 1.  Each wave takes its own quarter's maximum and sum, so that no wave waits
-// for another before the end.
-template <bool GREEDY, int NP>
+// One piece of a row.  Each wave takes its own quarter's maximum and sum, so that no wave waits for another before the end.
+// (With the walk 64 rows of 248320 logits take 32.4 us, 40 rows 26.2; two pieces a block 34.4 and 26.0, blocks that go from
+// piece to piece with the next one's loads under way 32.3 and 25.6.)
+template <bool GREEDY>
 __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyLaunch p, int pieces) {
     constexpr int kWaves = kStatThreads / kWave;
-    __shared__ Stat part[NP][kWaves];
-    __shared__ uint64_t best[NP][kWaves];
-    const int node = blockIdx.y, wid = threadIdx.x / kWave;
+    __shared__ Stat part[kWaves];
+    __shared__ uint64_t best[kWaves];
+    const int node = blockIdx.y, piece = blockIdx.x, v0 = piece * kPiece, wid = threadIdx.x / kWave;
     const VerifyWs ws = verify_ws(p.ws, p.nodes, p.vocab);
+    float x[kPer / 4][4];
+    load_piece(p.logits + node * p.ld, p.vocab, v0, aligned_rows(p.logits, p.ld), -INFINITY, x);
     const double scale = p.inv_t * kLog2e;
-    const bool al = aligned_rows(p.logits, p.ld);
-    float x[NP][kPer / 4][4];
+    if constexpr (GREEDY) {
+        uint64_t key = 0;
 #pragma unroll
-    for (int n = 0; n < NP; ++n)
-        load_piece(p.logits + node * p.ld, p.vocab, (static_cast<int>(blockIdx.x) * NP + n) * kPiece, al, -INFINITY, x[n]);
+        for (int u = 0; u < kPer / 4; ++u)
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-        const int v0 = (static_cast<int>(blockIdx.x) * NP + n) * kPiece;
-        if constexpr (GREEDY) {
-            uint64_t key = 0;
+            for (int e = 0; e < 4; ++e) key = u64_max(key, argmax_key(x[u][e], static_cast<uint32_t>(at_of(v0, u) + e)));
+        key = wave_max_u64(key);
+        if ((threadIdx.x & (kWave - 1)) == 0) best[wid] = key;
+    } else {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kPer / 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = fmaxf(m, x[u][e]);
+        m = wave_max(m);
+        double sum = 0.0;
+        // (fp64 operations are what this pass waits for: the clamp in fp32, one multiply-add for the exponent.
+        // Logits at the clamp, minus infinity among them, add 2^-1000 of the maximum: nothing.)
+        const float low = m - static_cast<float>(1000.0 / scale);
+        const double off = m * scale;
+        if (m > -INFINITY && m < INFINITY && low < m) {  // wave-uniform
 #pragma unroll
             for (int u = 0; u < kPer / 4; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) key = u64_max(key, argmax_key(x[n][u][e], static_cast<uint32_t>(at_of(v0, u) + e)));
-            key = wave_max_u64(key);
-            if ((threadIdx.x & (kWave - 1)) == 0) best[n][wid] = key;
-        } else {
-            float m = -INFINITY;
+                for (int e = 0; e < 4; ++e) sum += exp2_f64(fma(static_cast<double>(fmaxf(x[u][e], low)), scale, -off));
+        } else if (m > -INFINITY) {
 #pragma unroll
             for (int u = 0; u < kPer / 4; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) m = fmaxf(m, x[n][u][e]);
-            m = wave_max(m);
-            double sum = 0.0;
-            // (fp64 operations are what this pass waits for: the clamp in fp32, one multiply-add for the exponent.
-            // Logits at the clamp, minus infinity among them, add 2^-1000 of the maximum: nothing.)
-            const float low = m - static_cast<float>(1000.0 / scale);
-            const double off = m * scale;
-            if (m > -INFINITY && m < INFINITY && low < m) {  // wave-uniform
-#pragma unroll
-                for (int u = 0; u < kPer / 4; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum += exp2_f64(fma(static_cast<double>(fmaxf(x[n][u][e], low)), scale, -off));
-            } else if (m > -INFINITY) {
-#pragma unroll
-                for (int u = 0; u < kPer / 4; ++u)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum += weight_of(x[n][u][e], m, scale);
-            }
-            sum = wave_sum_f64(sum);
-            if ((threadIdx.x & (kWave - 1)) == 0) part[n][wid] = Stat{sum, m, 0};
+                for (int e = 0; e < 4; ++e) sum += weight_of(x[u][e], m, scale);
         }
+        sum = wave_sum_f64(sum);
+        if ((threadIdx.x & (kWave - 1)) == 0) part[wid] = Stat{sum, m, 0};
     }
     __syncthreads();
-    const int piece = static_cast<int>(blockIdx.x) * NP + static_cast<int>(threadIdx.x);
-    if (threadIdx.x >= NP || piece >= pieces) return;
+    if (threadIdx.x != 0) return;
     Stat r{0.0, -INFINITY, 0};
     if constexpr (GREEDY) {
         uint64_t key = 0;
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) key = u64_max(key, best[threadIdx.x][i]);
+        for (int i = 0; i < kWaves; ++i) key = u64_max(key, best[i]);
         r.m = float_from_order_key(static_cast<uint32_t>(key >> 32));
         r.arg = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key));
     } else {
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) r.m = fmaxf(r.m, part[threadIdx.x][i].m);
+        for (int i = 0; i < kWaves; ++i) r.m = fmaxf(r.m, part[i].m);
 #pragma unroll
         for (int i = 0; i < kWaves; ++i)
-            if (part[threadIdx.x][i].m > -INFINITY) r.sum += part[threadIdx.x][i].sum * weight_of(part[threadIdx.x][i].m, r.m, scale);
+            if (part[i].m > -INFINITY) r.sum += part[i].sum * weight_of(part[i].m, r.m, scale);
     }
     ws.stat[node * static_cast<size_t>(pieces) + piece] = r;
     if (piece == 0 && node == 0) *ws.done = 0;
@@ -598,18 +591,11 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyLaunch 
 
 hipError_t launch_verify(const VerifyLaunch& p, hipStream_t s) {
     const int pieces = verify_pieces(p.vocab);
-    // two pieces a block where one each would not be resident at once (8 blocks a CU): 40 rows of 248320 logits 14.7 us, one
-    // piece each 15.1 to 16.3; 6 rows one each 4.3
-    const bool two = static_cast<int64_t>(pieces) * p.nodes > 2048;
-    const dim3 grid(two ? (pieces + 1) / 2 : pieces, p.nodes);
-    if (p.inv_t > 0.0f && two)
-        hipLaunchKernelGGL((verify_stats_kernel<false, 2>), grid, dim3(kStatThreads), 0, s, p, pieces);
-    else if (p.inv_t > 0.0f)
-        hipLaunchKernelGGL((verify_stats_kernel<false, 1>), grid, dim3(kStatThreads), 0, s, p, pieces);
-    else if (two)
-        hipLaunchKernelGGL((verify_stats_kernel<true, 2>), grid, dim3(kStatThreads), 0, s, p, pieces);
+    const dim3 grid(pieces, p.nodes);
+    if (p.inv_t > 0.0f)
+        hipLaunchKernelGGL(verify_stats_kernel<false>, grid, dim3(kStatThreads), 0, s, p, pieces);
     else
-        hipLaunchKernelGGL((verify_stats_kernel<true, 1>), grid, dim3(kStatThreads), 0, s, p, pieces);
+        hipLaunchKernelGGL(verify_stats_kernel<true>, grid, dim3(kStatThreads), 0, s, p, pieces);
     if (p.draft)
         for (int r = 1; r < p.max_children; ++r)
             hipLaunchKernelGGL(verify_rest_kernel, dim3(pieces, p.nodes), dim3(kStatThreads), 0, s, p, r);
