@@ -163,17 +163,15 @@ __device__ __forceinline__ double wave_scan(double v) {
     return v + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? b : c);
 }
 
-// sum over the block in a fixed order; every thread gets it
+// sum over the block's up to 16 waves in a fixed order; each wave's first 16 lanes get it
 template <int THREADS>
 __device__ __forceinline__ double block_sum_f64(double v, double* red) {
+    const int lane = threadIdx.x & (kWave - 1);
     v = wave_sum_f64(v);
     __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x / kWave] = v;
+    if (lane == 0) red[threadIdx.x / kWave] = v;
     __syncthreads();
-    double t = 0.0;
-#pragma unroll
-    for (int i = 0; i < THREADS / kWave; ++i) t += red[i];
-    return t;
+    return row_sum_f64(lane < THREADS / kWave ? red[lane] : 0.0);
 }
 
 __device__ __forceinline__ bool aligned_rows(const float* base, int64_t ld) {
@@ -557,24 +555,15 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyLaunch 
     const double s4 = (w[0] + w[1]) + (w[2] + w[3]), upto = wave_scan(s4);
     if (lane == kWave - 1) red[wid] = upto;
     __syncthreads();
-    // each wave has the waves' sums; the first that passes `want` has the token (rounding can leave none: the last token
-    // with a weight then)
-    double pre = before_s, end = before_s;
-    const double want = want_s;
-    int first_wave = kWalkThreads / kWave, last_wave = -1;
-#pragma unroll
-    for (int i = 0; i < kWalkThreads / kWave; ++i) {
-        const double part = red[i];
-        if (i == wid) pre = end;
-        end += part;
-        if (part > 0.0) {
-            last_wave = i;
-            if (end > want && first_wave > i) first_wave = i;
-        }
-    }
-    const bool to_the_end = ends || first_wave == kWalkThreads / kWave;
-    if (wid != (to_the_end ? last_wave : first_wave)) return;
-    pre += upto - s4;
+    // each wave has the waves' sums, one a lane; the first that passes `want` has the token (rounding can leave none: the
+    // last token with a weight then)
+    constexpr int kWaves = kWalkThreads / kWave;
+    const double want = want_s, part = lane < kWaves ? red[lane] : 0.0, end = before_s + wave_scan(part);
+    const uint64_t holds = __builtin_amdgcn_ballot_w64(part > 0.0), passes = __builtin_amdgcn_ballot_w64(part > 0.0 && end > want);
+    const bool to_the_end = ends || !passes;
+    const int owner = to_the_end ? 63 - __builtin_clzll(holds | 1) : __builtin_ctzll(passes);
+    if (wid != owner || !holds) return;
+    double pre = readlane_f64(end - part, wid) + (upto - s4);
     int found = -1, at_least = -1;  // first token past `want`, last token with a weight
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
