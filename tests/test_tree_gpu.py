@@ -800,6 +800,47 @@ def test_verify_in_a_graph():
     xb.ck(L.xqhip_stream_destroy(s))
 
 
+# ---- LDS ------------------------------------------------------------------------
+def filled():
+    xb.ck(xb.hip().xqhip_lds_fill(math.nan, None))
+
+
+@KINDS
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_reads_no_lds_that_it_has_not_written(kind, hd):
+    rng = np.random.default_rng(hd)
+    for nq, nkv, T, pos0 in ((8, 2, 1, 0), (8, 2, 3, 300), (6, 2, 7, 90), (8, 2, 21, 700), (8, 1, 64, 40)):
+        cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, pos0)
+        par = to.random_tree(rng, T)
+        want = attend(cache, q, gate, pos0, par)
+        filled()
+        assert np.array_equal(attend(cache, q, gate, pos0, par), want)
+
+
+@pytest.mark.parametrize("dk", [64, 128])
+def test_linear_tree_reads_no_lds_that_it_has_not_written(dk):
+    rng = np.random.default_rng(dk)
+    for n in (1, 2, 7, 16, 17, 50):
+        c, par = linear_case(rng, 2, dk, 4, dk, 4, n), to.random_tree(rng, n)
+        want, _ = run_linear(c, 2, dk, 4, dk, 4, 1, par)
+        filled()
+        assert np.array_equal(run_linear(c, 2, dk, 4, dk, 4, 1, par)[0], want)
+
+
+@pytest.mark.parametrize("mode", ["point", "probs"])
+@pytest.mark.parametrize("inv_t", [0.0, 1.0])
+def test_verify_reads_no_lds_that_it_has_not_written(mode, inv_t):
+    rng = np.random.default_rng(5)
+    for n, vocab in ((1, 50), (9, 5000), (33, 9000)):
+        par = to.random_tree(rng, n, 3)
+        logits = rng.normal(0, 2, (n, vocab)).astype(np.float32)
+        draft = np.full((n, vocab), 1.0 / vocab, np.float32) if mode == "probs" else None
+        args = (logits, par, rng.integers(0, vocab, n).tolist(), draft, inv_t, rng.random(n) * 0.5, 0.7)
+        want = run_verify(*args)
+        filled()
+        assert run_verify(*args) == want
+
+
 # ---- a step of them together ----------------------------------------------------
 @KINDS
 def test_a_step_over_a_tree(kind):
