@@ -181,7 +181,7 @@ struct TreeBlock {
     static constexpr int kQuads = HD / 4;                 // float4 of an output row
     static constexpr int kMergeCols = kThreads / kQuads;  // columns per pass of the merge
     static constexpr int kPasses = kCols / kMergeCols;
-    static constexpr size_t kOutBytes = static_cast<size_t>(kCols) * KS * (kLdo + 2) * 4;
+    static constexpr size_t kOutBytes = static_cast<size_t>(kCols) * (KS * (kLdo + 3) + 1) * 4;
     static constexpr int kLdv = HD + 16;  // halves per V row: the 4 rows of a transposed read in distinct banks
     static_assert(kPasses * kThreads == kCols * kQuads, "merge");
     static_assert(kOutBytes >= tree_row_lds(kTreeMaxGroup, HD) * 4, "the general form runs in it");
@@ -362,6 +362,23 @@ __device__ __forceinline__ void add_scaled(float4& r, float f, float4 v) {
     r.w += f * v.w;
 }
 
+__device__ __forceinline__ float4 as_float4(u32x4 v) {
+    return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+}
+// writes the quad at `out`; whether its row has to be computed again
+__device__ __forceinline__ bool write_quad(float4 r, float L, bool gated, float4 gt, float* out) {
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
+    if (gated) {
+        y.x *= sigmoid_dev(gt.x);
+        y.y *= sigmoid_dev(gt.y);
+        y.z *= sigmoid_dev(gt.z);
+        y.w *= sigmoid_dev(gt.w);
+    }
+    *reinterpret_cast<float4*>(out) = y;
+    return !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
+}
+
 constexpr float kRaise = 6.0f;  // weights are held times 2^kRaise
 constexpr float kSlack = 6.0f;  // the max may outgrow the reference by 2^kSlack before it is moved
 
@@ -403,47 +420,53 @@ __device__ __forceinline__ void finish_columns(const TreeAttnLaunch& p, const Tr
         if (g == 0 && part == 0) *reinterpret_cast<float2*>(Ml + at * 2) = make_float2(m, l);
     }
     __syncthreads();
+    // a thread per column: the factors of its waves' outputs, and their sum
+    float* Fl = Ml + KS * F::kCols * 2;  // [waves][columns]
+    float* Ll = Fl + KS * F::kCols;      // [columns] the sums
+    auto row_of = [&](int c, int& hc, int& tc) {
+        hc = static_cast<int>(c * inv_t >> 16);
+        tc = c - hc * T;
+        return hc < group && tc < ntok;
+    };
+    if (threadIdx.x < F::kCols) {
+        const int c = threadIdx.x;
+        float M = -INFINITY, L = 0.0f;
+        for (int s = 0; s < waves; ++s) M = fmaxf(M, Ml[(c + s * F::kCols) * 2]);
+        for (int s = 0; s < waves; ++s) {
+            const float f = __builtin_amdgcn_exp2f(Ml[(c + s * F::kCols) * 2] - M);
+            L += f * Ml[(c + s * F::kCols) * 2 + 1];
+            Fl[c + s * F::kCols] = f;
+        }
+        Ll[c] = L;
+        int hc, tc;
+        if (!whole && row_of(c, hc, tc)) {
+            float2* pm = reinterpret_cast<float2*>(p.ws + static_cast<size_t>(grid.splits) * p.tokens * p.nq * HD) +
+                         static_cast<size_t>(sp) * p.tokens * p.nq;
+            pm[static_cast<size_t>(t0 + tc) * p.nq + kh * group + hc] = make_float2(M, L);
+        }
+    }
+    __syncthreads();
+    const int c0 = threadIdx.x / F::kQuads, d = 4 * (threadIdx.x % F::kQuads);
+    float4 r[F::kPasses] = {};
+    for (int s = 0; s < waves; ++s)
+#pragma unroll
+        for (int u = 0; u < F::kPasses; ++u) {
+            const int c = c0 + u * F::kMergeCols + s * F::kCols;
+            add_scaled(r[u], Fl[c], *reinterpret_cast<const float4*>(Ol + c * F::kLdo + d));
+        }
     float* po = p.ws + static_cast<size_t>(sp) * p.tokens * p.nq * HD;
-    float2* pm = reinterpret_cast<float2*>(p.ws + static_cast<size_t>(grid.splits) * p.tokens * p.nq * HD) +
-                 static_cast<size_t>(sp) * p.tokens * p.nq;
     bool bad = false;
 #pragma unroll
     for (int u = 0; u < F::kPasses; ++u) {
-        const int c = threadIdx.x / F::kQuads + u * F::kMergeCols, d = 4 * (threadIdx.x % F::kQuads);
-        const int hc = static_cast<int>(c * inv_t >> 16), tc = c - hc * T;
-        if (hc >= group || tc >= ntok) continue;
-        const int at = tc * p.out_stride + (kh * group + hc) * HD + d;
-        float ml[KS], M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-            if (s < waves) {  // block-uniform
-                ml[s] = Ml[(c + s * F::kCols) * 2];
-                M = fmaxf(M, ml[s]);
-            }
-        float4 r = float4{};
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-            if (s < waves) {
-                const float f = __builtin_amdgcn_exp2f(ml[s] - M);
-                L += f * Ml[(c + s * F::kCols) * 2 + 1];
-                add_scaled(r, f, *reinterpret_cast<const float4*>(Ol + (c + s * F::kCols) * F::kLdo + d));
-            }
+        int hc, tc;
+        if (!row_of(c0 + u * F::kMergeCols, hc, tc)) continue;
         if (!whole) {
             const size_t row = static_cast<size_t>(t0 + tc) * p.nq + kh * group + hc;
-            *reinterpret_cast<float4*>(po + row * HD + d) = r;
-            if (d == 0) pm[row] = make_float2(M, L);
+            *reinterpret_cast<float4*>(po + row * HD + d) = r[u];
             continue;
         }
-        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-        bad |= !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
-        float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
-        if (p.gate) {
-            y.x *= sigmoid_dev(__uint_as_float(gt[u][0]));
-            y.y *= sigmoid_dev(__uint_as_float(gt[u][1]));
-            y.z *= sigmoid_dev(__uint_as_float(gt[u][2]));
-            y.w *= sigmoid_dev(__uint_as_float(gt[u][3]));
-        }
-        *reinterpret_cast<float4*>(p.out + static_cast<size_t>(t0) * p.out_stride + at) = y;
+        bad |= write_quad(r[u], Ll[c0 + u * F::kMergeCols], p.gate, as_float4(gt[u]),
+                          p.out + static_cast<size_t>(t0 + tc) * p.out_stride + (kh * group + hc) * HD + d);
     }
     if (!whole) return;
     if (bad) *redo = 1;
@@ -920,22 +943,6 @@ struct TreeParts {
 __device__ __forceinline__ TreeParts tree_parts(const TreeAttnLaunch& p, const TreeGrid& grid, int hd) {
     const uint32_t rows = static_cast<uint32_t>(p.tokens) * p.nq, all = grid.splits * rows;
     return TreeParts{buf_rsrc(p.ws, all * hd * 4u), buf_rsrc(p.ws + static_cast<size_t>(all) * hd, all * 8u), rows};
-}
-__device__ __forceinline__ float4 as_float4(u32x4 v) {
-    return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
-}
-// writes the quad at `out`; whether its row has to be computed again
-__device__ __forceinline__ bool write_quad(float4 r, float L, bool gated, float4 gt, float* out) {
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
-    if (gated) {
-        y.x *= sigmoid_dev(gt.x);
-        y.y *= sigmoid_dev(gt.y);
-        y.z *= sigmoid_dev(gt.z);
-        y.w *= sigmoid_dev(gt.w);
-    }
-    *reinterpret_cast<float4*>(out) = y;
-    return !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
 }
 
 // The splits' partial outputs of one row and kv head joined, normalised and gated (nothing to do where one split held
