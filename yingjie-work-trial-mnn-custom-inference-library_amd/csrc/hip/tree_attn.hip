@@ -168,8 +168,8 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 constexpr int kTTile = 32;  // keys and columns of an MFMA tile
 constexpr int kTreeMaxSplits = 64;
-// A narrow call's splits hold two tiles or more: 8 rows of 256 dims after 2000 positions 16.4 us (one tile 18.3, four
-// 17.3), after 540 14.2 (14.7, 16.4); a wave each of one block, where that is all, needs no join.
+// A narrow call's splits hold two tiles or more: 8 rows of 256 dims after 540 positions 13.0 us (one tile 13.6, four 14.7),
+// after 2000 15.6 (18.6, 15.4); a wave each of one block, where that is all, needs no join.
 constexpr int kMinTiles = 2;
 
 // Columns, waves and output rows of a block: CT column tiles x KS key waves.
