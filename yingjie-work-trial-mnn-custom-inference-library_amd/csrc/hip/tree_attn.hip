@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(256) tree_attn_row_kernel(TreeAttnLaunch p) {
 //   chain of a launch's latencies in short ones (4 rows at position 0: 8 us).
 // tree_attn_wide_kernel: 64 columns, or 128.  What bounds it: the two products'
 //   two passes each and, beside them, the weights' exponentials and splits, which
-//   issue in turn with the MFMAs (64 rows after 131000 positions of an 8-bit
+//   issue in turn with the MFMAs (46 and 49 % of the time; 64 rows after 131000 positions of an 8-bit
 //   cache, 32 / 8 heads: 2.75e11 operations in 295 us, 0.93 PFLOP/s; 500 rows
 //   after 3584 80 us, of an fp16 cache 72: converting the codes is the
 //   difference).  A wave with two column tiles of its own read K and V half as
