@@ -770,6 +770,34 @@ def test_verify_of_rows_at_their_limits(mode):
                     assert run_verify(*args) == to.verify(*args), (tokens, ua, us, inv_t)
 
 
+@pytest.mark.parametrize("mode", ["point", "probs"])
+@pytest.mark.parametrize("inv_t,top", [
+    (1e3, 20), (1e4, 20), (1e5, 20), (1e6, 20), (1e7, 20), (1e8, 20), (3e8, 20), (1e12, 20), (3e38, 20), (1e6, 300), (1e7, 300),
+    (1e6, 2000), (1.0, 2.0**24), (100.0, 2.0**24), (0.25, 3e9), (1.0, 3e9), (1.0, 3e38), (1e8, -20), (1e-37, 20), (1e-37, 3e9),
+    (2e-36, 20), (1e-44, 20)])
+def test_verify_temperatures_and_logits_of_every_size(inv_t, top, mode):
+    """The maximum behind the first 4096 tokens, a tie or a close second beside it, others at minus infinity, and a
+    vocabulary that fills no whole number of 4096s."""
+    rng = np.random.default_rng(int(abs(top)) % 1000 + len(mode))
+    inv_t, vocab, par = float(np.float32(inv_t)), 12001, [-1, 0, 0, 1, 1, 3]
+    n = len(par)
+    for trial in range(8):
+        logits = (rng.normal(0, 2.5, (n, vocab)) * max(1.0, abs(top) / 64)).astype(np.float32)
+        logits = np.minimum(logits - logits.max(), 0).astype(np.float32) * np.float32(0.5) + np.float32(top - abs(top) / 4)
+        if trial % 2:
+            logits[:, rng.random(vocab) < 0.3] = -np.inf
+        best, second, other = (rng.permutation(3800)[:n] + at for at in (4100, 8200, 0))
+        rows = np.arange(n)
+        logits[rows, best] = top
+        logits[rows, second] = np.float32(top - float(rng.random()) * min(2 / inv_t, abs(top) / 8)) if trial % 3 else top
+        draft = np.zeros((n, vocab), np.float32)
+        draft[rows, best], draft[rows, second], draft[rows, other] = 0.4375, 0.3125, 0.25
+        tokens = [0] + [int((best, second, other)[int(rng.integers(3))][p]) for p in par[1:]]
+        ua = (rng.random(n) * (0.4 if trial < 4 else 1.0)).astype(np.float32)
+        args = (logits, par, tokens, draft if mode == "probs" else None, inv_t, ua, np.float32(rng.random()))
+        assert run_verify(*args) == to.verify(*args), trial
+
+
 def test_verify_in_a_graph():
     L = xb.hip()
     rng = np.random.default_rng(10)
