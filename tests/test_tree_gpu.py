@@ -690,6 +690,24 @@ def test_linear_rows_that_are_not_finite_stay_on_their_paths():
     assert np.isnan(got[hit]).all() and np.array_equal(got[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("what", ["a", "b"])
+@pytest.mark.parametrize("dk,n", [(128, 9), (128, 30), (64, 20)])
+def test_linear_gates_that_are_not_numbers_stay_on_their_paths(dk, n, what):
+    """A row's NaN decay or beta of one head reaches the row and those below it in that head, as it does in a scan, and
+    nothing else."""
+    rng = np.random.default_rng(n)
+    lk, lv, ks, row, head = 2, 4, 4, 4, 2
+    c = linear_case(rng, lk, dk, lv, dk, ks, n)
+    par = to.random_tree(rng, n, 5)
+    clean, _ = run_linear(c, lk, dk, lv, dk, ks, 1, par)
+    c[what][row, head] = np.nan
+    got, _ = run_linear(c, lk, dk, lv, dk, ks, 1, par)
+    hit = np.zeros((n, lv, dk), bool)
+    hit[to.path_masks(par)[:, row], head] = True
+    hit = hit.reshape(n, -1)
+    assert hit.any() and np.isnan(got[hit]).all() and np.array_equal(got[~hit], clean[~hit])
+
+
 # ---- verification ---------------------------------------------------------------
 def run_verify(logits, par, tokens, draft, inv_t, ua, us, ld=None, stream=None):
     n, vocab = logits.shape

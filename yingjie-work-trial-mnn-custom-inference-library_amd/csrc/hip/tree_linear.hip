@@ -8,7 +8,8 @@
 // which is S_i = g_i S_parent + k_i delta_i^T unrolled (custom_model.cpp:
 // 1074-1096 per row).  L in 64 bits: differences of sums over a long path lose
 // the digits that its length costs.  (Log gates below -1000 count as -1000: the
-// decay is 0 either way, and differences stay finite.)
+// decay is 0 either way, and differences stay finite.  NaN stays NaN, as in the
+// single-token step.)
 #include <algorithm>
 
 #include "xqhip_common.hpp"
@@ -30,6 +31,11 @@ __host__ __device__ inline LinWs lin_ws(const TreeLinearLaunch& p) {
     return LinWs{p.ws, p.ws + nk, p.ws + 2 * nk};
 }
 }  // namespace
+
+__device__ __forceinline__ float log_gate(const TreeLinearLaunch& p, int vh, float a) {
+    const float g = -expf(p.a_log[vh]) * softplus_dev(a + p.dt_bias[vh]);
+    return g < -1000.0f ? -1000.0f : g;  // (fmaxf would take -1000 for NaN)
+}
 
 // conv1d + SiLU of one head's channels of one row over its path (then the
 // history), q and k heads L2-normalised.  One wave per (row, head).
@@ -83,7 +89,7 @@ __global__ void __launch_bounds__(256) tree_delta_kernel(TreeLinearLaunch p) {
     if (tid < n) {
         const float a = p.a[static_cast<size_t>(tid) * p.stride + vh], b = p.b[static_cast<size_t>(tid) * p.stride + vh];
         beta[tid] = sigmoid_dev(b);
-        L[tid] = fmaxf(-expf(p.a_log[vh]) * softplus_dev(a + p.dt_bias[vh]), -1000.0f);
+        L[tid] = log_gate(p, vh, a);
     }
     __syncthreads();
     double sum = 0.0;
@@ -216,8 +222,7 @@ __device__ __forceinline__ void row_gates(const TreeLinearLaunch& p, int vh, dou
     const bool on = lane < p.nodes;
     const size_t at = static_cast<size_t>(on ? lane : 0) * p.stride + vh;
     const float a = p.a[at], b = p.b[at];
-    const float log_gate = fmaxf(-expf(p.a_log[vh]) * softplus_dev(a + p.dt_bias[vh]), -1000.0f);
-    const double mine = on ? static_cast<double>(log_gate) * 1.44269504088896340736 : 0.0;
+    const double mine = on ? static_cast<double>(log_gate(p, vh, a)) * 1.44269504088896340736 : 0.0;
     // path sums by doubling: before step s a lane has the sum of the last s rows of its path
     int up = on ? static_cast<int8_t>(p.links.words[lane / 4] >> 8 * (lane % 4)) : -1;
     double sum = mine;
