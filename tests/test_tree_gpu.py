@@ -368,6 +368,36 @@ def test_scores_of_every_size(kind, hd, scale):
 
 
 @KINDS
+@pytest.mark.parametrize("nq,nkv,hd,T", [(8, 2, 128, 3), (8, 2, 128, 10), (8, 2, 256, 10), (8, 2, 128, 40), (4, 2, 64, 10)])
+@pytest.mark.parametrize("scale", [1e3, 3e4])
+def test_scores_that_single_out_a_key(kind, nq, nkv, hd, T, scale):
+    """Every output of scores so large that a row's best key takes all its weight.  A score is off by E = (hd 2^-24 sum
+    |q_i k_i| + 2^-23 max|q| sum |k_i|) / sqrt(hd) at most (an fp32 sum of hd terms, q's 22 bits).  Where the best
+    leads by 2 E + 20 the others have 400 e^-20 = 1e-6 of the weight between them and the output is the best key's
+    value; elsewhere it lies between the values of the keys that are as near."""
+    rng = np.random.default_rng(hd + T)
+    pos0 = 333
+    cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, pos0)
+    q = (q * np.float32(scale)).astype(np.float32)
+    par = to.random_tree(rng, T)
+    see = to.path_masks(par)
+    k, v = cache.values()
+    got = attend(cache, q, gate, pos0, par) * (1 + np.exp(-gate.astype(np.float64)))
+    alone = 0
+    for t in range(T):
+        rows = np.concatenate([np.arange(pos0), pos0 + np.flatnonzero(see[t])])
+        for h in range(nq):
+            kh, qh = k[rows, h // (nq // nkv)], q[t, h].astype(np.float64)
+            vh, s = v[rows, h // (nq // nkv)], kh @ qh / math.sqrt(hd)
+            off = (hd * 2**-24 * (np.abs(kh) @ np.abs(qh)).max() + 2**-23 * np.abs(qh).max() * np.abs(kh).sum(1).max()) / math.sqrt(hd)
+            near = vh[s >= s.max() - 2 * off - 20]
+            alone += len(near) == 1
+            tol = 3e-5 * (1 + np.exp(-gate[t, h].astype(np.float64)))
+            assert (got[t, h] >= near.min(0) - tol).all() and (got[t, h] <= near.max(0) + tol).all(), (t, h)
+    assert alone >= 0.7 * T * nq
+
+
+@KINDS
 def test_attention_without_a_gate_and_unaligned_rows(kind):
     rng = np.random.default_rng(11)
     cache, q, _ = attention_case(rng, kind, 8, 2, 128, 6, 77)
