@@ -505,9 +505,9 @@ typedef struct xqhip_kv {
 
 /* xqhip_attn_prep_batch for a cache of either type and rows of a tree: per
  * query head (q, gate) split, q and k RMSNorm, partial RoPE at position *pos0 +
- * depth (tree == NULL: *pos0 + t, and any number of tokens), k and v written
- * to slot *pos0 + t of `kv` (custom_model.cpp:301-370, 673-753).  tokens: the
- * tree's nodes.  rope_cs: `kv->capacity` positions of xqhip_rope_table.
+ * depth (tree == NULL: *pos0 + t), k and v written to slot *pos0 + t of `kv`
+ * (custom_model.cpp:301-370, 673-753).  tokens: the tree's nodes (tree == NULL:
+ * up to 65535).  rope_cs: `kv->capacity` positions of xqhip_rope_table.
  * gate_out may be NULL when gated == 0.  A token whose slot or position lies
  * outside the cache's capacity writes no cache row, and NaN as its q. */
 XQHIP_API int xqhip_attn_prep_kv(const float* q_src, const float* k_src, const float* v_src, int gated, int nq,
@@ -525,14 +525,22 @@ XQHIP_API int xqhip_kv_read(const xqhip_kv* kv, int first, int count, int out_ty
 /* Attention of the rows over a cache of either type:
  *   out[t] = softmax_s(q[t] k[s] / sqrt(head_dim)) v[s] * sigmoid(gate[t])
  * over s in [0, *pos0) and the rows of the tree's mask (slot *pos0 + j for bit
- * j; tree == NULL: the rows 0 .. t, any number of tokens: a prompt chunk).  A
+ * j; tree == NULL: the rows 0 .. t of up to 65535 tokens: a prompt chunk).  A
  * row that sees nothing, or scores of minus infinity only, gives 0; what a row
  * does not see never reaches it, infinities and NaN included.  q, gate:
  * [tokens][q_stride], gate may be NULL (no gate); out: [tokens][out_stride].
  * Scores, weights and sums are held to fp32 accuracy.  The cache must hold the
  * rows: slots past its capacity are not read.  workspace: 16-byte aligned, of
- * workspace_bytes >= xqhip_tree_attention_workspace_bytes(...), no
- * initialisation; calls that can overlap need one each.  nq / nkv <= 8. */
+ * workspace_bytes >= xqhip_tree_attention_workspace_bytes(...) for this call's
+ * tokens (fewer tokens can take more: one workspace for several lengths has
+ * the largest of their sizes), no initialisation; calls that can overlap need
+ * one each.  Limits, with g = nq / nkv: g <= 8, head_dim <= 1024 and g * (2 *
+ * head_dim + 67) <= 16384; the size is 0 for shapes and token counts that are refused.
+ * Made for heads of 128 and 256 dims, q, gate and out 16-byte aligned with
+ * strides that are multiples of 4.  Other calls give the same results in a
+ * general form that reads each row's whole context in one block per kv head
+ * (one row after 8100 positions 2 to 4 ms instead of 13 us); so does a row
+ * beside which an infinity or NaN lies in an fp16 cache's values. */
 XQHIP_API size_t xqhip_tree_attention_workspace_bytes(int nq, int nkv, int head_dim, int tokens);
 XQHIP_API int xqhip_tree_attention(const float* q, const float* gate, const xqhip_kv* kv, int nq,
                                    const xqhip_tree* tree, int tokens, int q_stride, const int32_t* pos0, float* out,

@@ -106,6 +106,27 @@ def test_attention_workspace():
             refused(attend(kv=kv(nkv=nkv, hd=hd), nq=nq, tokens=n, qs=1 << 14, os=1 << 14, size=size - 1), "workspace")
 
 
+@pytest.mark.parametrize("group,hd", [(8, 990), (7, 1024), (4, 1024), (1, 1024)])
+def test_attention_up_to_its_largest_heads(group, hd):
+    """group (2 head_dim + 67) floats within 64 KiB: accepted by the size's check and refused for the workspace alone;
+    one dim more, or a group of more than eight, is not (heads have up to 1024 dims)."""
+    need = xb.hip().xqhip_tree_attention_workspace_bytes
+    o = dict(nq=2 * group, qs=1 << 14, os=1 << 14)
+    assert group * (2 * hd + 67) <= 16384 and need(2 * group, 2, hd, 3) == 16
+    refused(attend(kv=kv(hd=hd), size=15, **o), "workspace")
+    assert need(2 * group, 2, hd + 1, 3) == 0
+    refused(attend(kv=kv(hd=hd + 1), **o), "heads")
+    assert need(18, 2, 64, 3) == 0
+
+
+def test_attention_sizes_for_several_lengths():
+    """A prompt chunk whose blocks fill the card needs less than a few rows do: each call is checked for its own."""
+    need = xb.hip().xqhip_tree_attention_workspace_bytes
+    small, large = need(32, 8, 128, 1024), need(32, 8, 128, 64)
+    assert small < large
+    refused(attend(kv=kv(nkv=8), nq=32, tokens=64, qs=4096, os=4096, size=small), "workspace")
+
+
 def linear(**o):
     a = dict(m=P, a=P, b=P, stride=4096, hist=P, pos=P, w=P, al=P, dt=P, state=P, lk=2, dk=128, lv=4, dv=128, ks=4,
              tree=xb.tree([-1, 0, 0]), out=P, os=512, ws=P, size=1 << 40)
