@@ -579,10 +579,17 @@ XQHIP_API int xqhip_linear_attn_tree(const float* mixed, const float* a, const f
  * p(0) + .. + p(i) > u_sample * sum.  (Should a rejection leave nothing, p
  * itself is sampled.)  Greedy: the child whose token is the row's argmax (ties
  * to the lowest index) is accepted, the last token is that argmax.  The
- * outcome is distributed as sampling from the target alone.  NaN logits count
- * as minus infinity; a row with no finite or plus-infinite logit accepts
- * nothing and samples -1.  Tokens outside [0, vocab) are never accepted.  Sums
- * and probabilities are held in 64 bits.
+ * outcome is distributed as sampling from the target alone where a row's
+ * children were drawn from its q independently of each other (a token may then
+ * come twice; siblings that were drawn to differ, a top-k of q say, are not),
+ * or, without q, chosen in any way that the random numbers here have no part
+ * in.  NaN logits count as minus infinity; a row with no finite or
+ * plus-infinite logit accepts nothing and samples -1.  Tokens outside [0,
+ * vocab) are never accepted, and a rejected child takes q off whatever its
+ * token: a padding row of a sampled step with draft probabilities continues a
+ * row without drafted children whose draft row holds zeros, which changes
+ * nothing.  Sums and probabilities are held in 64 bits, the exponentials to
+ * 1e-11 of their value.
  * out_count: rows kept, row 0 included = new tokens, 1 .. nodes.  out_path
  * [nodes]: the kept rows, then -1.  out_tokens [nodes]: the new tokens (the
  * kept drafts', then the sampled one), then -1.  The tree has one root.

@@ -846,6 +846,29 @@ def test_verify_temperatures_and_logits_of_every_size(inv_t, top, mode):
         assert run_verify(*args) == to.verify(*args), trial
 
 
+@pytest.mark.parametrize("inv_t", [0.0, 1.0])
+@pytest.mark.parametrize("mode", ["point", "probs"])
+def test_verify_of_a_padded_tree(mode, inv_t):
+    """Rows of token -1 below the leaves, their draft rows zeros: the outcome of the tree without them."""
+    rng = np.random.default_rng(17)
+    vocab, par = 5000, [-1, 0, 0, 1, 1, 2]
+    n, padded = len(par), par + [3, 4, 5, 6, 3, 9]
+    for trial in range(20):
+        logits = rng.normal(0, 2.5, (len(padded), vocab)).astype(np.float32)
+        draft = np.exp(logits + rng.normal(0, 0.7, logits.shape))
+        draft = (draft / draft.sum(1, keepdims=True)).astype(np.float32)
+        draft[3:] = 0
+        if trial % 2:
+            tokens = [0] + [int(np.argsort(-logits[p])[int(rng.integers(0, 3))]) for p in par[1:]]
+        else:
+            tokens = [0] + [int(rng.choice(vocab, p=draft[p].astype(np.float64) / draft[p].sum(dtype=np.float64))) for p in par[1:]]
+        ua, us = (rng.random(len(padded)) * 0.5).astype(np.float32), np.float32(rng.random())
+        ua[n:] = 0
+        probs = draft if mode == "probs" else None
+        want = to.verify(logits[:n], par, tokens, None if probs is None else probs[:n], inv_t, ua[:n], us)
+        assert run_verify(logits, padded, tokens + [-1] * (len(padded) - n), probs, inv_t, ua, us) == want, trial
+
+
 def test_verify_in_a_graph():
     L = xb.hip()
     rng = np.random.default_rng(10)
