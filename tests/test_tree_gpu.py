@@ -287,6 +287,21 @@ def test_tree_attention(kind, nq, nkv, hd, T, pos0):
 
 
 @KINDS
+@pytest.mark.parametrize("nq,nkv,hd,T,pos0", [(16, 2, 990, 5, 70), (14, 2, 1024, 3, 64), (2, 2, 1024, 9, 63), (3, 1, 1, 6, 65)])
+def test_attention_of_the_largest_and_smallest_heads(kind, nq, nkv, hd, T, pos0):
+    """A score, an fp32 sum of up to 1024 terms, is off by 1024 2^-24 sum |q_i k_i| / sqrt(hd) <= 1024 2^-24 0.64 sqrt(1024) =
+    1.3e-3 at most, and an output, an average of |v| <= 6, by 2 x 6 times that.  Roundings of either sign add up to sqrt(1024)
+    2^-24 of partial sums of sqrt(1024), 2e-6 of a score; for the norm ten times that is allowed."""
+    rng = np.random.default_rng(hd + T)
+    cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, pos0)
+    par = to.random_tree(rng, T)
+    k, v = cache.values()
+    want = to.attention(q, gate, k, v, pos0, to.path_masks(par))
+    got = attend(cache, q, gate, pos0, par)
+    assert np.abs(got - want).max() <= 1.6e-2 and np.linalg.norm(got - want) <= 2e-5 * np.linalg.norm(want)
+
+
+@KINDS
 @pytest.mark.parametrize("nq,nkv,hd,T,pos0", [(32, 8, 128, 1, 5), (32, 8, 128, 3, 40), (32, 8, 128, 8, 300), (16, 4, 256, 2, 31),
                                               (32, 8, 128, 65, 0), (32, 8, 128, 130, 70),
                                               (32, 8, 128, 1030, 21), (16, 4, 256, 100, 3), (16, 4, 256, 300, 513), (6, 3, 64, 70, 9)])
