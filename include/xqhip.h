@@ -467,8 +467,9 @@ XQHIP_API int xqhip_linear_attn_scan_ws(const float* mixed, const float* a, cons
  * state stays as it is), the lm_head's logits go to xqhip_spec_verify, and
  * xqhip_tree_keep moves the rows on the accepted path together: cache slots
  * *pos0 .. *pos0 + count - 1, and the rows over which xqhip_linear_attn_scan
- * then advances each linear-attention state.  No call's outputs may overlap
- * its inputs. */
+ * then advances each linear-attention state (the scan takes position and count
+ * as host integers: *out_count is copied back before it).  No call's outputs
+ * may overlap its inputs. */
 #define XQHIP_TREE_MAX 64
 typedef struct xqhip_tree {
     int32_t nodes;                   /* rows, 1 .. XQHIP_TREE_MAX                  */

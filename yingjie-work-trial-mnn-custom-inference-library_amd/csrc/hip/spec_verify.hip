@@ -27,7 +27,8 @@
 // once; the exponentials' fp64 work (15 operations a logit) takes about as long
 // as the memory and half hides behind it (40 rows of 248320 logits: 15 us for
 // 39.7 MB, 2.6 TB/s); the walk is a chain of a dozen steps that wait for each
-// other (11 to 13 us for 6 as for 40 rows).
+// other (11 to 13 us for 6 as for 40 rows).  Greedy calls take 7.6 us for 6 rows
+// and 16.0 for 40, walk and all.
 #include <algorithm>
 
 #include "xqhip_common.hpp"
@@ -179,8 +180,8 @@ __device__ __forceinline__ bool aligned_rows(const float* base, int64_t ld) {
 }
 
 // One piece of a row.  Each wave takes its own quarter's maximum and sum, so that no wave waits for another before the end.
-// (With the walk 64 rows of 248320 logits take 32.4 us, 40 rows 26.2; two pieces a block 34.4 and 26.0, blocks that go from
-// piece to piece with the next one's loads under way 32.3 and 25.6.)
+// (With the walk, when it was chosen, 64 rows of 248320 logits took 32.4 us and 40 rows 26.2, now 31.7 and 25.1; two pieces
+// a block 34.4 and 26.0, blocks that go from piece to piece with the next one's loads under way 32.3 and 25.6.)
 template <bool GREEDY>
 __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyLaunch p, int pieces) {
     constexpr int kWaves = kStatThreads / kWave;

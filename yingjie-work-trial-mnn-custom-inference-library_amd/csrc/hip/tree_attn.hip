@@ -150,26 +150,29 @@ __global__ void __launch_bounds__(256) tree_attn_row_kernel(TreeAttnLaunch p) {
 // happens a sum is not finite or the weights sum to 0: the block that writes
 // such an output computes its rows again by attend_row.
 //
+// Times here and below are of whole calls, one behind the other in a graph, with
+// 32 / 8 heads of 128 dims where nothing else is said.
+//
 // tree_attn_narrow_kernel: calls of up to 16 or 32 columns (a decode step's few
 //   rows).  What bounds it: the cache's bytes in long contexts (one row after
-//   120000 positions of an 8-bit cache, 8 heads: 246 MB in 56 us, 4.4 TB/s), a
-//   chain of a launch's latencies in short ones (4 rows at position 0: 8 us).
+//   120000 positions of an 8-bit cache: 253 MB in 56 us, 4.5 TB/s), a chain of a
+//   launch's latencies in short ones (4 rows at position 0: 7.5 us).
 // tree_attn_wide_kernel: 64 columns, or 128.  What bounds it: the two products'
 //   two passes each and, beside them, the weights' exponentials and splits, which
-//   issue in turn with the MFMAs (46 and 49 % of the time; 64 rows after 131000 positions of an 8-bit
-//   cache, 32 / 8 heads: 2.75e11 operations in 295 us, 0.93 PFLOP/s; 500 rows
-//   after 3584 80 us, of an fp16 cache 72: converting the codes is the
-//   difference).  A wave with two column tiles of its own read K and V half as
-//   often and was slower below 100000 positions: twice the registers, half the
-//   waves.
+//   issue in turn with the MFMAs (46 and 49 % of the time; a tree of 64 rows after
+//   131000 positions of an 8-bit cache: 2.75e11 operations in the two passes,
+//   285 to 291 us, 0.95 PFLOP/s; 500 rows after 3584 81 us, of an fp16
+//   cache 70: converting the codes is the difference).  A wave with two column
+//   tiles of its own read K and V half as often and, when it was tried, was slower
+//   below 100000 positions: twice the registers, half the waves.
 // ---------------------------------------------------------------------------
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 constexpr int kTTile = 32;  // keys and columns of an MFMA tile
 constexpr int kTreeMaxSplits = 64;
-// A narrow call's splits hold two tiles or more: 8 rows of 256 dims after 540 positions 13.0 us (one tile 13.6, four 14.7),
-// after 2000 15.6 (18.6, 15.4); a wave each of one block, where that is all, needs no join.
+// A narrow call's splits hold two tiles or more: 8 rows of 16 / 4 heads of 256 dims after 540 positions 12.8 us (one tile
+// 13.5, four 14.7), after 2000 15.1 (17.7, 15.6); a wave each of one block, where that is all, needs no join.
 constexpr int kMinTiles = 2;
 
 // Columns, waves and output rows of a block: CT column tiles x KS key waves.
@@ -483,7 +486,7 @@ __device__ __forceinline__ void finish_columns(const TreeAttnLaunch& p, const Tr
 // the wave's own LDS, the next tile's K and V on their way meanwhile.
 // HALF: up to 16 columns, q's hi parts in the tile's first 16 columns and its lo parts in the others.  One MFMA then does
 // what two do, a lane and its neighbour 16 lanes on add their scores and take eight keys each, and the weights' hi and lo
-// parts go back into the two halves.  One row after 8100 positions 11.8 us, in 32 columns 14.0.
+// parts go back into the two halves.  One row after 8100 positions 11.7 us, in 32 columns 13.3.
 template <int HD, bool I8, int KS, bool HALF>
 __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) tree_attn_narrow_kernel(TreeAttnLaunch p, TreeGrid grid) {
     using F = NarrowTile<HD, I8, KS, HALF ? 16 : 32>;
@@ -1006,7 +1009,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_kernel(TreeAttn
 }
 
 // ... of up to kFewSplits splits (calls of many rows): each thread has an output's partials by itself, a block several
-// kv heads of a row.  256 rows, two splits: 16.5 us in all, with the kernel above 22.7.
+// kv heads of a row.  256 rows at position 0, two splits: 16.1 us in all, with the kernel above 22.3.
 template <typename F, int HD, bool I8>
 __global__ void __launch_bounds__(kMergeThreads) tree_attn_merge_few_kernel(TreeAttnLaunch p, TreeGrid grid, int T) {
     extern __shared__ float smem[];  // attend_row's
@@ -1059,14 +1062,15 @@ bool tree_attn_supported(int nq, int nkv, int head_dim) {
 }
 
 // The columns of a call's blocks.  Few rows are bound by latency and bytes, where the narrow kernel's waves run apart:
-// 4 rows of 4 heads after 8100 positions 12.7 us in 16 columns, 14.7 in 32, 16.4 in the wide kernel's 64; 8 rows 15.7
-// in 32, 17.4 in 64.
+// 4 rows after 8100 positions of an 8-bit cache 12.6 us in 16 columns, 14.1 in 32, 15.8 in the wide kernel's 64; 8 rows
+// 14.7 in 32, 16.5 in 64.
 // With 128 columns each key and value is staged (8-bit codes converted) for four column tiles instead of two, but there
-// are half as many row tiles.  Where those still give every CU a block: 2048 rows after 2000 positions 229 us (64 columns
-// 262), 1024 after 4000 177 (189), after none 45.5 (43.3).  Where they take splits that have to be joined it depends on the
-// context: 64 rows after 131000 positions of an 8-bit cache 320 us (352 on the same card), 512 after 16000 318 (345), 64
-// after 8000 36.3 (34.7), 512 after none 27 (18).  How long it is only the device knows; a cache that can hold kFar
-// positions is taken for one that does.
+// are half as many row tiles.  Where those still give every CU a block: 2048 rows after 2000 positions 220 us (64 columns
+// 251), 1024 after 4000 170 (180), after none 42 (38).  Where they take splits that have to be joined it depends on the
+// context: 64 rows after 131000 positions of an 8-bit cache 291 us (321), 512 after 16000 278 (304), 64 after 8000 33.9
+// (32.7), 64 after 1000 23.4 (18.6), 512 after none 27.3 (18.2); over fp16 caches the same by ratio.  How long it is only
+// the device knows; a cache that can hold kFar positions is taken for one that does.  So a cache allocated for long
+// contexts pays the larger figure of the last two cases while its context is short.
 constexpr int kFar = 1 << 15;
 static int tree_cols(int nq, int nkv, int hd, int tokens, bool far) {
     const int group = nq / nkv, cols = tokens * group, T = 128 / group;
@@ -1074,9 +1078,9 @@ static int tree_cols(int nq, int nkv, int hd, int tokens, bool far) {
     const bool full = static_cast<int64_t>((tokens + T - 1) / T) * nkv >= 256;
     return (far || full) && cols >= 128 && hd == 128 ? 128 : 64;
 }
-// Row tiles, and key splits that give every CU a block.  Twice or half as many blocks: one row after 8100 positions 11.8 us
-// (16.0, 13.0), 64 rows after 131000 319 (325, 517), 128 rows after 2000 24.8 (34.6, 29.5); half as many is better only
-// where there is next to no context (256 rows at position 0 16.5, 13.5).
+// Row tiles, and key splits that give every CU a block.  Twice or half as many blocks: one row after 8100 positions 11.7 us
+// (16.2, 12.9), 64 rows after 8000 32.7 (38.8, 43.2), after 131000 293 (304, 450), 128 rows after 2000 23.6 (34.5, 29.3);
+// half as many is better only where there is next to no context (256 rows at position 0 15.7, 13.5).
 static TreeGrid tree_grid(int nq, int nkv, int hd, int tokens, bool far) {
     const int T = tree_cols(nq, nkv, hd, tokens, far) / (nq / nkv);
     const int tiles = (tokens + T - 1) / T;

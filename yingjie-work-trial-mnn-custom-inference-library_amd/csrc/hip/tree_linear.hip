@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(256) tree_delta_kernel(TreeLinearLaunch p) {
 //
 // What bounds it: latency (a launch, rounds of loads, the steps); the bytes (the
 // state, 2 MB for 32 heads, and 128 KB a row) are 1 us.  With 16 / 32 heads: 6 rows
-// 5.9 us, a tree of 64 rows (three children a row) 14.4, a chain of 64 19.7.  Weights
+// 5.8 us, a tree of 64 rows (three children a row) 14.4, a chain of 64 19.2.  Weights
 // with decay and mask applied beforehand left the chain's step as long.
 // ---------------------------------------------------------------------------
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -349,8 +349,8 @@ struct RowsSmem {
 inline size_t rows_lds(int nodes) { return sizeof(RowsSmem) + static_cast<size_t>(4) * fast_rows(nodes) * kTLLd * 2; }
 
 // ALONE: up to 16 rows, without the first launch: each block convolves its own key head's rows and its own columns of v,
-// 16 times over in all, which costs less than a launch and its round trip: with 16 / 32 heads 1 row 4.7 us (two launches
-// 7.6), 6 rows 5.9 (8.3), a chain of 16 8.5 (9.8).
+// 16 times over in all, which costs less than a launch and its round trip: with 16 / 32 heads 1 row 4.5 us (two launches
+// 7.2), 6 rows 5.8 (7.5), a chain of 16 8.5 (9.1).
 constexpr int kTLAlone = 16;
 template <bool ALONE>
 __global__ void __launch_bounds__(kWave* kTLWaves, 2) tree_linear_rows_kernel(TreeLinearLaunch p) {
