@@ -471,6 +471,96 @@ def test_attention_around_a_split_of_its_own(kind, hd, nkv, edge, T):
         assert np.abs(attend(cache, q, gate, n - T, par) - want).max() <= 3e-5, n
 
 
+@KINDS
+@pytest.mark.parametrize("nq,nkv,hd,T,pos0,tree", [
+    (64, 64, 128, 5, 200, True), (128, 64, 128, 3, 500, True), (96, 32, 128, 9, 333, True), (300, 300, 128, 2, 70, True),
+    (40, 40, 256, 7, 150, True), (64, 64, 128, 40, 90, True), (128, 128, 256, 20, 50, True), (64, 64, 128, 150, 40, False)])
+def test_attention_of_many_heads(kind, nq, nkv, hd, T, pos0, tree):
+    """So many kv heads that few splits, or one, are left to each."""
+    rng = np.random.default_rng(nq + T)
+    cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, pos0, spare=0)
+    par = to.random_tree(rng, T) if tree else None
+    see = to.path_masks(par) if tree else np.tril(np.ones((T, T), bool))
+    want = to.attention(q, gate, *cache.values(), pos0, see)
+    got = attend(cache, q, gate, pos0, par)
+    assert np.abs(got - want).max() <= 3e-5 and np.linalg.norm(got - want) <= 5e-6 * np.linalg.norm(want)
+
+
+@KINDS
+@pytest.mark.parametrize("off", [2, 4, 8, 12])
+@pytest.mark.parametrize("hd,T", [(128, 2), (128, 7), (128, 30), (256, 3), (256, 30)])
+def test_caches_at_any_address(kind, off, hd, T):
+    """Caches that begin `off` bytes behind a 16-byte border: attention, the write, the read-back."""
+    rng = np.random.default_rng(off + T)
+    nq, nkv, pos0, rotary = 8, 2, 100, 32
+    cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, pos0, spare=T)
+    par = to.random_tree(rng, T)
+    want = to.attention(q, gate, *cache.values(), pos0, to.path_masks(par))
+    size = 1 if kind == xb.KV_I8 else 2
+    raw = cache.raw()
+
+    class Moved(Cache):
+        def __init__(self):
+            self.kind, self.shape = kind, cache.shape
+            held = [np.concatenate([np.zeros(off, np.uint8), x.view(np.uint8).ravel()]) for x in raw[:2]]
+            self.buf = [dev(held[0]), dev(held[1]), dev(raw[2]), dev(raw[3])]
+            self.kv = xb.Kv(kind, nkv, hd, cache.shape[0], *(ctypes.c_void_p(b.ptr.value + off) for b in self.buf[:2]),
+                            *(b.ptr if kind == xb.KV_I8 else None for b in self.buf[2:]))
+            self.ref = ctypes.byref(self.kv)
+
+        def codes(self, i):
+            b = self.buf[i].download(np.uint8, self.buf[i].nbytes)[off:]
+            return b.view(np.int8 if size == 1 else np.float16).reshape(self.shape)
+
+    moved = Moved()
+    assert np.abs(attend(moved, q, gate, pos0, par) - want).max() <= 3e-5
+    x = rng.normal(0, 1, (T, 2 * nq * hd + 2 * nkv * hd)).astype(np.float32)
+    prep(np.random.default_rng(1), cache, nq, rotary, pos0 + T, T, par, x=x)
+    prep(np.random.default_rng(1), moved, nq, rotary, pos0 + T, T, par, x=x)
+    raw = cache.raw()
+    for i in (0, 1):
+        assert np.array_equal(moved.codes(i), raw[i])
+    if kind == xb.KV_I8:
+        n = 2 * T * nkv * hd
+        for t, dt in ((xb.F32, np.float32), (xb.F16, np.float16)):
+            outs = [dev(np.zeros(n, dt)) for _ in range(2)]
+            xb.ck(xb.hip().xqhip_kv_read(cache.ref, pos0, 2 * T, t, None, outs[0].ptr, None))
+            xb.ck(xb.hip().xqhip_kv_read(moved.ref, pos0, 2 * T, t, None, outs[1].ptr, None))
+            a, b = (o.download(dt, n) for o in outs)
+            assert a.any() and np.array_equal(a, b)
+
+
+@KINDS
+@pytest.mark.parametrize("nq,nkv,hd,T,pos0", [(8, 2, 128, 4, 0), (8, 2, 128, 4, 900), (8, 2, 128, 30, 900), (8, 2, 128, 130, 5),
+                                              (8, 2, 256, 6, 300), (4, 2, 64, 6, 50)])
+def test_rows_that_are_not_numbers_stay_alone(kind, nq, nkv, hd, T, pos0):
+    """NaN in one row's q, and in one gate of another row: the other outputs are those without them."""
+    rng = np.random.default_rng(T + hd)
+    cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, pos0)
+    want = to.attention(q, gate, *cache.values(), pos0, np.tril(np.ones((T, T), bool)))
+    q[1, 3, 7] = np.nan
+    gate[2, 1, 5] = np.nan
+    got = attend(cache, q, gate, pos0)
+    clean = np.ones(want.shape, bool)
+    clean[1, 3], clean[2, 1, 5] = False, False
+    assert np.isnan(got[~clean]).all() and np.abs(got - want)[clean].max() <= 3e-5
+
+
+@KINDS
+@pytest.mark.parametrize("nq,nkv,hd,T", [(8, 2, 128, 3), (8, 2, 128, 40), (8, 2, 256, 20), (4, 2, 64, 9)])
+def test_chunk_past_the_capacity(kind, nq, nkv, hd, T):
+    """A prompt chunk that the cache cannot hold: its rows see the slots that are there."""
+    rng = np.random.default_rng(T)
+    cache, q, gate = attention_case(rng, kind, nq, nkv, hd, T, 50, spare=0)
+    k, v = cache.values()
+    for pos0 in (50 + T // 2, 50 + T - 1, 50 + T, 50 + T + 9):
+        held = max(0, 50 + T - pos0)
+        see = np.tril(np.ones((T, T), bool))
+        see[:, held:] = False
+        want = to.attention(q, gate, k, v, min(pos0, 50 + T), see)
+        assert np.abs(attend(cache, q, gate, pos0) - want).max() <= 3e-5
+
+
 @pytest.mark.parametrize("T", [1000, 5000])
 def test_attention_of_a_long_chunk(T):
     """Many row tiles, so that few splits are left, and a row of infinities in the middle of them."""
@@ -797,6 +887,23 @@ def test_verify(vocab, n, reach, ld, mode, inv_t):
 
 
 @pytest.mark.parametrize("mode", ["point", "probs"])
+@pytest.mark.parametrize("vocab,n,shape", [(1100003, 3, "chain"), (1 << 24, 1, "chain"), (4096, 64, "star"), (9001, 64, "star"),
+                                           (5000, 64, "chain"), (300, 33, "pairs")])
+def test_verify_of_long_rows_and_wide_trees(vocab, n, shape, mode):
+    """More than 64 pieces of a row; 63 children of one row; a path of 64; drafts that are mostly rejected."""
+    rng = np.random.default_rng(vocab % 1000 + n)
+    par = {"chain": list(range(-1, n - 1)), "star": [-1] + [0] * (n - 1), "pairs": [-1] + [(i - 1) // 2 for i in range(1, n)]}[shape]
+    for trial in range(1 if vocab > 100000 else 5):
+        logits = rng.normal(0, 2.5, (n, vocab)).astype(np.float32)
+        draft = np.exp(np.minimum(logits + rng.normal(0, 1.5, logits.shape), 12)).astype(np.float32)
+        draft = (draft / draft.sum(1, keepdims=True, dtype=np.float64)).astype(np.float32)
+        tokens = [0] + [int(np.argmax(logits[p])) if rng.random() < (0.5 if trial % 2 else 0.02) else int(rng.integers(vocab)) for p in par[1:]]
+        ua, us = (rng.random(n) * 0.3 + 0.7 * (trial > 2)).astype(np.float32), np.float32(rng.random())
+        args = (logits, par, tokens, draft if mode == "probs" else None, 1.0, ua, us)
+        assert run_verify(*args) == to.verify(*args), trial
+
+
+@pytest.mark.parametrize("mode", ["point", "probs"])
 def test_verify_of_rows_at_their_limits(mode):
     """Rows of minus infinity, NaN, plus infinity, ties; drafts outside the vocabulary, drafted twice; a draft equal to
     the target; random numbers of 0 and just below 1."""
@@ -859,6 +966,23 @@ def test_verify_temperatures_and_logits_of_every_size(inv_t, top, mode):
         ua = (rng.random(n) * (0.4 if trial < 4 else 1.0)).astype(np.float32)
         args = (logits, par, tokens, draft if mode == "probs" else None, inv_t, ua, np.float32(rng.random()))
         assert run_verify(*args) == to.verify(*args), trial
+
+
+@pytest.mark.parametrize("kids", [1, 2, 16, 30])
+@pytest.mark.parametrize("first", [0, 4097])
+def test_verify_where_rejections_leave_next_to_nothing(kids, first):
+    """Two tokens of probabilities 0.6 and 0.4 against a draft of one half each, all children the second: one after the
+    other rejected, they leave the first token with 0.1 x 2^-(kids - 1) of the row's distribution, up to 2 10^-10, and the
+    second with nothing."""
+    vocab, n = first + 2, kids + 1
+    logits = np.full((n, vocab), -np.inf, np.float32)
+    logits[:, first], logits[:, first + 1] = np.log(0.6), np.log(0.4)
+    draft = np.zeros((n, vocab), np.float32)
+    draft[:, first:] = 0.5
+    top = np.float32(1) - np.float32(2**-24)
+    for us in (0.0, 0.5, 0.7, top):
+        got = run_verify(logits, [-1] + [0] * kids, [0] + [first + 1] * kids, draft, 1.0, np.full(n, top), np.float32(us))
+        assert got == ([0], [first])
 
 
 @pytest.mark.parametrize("inv_t", [0.0, 1.0])
