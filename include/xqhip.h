@@ -619,6 +619,156 @@ typedef struct xqhip_rows {
 XQHIP_API int xqhip_tree_keep(const xqhip_rows* sets, int n_sets, const int32_t* path, const int32_t* count,
                               int max_rows, void* stream);
 
+/* ---- several sequences in one step: caches in pages ----------------------- */
+/* Decodes and prefills several sequences at once; no counterpart in the
+ * reference, whose session holds one sequence (session.cpp:304-421).  A step's
+ * rows are the new tokens of its sequences, one sequence behind the other: one
+ * row for a sequence that decodes, many for a prompt chunk.  Full-attention
+ * layers run xqhip_attn_prep_paged and xqhip_paged_attention, the lm_head's
+ * logits go to xqhip_token_logprobs where a program answers with
+ * probabilities.  No call's outputs may overlap its inputs. */
+#define XQHIP_STEP_SEQS 1024
+typedef struct xqhip_step {
+    int32_t seqs;          /* sequences, 1 .. XQHIP_STEP_SEQS                       */
+    int32_t rows;          /* rows that the activations hold, 1 .. 65535            */
+    int32_t max_rows;      /* most rows of one sequence, 1 .. rows; rows past it are
+                              left as they were                                     */
+    int32_t max_pages;     /* entries of a row of the table, max_pages * page <= 2^20 */
+    const int32_t* row0;   /* device [seqs + 1], never falling: sequence s has the rows
+                              row0[s] .. row0[s + 1] - 1 (none: it takes no part);
+                              rows from row0[seqs] on are left as they were         */
+    const int32_t* past;   /* device [seqs]: positions held before the step: row j of
+                              sequence s goes to position past[s] + j (negative: its
+                              rows have no position)                                */
+    const int32_t* table;  /* device [seqs][max_pages]: page of the positions page * i
+                              .. page * i + page - 1; entries past a sequence's
+                              positions are not read                                */
+    const int32_t* open;   /* device [seqs]: each sequence's open page (PAGES_I8: its
+                              row of k_open and v_open, another for every sequence) */
+} xqhip_step;
+
+/* Key/value cache of one full-attention layer in pages of `page` positions, in
+ * pieces of 16 bytes that are operands of the matrix cores as they lie (e = 8
+ * fp16 values or 16 codes):
+ *   k [pages][nkv][head_dim / e][page][e]    v [pages][nkv][page / e][head_dim][e]
+ * A page may stand in several sequences' tables (a prompt they share); a step
+ * writes a page for one sequence only.
+ * PAGES_F16: fp16 values (rounded from fp32).
+ * PAGES_I8: signed 8-bit codes of the fp16 values, with one fp32 scale per page
+ * and kv head ([pages][nkv]): scale = max |x| / 127 over the page's positions
+ * so far, code = 127 x / max |x| to the nearest (ties to even), value = code *
+ * scale.  When a later position raises the maximum the page's codes are taken
+ * anew from the fp16 values, which k_open and v_open ([opens][nkv][page]
+ * [head_dim]) keep of the page that a sequence's last append ended in; so a
+ * page's codes do not depend on the steps that it came in.  A scale never falls
+ * while its page is filled.  A sequence may go back (a smaller past[s]) within
+ * the page that its last append ended in, or to any page's first position.
+ * Infinities and values past fp16's range are held as fp16's largest value,
+ * values that are no numbers as 0.
+ * One step's appends to one open page must not overlap. */
+enum { XQHIP_PAGES_F16 = 0, XQHIP_PAGES_I8 = 1 };
+typedef struct xqhip_pages {
+    int32_t type;
+    int32_t nkv, head_dim; /* head_dim: a multiple of 16, up to 256; nkv up to 1024  */
+    int32_t page;          /* 32, 64 or 128                                         */
+    int32_t pages;         /* of the pool                                           */
+    int32_t opens;         /* PAGES_I8: open pages                                  */
+    void* k;               /* device, 16-byte aligned                               */
+    void* v;
+    float* k_scale;        /* PAGES_I8 only, as what follows                        */
+    float* v_scale;
+    void* k_open;          /* fp16, 16-byte aligned                                 */
+    void* v_open;
+} xqhip_pages;
+
+/* Rotation over one or several position axes: pair i (dims i and i +
+ * rotary_dim / 2 of a head) is turned by the angles of row pos[axis[i]] of the
+ * table, as applyRopeVector does with one position (custom_model.cpp:351-370).
+ * Axes are time, height and width of an image's or video's patches, say. */
+#define XQHIP_ROTARY_PAIRS 128
+typedef struct xqhip_rotary {
+    const float* cs;      /* device: xqhip_rope_table of `positions` positions       */
+    int32_t positions;
+    int32_t rotary_dim;
+    int32_t axes;         /* 1 .. 4                                                  */
+    uint8_t axis[XQHIP_ROTARY_PAIRS];
+    const int32_t* pos;   /* device [axes][rows of the step], or NULL: each row's
+                             position in its sequence on every axis                  */
+} xqhip_rotary;
+/* Host helper: sections[a] pairs for axis a, their sum rotary_dim / 2.
+ * interleaved == 0: one axis' pairs after the other's.  interleaved != 0: pair
+ * i belongs to axis a = i % axes while i < axes * sections[a], to axis 0
+ * otherwise (refused where that gives other numbers of pairs). */
+XQHIP_API int xqhip_rotary_init(const float* cs, int positions, int rotary_dim, const int32_t* sections, int axes,
+                                int interleaved, const int32_t* pos, xqhip_rotary* out);
+
+/* xqhip_attn_prep_batch for a step over several sequences: per query head (q,
+ * gate) split, q and k RMSNorm, rotation, k and v written to their positions'
+ * pages (custom_model.cpp:301-370, 673-753).  Row r reads its projections at
+ * q_src/k_src/v_src + r * src_stride and writes q and gate at r * out_stride.
+ * rotary == NULL: no rotation.  gate_out may be NULL when gated == 0 (else 0 is
+ * written there).  The normalised and rotated key is computed in 64 bits and
+ * rounded to fp32, then to fp16.  A row without a position or whose position has
+ * no page (a table entry outside [0, pages), a position past the table, an open
+ * page outside [0, opens)) or whose rotary positions lie outside the table writes no cache
+ * row, and NaN as its q. */
+XQHIP_API int xqhip_attn_prep_paged(const float* q_src, const float* k_src, const float* v_src, int gated, int nq,
+                                    const float* q_norm, const float* k_norm, float eps, const xqhip_rotary* rotary,
+                                    const xqhip_step* step, int src_stride, int out_stride, float* q_out,
+                                    float* gate_out, const xqhip_pages* kv, void* stream);
+/* The step's positions read back: row r of the outputs ([rows][nkv][head_dim] of
+ * out_type, XQHIP_F32 or XQHIP_F16: code * scale in fp32, then rounded once)
+ * holds the key and value of its position.  With row0 and past of a program's
+ * choice this reads any positions of any sequences (to move a cache, say);
+ * max_rows counts here too, `open` is not read.  k_out, v_out: either may be
+ * NULL.  Rows without a page read 0. */
+XQHIP_API int xqhip_paged_read(const xqhip_pages* kv, const xqhip_step* step, int out_type, void* k_out, void* v_out,
+                               void* stream);
+
+/* Attention of the step's rows over their sequences' pages, as they stand:
+ *   out[r] = softmax_p(q[r] k[p] / sqrt(head_dim)) v[p] * sigmoid(gate[r])
+ * row j of sequence s over the positions p = 0 .. past[s] + j.  Positions
+ * without a page (as above) are not seen; a row that sees nothing, or scores of
+ * minus infinity only, gives 0; what a row does not see never reaches it,
+ * infinities and NaN included.  q, gate: [rows][q_stride], gate may be NULL (no
+ * gate); out: [rows][out_stride].  Scores, weights and sums are held to fp32
+ * accuracy.  nq / nkv <= 16.  workspace: 16-byte aligned, of workspace_bytes >=
+ * xqhip_paged_attention_workspace_bytes(...) (0 for refused shapes), no
+ * initialisation, one size for every step; calls that can overlap need one
+ * each.  Graph-capturable: lengths, rows and tables may change between replays
+ * within seqs, rows, max_rows and max_pages. */
+XQHIP_API size_t xqhip_paged_attention_workspace_bytes(int nq, int nkv, int head_dim);
+XQHIP_API int xqhip_paged_attention(const float* q, const float* gate, const xqhip_pages* kv, int nq,
+                                    const xqhip_step* step, int q_stride, float* out, int out_stride, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens: with p = softmax(logits * inv_temperature)
+ * of a row (logits [rows][ld] of type XQHIP_F32 or XQHIP_F16, `vocab` of each),
+ *   out_logprob[r]   log p(tokens[r])
+ *   out_entropy[r]   - sum p log p
+ *   out_rank[r]      how many tokens come before tokens[r]: a larger logit, or
+ *                    the same at a lower index
+ *   out_top, out_top_logprob [rows][top]: the `top` <= XQHIP_TOP_MAX first
+ *                    tokens in that order and their log probabilities
+ * Any output may be NULL (tokens too, when neither log probabilities of them
+ * nor ranks are asked for).  The reference's only such output is the debug
+ * JSON's top logits (custom_model.cpp:1281-1338).  NaN logits count as minus
+ * infinity.  Plus infinities share the probability.  In a row that has nothing
+ * above minus infinity every token's log probability is minus infinity, the
+ * entropy 0.  Tokens of probability zero because of their logit are not listed:
+ * places of out_top that are left hold -1 and minus infinity.  A token outside
+ * [0, vocab) has log probability minus infinity and the rank -1.  Sums are held
+ * without the maximum's own term, so log probabilities near 0 keep their
+ * digits.  inv_temperature > 0.  rows <= 65535, vocab <= 2^24.  workspace:
+ * 16-byte aligned, of workspace_bytes >= xqhip_token_logprobs_workspace_bytes
+ * (...), no initialisation; calls that can overlap need one each. */
+#define XQHIP_TOP_MAX 64
+XQHIP_API size_t xqhip_token_logprobs_workspace_bytes(int rows, int vocab, int top);
+XQHIP_API int xqhip_token_logprobs(const void* logits, int type, int ld, int rows, int vocab, float inv_temperature,
+                                   const int32_t* tokens, int top, float* out_logprob, float* out_entropy,
+                                   int32_t* out_rank, int32_t* out_top, float* out_top_logprob, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
 /* One kernel of one thread that stores the device's 100 MHz realtime counter
  * (s_memrealtime) to *slot with a system-scope store; slot may be device or
  * coherent host memory (xqhip_host_alloc_coherent).  Between two kernels on a

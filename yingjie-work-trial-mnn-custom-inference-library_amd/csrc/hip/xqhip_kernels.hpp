@@ -356,4 +356,86 @@ struct VerifyLaunch {
 size_t verify_workspace_bytes(int nodes, int vocab);
 hipError_t launch_verify(const VerifyLaunch& p, hipStream_t s);
 
+// ---- a step over several sequences, caches in pages ------------------------------
+struct PagedCache {  // include/xqhip.h, xqhip_pages
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    _Float16* k_open;
+    _Float16* v_open;
+    int i8, nkv, head_dim, page, pages, opens;
+};
+struct PagedStep {  // xqhip_step
+    int seqs, rows, max_rows, max_pages;
+    const int32_t* row0;
+    const int32_t* past;
+    const int32_t* table;
+    const int32_t* open;
+};
+
+// paged_cache.hip
+struct RotaryAxes {
+    const float2* cs;    // [positions][pairs]
+    const int32_t* pos;  // [axes][rows], or nullptr
+    int positions, pairs, axes;
+    uint32_t axis[8];  // two bits per pair
+};
+struct PagedPrepLaunch {
+    const float* q_src;
+    const float* k_src;
+    const float* v_src;
+    const float* q_norm;
+    const float* k_norm;
+    float* q_out;
+    float* gate_out;
+    int gated, nq, src_stride, out_stride;
+    float eps;
+    RotaryAxes rot;
+    PagedStep step;
+    PagedCache kv;
+};
+hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s);
+
+struct PagedReadLaunch {
+    PagedCache kv;
+    PagedStep step;
+    int f16;
+    void* k_out;
+    void* v_out;
+};
+hipError_t launch_paged_read(const PagedReadLaunch& p, hipStream_t s);
+
+// paged_attn.hip
+struct PagedAttnLaunch {
+    const float* q;     // [rows][q_stride], heads [nq][hd]
+    const float* gate;  // same layout, or nullptr
+    PagedCache kv;
+    PagedStep step;
+    int nq, q_stride, out_stride;
+    float* out;
+    float* ws;  // paged_attn_workspace_bytes
+};
+size_t paged_attn_workspace_bytes(int nq, int nkv, int head_dim);
+hipError_t launch_paged_attn(const PagedAttnLaunch& p, hipStream_t s);
+
+// token_logprobs.hip
+struct LogprobsLaunch {
+    const void* logits;
+    int f16;
+    int64_t ld;
+    int rows, vocab;
+    float inv_t;
+    const int32_t* tokens;
+    int top;
+    float* out_logprob;
+    float* out_entropy;
+    int32_t* out_rank;
+    int32_t* out_top;
+    float* out_top_logprob;
+    void* ws;
+};
+size_t logprobs_workspace_bytes(int rows, int vocab, int top);
+hipError_t launch_logprobs(const LogprobsLaunch& p, hipStream_t s);
+
 }  // namespace xqhip

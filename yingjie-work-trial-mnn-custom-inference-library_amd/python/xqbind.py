@@ -72,6 +72,31 @@ class Rows(ctypes.Structure):
     _fields_ = [("base", c_void_p), ("row_bytes", c_uint64), ("rows", ctypes.c_int64), ("first", c_void_p)]
 
 
+PAGES_F16, PAGES_I8 = 0, 1
+STEP_SEQS, ROTARY_PAIRS, TOP_MAX = 1024, 128, 64
+
+
+class Step(ctypes.Structure):
+    """Mirror of xqhip_step (include/xqhip.h)."""
+    _fields_ = [("seqs", ctypes.c_int32), ("rows", ctypes.c_int32), ("max_rows", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32), ("row0", c_void_p), ("past", c_void_p), ("table", c_void_p),
+                ("open", c_void_p)]
+
+
+class Pages(ctypes.Structure):
+    """Mirror of xqhip_pages (include/xqhip.h)."""
+    _fields_ = [("type", ctypes.c_int32), ("nkv", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page", ctypes.c_int32), ("pages", ctypes.c_int32), ("opens", ctypes.c_int32), ("k", c_void_p),
+                ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_open", c_void_p),
+                ("v_open", c_void_p)]
+
+
+class Rotary(ctypes.Structure):
+    """Mirror of xqhip_rotary (include/xqhip.h)."""
+    _fields_ = [("cs", c_void_p), ("positions", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+                ("axes", ctypes.c_int32), ("axis", ctypes.c_uint8 * ROTARY_PAIRS), ("pos", c_void_p)]
+
+
 _P = ctypes.POINTER
 
 _HIP_SIGS = {
@@ -176,6 +201,16 @@ _HIP_SIGS = {
     "xqhip_spec_verify": (c_int, [c_void_p, c_int, c_int, _P(Tree), c_void_p, c_void_p, c_int, c_float, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "xqhip_tree_keep": (c_int, [_P(Rows), c_int, c_void_p, c_void_p, c_int, c_void_p]),
+    "xqhip_rotary_init": (c_int, [c_void_p, c_int, c_int, _P(ctypes.c_int32), c_int, c_int, c_void_p, _P(Rotary)]),
+    "xqhip_attn_prep_paged": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_float,
+                                      _P(Rotary), _P(Step), c_int, c_int, c_void_p, c_void_p, _P(Pages), c_void_p]),
+    "xqhip_paged_read": (c_int, [_P(Pages), _P(Step), c_int, c_void_p, c_void_p, c_void_p]),
+    "xqhip_paged_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "xqhip_paged_attention": (c_int, [c_void_p, c_void_p, _P(Pages), c_int, _P(Step), c_int, c_void_p, c_int, c_void_p,
+                                      c_size_t, c_void_p]),
+    "xqhip_token_logprobs_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "xqhip_token_logprobs": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "xqhip_rmsnorm": (c_int, [c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p]),
     "xqhip_lds_fill": (c_int, [c_float, c_void_p]),
     "xqhip_timestamp": (c_int, [c_void_p, c_void_p]),
@@ -248,6 +283,14 @@ def tree(parents):
 def rows(sets):
     """An array of xqhip_rows from (base, row_bytes, rows, first) tuples."""
     return (Rows * len(sets))(*[Rows(*s) for s in sets])
+
+
+def rotary(cs, positions, rotary_dim, sections, interleaved=False, pos=None):
+    """The xqhip_rotary of a table and the axes' sections (xqhip_rotary_init)."""
+    r = Rotary()
+    a = (ctypes.c_int32 * max(1, len(sections)))(*sections)
+    ck(hip().xqhip_rotary_init(cs, positions, rotary_dim, a, len(sections), int(interleaved), pos, ctypes.byref(r)))
+    return r
 
 
 def ptr(a):
