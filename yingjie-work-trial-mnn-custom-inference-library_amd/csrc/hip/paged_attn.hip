@@ -1,6 +1,7 @@
 // paged_attn.hip - attention of a step's rows over their sequences' pages.
 #include <algorithm>
 
+#include "attn_mfma.hpp"
 #include "paged_common.hpp"
 
 namespace xqhip {
@@ -112,13 +113,619 @@ __global__ void __launch_bounds__(256) paged_attn_row_kernel(PagedAttnLaunch p) 
     attend_paged_row<256>(p, s, sr, row, blockIdx.y, smem);
 }
 
+// ---------------------------------------------------------------------------
+// Matrix-core forms, heads of 128 and 256 dims.  A block takes some columns of
+// one sequence and kv head and a range of its keys, a column being one (row,
+// query head) pair: column c of C is head c / T of the kv head's `group` and row
+// t0 + c % T, T = C / group.  Its waves share the keys in 32-key tiles, each with
+// its own running max, sum and output, joined through LDS at the end.
+//
+// Scores are formed transposed, S^T = K Q^T (keys are the MFMA rows).  The pages
+// hold keys and values as the operands are: a lane's eight (or sixteen) values
+// are 16 bytes in a row, 32 lanes' 512 bytes, so K and V go from memory to the
+// matrix cores without a transposition.  An MFMA leaves a lane rows 8 (v / 4) + 4
+// (l >> 5) + v % 4; the order in which a tile's keys are given to the rows is
+// chosen so that those are eight keys in a row, the ones whose values the lane
+// loads (key_of_row).
+//
+// An 8-bit page's codes become fp16 integers, exactly; its scales enter as one
+// factor of a tile's scores and of its weights.
+//
+// Precision: q (scaled per column by a power of two to [2^12, 2^13)) and the
+// weights (times 2^6) are split into fp16 hi + lo, 22 bits together; fp32
+// accumulation.  The exponents' reference m is a column's largest score so far,
+// or up to 2^6 less; over 8-bit pages the largest of score + log2 of V's scale.
+//
+// A masked key has weight 0, but 0 times an infinity is not 0; values behind the
+// last position are replaced by 0, and where a sum is not finite for another
+// reason or the weights sum to 0 the block that writes such an output computes
+// its rows again by attend_paged_row.
+// ---------------------------------------------------------------------------
+constexpr int kNarrowCols = 16;     // up to 16 columns: paged_narrow_kernel
+constexpr int kNarrowBlocks = 256;  // blocks that share the narrow sequences' tiles
+constexpr int kWideCols = 64;
+constexpr int kWideUnits = 512;  // splits that a step of few row tiles is cut into, at most
+
+// the key of a tile that MFMA row r stands for: a lane's slots are then keys 16 (slot / 8) + 8 (lane / 32) + slot % 8
+// (fp16: pieces of 8 positions), or 16 (lane / 32) + 8 (slot / 8) + slot % 8 (8 bits: pieces of 16)
+template <bool I8>
+__device__ __forceinline__ int key_of_row(int r) {
+    const int e = r & 3, g = r >> 2 & 1, a0 = r >> 3 & 1, a1 = r >> 4;
+    return I8 ? 16 * g + 8 * a1 + 4 * a0 + e : 16 * a1 + 8 * g + 4 * a0 + e;
+}
+
+// Rows and keys of a sequence in an attention call.
+struct SeqKeys {
+    SeqRows r;
+    int cap;  // positions that the table holds
+    __device__ __forceinline__ SeqKeys(const PagedAttnLaunch& p, int s) : r(seq_rows(p.step, s)), cap(table_positions(p.step, p.kv)) {}
+    // last position that row j sees, -1: none
+    __device__ __forceinline__ int last(int j) const {
+        return r.past < 0 ? -1 : static_cast<int>(min(static_cast<int64_t>(r.past) + j, static_cast<int64_t>(cap) - 1));
+    }
+};
+
+// The narrow kernel's work: sequences of up to 16 columns, their 32-key tiles in units of q, for each kv head, one behind
+// the other; `blocks` blocks take equal ranges of them.  Few tiles: a block has one unit, and a unit lies in one
+// sequence and head.  Many: q = 1, and a block's range may end inside one and go on in the next.
+struct NarrowWork {
+    int q, blocks;
+    int units;  // of all sequences, one kv head
+};
+constexpr int kMinTiles = 2;   // smallest unit of few tiles
+constexpr int kMaxTiles = 16;  // largest
+
+__device__ __forceinline__ bool is_narrow(int rows, int group) { return rows > 0 && rows * group <= kNarrowCols; }
+__device__ __forceinline__ int tiles_of(int last) { return max(0, last) / kTTile + 1; }
+__device__ __forceinline__ int64_t range_begin(const NarrowWork& w, int nkv, int b) {
+    return static_cast<int64_t>(w.units) * nkv * b / w.blocks;
+}
+
+__device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int u = __shfl_up(v, o, kWave);
+        v += (threadIdx.x & (kWave - 1)) >= o ? u : 0;
+    }
+    return v;
+}
+
+// Units before each sequence into pre[0 .. seqs], by the whole block.
+template <int THREADS>
+__device__ NarrowWork narrow_work(const PagedAttnLaunch& p, int* pre, int* red) {
+    constexpr int kWaves = THREADS / kWave, kPer = (1024 + THREADS - 1) / THREADS;
+    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, group = p.nq / p.kv.nkv;
+    int tiles[kPer], sum = 0, active = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int s = i * THREADS + threadIdx.x;
+        tiles[i] = 0;
+        if (s < p.step.seqs) {
+            const SeqKeys k(p, s);
+            if (is_narrow(k.r.rows, group)) {
+                tiles[i] = tiles_of(k.last(k.r.rows - 1));
+                ++active;
+            }
+        }
+        sum += tiles[i];
+    }
+    {
+        int a = active, t = sum;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            a += __shfl_xor(a, o, kWave);
+            t += __shfl_xor(t, o, kWave);
+        }
+        if (lane == 0) {
+            red[wid] = a;
+            red[kWaves + wid] = t;
+        }
+    }
+    __syncthreads();
+    active = sum = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        active += red[i];
+        sum += red[kWaves + i];
+    }
+    NarrowWork w;
+    // the smallest unit with which every unit has a block of its own
+    const int64_t room = kNarrowBlocks - static_cast<int64_t>(active) * p.kv.nkv;
+    const int64_t fit = room > 0 ? (static_cast<int64_t>(sum) * p.kv.nkv + room - 1) / room : kMaxTiles + 1;
+    w.q = fit <= kMaxTiles ? max(static_cast<int>(fit), kMinTiles) : 1;
+    int base = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int s = i * THREADS + threadIdx.x;
+        const int u = (tiles[i] + w.q - 1) / w.q, in = wave_scan_int(u);
+        if (lane == kWave - 1) red[wid] = in;
+        __syncthreads();
+        int before = base, all = base;
+#pragma unroll
+        for (int j = 0; j < kWaves; ++j) {
+            before += j < wid ? red[j] : 0;
+            all += red[j];
+        }
+        if (s < p.step.seqs) pre[s + 1] = before + in;
+        base = all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) pre[0] = 0;
+    __syncthreads();
+    w.units = base;
+    w.blocks = static_cast<int>(min(static_cast<int64_t>(kNarrowBlocks), static_cast<int64_t>(base) * p.kv.nkv));
+    return w;
+}
+
+// the sequence whose units hold unit x of nkv heads: the last with nkv pre[s] <= x, by a wave
+__device__ __forceinline__ int seq_of_unit(const int* pre, int seqs, int nkv, int64_t x) {
+    const int lane = threadIdx.x & (kWave - 1);
+    int n = 0;
+    for (int b = 1; b <= seqs; b += kWave) {
+        const int s = b + lane;
+        const uint64_t on = __builtin_amdgcn_ballot_w64(s <= seqs && static_cast<int64_t>(pre[min(s, seqs)]) * nkv <= x);
+        n += __popcll(on);
+        if (on != ~uint64_t(0)) break;
+    }
+    return __builtin_amdgcn_readfirstlane(n);
+}
+
+// Workspace: the narrow work's prefix for the merge, the wide kernel's units, partial outputs.
+struct WideUnit {
+    int seq, tile, begin, end;  // chunks [begin, end) of a row tile
+};
+constexpr size_t kWsHead = 4 * (8 + 1024 + 8);
+struct PagedWs {
+    int* head;        // [0] q, [1] blocks, [2] units; [3] wide units; from [8] the prefix
+    int* again;       // [seqs][nkv]: outputs of one block that have to be computed again
+    float* narrow;    // [2 blocks][16][hd + 2]
+    WideUnit* units;  // followed by their split counts
+    float* wide;      // [units][64][hd + 2]
+};
+
+template <int HD, int KS, int COLS>
+struct PagedBlock {
+    static constexpr int kThreads = kWave * KS, kCols = COLS;
+    static constexpr int kLdo = HD + 4;                                            // floats per column of a wave's output
+    static constexpr int kQuads = HD / 4;                                          // float4 of an output row
+    static constexpr size_t kOutBytes = static_cast<size_t>(kCols) * (KS * (kLdo + 3) + 1) * 4;
+};
+
+// writes the quad at `out`; whether its row has to be computed again
+__device__ __forceinline__ bool write_paged_quad(float4 r, float L, const float* gate, float* out) {
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
+    if (gate) {
+        const float4 gt = *reinterpret_cast<const float4*>(gate);
+        y.x *= sigmoid_dev(gt.x);
+        y.y *= sigmoid_dev(gt.y);
+        y.z *= sigmoid_dev(gt.z);
+        y.w *= sigmoid_dev(gt.w);
+    }
+    *reinterpret_cast<float4*>(out) = y;
+    return !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
+}
+
+// The key waves of a block's columns joined, then written: a partial output (to part_out: [COLS][HD], then [COLS][2]), or
+// the output, and to *again whether it has to be computed again.  CT column tiles x KS key waves; HALF: hi and lo columns
+// of one tile.
+template <int HD, int CT, int KS, int COLS, bool HALF, int N>
+__device__ __forceinline__ void finish_paged(const PagedAttnLaunch& p, const SeqRows& sr, int kh, int t0, int ntok, int T, uint32_t inv_t,
+                                             float* part_out, int* again, bool live, const floatx16 (&o)[N], float m, float l, void* lds, int* redo) {
+    static_assert(HD == 32 * N, "dim tiles");
+    using F = PagedBlock<HD, KS, COLS>;
+    constexpr int kThreads = kWave * CT * KS;
+    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, cl = lane & 31, g = lane >> 5;
+    const int group = p.nq / p.kv.nkv;
+    float* Ol = static_cast<float*>(lds);          // [KS][columns][kLdo]
+    float* Ml = Ol + KS * F::kCols * F::kLdo;      // [KS][columns][2]
+    float* Fl = Ml + KS * F::kCols * 2;            // [KS][columns]
+    float* Ll = Fl + KS * F::kCols;                // [columns] the sums
+    l = xor_pair_sum<32>(l);
+    if constexpr (HALF) l = xor_pair_sum<16>(l);
+    const int cw = HALF ? cl & 15 : cl, half = HALF ? cl >> 4 : 0;
+    const int ct = wid % CT, ks = wid / CT;
+    __syncthreads();  // every wave is done with what lay here
+    // (HALF: the hi and lo columns' sums; every lane takes part in them)
+    const int at = ks * F::kCols + ct * 32 + cw;
+    float* oc = Ol + at * F::kLdo + 4 * g + 16 * half;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int a = 0; a < (HALF ? 2 : 4); ++a) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = HALF ? rows_sum(o[j][4 * a + e], o[j][(8 + 4 * a + e) % 16]) : o[j][4 * a + e];
+            if (live) *reinterpret_cast<float4*>(oc + 32 * j + 8 * a) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    if (live && g == 0 && half == 0) *reinterpret_cast<float2*>(Ml + at * 2) = make_float2(m, l);
+    if (threadIdx.x == 0) *redo = 0;
+    __syncthreads();
+    auto row_of = [&](int c, int& hc, int& tc) {
+        hc = static_cast<int>(c * inv_t >> 16);
+        tc = c - hc * T;
+        return hc < group && tc < ntok;
+    };
+    if (threadIdx.x < F::kCols) {  // a thread per column: the factors of its waves' outputs, and their sum
+        const int c = threadIdx.x;
+        int hc, tc;
+        if (row_of(c, hc, tc)) {
+            float M = -INFINITY, L = 0.0f;
+            for (int i = 0; i < KS; ++i) M = fmaxf(M, Ml[(c + i * F::kCols) * 2]);
+            for (int i = 0; i < KS; ++i) {
+                const float f = __builtin_amdgcn_exp2f(Ml[(c + i * F::kCols) * 2] - M);
+                L += f * Ml[(c + i * F::kCols) * 2 + 1];
+                Fl[c + i * F::kCols] = f;
+            }
+            Ll[c] = L;
+            if (part_out) reinterpret_cast<float2*>(part_out + F::kCols * HD)[c] = make_float2(M, L);
+        }
+    }
+    __syncthreads();
+    bool bad = false;
+    for (int i = threadIdx.x; i < F::kCols * F::kQuads; i += kThreads) {
+        const int c = i / F::kQuads, d = 4 * (i % F::kQuads);
+        int hc, tc;
+        if (!row_of(c, hc, tc)) continue;
+        float4 r = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) add_scaled(r, Fl[c + k * F::kCols], *reinterpret_cast<const float4*>(Ol + (c + k * F::kCols) * F::kLdo + d));
+        if (part_out) {
+            *reinterpret_cast<float4*>(part_out + c * HD + d) = r;
+            continue;
+        }
+        const size_t row = sr.row0 + t0 + tc, col = static_cast<size_t>(kh * group + hc) * HD + d;
+        bad |= write_paged_quad(r, Ll[c], p.gate ? p.gate + row * p.q_stride + col : nullptr, p.out + row * p.out_stride + col);
+    }
+    if (part_out) return;
+    if (bad) *redo = 1;
+    __syncthreads();
+    if (threadIdx.x == 0) *again = *redo;
+}
+
+// Where the tiles of a wave lie: lane i holds the page (and its scales) of the wave's tile i, of 64.
+struct TilePages {
+    int page, first, step, end;  // tiles first, first + step, .. < end
+    float ks, vs;
+    __device__ __forceinline__ void fill(const PagedAttnLaunch& p, int s, int kh, int i0, int last) {
+        const int tile = first + (i0 + static_cast<int>(threadIdx.x & (kWave - 1))) * step;
+        page = tile < end && tile * kTTile <= last ? page_at(p.step, p.kv, s, tile * kTTile / p.kv.page) : -1;
+        if (p.kv.i8) {
+            const size_t at = static_cast<size_t>(max(page, 0)) * p.kv.nkv + kh;
+            ks = page >= 0 ? p.kv.k_scale[at] : 0.0f;
+            vs = page >= 0 ? p.kv.v_scale[at] : 0.0f;
+        }
+    }
+};
+
+template <bool I8, int HD>
+struct TileBase {
+    __amdgpu_buffer_rsrc_t k, v;
+    float ks, vs;
+    int valid;
+};
+// the resources of tile i of a wave's (empty where it has no page: loads then read 0)
+template <bool I8, int HD>
+__device__ __forceinline__ TileBase<I8, HD> tile_base(const PagedAttnLaunch& p, TilePages& tp, int s, int kh, int i, int last) {
+    constexpr uint32_t es = I8 ? 1u : 2u;
+    if ((i & 63) == 0) tp.fill(p, s, kh, i, last);  // wave-uniform
+    TileBase<I8, HD> b;
+    const int page = __builtin_amdgcn_readlane(tp.page, i & 63);
+    if constexpr (I8) {
+        b.ks = readlane_f32(tp.ks, i & 63);
+        b.vs = readlane_f32(tp.vs, i & 63);
+    }
+    b.valid = page >= 0;
+    const int off = (tp.first + i * tp.step) * kTTile & (p.kv.page - 1);
+    const size_t head = page_head(p.kv, max(page, 0), kh) * es;
+    const uint32_t kskip = off * 16u, vskip = static_cast<uint32_t>(off) * HD * es;
+    const uint32_t all = b.valid ? static_cast<uint32_t>(p.kv.page) * HD * es : 0u;
+    b.k = buf_rsrc(static_cast<const uint8_t*>(p.kv.k) + head + kskip, b.valid ? all - kskip : 0u);
+    b.v = buf_rsrc(static_cast<const uint8_t*>(p.kv.v) + head + vskip, b.valid ? all - vskip : 0u);
+    return b;
+}
+
+// the first n of eight fp16 values, 0 for the others
+__device__ __forceinline__ u32x4 first_halves(u32x4 v, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] &= n > 2 * i + 1 ? ~0u : (n > 2 * i ? 0xffffu : 0u);
+    return v;
+}
+
+// Up to 16 columns, q's hi parts in the tile's first 16 columns and its lo parts in the others: one MFMA does what two
+// do, a lane and its neighbour 16 lanes on add their scores and take eight keys each, and the weights' hi and lo parts go
+// back into the two halves.  Each wave takes its own 32-key tiles, K and V straight into registers, the next tile's on
+// their way meanwhile; no barrier before the waves join.
+template <int HD, bool I8, int KS>
+__global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(PagedAttnLaunch p, PagedWs ws, int has_wide) {
+    using F = PagedBlock<HD, KS, kNarrowCols>;
+    using Q = QueryStage<F, HD>;
+    constexpr int kSteps = HD / 16, kDimTiles = HD / 32;
+    constexpr int kKPieces = HD / (I8 ? 32 : 16), kVPieces = I8 ? kDimTiles : 2 * kDimTiles;
+    extern __shared__ uint4 paged_lds[];
+    __shared__ int pre[1025], red[2 * KS], redo;
+    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kNarrowCols / group;
+    const int lane = threadIdx.x & (kWave - 1), ks = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int cl = lane & 31, g = lane >> 5, col = cl & 15, part = cl >> 4;
+    const uint32_t inv_t = (65535u + T) / T;
+    const int ch = static_cast<int>(col * inv_t >> 16), ctok = col - ch * T;
+    const NarrowWork w = narrow_work<F::kThreads>(p, pre, red);
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i <= p.step.seqs; i += F::kThreads) ws.head[8 + i] = pre[i];
+        if (threadIdx.x == 0) {
+            ws.head[0] = w.q;
+            ws.head[1] = w.blocks;
+            ws.head[2] = w.units;
+        }
+    }
+    if (static_cast<int>(blockIdx.x) >= w.blocks) return;
+    const int64_t begin = range_begin(w, nkv, blockIdx.x), end = range_begin(w, nkv, blockIdx.x + 1);
+    const uint32_t kat = (static_cast<uint32_t>(g) * p.kv.page + key_of_row<I8>(cl)) * 16u, kstep = 32u * p.kv.page;
+    const uint32_t vat = (static_cast<uint32_t>(g) * HD + cl) * 16u;
+    const int lane_key = I8 ? 16 * g + 8 * part : 16 * part + 8 * g;  // of the lane's eight slots
+    for (int64_t at = begin; at < end;) {
+        const int s = seq_of_unit(pre, p.step.seqs, nkv, at);
+        const int units = pre[s + 1] - pre[s];
+        const int in = static_cast<int>(at - static_cast<int64_t>(pre[s]) * nkv);
+        const int kh = in / units, u0 = in - kh * units;
+        const int u1 = static_cast<int>(min(static_cast<int64_t>(units), u0 + (end - at)));
+        const bool whole = u0 == 0 && u1 == units;
+        float* part_out = whole ? nullptr : ws.narrow + (2 * static_cast<size_t>(blockIdx.x) + (at == begin ? 0 : 1)) * kNarrowCols * (HD + 2);
+        at += u1 - u0;
+        const SeqKeys sk(p, s);
+        const int ntok = sk.r.rows, last = sk.last(ntok - 1), sure = sk.last(0);
+        const bool live = ch < group && ctok < ntok;
+        const int qpos = live ? sk.last(ctok) : -1;
+        TilePages tp;
+        tp.first = u0 * w.q + ks;
+        tp.step = KS;
+        tp.end = min(u1 * w.q, tiles_of(last));
+        const int n = __builtin_amdgcn_readfirstlane(max(0, (tp.end - tp.first + KS - 1) / KS));
+        Q query;
+        query.load(p.q + static_cast<size_t>(sk.r.row0) * p.q_stride, p.q_stride, kh, ntok, group, T, inv_t);
+        u32x4 kr[kKPieces], vr[kVPieces];
+        TileBase<I8, HD> next = tile_base<I8, HD>(p, tp, s, kh, 0, last);
+        auto load_k = [&] {
+#pragma unroll
+            for (int u = 0; u < kKPieces; ++u) kr[u] = __builtin_amdgcn_raw_buffer_load_b128(next.k, kat, u * kstep, 0);
+        };
+        auto load_v = [&] {
+#pragma unroll
+            for (int h = 0; h < kVPieces / kDimTiles; ++h)
+#pragma unroll
+                for (int j = 0; j < kDimTiles; ++j)
+                    vr[h * kDimTiles + j] = __builtin_amdgcn_raw_buffer_load_b128(next.v, vat + (2u * h * HD + 32u * j) * 16u, 0, 0);
+        };
+        load_k();
+        load_v();
+        query.store(paged_lds);
+        __syncthreads();
+        half8 qf[kSteps];  // the lane's own part, hi or lo
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t) qf[t] = Q::part(paged_lds, part, col, I8 ? 32 * (t / 2) + 16 * g + 8 * (t % 2) : 16 * t + 8 * g);
+        const float sscale = Q::scale(paged_lds, col);
+        float m = -1.0e30f, l = 0.0f;  // reference of the exponents, this lane's part of the sum
+        floatx16 o[kDimTiles];
+#pragma unroll
+        for (int j = 0; j < kDimTiles; ++j) o[j] = floatx16{};
+        for (int i = 0; i < n; ++i) {
+            const int key0 = (tp.first + i * KS) * kTTile;
+            const float kscale = I8 ? sscale * next.ks : sscale, vscale = I8 ? next.vs : 1.0f;
+            const bool valid = next.valid;
+            floatx16 st = floatx16{};
+#pragma unroll
+            for (int t = 0; t < kSteps; ++t) {
+                half8 a;
+                if constexpr (I8) {
+                    const u32x2 w0 = codes_to_half(kr[t / 2][2 * (t % 2)]), w1 = codes_to_half(kr[t / 2][2 * (t % 2) + 1]);
+                    a = __builtin_bit_cast(half8, u32x4{w0.x, w0.y, w1.x, w1.y});
+                } else {
+                    a = __builtin_bit_cast(half8, kr[t]);
+                }
+                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[t], st, 0, 0, 0);
+            }
+            next = tile_base<I8, HD>(p, tp, s, kh, i + 1, last);
+            load_k();
+            float sc[8];
+#pragma unroll
+            for (int v = 0; v < 8; ++v) sc[v] = rows_sum(st[v], st[v + 8]);
+            if (key0 + kTTile - 1 > sure || !valid) {  // wave-uniform: keys that some column does not see
+                const int see = valid ? qpos - (key0 + lane_key) : -1;  // slots up to here
+#pragma unroll
+                for (int v = 0; v < 8; ++v) sc[v] = v <= see ? sc[v] : -INFINITY;
+                if constexpr (!I8)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < kDimTiles; ++j)
+                            vr[h * kDimTiles + j] = first_halves(vr[h * kDimTiles + j], last + 1 - (key0 + 16 * h + 8 * g));
+            }
+            float mc = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+            mc = pair32_max(xor16_max(mc)) * kscale;
+            if constexpr (I8) mc += scale_exponent(vscale);
+            // the reference moves only when a column's max has outgrown it (rarely after the first tiles)
+            const bool up = mc > m + kSlack;
+            if (__builtin_amdgcn_ballot_w64(up)) {
+                const float to = up ? mc : m, f = __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                l *= f;
+#pragma unroll
+                for (int j = 0; j < kDimTiles; ++j) o[j] *= f;
+            }
+            const float off = kRaise - m;
+            float x[8];
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+                x[v] = __builtin_amdgcn_exp2f(fmaf(sc[v], kscale, off));
+                l += x[v];
+                if constexpr (I8) {
+                    x[v] *= vscale;
+                    asm("" : "+v"(x[v]));  // the rounded product: hi and lo would else be taken from two roundings of it
+                }
+            }
+            half8 phi, plo;
+            split8(x, phi, plo);
+            half8 pw[2];  // lanes of the hi columns give their lo for the other 8 keys' hi
+            {
+                const u32x4 hi = __builtin_bit_cast(u32x4, phi), lo = __builtin_bit_cast(u32x4, plo);
+                u32x4 r0, r1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const auto r = __builtin_amdgcn_permlane16_swap(hi[e], lo[e], false, false);
+                    r0[e] = r[0];
+                    r1[e] = r[1];
+                }
+                pw[0] = __builtin_bit_cast(half8, r0);
+                pw[1] = __builtin_bit_cast(half8, r1);
+            }
+#pragma unroll
+            for (int j = 0; j < kDimTiles; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    half8 a;
+                    if constexpr (I8) {
+                        const u32x2 w0 = codes_to_half(vr[j][2 * h]), w1 = codes_to_half(vr[j][2 * h + 1]);
+                        a = __builtin_bit_cast(half8, u32x4{w0.x, w0.y, w1.x, w1.y});
+                    } else {
+                        a = __builtin_bit_cast(half8, vr[h * kDimTiles + j]);
+                    }
+                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pw[h], o[j], 0, 0, 0);
+                }
+            load_v();
+        }
+        finish_paged<HD, 1, KS, kNarrowCols, true>(p, sk.r, kh, 0, ntok, T, inv_t, part_out, ws.again + s * nkv + kh, live, o, m, l, paged_lds, &redo);
+        __syncthreads();
+    }
+}
+
+// The partial outputs of a sequence and kv head joined (nothing to do where one block had all of its tiles).
+constexpr int kMergeThreads = 512;
+template <int HD>
+__global__ void __launch_bounds__(kMergeThreads) paged_narrow_merge_kernel(PagedAttnLaunch p, PagedWs ws) {
+    extern __shared__ float smem[];  // attend_paged_row's
+    __shared__ float fac[kNarrowCols][kNarrowBlocks], total[kNarrowCols];
+    __shared__ float4 sums[kMergeThreads];
+    __shared__ int redo;
+    constexpr int kQuads = HD / 4, kSlot = kNarrowCols * (HD + 2);
+    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kNarrowCols / group, s = blockIdx.x, kh = blockIdx.y;
+    const NarrowWork w{ws.head[0], ws.head[1], ws.head[2]};
+    const int u0 = ws.head[8 + s], units = ws.head[9 + s] - u0;
+    const SeqRows sr = seq_rows(p.step, s);
+    if (units == 0) return;
+    const int64_t all = static_cast<int64_t>(w.units) * nkv, first = static_cast<int64_t>(u0) * nkv + static_cast<int64_t>(kh) * units;
+    auto block_of = [&](int64_t x) { return static_cast<int>(((x + 1) * w.blocks - 1) / all); };
+    const int b0 = block_of(first), n = block_of(first + units - 1) - b0 + 1;
+    if (n == 1) {
+        if (__builtin_expect(ws.again[s * nkv + kh] != 0, 0))
+            for (int t = 0; t < sr.rows; ++t) attend_paged_row<kMergeThreads>(p, s, sr, sr.row0 + t, kh, smem);
+        return;
+    }
+    auto slot_of = [&](int b) {
+        return ws.narrow + (2 * static_cast<size_t>(b) + (range_begin(w, nkv, b) >= first ? 0 : 1)) * kSlot;
+    };
+    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, cols = sr.rows * group;
+    auto column = [&](int i) { return i / sr.rows * T + i % sr.rows; };  // live column i
+    for (int i = wid; i < cols; i += kMergeThreads / kWave) {
+        const int c = column(i);
+        float M = -INFINITY, L = 0.0f;
+        for (int b = lane; b < n; b += kWave) M = fmaxf(M, slot_of(b0 + b)[kNarrowCols * HD + 2 * c]);
+        M = wave_max(M);
+        for (int b = lane; b < n; b += kWave) {
+            const float2 ml = *reinterpret_cast<const float2*>(slot_of(b0 + b) + kNarrowCols * HD + 2 * c);
+            const float f = __builtin_amdgcn_exp2f(ml.x - M);
+            fac[i][b] = f;
+            L += f * ml.y;
+        }
+        L = wave_sum(L);
+        if (lane == 0) total[i] = L;
+    }
+    if (threadIdx.x == 0) redo = 0;
+    __syncthreads();
+    const int items = cols * kQuads, slices = max(1, kMergeThreads / items);
+    bool bad = false;
+    for (int base = 0; base < items; base += kMergeThreads) {
+        const int item = slices > 1 ? threadIdx.x % items : base + threadIdx.x, slice = slices > 1 ? threadIdx.x / items : 0;
+        const int i = item / kQuads, d = 4 * (item % kQuads);
+        float4 r = {};
+        const bool on = item < items && slice < slices;
+        if (on) {
+            const float* at = ws.narrow + column(i) * HD + d;
+#pragma unroll 4
+            for (int b = slice; b < n; b += slices) add_scaled(r, fac[i][b], *reinterpret_cast<const float4*>(at + (slot_of(b0 + b) - ws.narrow)));
+        }
+        if (slices > 1) {
+            sums[threadIdx.x] = r;
+            __syncthreads();
+            if (slice == 0)
+                for (int k = 1; k < slices; ++k) add_scaled(r, 1.0f, sums[k * items + item]);
+        }
+        if (on && slice == 0) {
+            const size_t row = sr.row0 + i % sr.rows, colm = static_cast<size_t>(kh * group + i / sr.rows) * HD + d;
+            bad |= write_paged_quad(r, total[i], p.gate ? p.gate + row * p.q_stride + colm : nullptr, p.out + row * p.out_stride + colm);
+        }
+    }
+    if (bad) redo = 1;
+    __syncthreads();
+    if (__builtin_expect(!redo, 1)) return;
+    for (int t = 0; t < sr.rows; ++t) attend_paged_row<kMergeThreads>(p, s, sr, sr.row0 + t, kh, smem);
+}
+
+// Rows of the sequences that the narrow kernel does not take, in the general form.
+__global__ void __launch_bounds__(256) paged_rest_row_kernel(PagedAttnLaunch p) {
+    extern __shared__ float smem[];
+    const int row = blockIdx.x;
+    const int s = __builtin_amdgcn_readfirstlane(seq_of_row(p.step, row));
+    if (s >= p.step.seqs) return;
+    const SeqRows sr = seq_rows(p.step, s);
+    if (row < sr.row0 || row - sr.row0 >= sr.rows || is_narrow(sr.rows, p.nq / p.kv.nkv)) return;
+    attend_paged_row<256>(p, s, sr, row, blockIdx.y, smem);
+}
+
+static size_t again_bytes(int nkv) { return (sizeof(int) * 1024 * nkv + 15) / 16 * 16; }
+static PagedWs paged_ws(float* base, int hd, int nkv) {
+    PagedWs w{};
+    w.head = reinterpret_cast<int*>(base);
+    w.again = w.head + kWsHead / 4;
+    w.narrow = base + (kWsHead + again_bytes(nkv)) / 4;
+    w.wide = w.narrow + static_cast<size_t>(2) * kNarrowBlocks * kNarrowCols * (hd + 2);
+    return w;
+}
+
 size_t paged_attn_workspace_bytes(int nq, int nkv, int head_dim) {
     if (nkv <= 0 || nq <= 0 || nq % nkv || nq / nkv > kPagedMaxGroup || head_dim <= 0 || head_dim > 256 || head_dim % 16) return 0;
-    return 16;
+    if (head_dim != 128 && head_dim != 256) return 16;
+    return kWsHead + again_bytes(nkv) + sizeof(float) * 2 * kNarrowBlocks * kNarrowCols * (head_dim + 2);
+}
+
+template <int HD, bool I8>
+static hipError_t launch_paged_heads(const PagedAttnLaunch& p, hipStream_t s) {
+    constexpr int KS = HD == 128 ? 8 : 4;
+    using F = PagedBlock<HD, KS, kNarrowCols>;
+    constexpr size_t kLds = std::max(F::kOutBytes, QueryStage<F, HD>::kBytes);
+    const int group = p.nq / p.kv.nkv;
+    const bool wide = p.step.max_rows * static_cast<int64_t>(group) > kNarrowCols;
+    const PagedWs ws = paged_ws(p.ws, HD, p.kv.nkv);
+    const size_t row_lds = paged_row_lds(group, HD);
+    auto kernel = &paged_narrow_kernel<HD, I8, KS>;
+    if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
+        e != hipSuccess)
+        return e;
+    hipLaunchKernelGGL(kernel, dim3(kNarrowBlocks), dim3(F::kThreads), kLds, s, p, ws, wide);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    hipLaunchKernelGGL(paged_narrow_merge_kernel<HD>, dim3(p.step.seqs, p.kv.nkv), dim3(kMergeThreads), row_lds, s, p, ws);
+    if (wide) hipLaunchKernelGGL(paged_rest_row_kernel, dim3(p.step.rows, p.kv.nkv), dim3(256), row_lds, s, p);
+    return hipGetLastError();
 }
 
 hipError_t launch_paged_attn(const PagedAttnLaunch& p, hipStream_t s) {
-    hipLaunchKernelGGL(paged_attn_row_kernel, dim3(p.step.rows, p.kv.nkv), dim3(256), paged_row_lds(p.nq / p.kv.nkv, p.kv.head_dim), s, p);
+    const int hd = p.kv.head_dim;
+    // the matrix-core kernels take rows in 16-byte pieces and their offsets within 64 rows in 32 bits
+    const bool al = ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.gate) | reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0 &&
+                    p.q_stride % 4 == 0 && p.out_stride % 4 == 0 && p.q_stride < 1 << 21 && p.out_stride < 1 << 21;
+    if (al && hd == 128) return p.kv.i8 ? launch_paged_heads<128, true>(p, s) : launch_paged_heads<128, false>(p, s);
+    if (al && hd == 256) return p.kv.i8 ? launch_paged_heads<256, true>(p, s) : launch_paged_heads<256, false>(p, s);
+    hipLaunchKernelGGL(paged_attn_row_kernel, dim3(p.step.rows, p.kv.nkv), dim3(256), paged_row_lds(p.nq / p.kv.nkv, hd), s, p);
     return hipGetLastError();
 }
 
