@@ -669,7 +669,7 @@ typedef struct xqhip_step {
 enum { XQHIP_PAGES_F16 = 0, XQHIP_PAGES_I8 = 1 };
 typedef struct xqhip_pages {
     int32_t type;
-    int32_t nkv, head_dim; /* head_dim: a multiple of 16, up to 256; nkv up to 1024  */
+    int32_t nkv, head_dim; /* head_dim: a multiple of 16, up to 256; nkv up to 256   */
     int32_t page;          /* 32, 64 or 128                                         */
     int32_t pages;         /* of the pool                                           */
     int32_t opens;         /* PAGES_I8: open pages                                  */

@@ -63,7 +63,7 @@ def bad_axis():
     return ctypes.byref(r)
 
 
-BAD_PAGES = [dict(type=2), dict(type=-1), dict(nkv=0), dict(nkv=1025), dict(hd=0), dict(hd=24), dict(hd=272), dict(page=16),
+BAD_PAGES = [dict(type=2), dict(type=-1), dict(nkv=0), dict(nkv=257), dict(hd=0), dict(hd=24), dict(hd=272), dict(page=16),
              dict(page=48), dict(page=256), dict(pages=0), dict(k=None), dict(v=None), dict(k=odd(8)), dict(v=odd(2)),
              dict(ks=None), dict(vs=None)]
 BAD_OPENS = [dict(opens=0), dict(ko=None), dict(vo=None), dict(ko=odd(8)), dict(vo=odd(4))]
@@ -112,7 +112,7 @@ def test_attention_refuses(o):
     refused(xb.hip().xqhip_paged_attention(*a.values(), None), "xqhip_paged_attention")
 
 
-@pytest.mark.parametrize("shape", [(7, 2, 128), (0, 1, 128), (8, 0, 128), (34, 2, 128), (8, 2, 24), (8, 2, 272), (8, 2, 0)])
+@pytest.mark.parametrize("shape", [(7, 2, 128), (0, 1, 128), (8, 0, 128), (34, 2, 128), (8, 2, 24), (8, 2, 272), (8, 2, 0), (257, 257, 128)])
 def test_attention_workspace_of_refused_shapes(shape):
     assert xb.hip().xqhip_paged_attention_workspace_bytes(*shape) == 0
 

@@ -593,6 +593,22 @@ def test_large_and_small_values(kind):
         assert np.abs(got[row] - want[row]).max() <= 6e-4 * np.abs(seen).max(), row
 
 
+@pytest.mark.parametrize("rows", [[1, 1], [37, 1]])
+@pytest.mark.parametrize("zero", ["k", "v", "kv"])
+def test_pages_of_zeros(rows, zero):
+    """8-bit pages with the scale 0, wholly and partly seen."""
+    rng = np.random.default_rng(27)
+    plan = Plan(rng, 64, [20, 150], rows)
+    k, v = (rng.normal(0, 1, (plan.pages, 2, 64, 128)).astype(np.float16) for _ in "kv")
+    for m, x in (("k", k), ("v", v)):
+        if m in zero:
+            x[plan.table[0]] = 0
+            x[plan.table[1, [0, 2]]] = 0
+    pool = Pool(I8, 2, 128, 64, plan.pages, 1, k, v)
+    q = rng.normal(0, 1, (plan.total, 8 * 128)).astype(np.float32)
+    check(attention(pool, plan, 8, q, None), attend_oracle(pool, plan, 8, q, None))
+
+
 def test_sequences_share_pages():
     """A prompt's pages in three tables."""
     rng = np.random.default_rng(18)

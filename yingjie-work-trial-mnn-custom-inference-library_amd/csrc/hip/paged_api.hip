@@ -38,7 +38,7 @@ bool workspace_ok(const void* ws, size_t have, size_t need) { return ws && align
 
 const char* pages_fault(const xqhip_pages* kv, bool opens) {
     if (kv->type != XQHIP_PAGES_F16 && kv->type != XQHIP_PAGES_I8) return "page type";
-    if (kv->nkv <= 0 || kv->nkv > 1024) return "kv heads (1 to 1024)";
+    if (kv->nkv <= 0 || kv->nkv > 256) return "kv heads (1 to 256)";
     if (kv->head_dim <= 0 || kv->head_dim > 256 || kv->head_dim % 16) return "head_dim (a multiple of 16, up to 256)";
     if (kv->page != 32 && kv->page != 64 && kv->page != 128) return "page (32, 64 or 128 positions)";
     if (kv->pages <= 0) return "pages of the pool";

@@ -14,13 +14,14 @@ constexpr size_t paged_row_lds(int group, int hd) {
 }
 
 // ---------------------------------------------------------------------------
-// One row and the `group` query heads of kv head kh, any head size: the
+// One row and the `group` query heads of kv head kh (of which h0 .. h1 - 1 are
+// written), any head size: the
 // positions in chunks of 32 with a running max and sum (rescaled by exp(m_old -
 // m_new)).  What the row does not see is passed over, so nothing in it can reach
 // the row; a chunk without a score above minus infinity leaves the sums.
 // ---------------------------------------------------------------------------
 template <int THREADS>
-__device__ void attend_paged_row(const PagedAttnLaunch& p, int s, const SeqRows& sr, int row, int kh, float* smem) {
+__device__ void attend_paged_row(const PagedAttnLaunch& p, int s, const SeqRows& sr, int row, int kh, float* smem, int h0 = 0, int h1 = kPagedMaxGroup) {
     static_assert(THREADS >= 8 * kRowChunk, "eight threads per key");
     const int hd = p.kv.head_dim, nkv = p.kv.nkv, group = p.nq / nkv;
     const int64_t want = static_cast<int64_t>(max(sr.past, 0)) + (row - sr.row0) + 1;
@@ -95,7 +96,7 @@ __device__ void attend_paged_row(const PagedAttnLaunch& p, int s, const SeqRows&
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < group * hd; i += THREADS) {
+    for (int i = h0 * hd + threadIdx.x; i < min(h1, group) * hd; i += THREADS) {
         const float l = ml[2 * (i / hd) + 1];
         const float r = l == 0.0f ? 0.0f : osum[i] / l;
         const float gate = p.gate ? sigmoid_dev(p.gate[static_cast<size_t>(row) * p.q_stride + head + i]) : 1.0f;
@@ -143,8 +144,9 @@ __global__ void __launch_bounds__(256) paged_attn_row_kernel(PagedAttnLaunch p) 
 // ---------------------------------------------------------------------------
 constexpr int kNarrowCols = 16;     // up to 16 columns: paged_narrow_kernel
 constexpr int kNarrowBlocks = 256;  // blocks that share the narrow sequences' tiles
-constexpr int kWideCols = 64;
-constexpr int kWideUnits = 512;  // splits that a step of few row tiles is cut into, at most
+constexpr int kWideCols = 64;       // other sequences: paged_wide_kernel
+constexpr int kWideBlocks = 256;    // blocks that few row tiles' keys are split over
+constexpr int kMostUnits = 65535 * kPagedMaxGroup / kWideCols + 1024 + kWideBlocks;  // row tiles and splits of a step
 
 // the key of a tile that MFMA row r stands for: a lane's slots are then keys 16 (slot / 8) + 8 (lane / 32) + slot % 8
 // (fp16: pieces of 8 positions), or 16 (lane / 32) + 8 (slot / 8) + slot % 8 (8 bits: pieces of 16)
@@ -271,18 +273,22 @@ __device__ __forceinline__ int seq_of_unit(const int* pre, int seqs, int nkv, in
     return __builtin_amdgcn_readfirstlane(n);
 }
 
-// Workspace: the narrow work's prefix for the merge, the wide kernel's units, partial outputs.
+// Chunks [begin, end) of the keys of a row tile; its `splits` units lie one behind the other, and of a tile with several
+// so do their partial outputs' slots.
 struct WideUnit {
-    int seq, tile, begin, end;  // chunks [begin, end) of a row tile
+    int seq, tile, begin, end, splits, slot;
+};
+// Workspace: the narrow work's prefix for the merge, the wide kernel's units, partial outputs.
+struct PagedWs {
+    int* head;        // [0] q, [1] blocks, [2] units; [4] wide units, [5] their slots; from [8] the prefix
+    int* again;       // [seqs][nkv]: outputs of one block that have to be computed again
+    int* again_wide;  // [wide units][nkv]
+    int* first;       // [slots]: first unit of the slot's row tile
+    WideUnit* units;
+    float* narrow;    // [2 blocks][16][hd + 2]
+    float* wide;      // [slots][nkv][64][hd + 2]
 };
 constexpr size_t kWsHead = 4 * (8 + 1024 + 8);
-struct PagedWs {
-    int* head;        // [0] q, [1] blocks, [2] units; [3] wide units; from [8] the prefix
-    int* again;       // [seqs][nkv]: outputs of one block that have to be computed again
-    float* narrow;    // [2 blocks][16][hd + 2]
-    WideUnit* units;  // followed by their split counts
-    float* wide;      // [units][64][hd + 2]
-};
 
 template <int HD, int KS, int COLS>
 struct PagedBlock {
@@ -393,7 +399,7 @@ struct TilePages {
         page = tile < end && tile * kTTile <= last ? page_at(p.step, p.kv, s, tile * kTTile / p.kv.page) : -1;
         if (p.kv.i8) {
             const size_t at = static_cast<size_t>(max(page, 0)) * p.kv.nkv + kh;
-            ks = page >= 0 ? p.kv.k_scale[at] : 0.0f;
+            ks = page >= 0 ? p.kv.k_scale[at] : 1.0f;
             vs = page >= 0 ? p.kv.v_scale[at] : 0.0f;
         }
     }
@@ -426,6 +432,13 @@ __device__ __forceinline__ TileBase<I8, HD> tile_base(const PagedAttnLaunch& p, 
     return b;
 }
 
+// The factor of a tile's scores in the exponent of 2.  A page of zeros has the scale 0, and a masked score of minus
+// infinity times 0 is no number: another factor of its scores, all 0, does as well.
+__device__ __forceinline__ float tile_scale(float column, float page) {
+    const float f = column * page;
+    return f == 0.0f ? 1.0e-37f : f;
+}
+
 // the first n of eight fp16 values, 0 for the others
 __device__ __forceinline__ u32x4 first_halves(u32x4 v, int n) {
 #pragma unroll
@@ -433,12 +446,106 @@ __device__ __forceinline__ u32x4 first_halves(u32x4 v, int n) {
     return v;
 }
 
+template <int HD>
+struct WideShape {
+    static constexpr int CT = 2, KS = HD == 128 ? 4 : 2;
+    static constexpr int kThreads = kWave * CT * KS, kKeys = kTTile * KS, kCols = kWideCols;
+    using F = PagedBlock<HD, KS, kWideCols>;
+    struct Q {  // of QueryStage
+        static constexpr int kThreads = WideShape::kThreads, kCols = kWideCols;
+    };
+    static constexpr int kBuf = kKeys * HD;  // halves
+    static constexpr size_t kKvBytes = 4 * static_cast<size_t>(kBuf) * 2;
+    static constexpr size_t kLds = kKvBytes > F::kOutBytes ? kKvBytes : F::kOutBytes;
+    static_assert(QueryStage<Q, HD>::kBytes <= kLds && kLds + 64 <= 160 * 1024, "LDS");
+};
+
+// The units of the sequences that the narrow kernel does not take, by one block: a row tile's keys are split in proportion
+// to their number where there are fewer tiles than blocks that fill the card.
+template <int THREADS, int HD>
+__device__ void plan_wide(const PagedAttnLaunch& p, const PagedWs& ws, int* pre, int* red) {
+    constexpr int kWaves = THREADS / kWave, kPer = (1024 + THREADS - 1) / THREADS, kKeys = WideShape<HD>::kKeys;
+    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kWideCols / group, seqs = p.step.seqs;
+    auto block_scan = [&](int v, int& all) {  // before this thread; all: of every thread
+        const int in = wave_scan_int(v);
+        __syncthreads();
+        if (lane == kWave - 1) red[wid] = in;
+        __syncthreads();
+        int before = in - v;
+        all = 0;
+        for (int i = 0; i < kWaves; ++i) {
+            before += i < wid ? red[i] : 0;
+            all += red[i];
+        }
+        return before;
+    };
+    int base = 0;
+    for (int i = 0; i < kPer; ++i) {
+        const int s = i * THREADS + threadIdx.x;
+        int n = 0;
+        if (s < seqs) {
+            const SeqRows r = seq_rows(p.step, s);
+            if (r.rows > 0 && !is_narrow(r.rows, group)) n = (r.rows + T - 1) / T;
+        }
+        int all;
+        const int before = block_scan(n, all);
+        if (s < seqs) pre[s] = base + before;
+        base += all;
+    }
+    __syncthreads();
+    const int tiles = base;
+    auto tile_at = [&](int f, int& s, int& tile) {  // chunks of row tile f
+        int lo = 0, hi = seqs - 1;  // the last sequence with pre <= f
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (pre[mid] <= f)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        s = lo;
+        tile = f - pre[lo];
+        const SeqKeys k(p, lo);
+        return max(0, k.last(min((tile + 1) * T, k.r.rows) - 1)) / kKeys + 1;
+    };
+    int64_t chunks = 0;
+    for (int f0 = 0; f0 < tiles; f0 += THREADS) {
+        const int f = f0 + threadIdx.x;
+        int s, tile, all;
+        block_scan(f < tiles ? tile_at(f, s, tile) : 0, all);
+        chunks += all;
+    }
+    const int room = kWideBlocks / nkv;
+    int units = 0;  // unit count, slots << 16
+    for (int f0 = 0; f0 < tiles; f0 += THREADS) {
+        const int f = tiles - 1 - (f0 + static_cast<int>(threadIdx.x));  // later rows, which see more, first
+        int s = 0, tile = 0, n = 0, c = 0;
+        if (f >= 0) {
+            c = tile_at(f, s, tile);
+            n = static_cast<int>(min(static_cast<int64_t>(c), max(int64_t(1), static_cast<int64_t>(c) * room / chunks)));
+        }
+        int all;
+        const int at = units + block_scan(n + (n > 1 ? n << 16 : 0), all);
+        units += all;
+        for (int i = 0; i < n; ++i) {
+            const int u = (at & 0xffff) + i, slot = (at >> 16) + i;
+            ws.units[u] = WideUnit{s, tile, static_cast<int>(static_cast<int64_t>(c) * i / n), static_cast<int>(static_cast<int64_t>(c) * (i + 1) / n), n, slot};
+            if (n > 1) ws.first[slot] = at & 0xffff;
+        }
+    }
+    if (threadIdx.x == 0) {
+        ws.head[4] = units & 0xffff;
+        ws.head[5] = units >> 16;
+    }
+}
+
 // Up to 16 columns, q's hi parts in the tile's first 16 columns and its lo parts in the others: one MFMA does what two
 // do, a lane and its neighbour 16 lanes on add their scores and take eight keys each, and the weights' hi and lo parts go
 // back into the two halves.  Each wave takes its own 32-key tiles, K and V straight into registers, the next tile's on
 // their way meanwhile; no barrier before the waves join.
 template <int HD, bool I8, int KS>
-__global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(PagedAttnLaunch p, PagedWs ws, int has_wide) {
+__global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(PagedAttnLaunch p, PagedWs ws) {
     using F = PagedBlock<HD, KS, kNarrowCols>;
     using Q = QueryStage<F, HD>;
     constexpr int kSteps = HD / 16, kDimTiles = HD / 32;
@@ -450,6 +557,10 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(P
     const int cl = lane & 31, g = lane >> 5, col = cl & 15, part = cl >> 4;
     const uint32_t inv_t = (65535u + T) / T;
     const int ch = static_cast<int>(col * inv_t >> 16), ctok = col - ch * T;
+    if (blockIdx.x == kNarrowBlocks) {
+        plan_wide<F::kThreads, HD>(p, ws, pre, red);
+        return;
+    }
     const NarrowWork w = narrow_work<F::kThreads>(p, pre, red);
     if (blockIdx.x == 0) {
         for (int i = threadIdx.x; i <= p.step.seqs; i += F::kThreads) ws.head[8 + i] = pre[i];
@@ -511,7 +622,7 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(P
         for (int j = 0; j < kDimTiles; ++j) o[j] = floatx16{};
         for (int i = 0; i < n; ++i) {
             const int key0 = (tp.first + i * KS) * kTTile;
-            const float kscale = I8 ? sscale * next.ks : sscale, vscale = I8 ? next.vs : 1.0f;
+            const float kscale = I8 ? tile_scale(sscale, next.ks) : sscale, vscale = I8 ? next.vs : 1.0f;
             const bool valid = next.valid;
             floatx16 st = floatx16{};
 #pragma unroll
@@ -602,13 +713,12 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(P
 // The partial outputs of a sequence and kv head joined (nothing to do where one block had all of its tiles).
 constexpr int kMergeThreads = 512;
 template <int HD>
-__global__ void __launch_bounds__(kMergeThreads) paged_narrow_merge_kernel(PagedAttnLaunch p, PagedWs ws) {
-    extern __shared__ float smem[];  // attend_paged_row's
+__device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s, int kh, float* smem) {
     __shared__ float fac[kNarrowCols][kNarrowBlocks], total[kNarrowCols];
     __shared__ float4 sums[kMergeThreads];
     __shared__ int redo;
     constexpr int kQuads = HD / 4, kSlot = kNarrowCols * (HD + 2);
-    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kNarrowCols / group, s = blockIdx.x, kh = blockIdx.y;
+    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kNarrowCols / group;
     const NarrowWork w{ws.head[0], ws.head[1], ws.head[2]};
     const int u0 = ws.head[8 + s], units = ws.head[9 + s] - u0;
     const SeqRows sr = seq_rows(p.step, s);
@@ -671,50 +781,346 @@ __global__ void __launch_bounds__(kMergeThreads) paged_narrow_merge_kernel(Paged
     for (int t = 0; t < sr.rows; ++t) attend_paged_row<kMergeThreads>(p, s, sr, sr.row0 + t, kh, smem);
 }
 
-// Rows of the sequences that the narrow kernel does not take, in the general form.
-__global__ void __launch_bounds__(256) paged_rest_row_kernel(PagedAttnLaunch p) {
-    extern __shared__ float smem[];
-    const int row = blockIdx.x;
-    const int s = __builtin_amdgcn_readfirstlane(seq_of_row(p.step, row));
-    if (s >= p.step.seqs) return;
-    const SeqRows sr = seq_rows(p.step, s);
-    if (row < sr.row0 || row - sr.row0 >= sr.rows || is_narrow(sr.rows, p.nq / p.kv.nkv)) return;
-    attend_paged_row<256>(p, s, sr, row, blockIdx.y, smem);
+// 64 columns: CT column tiles x KS key waves.  K and V are staged chunk by chunk (32 KS keys, shared by the column tiles) in
+// LDS as the pages hold them (8-bit codes as fp16), twice each: one barrier a chunk, the next chunk's loads over a whole
+// chunk ahead, and a chunk's products with V beside the next one's softmax.
+template <int HD, bool I8>
+__global__ void __launch_bounds__(WideShape<HD>::kThreads, (WideShape<HD>::kThreads / kWave + 3) / 4) paged_wide_kernel(PagedAttnLaunch p, PagedWs ws) {
+    using S = WideShape<HD>;
+    using Q = QueryStage<typename S::Q, HD>;
+    constexpr int CT = S::CT, KS = S::KS, kSteps = HD / 16, kDimTiles = HD / 32, kKeys = S::kKeys;
+    constexpr uint32_t es = I8 ? 1u : 2u;
+    constexpr int kKLoads = HD / (I8 ? 32 : 16) / CT, kVLoads = (I8 ? 2 : 4) * HD / 64 / CT;  // of a wave and chunk, 1 KiB each
+    extern __shared__ uint4 paged_lds[];
+    __shared__ int redo;
+    const int nkv = p.kv.nkv, kh = blockIdx.x % nkv, group = p.nq / nkv, T = kWideCols / group;
+    const int unit = blockIdx.x / nkv;
+    if (unit >= ws.head[4]) return;
+    const WideUnit un = ws.units[unit];
+    const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int ct = wid % CT, ks = wid / CT, cl = lane & 31, g = lane >> 5;
+    const uint32_t inv_t = (65535u + T) / T;  // c / T = c inv_t >> 16 for c < 64
+    const int s = __builtin_amdgcn_readfirstlane(un.seq), t0 = __builtin_amdgcn_readfirstlane(un.tile) * T;
+    const int begin = __builtin_amdgcn_readfirstlane(un.begin), end = __builtin_amdgcn_readfirstlane(un.end);
+    const SeqKeys sk(p, s);
+    const int ntok = min(T, sk.r.rows - t0);
+    Q query;
+    query.load(p.q + static_cast<size_t>(sk.r.row0 + t0) * p.q_stride, p.q_stride, kh, ntok, group, T, inv_t);
+    const int col = ct * kTTile + cl, ch = static_cast<int>(col * inv_t >> 16), ctok = col - ch * T;
+    const bool live = ch < group && ctok < ntok;
+    const int last = sk.last(t0 + ntok - 1), sure = sk.last(t0), qpos = live ? sk.last(t0 + ctok) : -1;
+    TilePages tp;
+    tp.first = begin * KS + ks;
+    tp.step = KS;
+    tp.end = end * KS;
+    struct Ref {  // a wave's 32 keys of a chunk
+        int page;
+        float ks, vs;
+    };
+    auto ref_of = [&](int c) {
+        const int i = c - begin;
+        if ((i & 63) == 0) tp.fill(p, s, kh, i, last);  // wave-uniform; chunks are asked for in their order
+        Ref r;
+        r.page = __builtin_amdgcn_readlane(tp.page, i & 63);
+        r.ks = I8 ? readlane_f32(tp.ks, i & 63) : 1.0f;
+        r.vs = I8 ? readlane_f32(tp.vs, i & 63) : 1.0f;
+        return r;
+    };
+    // (without a page, or past `end`: loads read 0)
+    auto rows_of = [&](const void* pool, const Ref& r, int c, uint32_t skip) {
+        const uint32_t off = static_cast<uint32_t>((c * KS + ks) * kTTile & (p.kv.page - 1)) * skip;
+        return buf_rsrc(static_cast<const uint8_t*>(pool) + page_head(p.kv, max(r.page, 0), kh) * es + off,
+                        r.page >= 0 ? static_cast<uint32_t>(p.kv.page) * HD * es - off : 0u);
+    };
+    u32x4 kr[kKLoads], vr[kVLoads];
+    auto load_k = [&](const Ref& r, int c) {
+        const __amdgpu_buffer_rsrc_t rs = rows_of(p.kv.k, r, c, 16u);
+        const uint32_t at = (static_cast<uint32_t>(2 * ct * kKLoads + g) * p.kv.page + cl) * 16u;
+#pragma unroll
+        for (int u = 0; u < kKLoads; ++u) kr[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, at, u * 32u * p.kv.page, 0);
+    };
+    auto load_v = [&](const Ref& r, int c) {
+        const __amdgpu_buffer_rsrc_t rs = rows_of(p.kv.v, r, c, HD * es);
+#pragma unroll
+        for (int u = 0; u < kVLoads; ++u)
+            vr[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, static_cast<uint32_t>(ct * kVLoads * kWave + lane) * 16u, u * 1024, 0);
+    };
+    // LDS, in halves: K [2][KS][HD / 8][32][8], V [2][KS][4][HD][8]
+    _Float16* Kl = reinterpret_cast<_Float16*>(paged_lds);
+    _Float16* Vl = Kl + 2 * S::kBuf;
+    auto both_halves = [&](_Float16* at, int next, u32x4 c) {  // sixteen codes: two pieces, `next` halves apart
+        const u32x2 a = codes_to_half(c[0]), b = codes_to_half(c[1]), d = codes_to_half(c[2]), e = codes_to_half(c[3]);
+        *reinterpret_cast<u32x4*>(at) = u32x4{a.x, a.y, b.x, b.y};
+        *reinterpret_cast<u32x4*>(at + next) = u32x4{d.x, d.y, e.x, e.y};
+    };
+    auto store_k = [&](int c) {
+        _Float16* d = Kl + (c & 1) * S::kBuf + ks * kTTile * HD;
+#pragma unroll
+        for (int u = 0; u < kKLoads; ++u) {
+            const int b = 2 * (ct * kKLoads + u);  // block of dims of lane 0
+            if constexpr (I8)
+                both_halves(d + (2 * (b + g) * 32 + cl) * 8, 256, kr[u]);
+            else
+                *reinterpret_cast<u32x4*>(d + (b * 32 + lane) * 8) = kr[u];
+        }
+    };
+    auto store_v = [&](int c, bool masked) {
+        _Float16* d = Vl + (c & 1) * S::kBuf + ks * kTTile * HD;
+#pragma unroll
+        for (int u = 0; u < kVLoads; ++u) {
+            const int i = ct * kVLoads + u, pb = i / (HD / 64), dim = i % (HD / 64) * 64 + lane;
+            if constexpr (I8) {
+                both_halves(d + (2 * pb * HD + dim) * 8, HD * 8, vr[u]);
+            } else {
+                if (masked) vr[u] = first_halves(vr[u], last + 1 - ((c * KS + ks) * kTTile + 8 * pb));
+                *reinterpret_cast<u32x4*>(d + (pb * HD + dim) * 8) = vr[u];
+            }
+        }
+    };
+    Ref r0 = ref_of(begin), r1;
+    load_k(r0, begin);
+    load_v(r0, begin);
+    half8 qhi[kSteps], qlo[kSteps];  // lane supplies dims 16 t + 8 g .. + 7 of its column
+    query.store(paged_lds);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+        qhi[t] = Q::part(paged_lds, 0, col, 16 * t + 8 * g);
+        qlo[t] = Q::part(paged_lds, 1, col, 16 * t + 8 * g);
+    }
+    const float sscale = Q::scale(paged_lds, col);
+    __syncthreads();  // every wave has its q: K and V may take its place
+    store_k(begin);
+    r1 = ref_of(begin + 1);
+    __syncthreads();
+    load_k(r1, begin + 1);
+    float m = -1.0e30f, l = 0.0f;  // reference of the exponents, this lane's part of the sum
+    floatx16 o[kDimTiles];
+#pragma unroll
+    for (int j = 0; j < kDimTiles; ++j) o[j] = floatx16{};
+    half8 phi[2], plo[2];  // the weights of the chunk before
+    auto add_values = [&](int c) {
+        const _Float16* vb = Vl + (c & 1) * S::kBuf + (ks * 4 * HD + g * HD + cl) * 8;
+#pragma unroll
+        for (int j = 0; j < kDimTiles; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const half8 a = *reinterpret_cast<const half8*>(vb + (2 * h * HD + 32 * j) * 8);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, plo[h], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, phi[h], o[j], 0, 0, 0);
+            }
+    };
+    const int krow = (ks * (HD / 8) + g) * 32 + key_of_row<false>(cl);
+    // One chunk: its scores, the values of the chunk before (the matrix cores work on them while the softmax runs), the
+    // next keys and this chunk's values into LDS.  One barrier: both are double-buffered.
+    auto chunk = [&](int c, auto first, auto masked) {
+        constexpr bool FIRST = decltype(first)::value, MASKED = decltype(masked)::value;
+        const int key0 = c * kKeys + ks * kTTile;
+        floatx16 st = floatx16{};
+        const _Float16* kb = Kl + (c & 1) * S::kBuf + krow * 8;
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t) {
+            const half8 a = *reinterpret_cast<const half8*>(kb + t * 512);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qlo[t], st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qhi[t], st, 0, 0, 0);
+        }
+        // (past `end`: loads read 0 into buffers that no one reads)
+        store_k(c + 1);
+        store_v(c, MASKED);
+        const Ref r2 = ref_of(c + 2);
+        load_v(r1, c + 1);
+        load_k(r2, c + 2);
+        if constexpr (!FIRST) add_values(c - 1);
+        const float kscale = I8 ? tile_scale(sscale, r0.ks) : sscale, vscale = r0.vs;
+        if (MASKED || r0.page < 0) {
+            const int see = r0.page < 0 ? -1 : qpos - (key0 + 8 * g);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) st[v] = 16 * (v / 8) + v % 8 <= see ? st[v] : -INFINITY;
+        }
+        float mc = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mc = fmaxf(mc, st[v]);
+        mc = pair32_max(mc) * kscale;
+        if constexpr (I8) mc += scale_exponent(vscale);
+        // the reference moves only when a column's max has outgrown it (rarely after the first chunks)
+        const bool up = mc > m + kSlack;
+        const float to = up ? mc : m, f = __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= f;
+        const float off = kRaise - m;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(fmaf(st[8 * h + e], kscale, off));
+                l += x[e];
+                if constexpr (I8) {
+                    x[e] *= vscale;
+                    asm("" : "+v"(x[e]));  // the rounded product: hi and lo would else be taken from two roundings of it
+                }
+            }
+            split8(x, phi[h], plo[h]);
+        }
+        if (__builtin_amdgcn_ballot_w64(up)) {
+#pragma unroll
+            for (int j = 0; j < kDimTiles; ++j) o[j] *= f;
+        }
+        r0 = r1;
+        r1 = r2;
+        __syncthreads();  // the next keys and these values are staged; every wave is done with the buffers they replace
+    };
+    const int clear = min(end, max(begin, (sure + 1) / kKeys));  // chunks [begin, clear) that every column sees whole
+    int c = begin;
+    if (c < clear)
+        chunk(c++, std::true_type{}, std::false_type{});
+    else
+        chunk(c++, std::true_type{}, std::true_type{});
+    for (; c < clear; ++c) chunk(c, std::false_type{}, std::false_type{});
+    for (; c < end; ++c) chunk(c, std::false_type{}, std::true_type{});
+    add_values(end - 1);
+    float* part_out = un.splits > 1 ? ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * kWideCols * (HD + 2) : nullptr;
+    finish_paged<HD, CT, KS, kWideCols, false>(p, sk.r, kh, t0, ntok, T, inv_t, part_out, ws.again_wide + unit * nkv + kh, live, o, m, l, paged_lds,
+                                               &redo);
 }
 
-static size_t again_bytes(int nkv) { return (sizeof(int) * 1024 * nkv + 15) / 16 * 16; }
-static PagedWs paged_ws(float* base, int hd, int nkv) {
+// The splits of a row tile joined, each slot's block a share of the columns; and outputs that have to be computed again.
+template <int HD>
+__device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int block, int blocks, float* smem) {
+    __shared__ float fac[kWideCols + kWideBlocks], total[kWideCols];  // a block's columns times the splits
+    __shared__ int list[kMergeThreads], count, redo;
+    constexpr int kQuads = HD / 4, kSlot = kWideCols * (HD + 2);
+    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kWideCols / group;
+    const int units = ws.head[4], slots = ws.head[5], slot = block / nkv, kh = block % nkv;
+    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+    if (slot < slots) {
+        const WideUnit un = ws.units[ws.first[slot]];
+        const SeqRows sr = seq_rows(p.step, un.seq);
+        const int n = un.splits, k = slot - un.slot, t0 = un.tile * T, ntok = min(T, sr.rows - t0);
+        const int c0 = kWideCols * k / n, c1 = kWideCols * (k + 1) / n;
+        const size_t stride = static_cast<size_t>(nkv) * kSlot;
+        const float* base = ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * kSlot;
+        for (int c = c0 + wid; c < c1; c += kMergeThreads / kWave) {
+            float M = -INFINITY, L = 0.0f;
+            const bool on = c / T < group && c % T < ntok;  // (others' sums were not written)
+            for (int b = lane; on && b < n; b += kWave) M = fmaxf(M, base[b * stride + kWideCols * HD + 2 * c]);
+            M = wave_max(M);
+            for (int b = lane; on && b < n; b += kWave) {
+                const float2 ml = *reinterpret_cast<const float2*>(base + b * stride + kWideCols * HD + 2 * c);
+                const float f = __builtin_amdgcn_exp2f(ml.x - M);
+                fac[(c - c0) * n + b] = f;
+                L += f * ml.y;
+            }
+            L = wave_sum(L);
+            if (lane == 0) total[c] = L;
+        }
+        if (threadIdx.x == 0) redo = 0;
+        __syncthreads();
+        bool bad = false;
+        for (int i = threadIdx.x; i < (c1 - c0) * kQuads; i += kMergeThreads) {
+            const int c = c0 + i / kQuads, d = 4 * (i % kQuads), hc = c / T, tc = c % T;
+            if (hc >= group || tc >= ntok) continue;
+            float4 r = {};
+#pragma unroll 4
+            for (int b = 0; b < n; ++b) add_scaled(r, fac[(c - c0) * n + b], *reinterpret_cast<const float4*>(base + b * stride + c * HD + d));
+            const size_t row = sr.row0 + t0 + tc, colm = static_cast<size_t>(kh * group + hc) * HD + d;
+            bad |= write_paged_quad(r, total[c], p.gate ? p.gate + row * p.q_stride + colm : nullptr, p.out + row * p.out_stride + colm);
+        }
+        if (bad) redo = 1;
+        __syncthreads();
+        // (another block of the tile may write the same rows' other columns: the general form writes them all, with values
+        // that differ from the joined ones by roundings only, so each block takes its own columns' rows)
+        if (__builtin_expect(redo, 0)) {
+            for (int c = c0; c < c1; ++c)
+                if (c / T < group && c % T < ntok) attend_paged_row<kMergeThreads>(p, un.seq, sr, sr.row0 + t0 + c % T, kh, smem, c / T, c / T + 1);
+        }
+        __syncthreads();
+    }
+    // the units without a split, a share of them by each block
+    const int all = units * nkv, per = (all + blocks - 1) / blocks;
+    for (int i0 = block * per; i0 < min(all, (block + 1) * per); i0 += kMergeThreads) {
+        const int i = i0 + threadIdx.x;
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        if (i < min(all, (block + 1) * per) && ws.units[i / nkv].splits == 1 && ws.again_wide[i]) list[atomicAdd(&count, 1)] = i;
+        __syncthreads();
+        const int n = count;
+        for (int j = 0; j < n; ++j) {
+            const int at = list[j];
+            const WideUnit un = ws.units[at / nkv];
+            const SeqRows sr = seq_rows(p.step, un.seq);
+            for (int t = un.tile * T; t < min((un.tile + 1) * T, sr.rows); ++t) attend_paged_row<kMergeThreads>(p, un.seq, sr, sr.row0 + t, at % nkv, smem);
+        }
+        __syncthreads();
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedAttnLaunch p, PagedWs ws, int narrow_blocks, int wide_blocks) {
+    extern __shared__ float smem[];  // attend_paged_row's
+    if (static_cast<int>(blockIdx.x) < narrow_blocks)
+        merge_narrow<HD>(p, ws, blockIdx.x / p.kv.nkv, blockIdx.x % p.kv.nkv, smem);
+    else
+        merge_wide<HD>(p, ws, blockIdx.x - narrow_blocks, wide_blocks, smem);
+}
+
+static PagedWs paged_ws(float* base, int hd, int nkv, size_t* bytes) {
     PagedWs w{};
-    w.head = reinterpret_cast<int*>(base);
-    w.again = w.head + kWsHead / 4;
-    w.narrow = base + (kWsHead + again_bytes(nkv)) / 4;
-    w.wide = w.narrow + static_cast<size_t>(2) * kNarrowBlocks * kNarrowCols * (hd + 2);
+    char* at = reinterpret_cast<char*>(base);
+    auto take = [&](size_t n) {
+        char* r = at;
+        at += (n + 15) / 16 * 16;
+        return r;
+    };
+    w.head = reinterpret_cast<int*>(take(kWsHead));
+    w.again = reinterpret_cast<int*>(take(sizeof(int) * 1024 * nkv));
+    w.again_wide = reinterpret_cast<int*>(take(sizeof(int) * kMostUnits * nkv));
+    w.first = reinterpret_cast<int*>(take(sizeof(int) * kWideBlocks));
+    w.units = reinterpret_cast<WideUnit*>(take(sizeof(WideUnit) * kMostUnits));
+    w.narrow = reinterpret_cast<float*>(take(sizeof(float) * 2 * kNarrowBlocks * kNarrowCols * (hd + 2)));
+    w.wide = reinterpret_cast<float*>(take(sizeof(float) * std::max(kWideBlocks, nkv) * kWideCols * (hd + 2)));
+    if (bytes) *bytes = at - reinterpret_cast<char*>(base);
     return w;
 }
 
 size_t paged_attn_workspace_bytes(int nq, int nkv, int head_dim) {
-    if (nkv <= 0 || nq <= 0 || nq % nkv || nq / nkv > kPagedMaxGroup || head_dim <= 0 || head_dim > 256 || head_dim % 16) return 0;
+    if (nkv <= 0 || nkv > 256 || nq <= 0 || nq % nkv || nq / nkv > kPagedMaxGroup || head_dim <= 0 || head_dim > 256 || head_dim % 16) return 0;
     if (head_dim != 128 && head_dim != 256) return 16;
-    return kWsHead + again_bytes(nkv) + sizeof(float) * 2 * kNarrowBlocks * kNarrowCols * (head_dim + 2);
+    size_t n;
+    paged_ws(nullptr, head_dim, nkv, &n);
+    return n;
+}
+
+template <typename Kernel>
+static hipError_t allow_lds(Kernel kernel, size_t bytes) {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
 }
 
 template <int HD, bool I8>
 static hipError_t launch_paged_heads(const PagedAttnLaunch& p, hipStream_t s) {
     constexpr int KS = HD == 128 ? 8 : 4;
     using F = PagedBlock<HD, KS, kNarrowCols>;
+    using S = WideShape<HD>;
     constexpr size_t kLds = std::max(F::kOutBytes, QueryStage<F, HD>::kBytes);
-    const int group = p.nq / p.kv.nkv;
+    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kWideCols / group;
     const bool wide = p.step.max_rows * static_cast<int64_t>(group) > kNarrowCols;
-    const PagedWs ws = paged_ws(p.ws, HD, p.kv.nkv);
+    const PagedWs ws = paged_ws(p.ws, HD, nkv, nullptr);
     const size_t row_lds = paged_row_lds(group, HD);
-    auto kernel = &paged_narrow_kernel<HD, I8, KS>;
-    if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
-        e != hipSuccess)
-        return e;
-    hipLaunchKernelGGL(kernel, dim3(kNarrowBlocks), dim3(F::kThreads), kLds, s, p, ws, wide);
+    if (hipError_t e = allow_lds(&paged_narrow_kernel<HD, I8, KS>, kLds); e != hipSuccess) return e;
+    hipLaunchKernelGGL((paged_narrow_kernel<HD, I8, KS>), dim3(kNarrowBlocks + wide), dim3(F::kThreads), kLds, s, p, ws);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    hipLaunchKernelGGL(paged_narrow_merge_kernel<HD>, dim3(p.step.seqs, p.kv.nkv), dim3(kMergeThreads), row_lds, s, p, ws);
-    if (wide) hipLaunchKernelGGL(paged_rest_row_kernel, dim3(p.step.rows, p.kv.nkv), dim3(256), row_lds, s, p);
+    int wide_blocks = 0;
+    if (wide) {
+        // row tiles of any division of the rows among the sequences, and the splits on top of them
+        const int tiles = p.step.rows / T + std::min(p.step.seqs, p.step.rows);
+        wide_blocks = std::max(1, kWideBlocks / nkv) * nkv;
+        if (hipError_t e = allow_lds(&paged_wide_kernel<HD, I8>, S::kLds); e != hipSuccess) return e;
+        hipLaunchKernelGGL((paged_wide_kernel<HD, I8>), dim3(static_cast<unsigned>(tiles + kWideBlocks / nkv) * nkv), dim3(S::kThreads), S::kLds, s, p, ws);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    const size_t merge_lds = row_lds;
+    if (hipError_t e = allow_lds(&paged_merge_kernel<HD>, merge_lds); e != hipSuccess) return e;
+    hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3(p.step.seqs * nkv + wide_blocks), dim3(kMergeThreads), merge_lds, s, p, ws, p.step.seqs * nkv, wide_blocks);
     return hipGetLastError();
 }
 
