@@ -167,128 +167,112 @@ struct SeqKeys {
     }
 };
 
+__device__ __forceinline__ bool is_narrow(int rows, int group) { return rows > 0 && rows * group <= kNarrowCols; }
+__device__ __forceinline__ int tiles_of(int last) { return max(0, last) / kTTile + 1; }
+
+__device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    const int a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31), c = b + __builtin_amdgcn_readlane(v, 47);
+    const int row = (threadIdx.x & (kWave - 1)) >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
+}
+
 // The narrow kernel's work: sequences of up to 16 columns, their 32-key tiles in units of q, for each kv head, one behind
 // the other; `blocks` blocks take equal ranges of them.  Few tiles: a block has one unit, and a unit lies in one
 // sequence and head.  Many: q = 1, and a block's range may end inside one and go on in the next.
-struct NarrowWork {
-    int q, blocks;
-    int units;  // of all sequences, one kv head
-};
+// Each wave finds its block's place by itself, 64 sequences in its lanes at a time: no barrier, no launch before.
 constexpr int kMinTiles = 2;   // smallest unit of few tiles
 constexpr int kMaxTiles = 16;  // largest
+struct NarrowItem {
+    int s, kh, unit, units;  // of the sequence and head: the unit asked for, and how many there are
+};
+struct NarrowWork {
+    int q, blocks, units, per, rem;  // units: all sequences, one kv head; a block has per, the first rem one more
+    int group, nkv;
+    int before;           // lane c: units of the sequences up to 64 c + 63
+    int held, in, tiles;  // sequences 64 held + lane: units up to it, its tiles
 
-__device__ __forceinline__ bool is_narrow(int rows, int group) { return rows > 0 && rows * group <= kNarrowCols; }
-__device__ __forceinline__ int tiles_of(int last) { return max(0, last) / kTTile + 1; }
-__device__ __forceinline__ int64_t range_begin(const NarrowWork& w, int nkv, int b) {
-    return static_cast<int64_t>(w.units) * nkv * b / w.blocks;
-}
-
-__device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const int u = __shfl_up(v, o, kWave);
-        v += (threadIdx.x & (kWave - 1)) >= o ? u : 0;
+    __device__ __forceinline__ int load(const PagedAttnLaunch& p, int c) const {
+        const int s = c * kWave + static_cast<int>(threadIdx.x & (kWave - 1));
+        if (s >= p.step.seqs) return 0;
+        const SeqKeys k(p, s);
+        return is_narrow(k.r.rows, group) ? tiles_of(k.last(k.r.rows - 1)) : 0;
     }
-    return v;
-}
-
-// Units before each sequence into pre[0 .. seqs], by the whole block.
-template <int THREADS>
-__device__ NarrowWork narrow_work(const PagedAttnLaunch& p, int* pre, int* red) {
-    constexpr int kWaves = THREADS / kWave, kPer = (1024 + THREADS - 1) / THREADS;
-    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, group = p.nq / p.kv.nkv;
-    int tiles[kPer], sum = 0, active = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int s = i * THREADS + threadIdx.x;
-        tiles[i] = 0;
-        if (s < p.step.seqs) {
-            const SeqKeys k(p, s);
-            if (is_narrow(k.r.rows, group)) {
-                tiles[i] = tiles_of(k.last(k.r.rows - 1));
-                ++active;
-            }
+    __device__ __forceinline__ explicit NarrowWork(const PagedAttnLaunch& p) : group(p.nq / p.kv.nkv), nkv(p.kv.nkv) {
+        const int lane = threadIdx.x & (kWave - 1), chunks = (p.step.seqs + kWave - 1) / kWave;
+        int active = 0, sum = 0;
+        for (int c = 0; c < chunks; ++c) {
+            tiles = load(p, c);
+            sum += tiles;
+            active += __popcll(__builtin_amdgcn_ballot_w64(tiles > 0));
         }
-        sum += tiles[i];
-    }
-    {
-        int a = active, t = sum;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            a += __shfl_xor(a, o, kWave);
-            t += __shfl_xor(t, o, kWave);
+        const int64_t all = static_cast<int64_t>(__builtin_amdgcn_readlane(wave_scan_int(sum), kWave - 1)) * nkv;
+        // the smallest unit with which every unit has a block of its own
+        const int room = kNarrowBlocks - min(active * nkv, kNarrowBlocks);
+        if (room > 0 && all <= kMaxTiles * room)
+            q = max((static_cast<int>(all) + room - 1) / room, kMinTiles);
+        else
+            q = 1 + static_cast<int>(all >> 30);  // (units are counted in 32 bits)
+        before = 0;
+        for (int c = 0; c < chunks; ++c) {
+            if (chunks > 1) tiles = load(p, c);
+            in = wave_scan_int((tiles + q - 1) / q);
+            const int n = __builtin_amdgcn_readlane(in, kWave - 1);
+            before += lane >= c ? n : 0;
         }
-        if (lane == 0) {
-            red[wid] = a;
-            red[kWaves + wid] = t;
+        held = chunks - 1;
+        units = __builtin_amdgcn_readlane(before, kWave - 1);
+        const int total = units * nkv;
+        blocks = min(kNarrowBlocks, total);
+        per = total / max(blocks, 1);
+        rem = total - per * blocks;
+    }
+    __device__ __forceinline__ int begin(int b) const { return b * per + min(b, rem); }
+    __device__ __forceinline__ int block_of(int x) const {
+        const int edge = rem * (per + 1);
+        return x < edge ? x / (per + 1) : rem + (x - edge) / per;
+    }
+    __device__ __forceinline__ NarrowItem find(const PagedAttnLaunch& p, int x) {
+        const int y = x / nkv;
+        const int c = __popcll(__builtin_amdgcn_ballot_w64(before <= y));
+        const int base = c ? __builtin_amdgcn_readlane(before, c - 1) : 0;
+        if (c != held) {
+            tiles = load(p, c);
+            in = wave_scan_int((tiles + q - 1) / q);
+            held = c;
         }
+        const int n = __popcll(__builtin_amdgcn_ballot_w64(base + in <= y));
+        const int pre = n ? __builtin_amdgcn_readlane(in, n - 1) : 0;
+        NarrowItem it;
+        it.s = c * kWave + n;
+        it.units = __builtin_amdgcn_readlane(in, n) - pre;
+        const int at = x - (base + pre) * nkv;
+        it.kh = at / it.units;
+        it.unit = at - it.kh * it.units;
+        return it;
     }
-    __syncthreads();
-    active = sum = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        active += red[i];
-        sum += red[kWaves + i];
-    }
-    NarrowWork w;
-    // the smallest unit with which every unit has a block of its own
-    const int64_t room = kNarrowBlocks - static_cast<int64_t>(active) * p.kv.nkv;
-    const int64_t fit = room > 0 ? (static_cast<int64_t>(sum) * p.kv.nkv + room - 1) / room : kMaxTiles + 1;
-    w.q = fit <= kMaxTiles ? max(static_cast<int>(fit), kMinTiles) : 1;
-    int base = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int s = i * THREADS + threadIdx.x;
-        const int u = (tiles[i] + w.q - 1) / w.q, in = wave_scan_int(u);
-        if (lane == kWave - 1) red[wid] = in;
-        __syncthreads();
-        int before = base, all = base;
-#pragma unroll
-        for (int j = 0; j < kWaves; ++j) {
-            before += j < wid ? red[j] : 0;
-            all += red[j];
-        }
-        if (s < p.step.seqs) pre[s + 1] = before + in;
-        base = all;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) pre[0] = 0;
-    __syncthreads();
-    w.units = base;
-    w.blocks = static_cast<int>(min(static_cast<int64_t>(kNarrowBlocks), static_cast<int64_t>(base) * p.kv.nkv));
-    return w;
-}
-
-// the sequence whose units hold unit x of nkv heads: the last with nkv pre[s] <= x, by a wave
-__device__ __forceinline__ int seq_of_unit(const int* pre, int seqs, int nkv, int64_t x) {
-    const int lane = threadIdx.x & (kWave - 1);
-    int n = 0;
-    for (int b = 1; b <= seqs; b += kWave) {
-        const int s = b + lane;
-        const uint64_t on = __builtin_amdgcn_ballot_w64(s <= seqs && static_cast<int64_t>(pre[min(s, seqs)]) * nkv <= x);
-        n += __popcll(on);
-        if (on != ~uint64_t(0)) break;
-    }
-    return __builtin_amdgcn_readfirstlane(n);
-}
+};
 
 // Chunks [begin, end) of the keys of a row tile; its `splits` units lie one behind the other, and of a tile with several
 // so do their partial outputs' slots.
 struct WideUnit {
     int seq, tile, begin, end, splits, slot;
 };
-// Workspace: the narrow work's prefix for the merge, the wide kernel's units, partial outputs.
+// Workspace: where the merge finds the narrow sequences' parts, the wide kernel's units, partial outputs.
 struct PagedWs {
-    int* head;        // [0] q, [1] blocks, [2] units; [4] wide units, [5] their slots; from [8] the prefix
-    int* again;       // [seqs][nkv]: outputs of one block that have to be computed again
-    int* again_wide;  // [wide units][nkv]
+    int* head;        // [0] wide units, [1] their slots
+    int4* narrow_at;  // [seqs][nkv]: blocks that share the sequence's tiles, the first of them and its slot, whether a single
+                      // block's output has to be computed again
+    int4* wide_at;    // [wide units][nkv], of those without splits: as above
     int* first;       // [slots]: first unit of the slot's row tile
     WideUnit* units;
     float* narrow;    // [2 blocks][16][hd + 2]
     float* wide;      // [slots][nkv][64][hd + 2]
 };
-constexpr size_t kWsHead = 4 * (8 + 1024 + 8);
+constexpr size_t kWsHead = 16;
 
 template <int HD, int KS, int COLS>
 struct PagedBlock {
@@ -314,11 +298,11 @@ __device__ __forceinline__ bool write_paged_quad(float4 r, float L, const float*
 }
 
 // The key waves of a block's columns joined, then written: a partial output (to part_out: [COLS][HD], then [COLS][2]), or
-// the output, and to *again whether it has to be computed again.  CT column tiles x KS key waves; HALF: hi and lo columns
+// the output, and to *entry whether it has to be computed again.  CT column tiles x KS key waves; HALF: hi and lo columns
 // of one tile.
 template <int HD, int CT, int KS, int COLS, bool HALF, int N>
 __device__ __forceinline__ void finish_paged(const PagedAttnLaunch& p, const SeqRows& sr, int kh, int t0, int ntok, int T, uint32_t inv_t,
-                                             float* part_out, int* again, bool live, const floatx16 (&o)[N], float m, float l, void* lds, int* redo) {
+                                             float* part_out, int4* entry, bool live, const floatx16 (&o)[N], float m, float l, void* lds, int* redo) {
     static_assert(HD == 32 * N, "dim tiles");
     using F = PagedBlock<HD, KS, COLS>;
     constexpr int kThreads = kWave * CT * KS;
@@ -387,7 +371,7 @@ __device__ __forceinline__ void finish_paged(const PagedAttnLaunch& p, const Seq
     if (part_out) return;
     if (bad) *redo = 1;
     __syncthreads();
-    if (threadIdx.x == 0) *again = *redo;
+    if (threadIdx.x == 0) *entry = make_int4(1, 0, 0, *redo);
 }
 
 // Where the tiles of a wave lie: lane i holds the page (and its scales) of the wave's tile i, of 64.
@@ -408,7 +392,6 @@ struct TilePages {
 template <bool I8, int HD>
 struct TileBase {
     __amdgpu_buffer_rsrc_t k, v;
-    float ks, vs;
     int valid;
 };
 // the resources of tile i of a wave's (empty where it has no page: loads then read 0)
@@ -418,10 +401,6 @@ __device__ __forceinline__ TileBase<I8, HD> tile_base(const PagedAttnLaunch& p, 
     if ((i & 63) == 0) tp.fill(p, s, kh, i, last);  // wave-uniform
     TileBase<I8, HD> b;
     const int page = __builtin_amdgcn_readlane(tp.page, i & 63);
-    if constexpr (I8) {
-        b.ks = readlane_f32(tp.ks, i & 63);
-        b.vs = readlane_f32(tp.vs, i & 63);
-    }
     b.valid = page >= 0;
     const int off = (tp.first + i * tp.step) * kTTile & (p.kv.page - 1);
     const size_t head = page_head(p.kv, max(page, 0), kh) * es;
@@ -464,7 +443,7 @@ struct WideShape {
 // to their number where there are fewer tiles than blocks that fill the card.
 template <int THREADS, int HD>
 __device__ void plan_wide(const PagedAttnLaunch& p, const PagedWs& ws, int* pre, int* red) {
-    constexpr int kWaves = THREADS / kWave, kPer = (1024 + THREADS - 1) / THREADS, kKeys = WideShape<HD>::kKeys;
+    constexpr int kWaves = THREADS / kWave, kPer = 1024 / THREADS, kKeys = WideShape<HD>::kKeys;
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
     const int nkv = p.kv.nkv, group = p.nq / nkv, T = kWideCols / group, seqs = p.step.seqs;
     auto block_scan = [&](int v, int& all) {  // before this thread; all: of every thread
@@ -535,8 +514,8 @@ __device__ void plan_wide(const PagedAttnLaunch& p, const PagedWs& ws, int* pre,
         }
     }
     if (threadIdx.x == 0) {
-        ws.head[4] = units & 0xffff;
-        ws.head[5] = units >> 16;
+        ws.head[0] = units & 0xffff;
+        ws.head[1] = units >> 16;
     }
 }
 
@@ -551,7 +530,7 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(P
     constexpr int kSteps = HD / 16, kDimTiles = HD / 32;
     constexpr int kKPieces = HD / (I8 ? 32 : 16), kVPieces = I8 ? kDimTiles : 2 * kDimTiles;
     extern __shared__ uint4 paged_lds[];
-    __shared__ int pre[1025], red[2 * KS], redo;
+    __shared__ int pre[1024], red[KS], redo;
     const int nkv = p.kv.nkv, group = p.nq / nkv, T = kNarrowCols / group;
     const int lane = threadIdx.x & (kWave - 1), ks = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int cl = lane & 31, g = lane >> 5, col = cl & 15, part = cl >> 4;
@@ -561,28 +540,21 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(P
         plan_wide<F::kThreads, HD>(p, ws, pre, red);
         return;
     }
-    const NarrowWork w = narrow_work<F::kThreads>(p, pre, red);
-    if (blockIdx.x == 0) {
-        for (int i = threadIdx.x; i <= p.step.seqs; i += F::kThreads) ws.head[8 + i] = pre[i];
-        if (threadIdx.x == 0) {
-            ws.head[0] = w.q;
-            ws.head[1] = w.blocks;
-            ws.head[2] = w.units;
-        }
-    }
-    if (static_cast<int>(blockIdx.x) >= w.blocks) return;
-    const int64_t begin = range_begin(w, nkv, blockIdx.x), end = range_begin(w, nkv, blockIdx.x + 1);
+    NarrowWork w(p);
+    const int block = blockIdx.x;
+    if (block >= w.blocks) return;
+    const int begin = w.begin(block), end = w.begin(block + 1);
     const uint32_t kat = (static_cast<uint32_t>(g) * p.kv.page + key_of_row<I8>(cl)) * 16u, kstep = 32u * p.kv.page;
     const uint32_t vat = (static_cast<uint32_t>(g) * HD + cl) * 16u;
     const int lane_key = I8 ? 16 * g + 8 * part : 16 * part + 8 * g;  // of the lane's eight slots
-    for (int64_t at = begin; at < end;) {
-        const int s = seq_of_unit(pre, p.step.seqs, nkv, at);
-        const int units = pre[s + 1] - pre[s];
-        const int in = static_cast<int>(at - static_cast<int64_t>(pre[s]) * nkv);
-        const int kh = in / units, u0 = in - kh * units;
-        const int u1 = static_cast<int>(min(static_cast<int64_t>(units), u0 + (end - at)));
-        const bool whole = u0 == 0 && u1 == units;
-        float* part_out = whole ? nullptr : ws.narrow + (2 * static_cast<size_t>(blockIdx.x) + (at == begin ? 0 : 1)) * kNarrowCols * (HD + 2);
+    for (int at = begin; at < end;) {
+        const NarrowItem it = w.find(p, at);
+        const int s = it.s, kh = it.kh, u0 = it.unit, u1 = min(it.units, u0 + (end - at));
+        const bool whole = u0 == 0 && u1 == it.units;
+        const int slot = at == begin ? 0 : 1;
+        float* part_out = whole ? nullptr : ws.narrow + (2 * static_cast<size_t>(block) + slot) * kNarrowCols * (HD + 2);
+        int4* entry = ws.narrow_at + s * nkv + kh;
+        if (u0 == 0 && !whole && threadIdx.x == 0) *entry = make_int4(w.block_of(at + it.units - 1) - block + 1, block, slot, 0);
         at += u1 - u0;
         const SeqKeys sk(p, s);
         const int ntok = sk.r.rows, last = sk.last(ntok - 1), sure = sk.last(0);
@@ -622,7 +594,7 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(P
         for (int j = 0; j < kDimTiles; ++j) o[j] = floatx16{};
         for (int i = 0; i < n; ++i) {
             const int key0 = (tp.first + i * KS) * kTTile;
-            const float kscale = I8 ? tile_scale(sscale, next.ks) : sscale, vscale = I8 ? next.vs : 1.0f;
+            const float kscale = I8 ? tile_scale(sscale, readlane_f32(tp.ks, i & 63)) : sscale, vscale = I8 ? readlane_f32(tp.vs, i & 63) : 1.0f;
             const bool valid = next.valid;
             floatx16 st = floatx16{};
 #pragma unroll
@@ -705,7 +677,7 @@ __global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(P
                 }
             load_v();
         }
-        finish_paged<HD, 1, KS, kNarrowCols, true>(p, sk.r, kh, 0, ntok, T, inv_t, part_out, ws.again + s * nkv + kh, live, o, m, l, paged_lds, &redo);
+        finish_paged<HD, 1, KS, kNarrowCols, true>(p, sk.r, kh, 0, ntok, T, inv_t, part_out, entry, live, o, m, l, paged_lds, &redo);
         __syncthreads();
     }
 }
@@ -717,60 +689,76 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
     __shared__ float fac[kNarrowCols][kNarrowBlocks], total[kNarrowCols];
     __shared__ float4 sums[kMergeThreads];
     __shared__ int redo;
-    constexpr int kQuads = HD / 4, kSlot = kNarrowCols * (HD + 2);
+    constexpr int kQuads = HD / 4, kSlot = kNarrowCols * (HD + 2), kBatch = 4;
     const int nkv = p.kv.nkv, group = p.nq / nkv, T = kNarrowCols / group;
-    const NarrowWork w{ws.head[0], ws.head[1], ws.head[2]};
-    const int u0 = ws.head[8 + s], units = ws.head[9 + s] - u0;
+    const int4 at = ws.narrow_at[s * nkv + kh];
     const SeqRows sr = seq_rows(p.step, s);
-    if (units == 0) return;
-    const int64_t all = static_cast<int64_t>(w.units) * nkv, first = static_cast<int64_t>(u0) * nkv + static_cast<int64_t>(kh) * units;
-    auto block_of = [&](int64_t x) { return static_cast<int>(((x + 1) * w.blocks - 1) / all); };
-    const int b0 = block_of(first), n = block_of(first + units - 1) - b0 + 1;
+    if (!is_narrow(sr.rows, group)) return;
+    const int n = at.x;
     if (n == 1) {
-        if (__builtin_expect(ws.again[s * nkv + kh] != 0, 0))
+        if (__builtin_expect(at.w != 0, 0))
             for (int t = 0; t < sr.rows; ++t) attend_paged_row<kMergeThreads>(p, s, sr, sr.row0 + t, kh, smem);
         return;
     }
-    auto slot_of = [&](int b) {
-        return ws.narrow + (2 * static_cast<size_t>(b) + (range_begin(w, nkv, b) >= first ? 0 : 1)) * kSlot;
-    };
+    // the first block's part, and the following blocks' first ones
+    const float* base = ws.narrow + (2 * static_cast<size_t>(at.y) + at.z) * kSlot;
+    auto part = [&](int b) { return base + (2 * b - (b ? at.z : 0)) * kSlot; };
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, cols = sr.rows * group;
     auto column = [&](int i) { return i / sr.rows * T + i % sr.rows; };  // live column i
+    const int items = cols * kQuads, slices = max(1, kMergeThreads / items);
+    const int first = slices > 1 ? threadIdx.x % items : threadIdx.x, slice = slices > 1 ? threadIdx.x / items : 0;
+    float4 v[kBatch];
+    auto load = [&](int item, int b0) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int b = b0 + u * slices;
+            v[u] = item < items && slice < slices && b < n ? *reinterpret_cast<const float4*>(part(b) + column(item / kQuads) * HD + 4 * (item % kQuads)) : float4{};
+        }
+    };
+    load(first, slice);
     for (int i = wid; i < cols; i += kMergeThreads / kWave) {
         const int c = column(i);
         float M = -INFINITY, L = 0.0f;
-        for (int b = lane; b < n; b += kWave) M = fmaxf(M, slot_of(b0 + b)[kNarrowCols * HD + 2 * c]);
+        float2 ml[kNarrowBlocks / kWave];
+#pragma unroll
+        for (int u = 0; u < kNarrowBlocks / kWave; ++u) {
+            const int b = lane + u * kWave;
+            ml[u] = b < n ? *reinterpret_cast<const float2*>(part(b) + kNarrowCols * HD + 2 * c) : make_float2(-INFINITY, 0.0f);
+            M = fmaxf(M, ml[u].x);
+        }
         M = wave_max(M);
-        for (int b = lane; b < n; b += kWave) {
-            const float2 ml = *reinterpret_cast<const float2*>(slot_of(b0 + b) + kNarrowCols * HD + 2 * c);
-            const float f = __builtin_amdgcn_exp2f(ml.x - M);
-            fac[i][b] = f;
-            L += f * ml.y;
+#pragma unroll
+        for (int u = 0; u < kNarrowBlocks / kWave; ++u) {
+            const float f = __builtin_amdgcn_exp2f(ml[u].x - M);
+            if (lane + u * kWave < n) fac[i][lane + u * kWave] = f;
+            L += f * ml[u].y;
         }
         L = wave_sum(L);
         if (lane == 0) total[i] = L;
     }
     if (threadIdx.x == 0) redo = 0;
     __syncthreads();
-    const int items = cols * kQuads, slices = max(1, kMergeThreads / items);
     bool bad = false;
-    for (int base = 0; base < items; base += kMergeThreads) {
-        const int item = slices > 1 ? threadIdx.x % items : base + threadIdx.x, slice = slices > 1 ? threadIdx.x / items : 0;
+    for (int item = first; item < items; item += kMergeThreads) {  // (more than one round only without slices)
         const int i = item / kQuads, d = 4 * (item % kQuads);
         float4 r = {};
-        const bool on = item < items && slice < slices;
-        if (on) {
-            const float* at = ws.narrow + column(i) * HD + d;
-#pragma unroll 4
-            for (int b = slice; b < n; b += slices) add_scaled(r, fac[i][b], *reinterpret_cast<const float4*>(at + (slot_of(b0 + b) - ws.narrow)));
-        }
+        if (item != first) load(item, 0);
+        if (slice < slices)
+            for (int b0 = slice;;) {
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u)
+                    if (b0 + u * slices < n) add_scaled(r, fac[i][b0 + u * slices], v[u]);
+                b0 += kBatch * slices;
+                if (b0 >= n) break;
+                load(item, b0);
+            }
         if (slices > 1) {
             sums[threadIdx.x] = r;
             __syncthreads();
             if (slice == 0)
                 for (int k = 1; k < slices; ++k) add_scaled(r, 1.0f, sums[k * items + item]);
         }
-        if (on && slice == 0) {
+        if (slice == 0) {
             const size_t row = sr.row0 + i % sr.rows, colm = static_cast<size_t>(kh * group + i / sr.rows) * HD + d;
             bad |= write_paged_quad(r, total[i], p.gate ? p.gate + row * p.q_stride + colm : nullptr, p.out + row * p.out_stride + colm);
         }
@@ -795,7 +783,7 @@ __global__ void __launch_bounds__(WideShape<HD>::kThreads, (WideShape<HD>::kThre
     __shared__ int redo;
     const int nkv = p.kv.nkv, kh = blockIdx.x % nkv, group = p.nq / nkv, T = kWideCols / group;
     const int unit = blockIdx.x / nkv;
-    if (unit >= ws.head[4]) return;
+    if (unit >= ws.head[0]) return;
     const WideUnit un = ws.units[unit];
     const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int ct = wid % CT, ks = wid / CT, cl = lane & 31, g = lane >> 5;
@@ -980,7 +968,7 @@ __global__ void __launch_bounds__(WideShape<HD>::kThreads, (WideShape<HD>::kThre
     for (; c < end; ++c) chunk(c, std::false_type{}, std::true_type{});
     add_values(end - 1);
     float* part_out = un.splits > 1 ? ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * kWideCols * (HD + 2) : nullptr;
-    finish_paged<HD, CT, KS, kWideCols, false>(p, sk.r, kh, t0, ntok, T, inv_t, part_out, ws.again_wide + unit * nkv + kh, live, o, m, l, paged_lds,
+    finish_paged<HD, CT, KS, kWideCols, false>(p, sk.r, kh, t0, ntok, T, inv_t, part_out, ws.wide_at + unit * nkv + kh, live, o, m, l, paged_lds,
                                                &redo);
 }
 
@@ -991,7 +979,7 @@ __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int bloc
     __shared__ int list[kMergeThreads], count, redo;
     constexpr int kQuads = HD / 4, kSlot = kWideCols * (HD + 2);
     const int nkv = p.kv.nkv, group = p.nq / nkv, T = kWideCols / group;
-    const int units = ws.head[4], slots = ws.head[5], slot = block / nkv, kh = block % nkv;
+    const int units = ws.head[0], slots = ws.head[1], slot = block / nkv, kh = block % nkv;
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
     if (slot < slots) {
         const WideUnit un = ws.units[ws.first[slot]];
@@ -1042,7 +1030,7 @@ __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int bloc
         const int i = i0 + threadIdx.x;
         if (threadIdx.x == 0) count = 0;
         __syncthreads();
-        if (i < min(all, (block + 1) * per) && ws.units[i / nkv].splits == 1 && ws.again_wide[i]) list[atomicAdd(&count, 1)] = i;
+        if (i < min(all, (block + 1) * per) && ws.units[i / nkv].splits == 1 && ws.wide_at[i].w) list[atomicAdd(&count, 1)] = i;
         __syncthreads();
         const int n = count;
         for (int j = 0; j < n; ++j) {
@@ -1073,8 +1061,8 @@ static PagedWs paged_ws(float* base, int hd, int nkv, size_t* bytes) {
         return r;
     };
     w.head = reinterpret_cast<int*>(take(kWsHead));
-    w.again = reinterpret_cast<int*>(take(sizeof(int) * 1024 * nkv));
-    w.again_wide = reinterpret_cast<int*>(take(sizeof(int) * kMostUnits * nkv));
+    w.narrow_at = reinterpret_cast<int4*>(take(sizeof(int4) * 1024 * nkv));
+    w.wide_at = reinterpret_cast<int4*>(take(sizeof(int4) * kMostUnits * nkv));
     w.first = reinterpret_cast<int*>(take(sizeof(int) * kWideBlocks));
     w.units = reinterpret_cast<WideUnit*>(take(sizeof(WideUnit) * kMostUnits));
     w.narrow = reinterpret_cast<float*>(take(sizeof(float) * 2 * kNarrowBlocks * kNarrowCols * (hd + 2)));

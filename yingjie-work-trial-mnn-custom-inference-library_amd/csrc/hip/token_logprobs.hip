@@ -30,6 +30,7 @@ constexpr int kMostSegments = 1024;
 constexpr int kPartWaves = 4;
 constexpr int kRowThreads = 512, kFewThreads = 256;
 constexpr int kCandidates = 2048;  // candidates of a row that are held
+constexpr int kMany = 512;         // ... that are put in order as they are
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct LogPart {
@@ -89,9 +90,9 @@ __global__ void __launch_bounds__(kWave* kPartWaves) logprobs_part_kernel(Logpro
     const float c = p.inv_t * kLog2e;
     float M = -INFINITY, S = 0.0f, H = 0.0f;  // the segment so far
     int arg = 0x7fffffff, before = 0;
-    const int t = p.out_rank ? p.tokens[row] : -1;
-    const bool has = t >= 0 && t < p.vocab;
-    const float xt = has ? logit_at<F16>(x0, t) : 0.0f;
+    int t = -1;
+    float xt = 0.0f;
+    bool has = false;
     for (int it = 0; it < 1 << shift; ++it) {
         const int i0 = ((seg << shift) + it) * kSegment;
         if (i0 >= p.vocab) break;
@@ -127,6 +128,11 @@ __global__ void __launch_bounds__(kWave* kPartWaves) logprobs_part_kernel(Logpro
                 const int i = i0 + element<F16, VEC>(lane, e);
                 x[e] = i < p.vocab ? logit_at<F16>(x0, i) : -INFINITY;
             }
+        }
+        if (it == 0 && p.out_rank) {  // (after the segment's own loads: two round trips beside them)
+            t = p.tokens[row];
+            has = t >= 0 && t < p.vocab;
+            xt = logit_at<F16>(x0, has ? t : 0);
         }
         float m = x[0];
 #pragma unroll
@@ -315,7 +321,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_row_kernel(LogprobsLaunch p,
         for (int i = 0; i < kPer; ++i)
             if (key[i] != 0 && key[i] >= limit) list[atomicAdd(&count, 1)] = i * THREADS + threadIdx.x;
         __syncthreads();
-        // the segments' logits by the block, kBatch loads of a thread in flight: each(key)
+        // the segments' logits by the block, kBatch loads of a thread in flight: each(logit, index)
         constexpr int N = VEC ? (F16 ? 8 : 4) : 1, kBatch = 8;
         const int loads = (count << (shift + 10)) / N, per = size / N;
         auto walk = [&](auto each) {
@@ -342,31 +348,45 @@ __global__ void __launch_bounds__(THREADS) logprobs_row_kernel(LogprobsLaunch p,
 #pragma unroll
                 for (int u = 0; u < kBatch; ++u)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) each(x[u][i] > -INFINITY ? argmax_key(x[u][i], at[u] + i) : uint64_t(0));
+                    for (int i = 0; i < N; ++i) each(x[u][i], at[u] + i);
             }
         };
-        uint64_t mine = 0;
-        walk([&](uint64_t v) { mine = u64_max(mine, v); });
-        __syncthreads();
-        keys[threadIdx.x] = mine;
-        if (threadIdx.x == 0) count = 0;
-        __syncthreads();
-        if (threadIdx.x < kWave) {
-            uint64_t v[THREADS / kWave];
-#pragma unroll
-            for (int i = 0; i < THREADS / kWave; ++i) v[i] = keys[i * kWave + lane];
-            const uint64_t l = kth_largest(v, k);
-            if (lane == 0) limit = l;
-        }
-        __syncthreads();
-        const uint64_t least = limit;
-        if (mine != 0 && mine >= least)
-            walk([&](uint64_t v) {
-                if (v == 0 || v < least) return;
+        // the candidates: logits that the k-th segment's maximum does not pass, not many more than k as a rule
+        auto collect = [&](uint64_t least) {
+            const float low = float_from_order_key(static_cast<uint32_t>(least >> 32));
+            walk([&](float x, int i) {
+                if (x < low || x == -INFINITY) return;
+                const uint64_t v = argmax_key(x, i);
+                if (v < least) return;
                 const int at = atomicAdd(&count, 1);
                 if (at < kCandidates) cand[at] = v;
             });
+        };
+        const uint64_t reached = limit;
         __syncthreads();
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        if (reached) collect(reached);
+        __syncthreads();
+        if (!reached || count > kMany) {  // few segments, or many candidates in one: the same once more with the threads' shares
+            __syncthreads();
+            uint64_t mine = 0;
+            walk([&](float x, int i) { mine = u64_max(mine, x > -INFINITY ? argmax_key(x, i) : 0); });
+            keys[threadIdx.x] = mine;
+            if (threadIdx.x == 0) count = 0;
+            __syncthreads();
+            if (threadIdx.x < kWave) {
+                uint64_t v[THREADS / kWave];
+#pragma unroll
+                for (int i = 0; i < THREADS / kWave; ++i) v[i] = keys[i * kWave + lane];
+                const uint64_t l = kth_largest(v, k);
+                if (lane == 0) limit = l;
+            }
+            __syncthreads();
+            const uint64_t least = u64_max(limit, 1);
+            if (mine >= least) collect(least);
+            __syncthreads();
+        }
         const int n = count;
         auto put = [&](int place, uint64_t v) {
             const size_t o = static_cast<size_t>(row) * k + place;
@@ -388,7 +408,10 @@ __global__ void __launch_bounds__(THREADS) logprobs_row_kernel(LogprobsLaunch p,
         uint64_t before_it = ~uint64_t(0);
         for (int i = 0; i < k; ++i) {
             uint64_t next = 0;
-            walk([&](uint64_t v) { next = v < before_it ? u64_max(next, v) : next; });
+            walk([&](float x, int at) {
+                const uint64_t v = x > -INFINITY ? argmax_key(x, at) : 0;
+                next = v < before_it ? u64_max(next, v) : next;
+            });
             before_it = block_most<THREADS>(next, red);
             if (threadIdx.x == 0) put(i, before_it);
         }
