@@ -23,12 +23,14 @@ namespace xqhip {
 //   no LDS.
 // logprobs_row_kernel: a block per row joins the segments.  A value that k
 //   segments' maxima reach is reached by the k first tokens: the lanes whose
-//   maxima reach it, in the segments that do, are all that is looked at again.
+//   maxima reach it, in those segments, are all that is looked at again.  With
+//   fewer than 8 k segments (of up to 256) the threads' shares of all lanes'
+//   maxima stand in for the segments: one row of 243 segments, 20 alternatives
+//   10.2 us (so 11.4), 64 alternatives 15.3 (13.3).
 // What bounds it: the logits' bytes and, with fp16 logits, 13 operations a
 // logit; for one row a chain of two launches.
 // ---------------------------------------------------------------------------
-constexpr int kMostSegments = 1024;
-constexpr int kMostTop = 64;  // alternatives
+constexpr int kMostSegments = 1024, kFewSegments = 256;
 constexpr int kPartWaves = 4;
 constexpr int kRowThreads = 512, kFewThreads = 256;
 constexpr int kCandidates = 2048;  // candidates of a row that are held
@@ -120,11 +122,14 @@ __global__ void __launch_bounds__(kWave* kPartWaves) logprobs_part_kernel(Logpro
         const float m = wave_max(lm);
         if (has && m >= xt) {  // wave-uniform
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = i0 + element<F16, VEC>(lane, e);
-                const float v = clean(x[e]);
-                before += __popcll(__builtin_amdgcn_ballot_w64(i < p.vocab && (v > xt || (v == xt && i < t))));
-            }
+            for (int e = 0; e < E; ++e) before += __popcll(__builtin_amdgcn_ballot_w64(x[e] > xt));
+            uint64_t ties = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) ties |= __builtin_amdgcn_ballot_w64(clean(x[e]) == xt);
+            if (ties)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    before += __popcll(__builtin_amdgcn_ballot_w64(clean(x[e]) == xt && i0 + element<F16, VEC>(lane, e) < t));
         }
         if (m > -INFINITY) {  // wave-uniform
             float s = 0.0f, h = 0.0f;
@@ -191,24 +196,29 @@ __device__ __forceinline__ uint64_t kth_largest(const uint64_t (&key)[R], int k)
 // A value that at least k and not many more of the wave's order keys reach, by halving the range between the least and the
 // largest; 0 where fewer than k are above 0, or ties leave no such value.
 template <int R>
-__device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[R], int k, uint32_t most) {
+__device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[R], int k) {
+    const int most = k + 4 + k / 4;
     auto count = [&](uint32_t to) {
         int n = 0;
 #pragma unroll
         for (int i = 0; i < R; ++i) n += __popcll(__builtin_amdgcn_ballot_w64(v[i] >= to));
         return n;
     };
-    uint32_t low = ~0u;
+    uint32_t low = ~0u, high = 0;
 #pragma unroll
-    for (int i = 0; i < R; ++i) low = v[i] ? min(low, v[i]) : low;
+    for (int i = 0; i < R; ++i) {
+        low = v[i] ? min(low, v[i]) : low;
+        high = max(high, v[i]);
+    }
     low = ~static_cast<uint32_t>(wave_max_u64(~low));
-    if (count(1) < k) return 0;
-    if (count(low) <= 2 * k) return low;
-    uint32_t high = most;  // low: more than 2 k reach it; high + 1: fewer than k
-    while (low < high) {
+    high = static_cast<uint32_t>(wave_max_u64(high));
+    const int all = count(1);
+    if (all < k) return 0;
+    if (all <= most) return low;
+    while (low < high) {  // more than `most` reach low, fewer than k reach high + 1
         const uint32_t mid = low + (high - low + 1) / 2;
         const int n = count(mid);
-        if (n >= k && n <= 2 * k) return mid;
+        if (n >= k && n <= most) return mid;
         if (n > k)
             low = mid;
         else
@@ -288,94 +298,114 @@ __global__ void __launch_bounds__(THREADS) logprobs_row_kernel(LogprobsLaunch p,
     } else {
         __shared__ uint64_t keys[kMostSegments];  // of segments, then of threads
         __shared__ uint64_t cand[kCandidates];
-        __shared__ int list[2 * kMostTop], lanes[kMostLanes];
+        __shared__ int list[kMostSegments], lanes[kMostLanes];
         __shared__ uint64_t limit;
         __shared__ int counts[3];  // segments, lanes, candidates
         constexpr int E = kLaneLogits<F16>, kPass = E * kWave;
         const int k = p.top;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) keys[i * THREADS + threadIdx.x] = key[i];
         if (threadIdx.x < 3) counts[threadIdx.x] = 0;
         __syncthreads();
         const float lz = finish();
-        if (wid == 0) {
-            auto threshold = [&](auto tag) {
-                constexpr int R = decltype(tag)::value;
-                uint32_t v[R];
+        const float* maxima = reinterpret_cast<const float*>(static_cast<const LogPart*>(p.ws) + static_cast<size_t>(p.rows) * sg.count) +
+                              static_cast<size_t>(row) * sg.count * kWave;
+        auto add_lane = [&](int e) {
+            const int at = atomicAdd(&counts[1], 1);
+            if (at < kMostLanes) lanes[at] = e;
+        };
+        uint32_t value;  // at least k logits reach it: order key
+        if (sg.count <= kFewSegments && sg.count < 8 * k) {  // block-uniform
+            // the threads' maxima of some lanes' each, in their order
+            constexpr int kMine = kFewSegments * kWave / THREADS;
+            float v[kMine];
+            const int all = sg.count * kWave;
+            float most = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < R; ++i) v[i] = static_cast<uint32_t>(keys[i * kWave + lane] >> 32);
-                uint64_t l = static_cast<uint64_t>(reached_by(v, k, static_cast<uint32_t>(best >> 32))) << 32;
-                if (l == 0) {  // few segments, or ties
-                    uint64_t u[R];
+            for (int u = 0; u < kMine; ++u) {
+                const int e = u * THREADS + threadIdx.x;
+                v[u] = e < all ? maxima[e] : -INFINITY;
+            }
 #pragma unroll
-                    for (int i = 0; i < R; ++i) u[i] = keys[i * kWave + lane];
-                    l = kth_largest(u, k);
+            for (int u = 0; u < kMine; ++u) most = fmaxf(most, v[u]);
+            keys[threadIdx.x] = most > -INFINITY ? float_order_key(most) : 0;
+            __syncthreads();
+            if (wid == 0) {
+                uint32_t w[kWaves];
+#pragma unroll
+                for (int i = 0; i < kWaves; ++i) w[i] = static_cast<uint32_t>(keys[i * kWave + lane]);
+                const uint32_t l = reached_by(w, k);
+                if (lane == 0) limit = l;
+            }
+            __syncthreads();
+            value = static_cast<uint32_t>(limit);
+            const float low = value ? float_from_order_key(value) : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kMine; ++u)
+                if (v[u] > -INFINITY && v[u] >= low) add_lane(u * THREADS + threadIdx.x);
+        } else {  // many more segments than alternatives: their maxima, then the lanes of those that reach
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) keys[i * THREADS + threadIdx.x] = key[i];
+            __syncthreads();
+            if (wid == 0) {
+                auto reached = [&](auto tag) {
+                    constexpr int R = decltype(tag)::value;
+                    uint32_t w[R];
+#pragma unroll
+                    for (int i = 0; i < R; ++i) w[i] = static_cast<uint32_t>(keys[i * kWave + lane] >> 32);
+                    return reached_by(w, k);
+                };
+                const uint32_t l = sg.count <= kFewSegments ? reached(std::integral_constant<int, kFewSegments / kWave>{})
+                                                            : reached(std::integral_constant<int, kMostSegments / kWave>{});
+                if (lane == 0) limit = l;
+            }
+            __syncthreads();
+            value = static_cast<uint32_t>(limit);
+            const float low = value ? float_from_order_key(value) : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (key[i] != 0 && part[i].m >= low) list[atomicAdd(&counts[0], 1)] = i * THREADS + threadIdx.x;
+            __syncthreads();
+            const int all = counts[0] * kWave;
+            for (int e0 = threadIdx.x; e0 < all; e0 += 4 * THREADS) {
+                float v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int e = e0 + u * THREADS;
+                    v[u] = e < all ? maxima[list[e / kWave] * kWave + e % kWave] : -INFINITY;
                 }
-                return l;
-            };
-            const uint64_t l = sg.count <= 4 * kWave ? threshold(std::integral_constant<int, 4>{})
-                                                     : threshold(std::integral_constant<int, kMostSegments / kWave>{});
-            if (lane == 0) limit = l;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int e = e0 + u * THREADS;
+                    if (v[u] > -INFINITY && v[u] >= low) add_lane(list[e / kWave] * kWave + e % kWave);
+                }
+            }
         }
         __syncthreads();
-        const uint64_t reach = u64_max(limit, 1);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (key[i] >= reach) list[atomicAdd(&counts[0], 1)] = i * THREADS + threadIdx.x;
-        __syncthreads();
-        const int segs = counts[0];
-        // an element of the listed segments, of the listed lanes
-        auto hold = [&](int i, uint64_t least) {
-            if (i >= p.vocab) return;
-            const float x = clean(static_cast<float>(x0[i]));
-            if (x == -INFINITY) return;
-            const uint64_t v = argmax_key(x, i);
-            if (v < least) return;
+        // a logit of a lane
+        auto index_of = [&](int ln, int e) { return (((ln >> 6) << sg.shift) + e / E) * kPass + element<F16, VEC>(ln & 63, e % E); };
+        const int n_lanes = counts[1], each = E << sg.shift;
+        auto hold = [&](uint64_t v) {
             const int at = atomicAdd(&counts[2], 1);
             if (at < kCandidates) cand[at] = v;
         };
-        auto index_of = [&](int seg, int ln, int e) { return ((seg << sg.shift) + e / E) * kPass + element<F16, VEC>(ln, e % E); };
-        // A segment's key orders it by its number, a logit's by its index: the value alone bounds the logits.  (Where the
-        // threshold is a tie's, too many may reach it: below.)
-        const uint32_t value = static_cast<uint32_t>(reach >> 32);
-        const float low = value ? float_from_order_key(value) : -INFINITY;
-        const float* maxima = reinterpret_cast<const float*>(static_cast<const LogPart*>(p.ws) + static_cast<size_t>(p.rows) * sg.count) +
-                              static_cast<size_t>(row) * sg.count * kWave;
-        for (int e0 = threadIdx.x; e0 < segs * kWave; e0 += 4 * THREADS) {
-            float v[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int e = e0 + u * THREADS;
-                v[u] = e < segs * kWave ? maxima[list[e / kWave] * kWave + e % kWave] : -INFINITY;
+        auto key_at = [&](int i) {
+            const float x = i < p.vocab ? clean(static_cast<float>(x0[i])) : -INFINITY;
+            return x > -INFINITY ? argmax_key(x, i) : uint64_t(0);
+        };
+        bool many = n_lanes > kMostLanes;  // block-uniform
+        if (!many) {
+            const uint64_t least = u64_max(static_cast<uint64_t>(value) << 32, 1);
+            for (int e = threadIdx.x; e < n_lanes * each; e += THREADS) {
+                const uint64_t v = key_at(index_of(lanes[e / each], e % each));
+                if (v >= least) hold(v);
             }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int e = e0 + u * THREADS;
-                if (v[u] == -INFINITY || v[u] < low) continue;
-                const int at = atomicAdd(&counts[1], 1);
-                if (at < kMostLanes) lanes[at] = list[e / kWave] << 6 | e % kWave;
-            }
-        }
-        __syncthreads();
-        const int n_lanes = counts[1], each = E << sg.shift;
-        bool whole = n_lanes > kMostLanes;  // block-uniform
-        if (!whole) {
-            for (int e = threadIdx.x; e < n_lanes * each; e += THREADS)
-                hold(index_of(lanes[e / each] >> 6, lanes[e / each] & 63, e % each), static_cast<uint64_t>(value) << 32);
             __syncthreads();
-            whole = counts[2] > kMany;
+            many = counts[2] > kMany;
             __syncthreads();
         }
-        if (whole) {  // few segments, ties, or many large logits in a few lanes: once more, with the k-th of the threads' shares
-            const int all = segs * kWave * each;
+        if (many) {  // ties, or many large logits in a few lanes: the whole row once more, with the k-th of the threads' shares
             uint64_t mine = 0;
-            auto key_at = [&](int e) {
-                const int i = index_of(list[e / (kWave * each)], e % kWave, e / kWave % each);
-                const float x = i < p.vocab ? clean(static_cast<float>(x0[i])) : -INFINITY;
-                return x > -INFINITY ? argmax_key(x, i) : uint64_t(0);
-            };
 #pragma unroll 8
-            for (int e = threadIdx.x; e < all; e += THREADS) mine = u64_max(mine, key_at(e));
+            for (int i = threadIdx.x; i < p.vocab; i += THREADS) mine = u64_max(mine, key_at(i));
             keys[threadIdx.x] = mine;
             if (threadIdx.x == 0) counts[2] = 0;
             __syncthreads();
@@ -389,19 +419,19 @@ __global__ void __launch_bounds__(THREADS) logprobs_row_kernel(LogprobsLaunch p,
             __syncthreads();
             const uint64_t least = limit;
             if (mine >= least)
-                for (int e = threadIdx.x; e < all; e += THREADS) {
-                    const uint64_t v = key_at(e);
-                    if (v < least) continue;
-                    const int at = atomicAdd(&counts[2], 1);
-                    if (at < kCandidates) cand[at] = v;
+#pragma unroll 8
+                for (int i = threadIdx.x; i < p.vocab; i += THREADS) {
+                    const uint64_t v = key_at(i);
+                    if (v >= least) hold(v);
                 }
             __syncthreads();
             if (counts[2] > kCandidates) {  // (a few threads' shares hold them all)
                 uint64_t last = ~uint64_t(0);
                 for (int i = 0; i < k; ++i) {
                     uint64_t next = 0;
-                    for (int e = threadIdx.x; e < all; e += THREADS) {
-                        const uint64_t v = key_at(e);
+#pragma unroll 8
+                    for (int j = threadIdx.x; j < p.vocab; j += THREADS) {
+                        const uint64_t v = key_at(j);
                         next = v < last ? u64_max(next, v) : next;
                     }
                     next = wave_max_u64(next);
