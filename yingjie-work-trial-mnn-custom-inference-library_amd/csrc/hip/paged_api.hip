@@ -155,7 +155,10 @@ int xqhip_attn_prep_paged(const float* q_src, const float* k_src, const float* v
         p.rot.positions = rotary->positions;
         p.rot.pairs = rotary->rotary_dim / 2;
         p.rot.axes = rotary->axes;
-        for (int i = 0; i < p.rot.pairs; ++i) p.rot.axis[i / 16] |= static_cast<uint32_t>(rotary->axis[i]) << 2 * (i % 16);
+        for (int i = 0; i < p.rot.pairs; ++i) {
+            p.rot.axis[i / 16] |= static_cast<uint32_t>(rotary->axis[i]) << 2 * (i % 16);
+            p.rot.used |= 1 << rotary->axis[i];
+        }
     }
     p.step = step_of(step);
     p.kv = cache_of(kv);

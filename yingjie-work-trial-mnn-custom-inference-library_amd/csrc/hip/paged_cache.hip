@@ -1,6 +1,7 @@
 // paged_cache.hip - the paged key/value cache of a step over several sequences:
 // head preparation with the append, and read-back.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_common.hpp"
 
@@ -16,8 +17,10 @@ namespace xqhip {
 // A head's values lie in a wave's lanes: lane l has the dims E l .. E l + E - 1
 // (VEC, one load) or l, l + 64, .. (other sizes).
 // ---------------------------------------------------------------------------
-constexpr int kPagedWaves = 4;
+constexpr int kPagedWaves = 8;
+constexpr int kPagedThreads = kWave * kPagedWaves;
 constexpr int kPagedMaxDim = 256;
+constexpr int kPagedMaxPage = 128;
 
 __device__ __forceinline__ double wave_sum_double(double v) {
     v += __builtin_bit_cast(double, dpp_u64<kDppXor1>(__builtin_bit_cast(uint64_t, v)));
@@ -71,36 +74,53 @@ struct HeadLanes {
     }
 };
 
-// The angles of a row: whether all of its positions lie in the table.
-template <int E, bool VEC>
-__device__ __forceinline__ bool row_angles(const PagedPrepLaunch& p, int row, int pos, int lane, float2 (&cs)[E]) {
-    typedef HeadLanes<E, VEC> L;
-    const int half = p.rot.pairs;
-    bool good = true;
+
+// The positions of a row on its axes (wave-uniform), and whether all that its pairs use lie in the table.
+struct RowAxes {
+    int at[4];
+    __device__ __forceinline__ void load(const RotaryAxes& r, int rows, int row, int pos) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int d = L::dim(lane, e);
-        cs[e] = make_float2(1.0f, 0.0f);
-        if (d >= 2 * half) continue;
-        const int i = d < half ? d : d - half, a = p.rot.axis[i / 16] >> 2 * (i % 16) & 3;
-        const int at = p.rot.pos ? p.rot.pos[static_cast<size_t>(a) * p.step.rows + row] : pos;
-        if (at >= 0 && at < p.rot.positions)
-            cs[e] = p.rot.cs[static_cast<size_t>(at) * half + i];
-        else
-            good = false;
+        for (int a = 0; a < 4; ++a) at[a] = r.pos && a < r.axes ? r.pos[static_cast<size_t>(a) * rows + row] : pos;
     }
-    return __builtin_amdgcn_ballot_w64(!good) == 0;
+    __device__ __forceinline__ bool good(const RotaryAxes& r) const {
+        bool all = true;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) all = all && (!(r.used >> a & 1) || (at[a] >= 0 && at[a] < r.positions));
+        return all;
+    }
+    // the angles of a lane's dims (those of a good row)
+    template <int E, bool VEC>
+    __device__ __forceinline__ void angles(const RotaryAxes& r, int lane, float2 (&cs)[E]) const {
+        const int half = r.pairs;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int d = HeadLanes<E, VEC>::dim(lane, e);
+            cs[e] = make_float2(1.0f, 0.0f);
+            if (d >= 2 * half) continue;
+            const int i = d < half ? d : d - half, a = r.axis[i / 16] >> 2 * (i % 16) & 3;
+            const int p = a == 0 ? at[0] : a == 1 ? at[1] : a == 2 ? at[2] : at[3];
+            cs[e] = r.cs[static_cast<size_t>(p) * half + i];
+        }
+    }
+};
+
+// 1 / sqrt(v): the hardware's estimate and two steps of Newton's, within 2^-50 (what is kept of it has 24 bits)
+__device__ __forceinline__ double inverse_sqrt(double v) {
+    double y = __builtin_amdgcn_rsq(v);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = fma(0.5 * y, fma(-v * y, y, 1.0), y);
+    return y;
 }
 
 // x normalised and turned, by a whole wave; turn: the wave's kPagedMaxDim doubles of LDS
 template <int E, bool VEC>
-__device__ __forceinline__ void turn_head(const float (&x)[E], const float (&w)[E], const float2 (&cs)[E], int hd, int half, float eps,
-                                          int lane, double* turn, float (&y)[E]) {
+__device__ __forceinline__ void turn_head(float (&x)[E], const float (&w)[E], const float2 (&cs)[E], int hd, int half, float eps, int lane,
+                                          double* turn) {
     typedef HeadLanes<E, VEC> L;
     double ss = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) ss += static_cast<double>(x[e]) * x[e];
-    const double inv = 1.0 / sqrt(wave_sum_double(ss) / hd + static_cast<double>(eps));
+    const double inv = inverse_sqrt(wave_sum_double(ss) / hd + static_cast<double>(eps));
     double v[E];
     wave_lds_sync();
 #pragma unroll
@@ -116,150 +136,238 @@ __device__ __forceinline__ void turn_head(const float (&x)[E], const float (&w)[
             v[e] = v[e] * cs[e].x - turn[half + d] * cs[e].y;
         else if (d < 2 * half)
             v[e] = v[e] * cs[e].x + turn[d - half] * cs[e].y;
-        y[e] = static_cast<float>(v[e]);
+        x[e] = static_cast<float>(v[e]);
     }
 }
 
-// Whether a row's key and value have a place: sequence s, position pos.
-__device__ __forceinline__ int place_of(const PagedPrepLaunch& p, int s, int64_t pos) {
-    if (pos < 0 || pos >= table_positions(p.step, p.kv)) return -1;
-    if (p.kv.i8) {
-        const int o = p.step.open[s];
-        if (o < 0 || o >= p.kv.opens) return -1;
+// Where a sequence's position goes.  (Both loads go out at once, from places that exist.)
+struct Place {
+    int page, open;
+    __device__ __forceinline__ Place(const PagedPrepLaunch& p, int s, int64_t pos) {
+        const int at = static_cast<int>(max(int64_t(0), min(pos, static_cast<int64_t>(table_positions(p.step, p.kv)) - 1))) / p.kv.page;
+        page = p.step.table[static_cast<size_t>(s) * p.step.max_pages + at];
+        open = p.kv.i8 ? p.step.open[s] : 0;
+        if (pos != at * static_cast<int64_t>(p.kv.page) + (pos & (p.kv.page - 1)) || page >= p.kv.pages || open < 0 || (p.kv.i8 && open >= p.kv.opens)) page = -1;
     }
-    return page_at(p.step, p.kv, s, static_cast<int>(pos) / p.kv.page);
-}
+    __device__ __forceinline__ bool none() const { return page < 0; }
+};
 
-// One head of one row per wave: q, gate, and k and v of fp16 pages.
+// `per` query heads of one row by a wave, h0 and every kPagedWaves-th from there: q and their gates.
+constexpr int kQueryHeads = 4;
 template <int E, bool VEC>
-__device__ void prep_unit(const PagedPrepLaunch& p, int unit, int row, double* turn) {
+__device__ __forceinline__ void query_unit(const PagedPrepLaunch& p, int h0, int per, int row, double* turn) {
     typedef HeadLanes<E, VEC> L;
-    const int lane = threadIdx.x & (kWave - 1), hd = p.kv.head_dim, nkv = p.kv.nkv;
-    const bool is_q = unit < p.nq, is_k = !is_q && unit < p.nq + nkv;
-    const int h = is_q ? unit : (is_k ? unit - p.nq : unit - p.nq - nkv);
-    const size_t off = static_cast<size_t>(row) * p.src_stride;
-    const float* src = is_q ? p.q_src + off + static_cast<size_t>(h) * (p.gated ? 2 * hd : hd)
-                            : (is_k ? p.k_src : p.v_src) + off + static_cast<size_t>(h) * hd;
+    const int lane = threadIdx.x & (kWave - 1), hd = p.kv.head_dim;
+    const float* src = p.q_src + static_cast<size_t>(row) * p.src_stride;
+    float x[kQueryHeads][E], gate[kQueryHeads][E], w[E];
+    auto on = [&](int i) { return i < per && h0 + i * kPagedWaves < p.nq; };  // wave-uniform
+#pragma unroll
+    for (int i = 0; i < kQueryHeads; ++i)
+        if (on(i)) {
+            const float* at = src + static_cast<size_t>(h0 + i * kPagedWaves) * (p.gated ? 2 * hd : hd);
+            L::load(at, lane, hd, x[i]);
+            if (p.gated) L::load(at + hd, lane, hd, gate[i]);
+        }
+    L::load(p.q_norm, lane, hd, w);
     const int s = __builtin_amdgcn_readfirstlane(seq_of_row(p.step, row));
     if (s >= p.step.seqs) return;
     const SeqRows sr = seq_rows(p.step, s);
     const int j = row - sr.row0;
     if (j < 0 || j >= sr.rows) return;
-    float x[E], w[E], gate[E] = {};
-    L::load(src, lane, hd, x);
-    if (is_q && p.gated) L::load(src + hd, lane, hd, gate);
-    if (is_q || is_k) L::load(is_q ? p.q_norm : p.k_norm, lane, hd, w);
     const int64_t pos = sr.past < 0 ? -1 : static_cast<int64_t>(sr.past) + j;
-    const int page = place_of(p, s, pos);
-    float2 cs[E];
-    const bool held = row_angles<E, VEC>(p, row, static_cast<int>(pos), lane, cs) && page >= 0;
-    if (is_q || is_k) {
-        float y[E];
-        turn_head<E, VEC>(x, w, cs, hd, p.rot.pairs, p.eps, lane, turn, y);
+    RowAxes axes;
+    axes.load(p.rot, p.step.rows, row, static_cast<int>(pos));
+    const Place place(p, s, pos);
+    const bool turned = axes.good(p.rot);
+    float2 cs[E] = {};
+    if (turned) axes.angles<E, VEC>(p.rot, lane, cs);
+    const bool held = turned && !place.none();
+    const size_t o = static_cast<size_t>(row) * p.out_stride;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = y[e];
-    }
-    if (is_q) {
-        const size_t o = static_cast<size_t>(row) * p.out_stride + static_cast<size_t>(h) * hd;
+    for (int i = 0; i < kQueryHeads; ++i) {
+        if (!on(i)) break;
+        turn_head<E, VEC>(x[i], w, cs, hd, p.rot.pairs, p.eps, lane, turn);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = held ? x[e] : __builtin_nanf("");
-        L::store(p.q_out + o, lane, hd, x);
-        if (p.gate_out) L::store(p.gate_out + o, lane, hd, gate);
-        return;
-    }
-    if (!held) return;
-    const int at = static_cast<int>(pos) % p.kv.page;
-    _Float16* d = static_cast<_Float16*>(is_k ? p.kv.k : p.kv.v) + page_head(p.kv, page, h);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (L::in(lane, e, hd)) {
-            const int dim = L::dim(lane, e);
-            d[is_k ? k_offset<8>(p.kv, at, dim) : v_offset<8>(p.kv, at, dim)] = static_cast<_Float16>(x[e]);
+        for (int e = 0; e < E; ++e) {
+            x[i][e] = held ? x[i][e] : __builtin_nanf("");
+            if (!p.gated) gate[i][e] = 0.0f;
         }
+        const size_t at = o + static_cast<size_t>(h0 + i * kPagedWaves) * hd;
+        L::store(p.q_out + at, lane, hd, x[i]);
+        if (p.gate_out) L::store(p.gate_out + at, lane, hd, gate[i]);
+    }
 }
 
 // The fp16 value that 8 bits are taken of: no infinities, no NaN.
 __device__ __forceinline__ _Float16 held_value(float x) {
     return static_cast<_Float16>(x == x ? fminf(fmaxf(x, -65504.0f), 65504.0f) : 0.0f);
 }
-// 127 x / mx to the nearest: 127 x is exact (18 bits), and the division correctly rounded: its quotient is half a code's
-// step exactly where the true one is
-__device__ __forceinline__ int8_t code_of(_Float16 x, float mx) {
-    const float c = mx > 0.0f ? rintf(__fdiv_rn(127.0f * static_cast<float>(x), mx)) : 0.0f;
-    return static_cast<int8_t>(fminf(fmaxf(c, -127.0f), 127.0f));  // (a row that was never written may pass the maximum)
+// 127 x / mx to the nearest, inv near 1 / mx: 127 x is exact (18 bits), the quotient's error is taken off by its exact
+// remainder, so it is half a code's step exactly where the true one is (which is then a number of few bits), and
+// elsewhere further from it (2^-12) than its own rounding
+__device__ __forceinline__ int code_of(_Float16 x, float mx, float inv) {
+    const float n = 127.0f * static_cast<float>(x);
+    float q = n * inv;
+    q = fmaf(fmaf(-mx, q, n), inv, q);
+    return static_cast<int>(__builtin_amdgcn_fmed3f(rintf(q), -127.0f, 127.0f));  // (a position never written may pass the maximum)
 }
 
-// One 8-bit page that the step touches, one kv head, k or v, by a block: the new rows' fp16 values into LDS and their
-// maximum taken, then codes of them, or of the whole page where the maximum rose.
-template <int E, bool VEC>
-__device__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int h, bool is_k, _Float16* vals, double* turn) {
+// One page that the step touches, one kv head, k or v, by a block.  The new rows' fp16 values go to LDS (four rows' loads of a
+// wave at a time), then to the page in 16-byte pieces; 8 bits: their maximum is taken on the way, and where it rose the
+// page's earlier values are fetched and the codes of all of them written.
+template <int E, bool VEC, bool I8>
+__device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int h, bool is_k, _Float16* vals, double* turn) {
     typedef HeadLanes<E, VEC> L;
+    constexpr int kBatch = E == 2 ? 4 : 2;
     __shared__ float wave_mx[kPagedWaves];
+    __shared__ uint8_t ok[kPagedMaxPage];
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
-    const int page = place_of(p, s, static_cast<int64_t>(index) * P);
-    if (page < 0) return;  // block-uniform
-    const int open = p.step.open[s];
-    const int base = index * P;                                                       // position of the page's first
+    const int base = index * P, ld = hd + 8;                                          // position of the page's first
     const int lead = max(0, sr.past - base), end = min(P, sr.past + sr.rows - base);  // new ones: [lead, end)
     const bool last = base + P >= sr.past + sr.rows;
-    const size_t head = page_head(p.kv, page, h);
-    _Float16* kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(open) * nkv + h) * P * hd;
-    float* scale = (is_k ? p.kv.k_scale : p.kv.v_scale) + static_cast<size_t>(page) * nkv + h;
-    float w[E], mx = 0.0f;
-    if (is_k) L::load(p.k_norm, lane, hd, w);
-    for (int t = lead + wid; t < end; t += kPagedWaves) {
-        const int row = sr.row0 + base + t - sr.past;
-        float x[E];
-        float2 cs[E];
-        L::load((is_k ? p.k_src : p.v_src) + static_cast<size_t>(row) * p.src_stride + static_cast<size_t>(h) * hd, lane, hd, x);
-        const bool held = row_angles<E, VEC>(p, row, base + t, lane, cs);
-        if (is_k) {
-            float y[E];
-            turn_head<E, VEC>(x, w, cs, hd, p.rot.pairs, p.eps, lane, turn, y);
+    float x[kBatch][E], w[E];
+    RowAxes axes[kBatch];
+    auto load = [&](int t0) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = y[e];
+        for (int b = 0; b < kBatch; ++b) {  // (rows behind the last: the last again)
+            const int row = sr.row0 + base + min(t0 + b * kPagedWaves, end - 1) - sr.past;
+            L::load((is_k ? p.k_src : p.v_src) + static_cast<size_t>(row) * p.src_stride + static_cast<size_t>(h) * hd, lane, hd, x[b]);
+            axes[b].load(p.rot, p.step.rows, row, base + t0 + b * kPagedWaves);
+        }
+    };
+    load(lead + wid);
+    if (is_k) L::load(p.k_norm, lane, hd, w);
+    const Place place(p, s, base);
+    if (place.none()) return;  // block-uniform
+    const int page = place.page;
+    const size_t sat = static_cast<size_t>(page) * nkv + h;
+    _Float16* kept = nullptr;
+    float was = 0.0f, mx = 0.0f;
+    if constexpr (I8) {
+        kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(place.open) * nkv + h) * P * hd;
+        was = lead ? (is_k ? p.kv.k_scale : p.kv.v_scale)[sat] : 0.0f;
+    }
+    for (int t0 = lead + wid; t0 < end; t0 += kBatch * kPagedWaves) {
+        float2 cs[kBatch][E];
+        bool held[kBatch];
+        if (t0 != lead + wid) load(t0);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            held[b] = t0 + b * kPagedWaves < end && axes[b].good(p.rot);
+            if (is_k && held[b]) axes[b].template angles<E, VEC>(p.rot, lane, cs[b]);
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (!L::in(lane, e, hd)) continue;
-            const int d = L::dim(lane, e);
-            // (a row that is not held leaves what is there: NaN marks it)
-            const _Float16 v = held ? held_value(x[e]) : static_cast<_Float16>(__builtin_nanf(""));
-            vals[t * hd + d] = v;
-            if (held) {
-                mx = fmaxf(mx, fabsf(static_cast<float>(v)));
-                if (last) kept[static_cast<size_t>(t) * hd + d] = v;
+        for (int b = 0; b < kBatch; ++b) {
+            const int t = t0 + b * kPagedWaves;
+            if (t >= end) break;  // wave-uniform
+            if (is_k && held[b]) turn_head<E, VEC>(x[b], w, cs[b], hd, p.rot.pairs, p.eps, lane, turn);
+            if (lane == 0) ok[t] = held[b];
+            _Float16 v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                v[e] = I8 ? held_value(x[b][e]) : static_cast<_Float16>(x[b][e]);
+                if (I8 && held[b] && L::in(lane, e, hd)) mx = fmaxf(mx, fabsf(static_cast<float>(v[e])));
+            }
+            auto put = [&](_Float16* d) {
+                if constexpr (VEC) {
+                    typedef _Float16 hv __attribute__((ext_vector_type(E)));
+                    hv y;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) y[e] = v[e];
+                    *reinterpret_cast<hv*>(d + lane * E) = y;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (L::in(lane, e, hd)) d[L::dim(lane, e)] = v[e];
+                }
+            };
+            put(vals + t * ld);
+            if (I8 && last && held[b]) put(kept + static_cast<size_t>(t) * hd);
+        }
+    }
+    int from = lead;
+    float inv = 0.0f;
+    if constexpr (I8) {
+        mx = wave_max(mx);
+        if (lane == 0) wave_mx[wid] = mx;
+    }
+    __syncthreads();
+    if constexpr (I8) {
+#pragma unroll
+        for (int i = 0; i < kPagedWaves; ++i) mx = fmaxf(mx, wave_mx[i]);
+        const float before = static_cast<float>(static_cast<_Float16>(was * 127.0f));  // the maximum, an fp16 value, exactly
+        const bool grew = mx > before;
+        mx = grew ? mx : before;
+        inv = mx > 0.0f ? 1.0f / mx : 0.0f;
+        if (grew && lead) {
+            from = 0;
+            for (int i = threadIdx.x; i < lead * (hd / 8); i += kPagedThreads) {
+                const int t = i / (hd / 8), b = i - t * (hd / 8);
+                *reinterpret_cast<u32x4*>(vals + t * ld + 8 * b) = *reinterpret_cast<const u32x4*>(kept + static_cast<size_t>(t) * hd + 8 * b);
+            }
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) (is_k ? p.kv.k_scale : p.kv.v_scale)[sat] = mx / 127.0f;
+    }
+    // positions to write: [from, lead) and the new ones that are held
+    uint64_t go[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = i * kWave + lane;
+        go[i] = __builtin_amdgcn_ballot_w64(t >= from && t < end && (t < lead || ok[t] != 0));
+    }
+    auto writes = [&](int t) { return (t < kWave ? go[0] >> t : go[1] >> (t - kWave)) & 1; };
+    constexpr int N = I8 ? 16 : 8;  // values of a piece
+    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+    typedef typename std::conditional<I8, int8_t, _Float16>::type T;
+    union Piece {
+        T v[N];
+        u32x4 all;
+    };
+    auto value = [&](_Float16 v) -> T {
+        if constexpr (I8)
+            return static_cast<T>(code_of(v, mx, inv));
+        else
+            return v;
+    };
+    T* d = static_cast<T*>(is_k ? p.kv.k : p.kv.v) + page_head(p.kv, page, h);
+    if (is_k) {  // lanes over positions, then blocks of dims
+        const int n = end - from;
+        for (int i = threadIdx.x; i < n * (hd / N); i += kPagedThreads) {
+            const int b = i / n, t = from + i - b * n;
+            if (!writes(t)) continue;
+            Piece o;
+#pragma unroll
+            for (int u = 0; u < N / 8; ++u) {
+                const half8 y = *reinterpret_cast<const half8*>(vals + t * ld + b * N + 8 * u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o.v[8 * u + e] = value(y[e]);
+            }
+            *reinterpret_cast<u32x4*>(d + (static_cast<size_t>(b) * P + t) * N) = o.all;
+        }
+    } else {  // lanes over dims, then blocks of positions
+        const int b0 = from / N, n = (end - 1) / N + 1 - b0;
+        for (int i = threadIdx.x; i < n * hd; i += kPagedThreads) {
+            const int b = b0 + i / hd, dim = i % hd, t0 = b * N;
+            const uint32_t on = static_cast<uint32_t>((t0 < kWave ? go[0] >> t0 : go[1] >> (t0 - kWave)) & ((1u << N) - 1));
+            T* at = d + (static_cast<size_t>(b) * hd + dim) * N;
+            if (on == (1u << N) - 1) {
+                Piece o;
+#pragma unroll
+                for (int e = 0; e < N; ++e) o.v[e] = value(vals[(t0 + e) * ld + dim]);
+                *reinterpret_cast<u32x4*>(at) = o.all;
+            } else {
+                for (int e = 0; e < N; ++e)
+                    if (on >> e & 1) at[e] = value(vals[(t0 + e) * ld + dim]);
             }
         }
     }
-    mx = wave_max(mx);
-    if (lane == 0) wave_mx[wid] = mx;
-    const float was = lead ? *scale : 0.0f;
-    __syncthreads();
-    mx = fmaxf(fmaxf(wave_mx[0], wave_mx[1]), fmaxf(wave_mx[2], wave_mx[3]));
-    const float before = static_cast<float>(static_cast<_Float16>(was * 127.0f));  // the maximum, an fp16 value, exactly
-    const bool grew = mx > before;
-    mx = grew ? mx : before;
-    int from = lead;
-    if (grew && lead) {
-        from = 0;
-        for (int i = threadIdx.x; i < lead * hd; i += kWave * kPagedWaves) vals[i] = kept[i];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) *scale = mx / 127.0f;
-    int8_t* d = static_cast<int8_t*>(is_k ? p.kv.k : p.kv.v) + head;
-    for (int i = from * hd + threadIdx.x; i < end * hd; i += kWave * kPagedWaves) {
-        const int t = i / hd, dim = i - t * hd;
-        const _Float16 v = vals[i];
-        if (t >= lead && v != v) continue;
-        d[is_k ? k_offset<16>(p.kv, t, dim) : v_offset<16>(p.kv, t, dim)] = code_of(v, mx);
-    }
 }
 
-// The 8-bit pages of a sequence, a block per page, kv head and k or v.  The first page and the last are one block's: the
-// first's earlier values lie where the last's are kept.
-template <int E, bool VEC>
-__device__ void hold_unit(const PagedPrepLaunch& p, int unit, _Float16* vals, double* turn) {
+// The pages of a sequence that the step touches, a block per page, kv head and k or v.  The first page and the last are one
+// block's: the first's earlier values lie where the last's are kept.
+template <int E, bool VEC, bool I8>
+__device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _Float16* vals, double* turn) {
     const bool is_k = (unit & 1) == 0;
     unit >>= 1;
     const int h = unit % p.kv.nkv;
@@ -270,33 +378,35 @@ __device__ void hold_unit(const PagedPrepLaunch& p, int unit, _Float16* vals, do
     if (sr.rows == 0 || sr.past < 0 || sr.past >= table_positions(p.step, p.kv)) return;
     const int first = sr.past / p.kv.page, last = (sr.past + sr.rows - 1) / p.kv.page;
     if (nth && first + nth >= last) return;
-    hold_page<E, VEC>(p, sr, s, first + nth, h, is_k, vals, turn);
-    if (nth || first == last) return;
-    __syncthreads();
-    hold_page<E, VEC>(p, sr, s, last, h, is_k, vals, turn);
+    for (int index = first + nth;; index = last) {
+        hold_page<E, VEC, I8>(p, sr, s, index, h, is_k, vals, turn);
+        if (nth || index == last) return;
+        __syncthreads();
+    }
 }
 
-template <int E, bool VEC>
-__global__ void __launch_bounds__(kWave* kPagedWaves) paged_prep_kernel(PagedPrepLaunch p, int hold_blocks, int row_blocks) {
-    extern __shared__ _Float16 page_vals[];
+template <int E, bool VEC, bool I8>
+__global__ void __launch_bounds__(kPagedThreads, 4) paged_prep_kernel(PagedPrepLaunch p, int hold_blocks, int row_blocks, int per) {
+    extern __shared__ uint4 page_lds[];
+    _Float16* page_vals = reinterpret_cast<_Float16*>(page_lds);
     __shared__ double turn[kPagedWaves][kPagedMaxDim];
     const int wid = threadIdx.x / kWave;
     if (static_cast<int>(blockIdx.x) < hold_blocks) {
-        hold_unit<E, VEC>(p, blockIdx.x, page_vals, turn[wid]);
+        hold_unit<E, VEC, I8>(p, blockIdx.x, page_vals, turn[wid]);
         return;
     }
-    const int b = blockIdx.x - hold_blocks, row = b / row_blocks, unit = (b - row * row_blocks) * kPagedWaves + wid;
-    if (unit < p.nq + (p.kv.i8 ? 0 : 2 * p.kv.nkv)) prep_unit<E, VEC>(p, unit, row, turn[wid]);
+    const int b = blockIdx.x - hold_blocks, row = b / row_blocks, h = (b - row * row_blocks) * kPagedWaves * per + wid;
+    if (h < p.nq) query_unit<E, VEC>(p, h, per, row, turn[wid]);
 }
 
 hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
     const int hd = p.kv.head_dim, P = p.kv.page;
     const int64_t touched = (p.step.max_rows + P - 2) / P + 1;  // most pages that one sequence's rows touch
-    const int64_t hold = p.kv.i8 ? 2 * std::max<int64_t>(1, touched - 1) * p.kv.nkv * p.step.seqs : 0;
-    const int row_blocks = (p.nq + (p.kv.i8 ? 0 : 2 * p.kv.nkv) + kPagedWaves - 1) / kPagedWaves;
+    const int64_t hold = 2 * std::max<int64_t>(1, touched - 1) * p.kv.nkv * p.step.seqs;
+    const int per = p.step.rows >= 128 ? kQueryHeads : 1, row_blocks = (p.nq + kPagedWaves * per - 1) / (kPagedWaves * per);
     const int64_t blocks = hold + static_cast<int64_t>(row_blocks) * p.step.rows;
     if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-    const size_t lds = p.kv.i8 ? static_cast<size_t>(P) * hd * 2 : 0;
+    const size_t lds = static_cast<size_t>(P) * (hd + 8) * 2;
     const uintptr_t ptrs = reinterpret_cast<uintptr_t>(p.q_src) | reinterpret_cast<uintptr_t>(p.k_src) |
                            reinterpret_cast<uintptr_t>(p.v_src) | reinterpret_cast<uintptr_t>(p.q_norm) |
                            reinterpret_cast<uintptr_t>(p.k_norm) | reinterpret_cast<uintptr_t>(p.q_out) |
@@ -307,56 +417,83 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
                                                static_cast<int>(lds));
             e != hipSuccess)
             return e;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kWave * kPagedWaves), lds, s, p, static_cast<int>(hold),
-                           row_blocks);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPagedThreads), lds, s, p, static_cast<int>(hold), row_blocks, per);
         return hipGetLastError();
     };
-    if (hd == 128 && al) return go(paged_prep_kernel<2, true>);
-    if (hd == 256 && al) return go(paged_prep_kernel<4, true>);
-    return go(paged_prep_kernel<kPagedMaxDim / kWave, false>);
+    if (hd == 128 && al) return p.kv.i8 ? go(paged_prep_kernel<2, true, true>) : go(paged_prep_kernel<2, true, false>);
+    if (hd == 256 && al) return p.kv.i8 ? go(paged_prep_kernel<4, true, true>) : go(paged_prep_kernel<4, true, false>);
+    constexpr int E = kPagedMaxDim / kWave;
+    return p.kv.i8 ? go(paged_prep_kernel<E, false, true>) : go(paged_prep_kernel<E, false, false>);
 }
 
 // ---------------------------------------------------------------------------
-// Positions read back: a block per row, k or v.
+// Positions read back, a block per sequence, 16 positions in a row of a page, kv
+// head, and k or v: 16-byte pieces in, a row's values out.
 // ---------------------------------------------------------------------------
+constexpr int kReadRows = 16, kReadThreads = 128;
 template <typename T>
-__global__ void __launch_bounds__(256) paged_read_kernel(PagedReadLaunch p) {
-    const int row = blockIdx.x, hd = p.kv.head_dim, nkv = p.kv.nkv;
-    const bool is_v = blockIdx.y != 0;
+__device__ __forceinline__ T paged_value(float x, float scale) {
+    float y = x * scale;
+    asm("" : "+v"(y));  // the fp32 product is a value of its own (else it is rounded to fp16 without it)
+    return static_cast<T>(y);
+}
+
+template <typename T, bool I8>
+__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(PagedReadLaunch p) {
+    constexpr int N = I8 ? 16 : 8;
+    typedef typename std::conditional<I8, int8_t, _Float16>::type V;
+    typedef V piece __attribute__((ext_vector_type(N)));
+    const int s = blockIdx.z, hd = p.kv.head_dim, nkv = p.kv.nkv, h = blockIdx.x >> 1;
+    const bool is_v = blockIdx.x & 1;
     T* out = static_cast<T*>(is_v ? p.v_out : p.k_out);
     if (!out) return;
-    const int s = __builtin_amdgcn_readfirstlane(seq_of_row(p.step, row));
-    if (s >= p.step.seqs) return;
     const SeqRows sr = seq_rows(p.step, s);
-    const int j = row - sr.row0;
-    if (j < 0 || j >= sr.rows) return;
-    const int64_t pos = sr.past < 0 ? -1 : static_cast<int64_t>(sr.past) + j;
-    const int page = pos < 0 || pos >= table_positions(p.step, p.kv) ? -1 : page_at(p.step, p.kv, s, static_cast<int>(pos) / p.kv.page);
-    const int at = page < 0 ? 0 : static_cast<int>(pos) % p.kv.page;
-    const void* pool = is_v ? p.kv.v : p.kv.k;
-    const float* scale = is_v ? p.kv.v_scale : p.kv.k_scale;
-    for (int i = threadIdx.x; i < nkv * hd; i += 256) {
-        const int h = i / hd, d = i - h * hd;
-        float x = 0.0f;
-        if (page >= 0) {
-            const size_t head = page_head(p.kv, page, h);
-            if (p.kv.i8) {
-                x = static_cast<float>(static_cast<const int8_t*>(pool)[head + (is_v ? v_offset<16>(p.kv, at, d) : k_offset<16>(p.kv, at, d))]) *
-                    scale[static_cast<size_t>(page) * nkv + h];
-                asm("" : "+v"(x));  // the fp32 product is a value of its own (else it is rounded to fp16 without it)
-            } else {
-                x = static_cast<float>(static_cast<const _Float16*>(pool)[head + (is_v ? v_offset<8>(p.kv, at, d) : k_offset<8>(p.kv, at, d))]);
+    // rows [j0, j1) of the sequence lie in one group of 16 positions; without a position they are grouped from the first
+    const int past = max(sr.past, 0);
+    const int64_t g0 = (static_cast<int64_t>(past / kReadRows) + blockIdx.y) * kReadRows;
+    const int j0 = static_cast<int>(max(g0 - past, int64_t(0))), j1 = static_cast<int>(min(g0 + kReadRows - past, static_cast<int64_t>(sr.rows)));
+    if (j0 >= j1) return;
+    const int page = sr.past < 0 || g0 >= table_positions(p.step, p.kv) ? -1 : page_at(p.step, p.kv, s, static_cast<int>(g0) / p.kv.page);
+    const size_t width = static_cast<size_t>(nkv) * hd;
+    T* rows = out + static_cast<size_t>(sr.row0 + j0) * width + h * hd;
+    const int n = j1 - j0;
+    if (page < 0) {
+        for (int i = threadIdx.x; i < n * hd; i += kReadThreads) rows[i / hd * width + i % hd] = static_cast<T>(0.0f);
+        return;
+    }
+    const int t0 = static_cast<int>(g0 % p.kv.page) + (past + j0 - static_cast<int>(g0));  // position of row j0 in the page
+    const V* pool = static_cast<const V*>(is_v ? p.kv.v : p.kv.k) + page_head(p.kv, page, h);
+    const float f = I8 ? (is_v ? p.kv.v_scale : p.kv.k_scale)[static_cast<size_t>(page) * nkv + h] : 1.0f;
+    if (is_v) {  // a thread has a dim's positions
+        const int b0 = t0 / N, blocks = (t0 + n - 1) / N + 1 - b0;
+        for (int i = threadIdx.x; i < blocks * hd; i += kReadThreads) {
+            const int b = i / hd, dim = i - b * hd;
+            const piece x = *reinterpret_cast<const piece*>(pool + (static_cast<size_t>(b0 + b) * hd + dim) * N);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int j = (b0 + b) * N + e - t0;
+                if (j >= 0 && j < n) rows[j * width + dim] = paged_value<T>(static_cast<float>(x[e]), f);
             }
         }
-        out[(static_cast<size_t>(row) * nkv + h) * hd + d] = static_cast<T>(x);
+    } else {  // a position's dims
+        const int per = hd / N;
+        for (int i = threadIdx.x; i < n * per; i += kReadThreads) {
+            const int j = i / per, b = i - j * per;
+            const piece x = *reinterpret_cast<const piece*>(pool + (static_cast<size_t>(b) * p.kv.page + t0 + j) * N);
+            T* at = rows + j * width + b * N;
+#pragma unroll
+            for (int e = 0; e < N; ++e) at[e] = paged_value<T>(static_cast<float>(x[e]), f);
+        }
     }
 }
 
 hipError_t launch_paged_read(const PagedReadLaunch& p, hipStream_t s) {
-    if (p.f16)
-        hipLaunchKernelGGL(paged_read_kernel<_Float16>, dim3(p.step.rows, 2), dim3(256), 0, s, p);
+    const dim3 grid(2 * p.kv.nkv, (p.step.max_rows + kReadRows - 2) / kReadRows + 1, p.step.seqs);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kReadThreads), 0, s, p); };
+    if (p.kv.i8)
+        p.f16 ? go(paged_read_kernel<_Float16, true>) : go(paged_read_kernel<float, true>);
     else
-        hipLaunchKernelGGL(paged_read_kernel<float>, dim3(p.step.rows, 2), dim3(256), 0, s, p);
+        p.f16 ? go(paged_read_kernel<_Float16, false>) : go(paged_read_kernel<float, false>);
     return hipGetLastError();
 }
 

@@ -378,8 +378,8 @@ struct PagedStep {  // xqhip_step
 struct RotaryAxes {
     const float2* cs;    // [positions][pairs]
     const int32_t* pos;  // [axes][rows], or nullptr
-    int positions, pairs, axes;
-    uint32_t axis[8];  // two bits per pair
+    int positions, pairs, axes, used;  // used: bit a: some pair turns with axis a
+    uint32_t axis[8];                  // two bits per pair
 };
 struct PagedPrepLaunch {
     const float* q_src;
