@@ -149,6 +149,7 @@ int xqhip_attn_prep_paged(const float* q_src, const float* k_src, const float* v
     p.src_stride = src_stride;
     p.out_stride = out_stride;
     p.eps = eps;
+    p.inv_hd = 1.0 / kv->head_dim;
     if (rotary && rotary->rotary_dim) {
         p.rot.cs = reinterpret_cast<const float2*>(rotary->cs);
         p.rot.pos = rotary->pos;

@@ -170,16 +170,6 @@ struct SeqKeys {
 __device__ __forceinline__ bool is_narrow(int rows, int group) { return rows > 0 && rows * group <= kNarrowCols; }
 __device__ __forceinline__ int tiles_of(int last) { return max(0, last) / kTTile + 1; }
 
-__device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    const int a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31), c = b + __builtin_amdgcn_readlane(v, 47);
-    const int row = (threadIdx.x & (kWave - 1)) >> 4;
-    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
-}
-
 // The narrow kernel's work: sequences of up to 16 columns, their 32-key tiles in units of q, for each kv head, one behind
 // the other; `blocks` blocks take equal ranges of them.  Few tiles: a block has one unit, and a unit lies in one
 // sequence and head.  Many: q = 1, and a block's range may end inside one and go on in the next.

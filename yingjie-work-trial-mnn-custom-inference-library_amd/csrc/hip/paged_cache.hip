@@ -114,13 +114,13 @@ __device__ __forceinline__ double inverse_sqrt(double v) {
 
 // x normalised and turned, by a whole wave; turn: the wave's kPagedMaxDim doubles of LDS
 template <int E, bool VEC>
-__device__ __forceinline__ void turn_head(float (&x)[E], const float (&w)[E], const float2 (&cs)[E], int hd, int half, float eps, int lane,
-                                          double* turn) {
+__device__ __forceinline__ void turn_head(float (&x)[E], const float (&w)[E], const float2 (&cs)[E], int hd, int half, double inv_hd, float eps,
+                                          int lane, double* turn) {
     typedef HeadLanes<E, VEC> L;
     double ss = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) ss += static_cast<double>(x[e]) * x[e];
-    const double inv = inverse_sqrt(wave_sum_double(ss) / hd + static_cast<double>(eps));
+    const double inv = inverse_sqrt(fma(wave_sum_double(ss), inv_hd, static_cast<double>(eps)));
     double v[E];
     wave_lds_sync();
 #pragma unroll
@@ -186,7 +186,7 @@ __device__ __forceinline__ void query_unit(const PagedPrepLaunch& p, int h0, int
 #pragma unroll
     for (int i = 0; i < kQueryHeads; ++i) {
         if (!on(i)) break;
-        turn_head<E, VEC>(x[i], w, cs, hd, p.rot.pairs, p.eps, lane, turn);
+        turn_head<E, VEC>(x[i], w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             x[i][e] = held ? x[i][e] : __builtin_nanf("");
@@ -218,7 +218,7 @@ __device__ __forceinline__ int code_of(_Float16 x, float mx, float inv) {
 template <int E, bool VEC, bool I8>
 __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int h, bool is_k, _Float16* vals, double* turn) {
     typedef HeadLanes<E, VEC> L;
-    constexpr int kBatch = E == 2 ? 4 : 2;
+    constexpr int kBatch = 2;
     __shared__ float wave_mx[kPagedWaves];
     __shared__ uint8_t ok[kPagedMaxPage];
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
@@ -250,22 +250,25 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     for (int t0 = lead + wid; t0 < end; t0 += kBatch * kPagedWaves) {
         float2 cs[kBatch][E];
         bool held[kBatch];
-        if (t0 != lead + wid) load(t0);
+        float y[kBatch][E];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             held[b] = t0 + b * kPagedWaves < end && axes[b].good(p.rot);
             if (is_k && held[b]) axes[b].template angles<E, VEC>(p.rot, lane, cs[b]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[b][e] = x[b][e];
         }
+        if (t0 + kBatch * kPagedWaves < end) load(t0 + kBatch * kPagedWaves);  // (wave-uniform; they come while these are turned)
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const int t = t0 + b * kPagedWaves;
             if (t >= end) break;  // wave-uniform
-            if (is_k && held[b]) turn_head<E, VEC>(x[b], w, cs[b], hd, p.rot.pairs, p.eps, lane, turn);
+            if (is_k && held[b]) turn_head<E, VEC>(y[b], w, cs[b], hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn);
             if (lane == 0) ok[t] = held[b];
             _Float16 v[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                v[e] = I8 ? held_value(x[b][e]) : static_cast<_Float16>(x[b][e]);
+                v[e] = I8 ? held_value(y[b][e]) : static_cast<_Float16>(y[b][e]);
                 if (I8 && held[b] && L::in(lane, e, hd)) mx = fmaxf(mx, fabsf(static_cast<float>(v[e])));
             }
             auto put = [&](_Float16* d) {
@@ -364,23 +367,37 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     }
 }
 
-// The pages of a sequence that the step touches, a block per page, kv head and k or v.  The first page and the last are one
-// block's: the first's earlier values lie where the last's are kept.
+// The pages that the step touches, a block per page, kv head and k or v, in the order of the sequences.  Where a sequence's
+// first 8-bit page holds earlier positions, it and the last are one block's: their values lie where the last's are kept.
+__device__ __forceinline__ int hold_blocks_of(const PagedPrepLaunch& p, const SeqRows& r) {
+    // (positions past the table have no page: the sums stay in 32 bits)
+    if (r.rows == 0 || r.past < 0 || r.past >= table_positions(p.step, p.kv)) return 0;
+    const int pages = (r.past + r.rows - 1) / p.kv.page - r.past / p.kv.page + 1;
+    return pages > 1 && p.kv.i8 && r.past % p.kv.page ? pages - 1 : pages;
+}
 template <int E, bool VEC, bool I8>
 __device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _Float16* vals, double* turn) {
     const bool is_k = (unit & 1) == 0;
     unit >>= 1;
-    const int h = unit % p.kv.nkv;
-    unit /= p.kv.nkv;
-    const int s = unit % p.step.seqs, nth = unit / p.step.seqs;
+    const int h = unit % p.kv.nkv, nth = unit / p.kv.nkv;  // block `nth` of the head
+    int before = 0, s = -1, first_block = 0;
+    for (int c = 0; c < p.step.seqs && s < 0; c += kWave) {  // each wave by itself
+        const int q = c + static_cast<int>(threadIdx.x & (kWave - 1));
+        const int in = before + wave_scan_int(q < p.step.seqs ? hold_blocks_of(p, seq_rows(p.step, q)) : 0);
+        const int n = __popcll(__builtin_amdgcn_ballot_w64(in <= nth));
+        if (n < kWave) {
+            s = c + n;
+            first_block = n ? __builtin_amdgcn_readlane(in, n - 1) : before;
+        }
+        before = __builtin_amdgcn_readlane(in, kWave - 1);
+    }
+    if (s < 0) return;  // fewer pages than blocks
     const SeqRows sr = seq_rows(p.step, s);
-    // (positions past the table have no page: the sum stays in 32 bits)
-    if (sr.rows == 0 || sr.past < 0 || sr.past >= table_positions(p.step, p.kv)) return;
-    const int first = sr.past / p.kv.page, last = (sr.past + sr.rows - 1) / p.kv.page;
-    if (nth && first + nth >= last) return;
-    for (int index = first + nth;; index = last) {
+    const int first = sr.past / p.kv.page, last = (sr.past + sr.rows - 1) / p.kv.page, at = nth - first_block;
+    const bool both = I8 && at == 0 && sr.past % p.kv.page;
+    for (int index = first + at;; index = last) {
         hold_page<E, VEC, I8>(p, sr, s, index, h, is_k, vals, turn);
-        if (nth || index == last) return;
+        if (!both || index == last) return;
         __syncthreads();
     }
 }
@@ -399,19 +416,116 @@ __global__ void __launch_bounds__(kPagedThreads, 4) paged_prep_kernel(PagedPrepL
     if (h < p.nq) query_unit<E, VEC>(p, h, per, row, turn[wid]);
 }
 
+// Steps of single tokens: a wave per sequence and head (query heads, then keys, then values), no barrier between them.
+constexpr int kTokenWaves = 4;
+template <int E, bool VEC, bool I8>
+__global__ void __launch_bounds__(kWave* kTokenWaves) paged_token_kernel(PagedPrepLaunch p, int row_blocks) {
+    typedef HeadLanes<E, VEC> L;
+    __shared__ double turn_lds[kTokenWaves][kPagedMaxDim];
+    const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
+    const int s = blockIdx.x / row_blocks, unit = (static_cast<int>(blockIdx.x) - s * row_blocks) * kTokenWaves + wid;
+    if (unit >= p.nq + 2 * nkv) return;
+    const SeqRows sr = seq_rows(p.step, s);
+    if (sr.rows == 0) return;
+    const int row = sr.row0;
+    const bool is_q = unit < p.nq, is_k = !is_q && unit < p.nq + nkv;
+    const int h = is_q ? unit : (is_k ? unit - p.nq : unit - p.nq - nkv);
+    const float* src = (is_q ? p.q_src : is_k ? p.k_src : p.v_src) + static_cast<size_t>(row) * p.src_stride +
+                       static_cast<size_t>(h) * (is_q && p.gated ? 2 * hd : hd);
+    float x[E], gate[E] = {}, w[E];
+    L::load(src, lane, hd, x);
+    if (is_q && p.gated) L::load(src + hd, lane, hd, gate);
+    if (is_q || is_k) L::load(is_q ? p.q_norm : p.k_norm, lane, hd, w);
+    const int64_t pos = sr.past < 0 ? -1 : sr.past;
+    RowAxes axes;
+    axes.load(p.rot, p.step.rows, row, static_cast<int>(pos));
+    const Place place(p, s, pos);
+    const bool turned = axes.good(p.rot);
+    float2 cs[E] = {};
+    if (turned && (is_q || is_k)) axes.template angles<E, VEC>(p.rot, lane, cs);
+    const bool held = turned && !place.none();
+    const int t = static_cast<int>(pos) & (P - 1);
+    float was = 0.0f;
+    const size_t sat = static_cast<size_t>(max(place.page, 0)) * nkv + h;
+    float* scale = is_k ? p.kv.k_scale : p.kv.v_scale;
+    if (I8 && !is_q && held && t) was = scale[sat];
+    if (is_q || is_k) turn_head<E, VEC>(x, w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn_lds[wid]);
+    if (is_q) {
+        const size_t o = static_cast<size_t>(row) * p.out_stride + static_cast<size_t>(h) * hd;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = held ? x[e] : __builtin_nanf("");
+        L::store(p.q_out + o, lane, hd, x);
+        if (p.gate_out) L::store(p.gate_out + o, lane, hd, gate);
+        return;
+    }
+    if (!held) return;
+    constexpr int N = I8 ? 16 : 8;
+    auto offset = [&](int pos_in, int dim) { return is_k ? k_offset<N>(p.kv, pos_in, dim) : v_offset<N>(p.kv, pos_in, dim); };
+    const size_t head = page_head(p.kv, place.page, h);
+    if constexpr (!I8) {
+        _Float16* d = static_cast<_Float16*>(is_k ? p.kv.k : p.kv.v) + head;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (L::in(lane, e, hd)) d[offset(t, L::dim(lane, e))] = static_cast<_Float16>(x[e]);
+    } else {
+        int8_t* d = static_cast<int8_t*>(is_k ? p.kv.k : p.kv.v) + head;
+        _Float16* kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(place.open) * nkv + h) * P * hd;
+        _Float16 v[E];
+        float mx = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            v[e] = held_value(x[e]);
+            if (!L::in(lane, e, hd)) continue;
+            mx = fmaxf(mx, fabsf(static_cast<float>(v[e])));
+            kept[static_cast<size_t>(t) * hd + L::dim(lane, e)] = v[e];
+        }
+        mx = wave_max(mx);
+        const float before = static_cast<float>(static_cast<_Float16>(was * 127.0f));  // the maximum, an fp16 value, exactly
+        const bool grew = mx > before;
+        mx = grew ? mx : before;
+        const float inv = mx > 0.0f ? 1.0f / mx : 0.0f;
+        if (lane == 0) scale[sat] = mx / 127.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (L::in(lane, e, hd)) d[offset(t, L::dim(lane, e))] = static_cast<int8_t>(code_of(v[e], mx, inv));
+        if (grew) {  // wave-uniform: the page's earlier codes anew (of 64 positions a maximum rises at five or so)
+#pragma unroll 4
+            for (int i = 0; i < t; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (L::in(lane, e, hd))
+                        d[offset(i, L::dim(lane, e))] = static_cast<int8_t>(code_of(kept[static_cast<size_t>(i) * hd + L::dim(lane, e)], mx, inv));
+        }
+    }
+}
+
 hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
     const int hd = p.kv.head_dim, P = p.kv.page;
-    const int64_t touched = (p.step.max_rows + P - 2) / P + 1;  // most pages that one sequence's rows touch
-    const int64_t hold = 2 * std::max<int64_t>(1, touched - 1) * p.kv.nkv * p.step.seqs;
-    const int per = p.step.rows >= 128 ? kQueryHeads : 1, row_blocks = (p.nq + kPagedWaves * per - 1) / (kPagedWaves * per);
-    const int64_t blocks = hold + static_cast<int64_t>(row_blocks) * p.step.rows;
-    if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-    const size_t lds = static_cast<size_t>(P) * (hd + 8) * 2;
     const uintptr_t ptrs = reinterpret_cast<uintptr_t>(p.q_src) | reinterpret_cast<uintptr_t>(p.k_src) |
                            reinterpret_cast<uintptr_t>(p.v_src) | reinterpret_cast<uintptr_t>(p.q_norm) |
                            reinterpret_cast<uintptr_t>(p.k_norm) | reinterpret_cast<uintptr_t>(p.q_out) |
                            reinterpret_cast<uintptr_t>(p.gate_out);
     const bool al = (ptrs & 15u) == 0 && p.src_stride % 4 == 0 && p.out_stride % 4 == 0;
+    if (p.step.max_rows == 1) {
+        const int row_blocks = (p.nq + 2 * p.kv.nkv + kTokenWaves - 1) / kTokenWaves;
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.step.seqs) * row_blocks), dim3(kWave * kTokenWaves), 0, s, p, row_blocks);
+            return hipGetLastError();
+        };
+        constexpr int E = kPagedMaxDim / kWave;
+        if (hd == 128 && al) return p.kv.i8 ? go(paged_token_kernel<2, true, true>) : go(paged_token_kernel<2, true, false>);
+        if (hd == 256 && al) return p.kv.i8 ? go(paged_token_kernel<4, true, true>) : go(paged_token_kernel<4, true, false>);
+        return p.kv.i8 ? go(paged_token_kernel<E, false, true>) : go(paged_token_kernel<E, false, false>);
+    }
+    const int per = p.step.rows >= 128 ? std::min(kQueryHeads, std::max(1, p.nq / kPagedWaves)) : 1;
+    const int row_blocks = (p.nq + kPagedWaves * per - 1) / (kPagedWaves * per);
+    // pages of any division of the rows among the sequences: n rows reach over n / P page borders, and one more; one more
+    // page than borders (one less block than pages: 8 bits)
+    const int64_t hold = 2 * static_cast<int64_t>(p.kv.nkv) * (p.step.rows / P + (p.kv.i8 ? 1 : 2) * std::min(p.step.seqs, p.step.rows));
+    const int64_t blocks = hold + static_cast<int64_t>(row_blocks) * p.step.rows;
+    if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+    const size_t lds = static_cast<size_t>(P) * (hd + 8) * 2;
     auto go = [&](auto kernel) {
         if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(lds));

@@ -35,6 +35,17 @@ __device__ __forceinline__ int seq_of_row(const PagedStep& st, int row) {
     return n;
 }
 
+// sum over the lanes up to each, of the whole wave
+__device__ __forceinline__ int wave_scan_int(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    const int a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31), c = b + __builtin_amdgcn_readlane(v, 47);
+    const int row = (threadIdx.x & (kWave - 1)) >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
+}
+
 // positions that the table has room for
 __device__ __forceinline__ int table_positions(const PagedStep& st, const PagedCache& kv) { return st.max_pages * kv.page; }
 

@@ -391,6 +391,7 @@ struct PagedPrepLaunch {
     float* gate_out;
     int gated, nq, src_stride, out_stride;
     float eps;
+    double inv_hd;  // 1 / head_dim
     RotaryAxes rot;
     PagedStep step;
     PagedCache kv;
