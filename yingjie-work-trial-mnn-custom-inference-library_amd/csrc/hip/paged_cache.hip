@@ -76,30 +76,44 @@ struct HeadLanes {
 
 
 // The positions of a row on its axes (wave-uniform), and whether all that its pairs use lie in the table.
+// (The first's, and what the others are more: a choice between four values held in an object becomes an indexed load of
+// it, from LDS, at an offset that takes the dispatch packet in host memory: 13 us.)
 struct RowAxes {
-    int at[4];
+    int a0, d1, d2, d3;
+    bool fine;
     __device__ __forceinline__ void load(const RotaryAxes& r, int rows, int row, int pos) {
-#pragma unroll
-        for (int a = 0; a < 4; ++a) at[a] = r.pos && a < r.axes ? r.pos[static_cast<size_t>(a) * rows + row] : pos;
+        auto at = [&](int a) { return r.pos && a < r.axes ? r.pos[static_cast<size_t>(a) * rows + row] : pos; };
+        auto in = [&](int a, int p) { return !(r.used >> a & 1) || (p >= 0 && p < r.positions); };
+        const int p0 = at(0), p1 = at(1), p2 = at(2), p3 = at(3);
+        fine = in(0, p0) && in(1, p1) && in(2, p2) && in(3, p3);
+        a0 = fine ? p0 : 0;  // (the angles of a row that is not: those of position 0)
+        d1 = fine ? p1 - p0 : 0;
+        d2 = fine ? p2 - p0 : 0;
+        d3 = fine ? p3 - p0 : 0;
     }
-    __device__ __forceinline__ bool good(const RotaryAxes& r) const {
-        bool all = true;
-#pragma unroll
-        for (int a = 0; a < 4; ++a) all = all && (!(r.used >> a & 1) || (at[a] >= 0 && at[a] < r.positions));
-        return all;
-    }
-    // the angles of a lane's dims (those of a good row)
-    template <int E, bool VEC>
-    __device__ __forceinline__ void angles(const RotaryAxes& r, int lane, float2 (&cs)[E]) const {
-        const int half = r.pairs;
+    __device__ __forceinline__ int of(int axis) const { return a0 + (axis == 1 ? d1 : 0) + (axis == 2 ? d2 : 0) + (axis == 3 ? d3 : 0); }
+};
+
+// The pairs of a lane's dims and their axes, the same for every row.
+template <int E, bool VEC>
+struct LanePairs {
+    int pair[E], axis[E];  // pair -1: a dim that is not turned
+    __device__ __forceinline__ LanePairs(const RotaryAxes& r, int lane) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int d = HeadLanes<E, VEC>::dim(lane, e);
+            const int d = HeadLanes<E, VEC>::dim(lane, e), i = d < r.pairs ? d : d - r.pairs;
+            uint32_t bits = 0;  // (selected from the arguments: indexed by lane they would be a load)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) bits = i / 16 == k ? r.axis[k] : bits;
+            pair[e] = d < 2 * r.pairs ? i : -1;
+            axis[e] = bits >> 2 * (i % 16) & 3;
+        }
+    }
+    __device__ __forceinline__ void angles(const RotaryAxes& r, const RowAxes& row, float2 (&cs)[E]) const {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
             cs[e] = make_float2(1.0f, 0.0f);
-            if (d >= 2 * half) continue;
-            const int i = d < half ? d : d - half, a = r.axis[i / 16] >> 2 * (i % 16) & 3;
-            const int p = a == 0 ? at[0] : a == 1 ? at[1] : a == 2 ? at[2] : at[3];
-            cs[e] = r.cs[static_cast<size_t>(p) * half + i];
+            if (pair[e] >= 0) cs[e] = r.cs[static_cast<size_t>(row.of(axis[e])) * r.pairs + pair[e]];
         }
     }
 };
@@ -112,31 +126,63 @@ __device__ __forceinline__ double inverse_sqrt(double v) {
     return y;
 }
 
-// x normalised and turned, by a whole wave; turn: the wave's kPagedMaxDim doubles of LDS
-template <int E, bool VEC>
-__device__ __forceinline__ void turn_head(float (&x)[E], const float (&w)[E], const float2 (&cs)[E], int hd, int half, double inv_hd, float eps,
-                                          int lane, double* turn) {
+__device__ __forceinline__ double lane_value(double v, int from) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_ds_bpermute(4 * from, static_cast<int>(static_cast<uint32_t>(u)));
+    const uint32_t hi = __builtin_amdgcn_ds_bpermute(4 * from, static_cast<int>(static_cast<uint32_t>(u >> 32)));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// B rows of a head normalised and turned, by a whole wave, their chains of 64-bit operations beside each other.  A dim's
+// partner in its pair lies `half` dims on: in another lane (VEC, half a multiple of E), or it is fetched through the wave's
+// kPagedMaxDim doubles of LDS, `turn`.
+template <int B, int E, bool VEC>
+__device__ __forceinline__ void turn_heads(float (&x)[B][E], const float (&w)[E], const float2 (&cs)[B][E], int hd, int half, double inv_hd,
+                                           float eps, int lane, double* turn) {
     typedef HeadLanes<E, VEC> L;
-    double ss = 0.0;
+    double v[B][E], inv[B];
 #pragma unroll
-    for (int e = 0; e < E; ++e) ss += static_cast<double>(x[e]) * x[e];
-    const double inv = inverse_sqrt(fma(wave_sum_double(ss), inv_hd, static_cast<double>(eps)));
-    double v[E];
-    wave_lds_sync();
+    for (int b = 0; b < B; ++b) {
+        inv[b] = 0.0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        v[e] = static_cast<double>(x[e]) * inv * w[e];
-        if (L::in(lane, e, hd)) turn[L::dim(lane, e)] = v[e];
+        for (int e = 0; e < E; ++e) inv[b] += static_cast<double>(x[b][e]) * x[b][e];
     }
-    wave_lds_sync();
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int d = L::dim(lane, e);
-        if (d < half)
-            v[e] = v[e] * cs[e].x - turn[half + d] * cs[e].y;
-        else if (d < 2 * half)
-            v[e] = v[e] * cs[e].x + turn[d - half] * cs[e].y;
-        x[e] = static_cast<float>(v[e]);
+    for (int b = 0; b < B; ++b) inv[b] = wave_sum_double(inv[b]);
+#pragma unroll
+    for (int b = 0; b < B; ++b) inv[b] = inverse_sqrt(fma(inv[b], inv_hd, static_cast<double>(eps)));
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[b][e] = static_cast<double>(x[b][e]) * inv[b] * w[e];
+    const bool by_lanes = VEC && half % E == 0;  // block-uniform
+    auto turned = [&](double a, double other, float2 c, int d) { return d < half ? a * c.x - other * c.y : (d < 2 * half ? a * c.x + other * c.y : a); };
+    if (by_lanes) {
+        const int from = lane * E < half ? lane + half / E : lane - half / E;
+        double other[B][E];
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int e = 0; e < E; ++e) other[b][e] = lane_value(v[b][e], from & (kWave - 1));
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[b][e] = static_cast<float>(turned(v[b][e], other[b][e], cs[b][e], L::dim(lane, e)));
+    } else {
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            wave_lds_sync();
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (L::in(lane, e, hd)) turn[L::dim(lane, e)] = v[b][e];
+            wave_lds_sync();
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int d = L::dim(lane, e);
+                const double other = d < half ? turn[half + d] : (d < 2 * half ? turn[d - half] : 0.0);
+                x[b][e] = static_cast<float>(turned(v[b][e], other, cs[b][e], d));
+            }
+        }
     }
 }
 
@@ -158,6 +204,7 @@ template <int E, bool VEC>
 __device__ __forceinline__ void query_unit(const PagedPrepLaunch& p, int h0, int per, int row, double* turn) {
     typedef HeadLanes<E, VEC> L;
     const int lane = threadIdx.x & (kWave - 1), hd = p.kv.head_dim;
+    const LanePairs<E, VEC> pairs(p.rot, lane);
     const float* src = p.q_src + static_cast<size_t>(row) * p.src_stride;
     float x[kQueryHeads][E], gate[kQueryHeads][E], w[E];
     auto on = [&](int i) { return i < per && h0 + i * kPagedWaves < p.nq; };  // wave-uniform
@@ -178,22 +225,25 @@ __device__ __forceinline__ void query_unit(const PagedPrepLaunch& p, int h0, int
     RowAxes axes;
     axes.load(p.rot, p.step.rows, row, static_cast<int>(pos));
     const Place place(p, s, pos);
-    const bool turned = axes.good(p.rot);
-    float2 cs[E] = {};
-    if (turned) axes.angles<E, VEC>(p.rot, lane, cs);
+    const bool turned = axes.fine;
+    float2 cs[1][E] = {};
+    pairs.angles(p.rot, axes, cs[0]);
     const bool held = turned && !place.none();
     const size_t o = static_cast<size_t>(row) * p.out_stride;
 #pragma unroll
     for (int i = 0; i < kQueryHeads; ++i) {
         if (!on(i)) break;
-        turn_head<E, VEC>(x[i], w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn);
+        float y[1][E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[0][e] = x[i][e];
+        turn_heads<1, E, VEC>(y, w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            x[i][e] = held ? x[i][e] : __builtin_nanf("");
+            y[0][e] = held ? y[0][e] : __builtin_nanf("");
             if (!p.gated) gate[i][e] = 0.0f;
         }
         const size_t at = o + static_cast<size_t>(h0 + i * kPagedWaves) * hd;
-        L::store(p.q_out + at, lane, hd, x[i]);
+        L::store(p.q_out + at, lane, hd, y[0]);
         if (p.gate_out) L::store(p.gate_out + at, lane, hd, gate[i]);
     }
 }
@@ -218,13 +268,15 @@ __device__ __forceinline__ int code_of(_Float16 x, float mx, float inv) {
 template <int E, bool VEC, bool I8>
 __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int h, bool is_k, _Float16* vals, double* turn) {
     typedef HeadLanes<E, VEC> L;
-    constexpr int kBatch = 2;
+    constexpr int kBatch = E == 2 ? 4 : 2;
     __shared__ float wave_mx[kPagedWaves];
     __shared__ uint8_t ok[kPagedMaxPage];
-    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
+    const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
     const int base = index * P, ld = hd + 8;                                          // position of the page's first
     const int lead = max(0, sr.past - base), end = min(P, sr.past + sr.rows - base);  // new ones: [lead, end)
     const bool last = base + P >= sr.past + sr.rows;
+    const LanePairs<E, VEC> pairs(p.rot, lane);
     float x[kBatch][E], w[E];
     RowAxes axes[kBatch];
     auto load = [&](int t0) {
@@ -232,7 +284,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
         for (int b = 0; b < kBatch; ++b) {  // (rows behind the last: the last again)
             const int row = sr.row0 + base + min(t0 + b * kPagedWaves, end - 1) - sr.past;
             L::load((is_k ? p.k_src : p.v_src) + static_cast<size_t>(row) * p.src_stride + static_cast<size_t>(h) * hd, lane, hd, x[b]);
-            axes[b].load(p.rot, p.step.rows, row, base + t0 + b * kPagedWaves);
+            axes[b].load(p.rot, p.step.rows, row, base + min(t0 + b * kPagedWaves, end - 1));
         }
     };
     load(lead + wid);
@@ -253,17 +305,17 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
         float y[kBatch][E];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            held[b] = t0 + b * kPagedWaves < end && axes[b].good(p.rot);
-            if (is_k && held[b]) axes[b].template angles<E, VEC>(p.rot, lane, cs[b]);
+            held[b] = t0 + b * kPagedWaves < end && axes[b].fine;
+            if (is_k) pairs.angles(p.rot, axes[b], cs[b]);
 #pragma unroll
             for (int e = 0; e < E; ++e) y[b][e] = x[b][e];
         }
         if (t0 + kBatch * kPagedWaves < end) load(t0 + kBatch * kPagedWaves);  // (wave-uniform; they come while these are turned)
+        if (is_k) turn_heads<kBatch, E, VEC>(y, w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn);
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const int t = t0 + b * kPagedWaves;
             if (t >= end) break;  // wave-uniform
-            if (is_k && held[b]) turn_head<E, VEC>(y[b], w, cs[b], hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn);
             if (lane == 0) ok[t] = held[b];
             _Float16 v[E];
 #pragma unroll
@@ -407,7 +459,7 @@ __global__ void __launch_bounds__(kPagedThreads, 4) paged_prep_kernel(PagedPrepL
     extern __shared__ uint4 page_lds[];
     _Float16* page_vals = reinterpret_cast<_Float16*>(page_lds);
     __shared__ double turn[kPagedWaves][kPagedMaxDim];
-    const int wid = threadIdx.x / kWave;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (static_cast<int>(blockIdx.x) < hold_blocks) {
         hold_unit<E, VEC, I8>(p, blockIdx.x, page_vals, turn[wid]);
         return;
@@ -433,7 +485,8 @@ __global__ void __launch_bounds__(kWave* kTokenWaves) paged_token_kernel(PagedPr
     const int h = is_q ? unit : (is_k ? unit - p.nq : unit - p.nq - nkv);
     const float* src = (is_q ? p.q_src : is_k ? p.k_src : p.v_src) + static_cast<size_t>(row) * p.src_stride +
                        static_cast<size_t>(h) * (is_q && p.gated ? 2 * hd : hd);
-    float x[E], gate[E] = {}, w[E];
+    float in[1][E], gate[E] = {}, w[E];
+    float(&x)[E] = in[0];
     L::load(src, lane, hd, x);
     if (is_q && p.gated) L::load(src + hd, lane, hd, gate);
     if (is_q || is_k) L::load(is_q ? p.q_norm : p.k_norm, lane, hd, w);
@@ -441,16 +494,16 @@ __global__ void __launch_bounds__(kWave* kTokenWaves) paged_token_kernel(PagedPr
     RowAxes axes;
     axes.load(p.rot, p.step.rows, row, static_cast<int>(pos));
     const Place place(p, s, pos);
-    const bool turned = axes.good(p.rot);
-    float2 cs[E] = {};
-    if (turned && (is_q || is_k)) axes.template angles<E, VEC>(p.rot, lane, cs);
+    const bool turned = axes.fine;
+    float2 cs[1][E] = {};
+    if (is_q || is_k) LanePairs<E, VEC>(p.rot, lane).angles(p.rot, axes, cs[0]);
     const bool held = turned && !place.none();
     const int t = static_cast<int>(pos) & (P - 1);
     float was = 0.0f;
     const size_t sat = static_cast<size_t>(max(place.page, 0)) * nkv + h;
     float* scale = is_k ? p.kv.k_scale : p.kv.v_scale;
     if (I8 && !is_q && held && t) was = scale[sat];
-    if (is_q || is_k) turn_head<E, VEC>(x, w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn_lds[wid]);
+    if (is_q || is_k) turn_heads<1, E, VEC>(in, w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn_lds[wid]);
     if (is_q) {
         const size_t o = static_cast<size_t>(row) * p.out_stride + static_cast<size_t>(h) * hd;
 #pragma unroll
