@@ -142,11 +142,13 @@ __global__ void __launch_bounds__(256) paged_attn_row_kernel(PagedAttnLaunch p) 
 // reason or the weights sum to 0 the block that writes such an output computes
 // its rows again by attend_paged_row.
 // ---------------------------------------------------------------------------
+template <int HD>
+constexpr int kBlockWaves = HD == 128 ? 8 : 4;  // registers for two waves, or one, per SIMD
 constexpr int kNarrowCols = 16;     // up to 16 columns: paged_narrow_kernel
 constexpr int kNarrowBlocks = 256;  // blocks that share the narrow sequences' tiles
-constexpr int kWideCols = 64;       // other sequences: paged_wide_kernel
+constexpr int kLeastCols = 64, kMostCols = 128;  // columns of other sequences' blocks: wide_block
 constexpr int kWideBlocks = 256;    // blocks that few row tiles' keys are split over
-constexpr int kMostUnits = 65535 * kPagedMaxGroup / kWideCols + 1024 + kWideBlocks;  // row tiles and splits of a step
+constexpr int kMostUnits = 65535 * kPagedMaxGroup / kLeastCols + 1024 + kWideBlocks;  // row tiles and splits of a step
 
 // the key of a tile that MFMA row r stands for: a lane's slots are then keys 16 (slot / 8) + 8 (lane / 32) + slot % 8
 // (fp16: pieces of 8 positions), or 16 (lane / 32) + 8 (slot / 8) + slot % 8 (8 bits: pieces of 16)
@@ -253,14 +255,15 @@ struct WideUnit {
 };
 // Workspace: where the merge finds the narrow sequences' parts, the wide kernel's units, partial outputs.
 struct PagedWs {
-    int* head;        // [0] wide units, [1] their slots
+    int* head;        // [0] wide units, [1] their slots, [2] blocks of the narrow work
     int4* narrow_at;  // [seqs][nkv]: blocks that share the sequence's tiles, the first of them and its slot, whether a single
                       // block's output has to be computed again
     int4* wide_at;    // [wide units][nkv], of those without splits: as above
     int* first;       // [slots]: first unit of the slot's row tile
     WideUnit* units;
     float* narrow;    // [2 blocks][16][hd + 2]
-    float* wide;      // [slots][nkv][64][hd + 2]
+    float* wide;      // [slots][nkv][columns][hd + 2]
+    int cols;         // of a wide block
 };
 constexpr size_t kWsHead = 16;
 
@@ -415,13 +418,13 @@ __device__ __forceinline__ u32x4 first_halves(u32x4 v, int n) {
     return v;
 }
 
-template <int HD>
+template <int HD, int CT>
 struct WideShape {
-    static constexpr int CT = 2, KS = HD == 128 ? 4 : 2;
-    static constexpr int kThreads = kWave * CT * KS, kKeys = kTTile * KS, kCols = kWideCols;
-    using F = PagedBlock<HD, KS, kWideCols>;
+    static constexpr int KS = kBlockWaves<HD> / CT;
+    static constexpr int kThreads = kWave * CT * KS, kKeys = kTTile * KS, kCols = kTTile * CT;
+    using F = PagedBlock<HD, KS, kCols>;
     struct Q {  // of QueryStage
-        static constexpr int kThreads = WideShape::kThreads, kCols = kWideCols;
+        static constexpr int kThreads = WideShape::kThreads, kCols = WideShape::kCols;
     };
     static constexpr int kBuf = kKeys * HD;  // halves
     static constexpr size_t kKvBytes = 4 * static_cast<size_t>(kBuf) * 2;
@@ -431,11 +434,12 @@ struct WideShape {
 
 // The units of the sequences that the narrow kernel does not take, by one block: a row tile's keys are split in proportion
 // to their number where there are fewer tiles than blocks that fill the card.
-template <int THREADS, int HD>
-__device__ void plan_wide(const PagedAttnLaunch& p, const PagedWs& ws, int* pre, int* red) {
-    constexpr int kWaves = THREADS / kWave, kPer = 1024 / THREADS, kKeys = WideShape<HD>::kKeys;
+constexpr int kPlanThreads = 1024;
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunch p, PagedWs ws, int kKeys) {
+    constexpr int THREADS = kPlanThreads, kWaves = THREADS / kWave, kPer = 1024 / THREADS;
+    __shared__ int pre[1024], red[kWaves];
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
-    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kWideCols / group, seqs = p.step.seqs;
+    const int nkv = p.kv.nkv, group = p.nq / nkv, T = ws.cols / group, seqs = p.step.seqs;
     auto block_scan = [&](int v, int& all) {  // before this thread; all: of every thread
         const int in = wave_scan_int(v);
         __syncthreads();
@@ -503,9 +507,13 @@ __device__ void plan_wide(const PagedAttnLaunch& p, const PagedWs& ws, int* pre,
             if (n > 1) ws.first[slot] = at & 0xffff;
         }
     }
-    if (threadIdx.x == 0) {
-        ws.head[0] = units & 0xffff;
-        ws.head[1] = units >> 16;
+    if (wid == 0) {
+        const NarrowWork w(p);
+        if (lane == 0) {
+            ws.head[0] = units & 0xffff;
+            ws.head[1] = units >> 16;
+            ws.head[2] = w.blocks;
+        }
     }
 }
 
@@ -514,24 +522,18 @@ __device__ void plan_wide(const PagedAttnLaunch& p, const PagedWs& ws, int* pre,
 // back into the two halves.  Each wave takes its own 32-key tiles, K and V straight into registers, the next tile's on
 // their way meanwhile; no barrier before the waves join.
 template <int HD, bool I8, int KS>
-__global__ void __launch_bounds__(kWave* KS, (KS + 3) / 4) paged_narrow_kernel(PagedAttnLaunch p, PagedWs ws) {
+__device__ __forceinline__ void narrow_block(const PagedAttnLaunch& p, const PagedWs& ws, int block, uint4* paged_lds) {
     using F = PagedBlock<HD, KS, kNarrowCols>;
     using Q = QueryStage<F, HD>;
     constexpr int kSteps = HD / 16, kDimTiles = HD / 32;
     constexpr int kKPieces = HD / (I8 ? 32 : 16), kVPieces = I8 ? kDimTiles : 2 * kDimTiles;
-    extern __shared__ uint4 paged_lds[];
-    __shared__ int pre[1024], red[KS], redo;
+    __shared__ int redo;
     const int nkv = p.kv.nkv, group = p.nq / nkv, T = kNarrowCols / group;
     const int lane = threadIdx.x & (kWave - 1), ks = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int cl = lane & 31, g = lane >> 5, col = cl & 15, part = cl >> 4;
     const uint32_t inv_t = (65535u + T) / T;
     const int ch = static_cast<int>(col * inv_t >> 16), ctok = col - ch * T;
-    if (blockIdx.x == kNarrowBlocks) {
-        plan_wide<F::kThreads, HD>(p, ws, pre, red);
-        return;
-    }
     NarrowWork w(p);
-    const int block = blockIdx.x;
     if (block >= w.blocks) return;
     const int begin = w.begin(block), end = w.begin(block + 1);
     const uint32_t kat = (static_cast<uint32_t>(g) * p.kv.page + key_of_row<I8>(cl)) * 16u, kstep = 32u * p.kv.page;
@@ -762,22 +764,21 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
 // 64 columns: CT column tiles x KS key waves.  K and V are staged chunk by chunk (32 KS keys, shared by the column tiles) in
 // LDS as the pages hold them (8-bit codes as fp16), twice each: one barrier a chunk, the next chunk's loads over a whole
 // chunk ahead, and a chunk's products with V beside the next one's softmax.
-template <int HD, bool I8>
-__global__ void __launch_bounds__(WideShape<HD>::kThreads, (WideShape<HD>::kThreads / kWave + 3) / 4) paged_wide_kernel(PagedAttnLaunch p, PagedWs ws) {
-    using S = WideShape<HD>;
+template <int HD, bool I8, int CT>
+__device__ __forceinline__ void wide_block(const PagedAttnLaunch& p, const PagedWs& ws, int index, uint4* paged_lds) {
+    using S = WideShape<HD, CT>;
     using Q = QueryStage<typename S::Q, HD>;
-    constexpr int CT = S::CT, KS = S::KS, kSteps = HD / 16, kDimTiles = HD / 32, kKeys = S::kKeys;
+    constexpr int KS = S::KS, kSteps = HD / 16, kDimTiles = HD / 32, kKeys = S::kKeys;
     constexpr uint32_t es = I8 ? 1u : 2u;
     constexpr int kKLoads = HD / (I8 ? 32 : 16) / CT, kVLoads = (I8 ? 2 : 4) * HD / 64 / CT;  // of a wave and chunk, 1 KiB each
-    extern __shared__ uint4 paged_lds[];
     __shared__ int redo;
-    const int nkv = p.kv.nkv, kh = blockIdx.x % nkv, group = p.nq / nkv, T = kWideCols / group;
-    const int unit = blockIdx.x / nkv;
+    const int nkv = p.kv.nkv, kh = index % nkv, group = p.nq / nkv, T = S::kCols / group;
+    const int unit = index / nkv;
     if (unit >= ws.head[0]) return;
     const WideUnit un = ws.units[unit];
     const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int ct = wid % CT, ks = wid / CT, cl = lane & 31, g = lane >> 5;
-    const uint32_t inv_t = (65535u + T) / T;  // c / T = c inv_t >> 16 for c < 64
+    const uint32_t inv_t = (65535u + T) / T;  // c / T = c inv_t >> 16 for c < 128, T <= 128
     const int s = __builtin_amdgcn_readfirstlane(un.seq), t0 = __builtin_amdgcn_readfirstlane(un.tile) * T;
     const int begin = __builtin_amdgcn_readfirstlane(un.begin), end = __builtin_amdgcn_readfirstlane(un.end);
     const SeqKeys sk(p, s);
@@ -957,34 +958,34 @@ __global__ void __launch_bounds__(WideShape<HD>::kThreads, (WideShape<HD>::kThre
     for (; c < clear; ++c) chunk(c, std::false_type{}, std::false_type{});
     for (; c < end; ++c) chunk(c, std::false_type{}, std::true_type{});
     add_values(end - 1);
-    float* part_out = un.splits > 1 ? ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * kWideCols * (HD + 2) : nullptr;
-    finish_paged<HD, CT, KS, kWideCols, false>(p, sk.r, kh, t0, ntok, T, inv_t, part_out, ws.wide_at + unit * nkv + kh, live, o, m, l, paged_lds,
+    float* part_out = un.splits > 1 ? ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * S::kCols * (HD + 2) : nullptr;
+    finish_paged<HD, CT, KS, S::kCols, false>(p, sk.r, kh, t0, ntok, T, inv_t, part_out, ws.wide_at + unit * nkv + kh, live, o, m, l, paged_lds,
                                                &redo);
 }
 
 // The splits of a row tile joined, each slot's block a share of the columns; and outputs that have to be computed again.
 template <int HD>
 __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int block, int blocks, float* smem) {
-    __shared__ float fac[kWideCols + kWideBlocks], total[kWideCols];  // a block's columns times the splits
+    __shared__ float fac[kMostCols + kWideBlocks], total[kMostCols];  // a block's columns times the splits
     __shared__ int list[kMergeThreads], count, redo;
-    constexpr int kQuads = HD / 4, kSlot = kWideCols * (HD + 2);
-    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kWideCols / group;
+    constexpr int kQuads = HD / 4;
+    const int cols = ws.cols, slot_size = cols * (HD + 2), nkv = p.kv.nkv, group = p.nq / nkv, T = cols / group;
     const int units = ws.head[0], slots = ws.head[1], slot = block / nkv, kh = block % nkv;
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
     if (slot < slots) {
         const WideUnit un = ws.units[ws.first[slot]];
         const SeqRows sr = seq_rows(p.step, un.seq);
         const int n = un.splits, k = slot - un.slot, t0 = un.tile * T, ntok = min(T, sr.rows - t0);
-        const int c0 = kWideCols * k / n, c1 = kWideCols * (k + 1) / n;
-        const size_t stride = static_cast<size_t>(nkv) * kSlot;
-        const float* base = ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * kSlot;
+        const int c0 = cols * k / n, c1 = cols * (k + 1) / n;
+        const size_t stride = static_cast<size_t>(nkv) * slot_size;
+        const float* base = ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * slot_size;
         for (int c = c0 + wid; c < c1; c += kMergeThreads / kWave) {
             float M = -INFINITY, L = 0.0f;
             const bool on = c / T < group && c % T < ntok;  // (others' sums were not written)
-            for (int b = lane; on && b < n; b += kWave) M = fmaxf(M, base[b * stride + kWideCols * HD + 2 * c]);
+            for (int b = lane; on && b < n; b += kWave) M = fmaxf(M, base[b * stride + cols * HD + 2 * c]);
             M = wave_max(M);
             for (int b = lane; on && b < n; b += kWave) {
-                const float2 ml = *reinterpret_cast<const float2*>(base + b * stride + kWideCols * HD + 2 * c);
+                const float2 ml = *reinterpret_cast<const float2*>(base + b * stride + cols * HD + 2 * c);
                 const float f = __builtin_amdgcn_exp2f(ml.x - M);
                 fac[(c - c0) * n + b] = f;
                 L += f * ml.y;
@@ -1056,7 +1057,7 @@ static PagedWs paged_ws(float* base, int hd, int nkv, size_t* bytes) {
     w.first = reinterpret_cast<int*>(take(sizeof(int) * kWideBlocks));
     w.units = reinterpret_cast<WideUnit*>(take(sizeof(WideUnit) * kMostUnits));
     w.narrow = reinterpret_cast<float*>(take(sizeof(float) * 2 * kNarrowBlocks * kNarrowCols * (hd + 2)));
-    w.wide = reinterpret_cast<float*>(take(sizeof(float) * std::max(kWideBlocks, nkv) * kWideCols * (hd + 2)));
+    w.wide = reinterpret_cast<float*>(take(sizeof(float) * std::max(kWideBlocks, nkv) * (hd == 128 ? kMostCols : kLeastCols) * (hd + 2)));
     if (bytes) *bytes = at - reinterpret_cast<char*>(base);
     return w;
 }
@@ -1069,36 +1070,72 @@ size_t paged_attn_workspace_bytes(int nq, int nkv, int head_dim) {
     return n;
 }
 
+// Steps of few rows per sequence.
+template <int HD, bool I8>
+__global__ void __launch_bounds__(kWave* kBlockWaves<HD>, kBlockWaves<HD> / 4) paged_narrow_kernel(PagedAttnLaunch p, PagedWs ws) {
+    extern __shared__ uint4 paged_lds[];
+    narrow_block<HD, I8, kBlockWaves<HD>>(p, ws, blockIdx.x, paged_lds);
+}
+// Steps with longer ones.  Among the first blocks every fifth eight (one block on each XCD) are narrow ones, as many as there is
+// work for: those wait for memory, the others for the matrix cores.  (Every fourth eight would all go to the same quarter
+// of an XCD.)
+template <int HD, bool I8, int CT>
+__global__ void __launch_bounds__(kWave* kBlockWaves<HD>, kBlockWaves<HD> / 4) paged_mixed_kernel(PagedAttnLaunch p, PagedWs ws) {
+    extern __shared__ uint4 paged_lds[];
+    const int b = blockIdx.x, all = ws.head[2];
+    const int n = b / 40 * 8 + max(0, b % 40 - 32);  // narrow ones before this, if they do not end
+    if (b % 40 >= 32 && n < all)
+        narrow_block<HD, I8, kBlockWaves<HD>>(p, ws, n, paged_lds);
+    else
+        wide_block<HD, I8, CT>(p, ws, b - min(n, all), paged_lds);
+}
+
 template <typename Kernel>
 static hipError_t allow_lds(Kernel kernel, size_t bytes) {
     return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
 }
 
+template <int HD, bool I8, int CT>
+static hipError_t launch_mixed(const PagedAttnLaunch& p, PagedWs ws, hipStream_t s) {
+    using S = WideShape<HD, CT>;
+    const int nkv = p.kv.nkv, T = S::kCols / (p.nq / nkv);
+    ws.cols = S::kCols;
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, ws, S::kKeys);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    // row tiles of any division of the rows among the sequences, and the splits on top of them
+    const int tiles = p.step.rows / T + std::min(p.step.seqs, p.step.rows);
+    const unsigned wide = static_cast<unsigned>(tiles + kWideBlocks / nkv) * nkv;
+    if (hipError_t e = allow_lds(&paged_mixed_kernel<HD, I8, CT>, S::kLds); e != hipSuccess) return e;
+    hipLaunchKernelGGL((paged_mixed_kernel<HD, I8, CT>), dim3(std::max(wide, 4u * kNarrowBlocks) + kNarrowBlocks), dim3(S::kThreads), S::kLds, s, p, ws);
+    return hipGetLastError();
+}
+
 template <int HD, bool I8>
 static hipError_t launch_paged_heads(const PagedAttnLaunch& p, hipStream_t s) {
-    constexpr int KS = HD == 128 ? 8 : 4;
-    using F = PagedBlock<HD, KS, kNarrowCols>;
-    using S = WideShape<HD>;
+    using F = PagedBlock<HD, kBlockWaves<HD>, kNarrowCols>;
     constexpr size_t kLds = std::max(F::kOutBytes, QueryStage<F, HD>::kBytes);
-    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kWideCols / group;
-    const bool wide = p.step.max_rows * static_cast<int64_t>(group) > kNarrowCols;
-    const PagedWs ws = paged_ws(p.ws, HD, nkv, nullptr);
+    const int nkv = p.kv.nkv, group = p.nq / nkv;
+    const bool mixed = p.step.max_rows * static_cast<int64_t>(group) > kNarrowCols;
+    PagedWs ws = paged_ws(p.ws, HD, nkv, nullptr);
     const size_t row_lds = paged_row_lds(group, HD);
-    if (hipError_t e = allow_lds(&paged_narrow_kernel<HD, I8, KS>, kLds); e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_narrow_kernel<HD, I8, KS>), dim3(kNarrowBlocks + wide), dim3(F::kThreads), kLds, s, p, ws);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     int wide_blocks = 0;
-    if (wide) {
-        // row tiles of any division of the rows among the sequences, and the splits on top of them
-        const int tiles = p.step.rows / T + std::min(p.step.seqs, p.step.rows);
+    if (mixed) {
         wide_blocks = std::max(1, kWideBlocks / nkv) * nkv;
-        if (hipError_t e = allow_lds(&paged_wide_kernel<HD, I8>, S::kLds); e != hipSuccess) return e;
-        hipLaunchKernelGGL((paged_wide_kernel<HD, I8>), dim3(static_cast<unsigned>(tiles + kWideBlocks / nkv) * nkv), dim3(S::kThreads), S::kLds, s, p, ws);
+        const bool many = getenv("XQ_CT4") != nullptr;
+        ws.cols = HD == 128 && many ? 128 : 64;
+        hipError_t e;
+        if constexpr (HD == 128)
+            e = many ? launch_mixed<HD, I8, 4>(p, ws, s) : launch_mixed<HD, I8, 2>(p, ws, s);
+        else
+            e = launch_mixed<HD, I8, 2>(p, ws, s);
+        if (e != hipSuccess) return e;
+    } else {
+        if (hipError_t e = allow_lds(&paged_narrow_kernel<HD, I8>, kLds); e != hipSuccess) return e;
+        hipLaunchKernelGGL((paged_narrow_kernel<HD, I8>), dim3(kNarrowBlocks), dim3(F::kThreads), kLds, s, p, ws);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
-    const size_t merge_lds = row_lds;
-    if (hipError_t e = allow_lds(&paged_merge_kernel<HD>, merge_lds); e != hipSuccess) return e;
-    hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3(p.step.seqs * nkv + wide_blocks), dim3(kMergeThreads), merge_lds, s, p, ws, p.step.seqs * nkv, wide_blocks);
+    if (hipError_t e = allow_lds(&paged_merge_kernel<HD>, row_lds); e != hipSuccess) return e;
+    hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3(p.step.seqs * nkv + wide_blocks), dim3(kMergeThreads), row_lds, s, p, ws, p.step.seqs * nkv, wide_blocks);
     return hipGetLastError();
 }
 
