@@ -255,7 +255,7 @@ struct WideUnit {
 };
 // Workspace: where the merge finds the narrow sequences' parts, the wide kernel's units, partial outputs.
 struct PagedWs {
-    int* head;        // [0] wide units, [1] their slots, [2] blocks of the narrow work
+    int* head;        // [0] wide units, [1] their slots, [2] blocks of the narrow work, [3] columns of a wide block
     int4* narrow_at;  // [seqs][nkv]: blocks that share the sequence's tiles, the first of them and its slot, whether a single
                       // block's output has to be computed again
     int4* wide_at;    // [wide units][nkv], of those without splits: as above
@@ -263,7 +263,6 @@ struct PagedWs {
     WideUnit* units;
     float* narrow;    // [2 blocks][16][hd + 2]
     float* wide;      // [slots][nkv][columns][hd + 2]
-    int cols;         // of a wide block
 };
 constexpr size_t kWsHead = 16;
 
@@ -432,44 +431,66 @@ struct WideShape {
     static_assert(QueryStage<Q, HD>::kBytes <= kLds && kLds + 64 <= 160 * 1024, "LDS");
 };
 
-// The units of the sequences that the narrow kernel does not take, by one block: a row tile's keys are split in proportion
-// to their number where there are fewer tiles than blocks that fill the card.
+// The units of the sequences that the narrow kernel does not take, by one block (5 us, a launch's and a dozen barriers'
+// latencies).
+//
+// Columns of a block: with 128 each key and value is staged for four column tiles instead of two, but there are half as many
+// row tiles.  128 where those still give every block of a round its own (three chunks of 512 rows after 2300 beside 21 tokens
+// 148 us, with 64 columns 171; 2000 rows after 2000 220, 243), or where a round's blocks have over kLong chunks each, so that
+// splits cost little beside them (512 rows after 16000 292, 312; 64 after 131000 289, 317); elsewhere 64 (500 rows after
+// 3584 85, 91; 64 after 1000 24, 27).
 constexpr int kPlanThreads = 1024;
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunch p, PagedWs ws, int kKeys) {
-    constexpr int THREADS = kPlanThreads, kWaves = THREADS / kWave, kPer = 1024 / THREADS;
-    __shared__ int pre[1024], red[kWaves];
-    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
-    const int nkv = p.kv.nkv, group = p.nq / nkv, T = ws.cols / group, seqs = p.step.seqs;
-    auto block_scan = [&](int v, int& all) {  // before this thread; all: of every thread
-        const int in = wave_scan_int(v);
-        __syncthreads();
-        if (lane == kWave - 1) red[wid] = in;
-        __syncthreads();
-        int before = in - v;
-        all = 0;
-        for (int i = 0; i < kWaves; ++i) {
-            before += i < wid ? red[i] : 0;
-            all += red[i];
+constexpr int kLong = 60;
+static_assert(kPlanThreads >= 1024, "a thread per sequence");
+template <int HD>
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunch p, PagedWs ws) {
+    constexpr int kWaves = kPlanThreads / kWave;
+    __shared__ int pre[kPlanThreads], rows[kPlanThreads], past[kPlanThreads], red[3][kWaves], length;
+    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, s = threadIdx.x;
+    const int nkv = p.kv.nkv, group = p.nq / nkv, seqs = p.step.seqs, cap = table_positions(p.step, p.kv);
+    const int room = max(1, kWideBlocks / nkv);  // units of a round of blocks
+    int mine = 0, keys = 0;                      // rows of this thread's sequence, positions
+    if (s < seqs) {
+        const SeqRows r = seq_rows(p.step, s);
+        if (r.rows > 0 && !is_narrow(r.rows, group)) mine = r.rows;
+        rows[s] = mine;
+        past[s] = r.past;
+        keys = r.past < 0 ? 0 : min(cap, r.past);
+    }
+    auto wave_total = [&](int v) { return __builtin_amdgcn_readlane(wave_scan_int(v), kWave - 1); };
+    auto tiles_of_rows = [&](int n, int cols) { return n ? (n + cols / group - 1) / (cols / group) : 0; };
+    int cols = kLeastCols;
+    const int n64 = tiles_of_rows(mine, kLeastCols), n128 = tiles_of_rows(mine, kMostCols);
+    {
+        // (chunks of 128 keys, in the order of their number)
+        const int chunks = n64 ? min(n64 * ((keys + mine / 2) / 128 + 1), 1 << 20) : 0;
+        const int a = wave_total(n64), b = wave_total(n128), c = wave_total(chunks);
+        if (lane == 0) {
+            red[0][wid] = a;
+            red[1][wid] = b;
+            red[2][wid] = c;
         }
-        return before;
-    };
-    int base = 0;
-    for (int i = 0; i < kPer; ++i) {
-        const int s = i * THREADS + threadIdx.x;
-        int n = 0;
-        if (s < seqs) {
-            const SeqRows r = seq_rows(p.step, s);
-            if (r.rows > 0 && !is_narrow(r.rows, group)) n = (r.rows + T - 1) / T;
-        }
-        int all;
-        const int before = block_scan(n, all);
-        if (s < seqs) pre[s] = base + before;
-        base += all;
     }
     __syncthreads();
-    const int tiles = base;
-    auto tile_at = [&](int f, int& s, int& tile) {  // chunks of row tile f
-        int lo = 0, hi = seqs - 1;  // the last sequence with pre <= f
+    int tiles = 0, tiles128 = 0, before = 0, before128 = 0;
+    int64_t chunks = 0;
+    for (int i = 0; i < kWaves; ++i) {
+        before += i < wid ? red[0][i] : 0;
+        before128 += i < wid ? red[1][i] : 0;
+        tiles += red[0][i];
+        tiles128 += red[1][i];
+        chunks += red[2][i];
+    }
+    if (HD == 128 && (tiles128 >= room || chunks * nkv > static_cast<int64_t>(kLong) * kWideBlocks)) {
+        cols = kMostCols;
+        tiles = tiles128;
+        before = before128;
+    }
+    const int own = cols == kMostCols ? n128 : n64, T = cols / group, chunk = kBlockWaves<HD> * kTTile * kTTile / cols;
+    pre[s] = before + wave_scan_int(own) - own;
+    __syncthreads();
+    auto tile_at = [&](int f, int& q, int& tile) {  // chunks of row tile f
+        int lo = 0, hi = seqs - 1;                  // the last sequence with pre <= f
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
             if (pre[mid] <= f)
@@ -477,33 +498,64 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
             else
                 hi = mid - 1;
         }
-        s = lo;
+        q = lo;
         tile = f - pre[lo];
-        const SeqKeys k(p, lo);
-        return max(0, k.last(min((tile + 1) * T, k.r.rows) - 1)) / kKeys + 1;
+        const int seen = past[lo] < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(past[lo]) + min((tile + 1) * T, rows[lo]), static_cast<int64_t>(cap)));
+        return max(0, seen - 1) / chunk + 1;
     };
-    int64_t chunks = 0;
-    for (int f0 = 0; f0 < tiles; f0 += THREADS) {
-        const int f = f0 + threadIdx.x;
-        int s, tile, all;
-        block_scan(f < tiles ? tile_at(f, s, tile) : 0, all);
-        chunks += all;
-    }
-    const int room = kWideBlocks / nkv;
-    int units = 0;  // unit count, slots << 16
-    for (int f0 = 0; f0 < tiles; f0 += THREADS) {
-        const int f = tiles - 1 - (f0 + static_cast<int>(threadIdx.x));  // later rows, which see more, first
-        int s = 0, tile = 0, n = 0, c = 0;
-        if (f >= 0) {
-            c = tile_at(f, s, tile);
-            n = static_cast<int>(min(static_cast<int64_t>(c), max(int64_t(1), static_cast<int64_t>(c) * room / chunks)));
+    // Splits: the shortest length with which all units fit one round of blocks; none where the tiles alone are more.  (Two
+    // rounds of splits instead of one and a half of tiles: the three chunks above 161 us, not 148.)
+    constexpr int kHeld = kWideBlocks / kWave;
+    if (wid == 0) {
+        int per = 1 << 20;  // (no tile has so many chunks)
+        if (tiles <= room) {
+            int c[kHeld], most = 0, sum = 0;
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                const int f = i * kWave + lane;
+                int q, tile;
+                c[i] = f < tiles ? tile_at(f, q, tile) : 0;
+                most = max(most, c[i]);
+                sum += c[i];
+            }
+            most = static_cast<int>(wave_max_u64(most));
+            int low = max(1, (wave_total(sum) + room - 1) / room), high = max(most, low);
+            while (low < high) {
+                const int mid = (low + high) / 2;
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) n += (c[i] + mid - 1) / mid;
+                if (wave_total(n) <= room)
+                    high = mid;
+                else
+                    low = mid + 1;
+            }
+            per = low;
         }
-        int all;
-        const int at = units + block_scan(n + (n > 1 ? n << 16 : 0), all);
-        units += all;
+        if (lane == 0) length = per;
+    }
+    __syncthreads();
+    const int per = length;
+    int units = 0;  // unit count, slots << 16
+    for (int f0 = 0; f0 < tiles; f0 += kPlanThreads) {
+        const int f = tiles - 1 - (f0 + static_cast<int>(threadIdx.x));  // later rows, which see more, first
+        int q = 0, tile = 0, n = 0, c = 0;
+        if (f >= 0) {
+            c = tile_at(f, q, tile);
+            n = (c + per - 1) / per;
+        }
+        const int v = n + (n > 1 ? n << 16 : 0), in = wave_scan_int(v);
+        __syncthreads();
+        if (lane == kWave - 1) red[0][wid] = in;
+        __syncthreads();
+        int at = units + in - v;
+        for (int i = 0; i < kWaves; ++i) {
+            at += i < wid ? red[0][i] : 0;
+            units += red[0][i];
+        }
         for (int i = 0; i < n; ++i) {
             const int u = (at & 0xffff) + i, slot = (at >> 16) + i;
-            ws.units[u] = WideUnit{s, tile, static_cast<int>(static_cast<int64_t>(c) * i / n), static_cast<int>(static_cast<int64_t>(c) * (i + 1) / n), n, slot};
+            ws.units[u] = WideUnit{q, tile, static_cast<int>(static_cast<int64_t>(c) * i / n), static_cast<int>(static_cast<int64_t>(c) * (i + 1) / n), n, slot};
             if (n > 1) ws.first[slot] = at & 0xffff;
         }
     }
@@ -513,6 +565,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
             ws.head[0] = units & 0xffff;
             ws.head[1] = units >> 16;
             ws.head[2] = w.blocks;
+            ws.head[3] = cols;
         }
     }
 }
@@ -969,7 +1022,7 @@ __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int bloc
     __shared__ float fac[kMostCols + kWideBlocks], total[kMostCols];  // a block's columns times the splits
     __shared__ int list[kMergeThreads], count, redo;
     constexpr int kQuads = HD / 4;
-    const int cols = ws.cols, slot_size = cols * (HD + 2), nkv = p.kv.nkv, group = p.nq / nkv, T = cols / group;
+    const int cols = ws.head[3], slot_size = cols * (HD + 2), nkv = p.kv.nkv, group = p.nq / nkv, T = cols / group;
     const int units = ws.head[0], slots = ws.head[1], slot = block / nkv, kh = block % nkv;
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
     if (slot < slots) {
@@ -1057,7 +1110,7 @@ static PagedWs paged_ws(float* base, int hd, int nkv, size_t* bytes) {
     w.first = reinterpret_cast<int*>(take(sizeof(int) * kWideBlocks));
     w.units = reinterpret_cast<WideUnit*>(take(sizeof(WideUnit) * kMostUnits));
     w.narrow = reinterpret_cast<float*>(take(sizeof(float) * 2 * kNarrowBlocks * kNarrowCols * (hd + 2)));
-    w.wide = reinterpret_cast<float*>(take(sizeof(float) * std::max(kWideBlocks, nkv) * (hd == 128 ? kMostCols : kLeastCols) * (hd + 2)));
+    w.wide = reinterpret_cast<float*>(take(sizeof(float) * kWideBlocks * (hd == 128 ? kMostCols : kLeastCols) * (hd + 2)));
     if (bytes) *bytes = at - reinterpret_cast<char*>(base);
     return w;
 }
@@ -1079,15 +1132,18 @@ __global__ void __launch_bounds__(kWave* kBlockWaves<HD>, kBlockWaves<HD> / 4) p
 // Steps with longer ones.  Among the first blocks every fifth eight (one block on each XCD) are narrow ones, as many as there is
 // work for: those wait for memory, the others for the matrix cores.  (Every fourth eight would all go to the same quarter
 // of an XCD.)
-template <int HD, bool I8, int CT>
+template <int HD, bool I8>
 __global__ void __launch_bounds__(kWave* kBlockWaves<HD>, kBlockWaves<HD> / 4) paged_mixed_kernel(PagedAttnLaunch p, PagedWs ws) {
     extern __shared__ uint4 paged_lds[];
     const int b = blockIdx.x, all = ws.head[2];
     const int n = b / 40 * 8 + max(0, b % 40 - 32);  // narrow ones before this, if they do not end
-    if (b % 40 >= 32 && n < all)
+    if (b % 40 >= 32 && n < all) {
         narrow_block<HD, I8, kBlockWaves<HD>>(p, ws, n, paged_lds);
-    else
-        wide_block<HD, I8, CT>(p, ws, b - min(n, all), paged_lds);
+    } else if (HD == 128 && ws.head[3] == kMostCols) {
+        if constexpr (HD == 128) wide_block<HD, I8, kMostCols / kTTile>(p, ws, b - min(n, all), paged_lds);
+    } else {
+        wide_block<HD, I8, kLeastCols / kTTile>(p, ws, b - min(n, all), paged_lds);
+    }
 }
 
 template <typename Kernel>
@@ -1095,45 +1151,34 @@ static hipError_t allow_lds(Kernel kernel, size_t bytes) {
     return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
 }
 
-template <int HD, bool I8, int CT>
-static hipError_t launch_mixed(const PagedAttnLaunch& p, PagedWs ws, hipStream_t s) {
-    using S = WideShape<HD, CT>;
-    const int nkv = p.kv.nkv, T = S::kCols / (p.nq / nkv);
-    ws.cols = S::kCols;
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, ws, S::kKeys);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    // row tiles of any division of the rows among the sequences, and the splits on top of them
-    const int tiles = p.step.rows / T + std::min(p.step.seqs, p.step.rows);
-    const unsigned wide = static_cast<unsigned>(tiles + kWideBlocks / nkv) * nkv;
-    if (hipError_t e = allow_lds(&paged_mixed_kernel<HD, I8, CT>, S::kLds); e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_mixed_kernel<HD, I8, CT>), dim3(std::max(wide, 4u * kNarrowBlocks) + kNarrowBlocks), dim3(S::kThreads), S::kLds, s, p, ws);
-    return hipGetLastError();
-}
+template <int HD>
+constexpr size_t kWideLds = std::max(WideShape<HD, kLeastCols / kTTile>::kLds, WideShape<HD, (HD == 128 ? kMostCols : kLeastCols) / kTTile>::kLds);
 
 template <int HD, bool I8>
 static hipError_t launch_paged_heads(const PagedAttnLaunch& p, hipStream_t s) {
     using F = PagedBlock<HD, kBlockWaves<HD>, kNarrowCols>;
     constexpr size_t kLds = std::max(F::kOutBytes, QueryStage<F, HD>::kBytes);
+    constexpr int kThreads = kWave * kBlockWaves<HD>;
     const int nkv = p.kv.nkv, group = p.nq / nkv;
     const bool mixed = p.step.max_rows * static_cast<int64_t>(group) > kNarrowCols;
-    PagedWs ws = paged_ws(p.ws, HD, nkv, nullptr);
+    const PagedWs ws = paged_ws(p.ws, HD, nkv, nullptr);
     const size_t row_lds = paged_row_lds(group, HD);
     int wide_blocks = 0;
     if (mixed) {
+        static_assert(kWideLds<HD> >= kLds, "narrow blocks among them");
+        hipLaunchKernelGGL(paged_plan_kernel<HD>, dim3(1), dim3(kPlanThreads), 0, s, p, ws);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        // row tiles of any division of the rows among the sequences, and the splits on top of them
+        const int tiles = p.step.rows / (kLeastCols / group) + std::min(p.step.seqs, p.step.rows);
+        const unsigned wide = static_cast<unsigned>(tiles + kWideBlocks / nkv) * nkv;
+        if (hipError_t e = allow_lds(&paged_mixed_kernel<HD, I8>, kWideLds<HD>); e != hipSuccess) return e;
+        hipLaunchKernelGGL((paged_mixed_kernel<HD, I8>), dim3(std::max(wide, 4u * kNarrowBlocks) + kNarrowBlocks), dim3(kThreads), kWideLds<HD>, s, p, ws);
         wide_blocks = std::max(1, kWideBlocks / nkv) * nkv;
-        const bool many = getenv("XQ_CT4") != nullptr;
-        ws.cols = HD == 128 && many ? 128 : 64;
-        hipError_t e;
-        if constexpr (HD == 128)
-            e = many ? launch_mixed<HD, I8, 4>(p, ws, s) : launch_mixed<HD, I8, 2>(p, ws, s);
-        else
-            e = launch_mixed<HD, I8, 2>(p, ws, s);
-        if (e != hipSuccess) return e;
     } else {
         if (hipError_t e = allow_lds(&paged_narrow_kernel<HD, I8>, kLds); e != hipSuccess) return e;
-        hipLaunchKernelGGL((paged_narrow_kernel<HD, I8>), dim3(kNarrowBlocks), dim3(F::kThreads), kLds, s, p, ws);
-        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        hipLaunchKernelGGL((paged_narrow_kernel<HD, I8>), dim3(kNarrowBlocks), dim3(kThreads), kLds, s, p, ws);
     }
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (hipError_t e = allow_lds(&paged_merge_kernel<HD>, row_lds); e != hipSuccess) return e;
     hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3(p.step.seqs * nkv + wide_blocks), dim3(kMergeThreads), row_lds, s, p, ws, p.step.seqs * nkv, wide_blocks);
     return hipGetLastError();
