@@ -657,12 +657,14 @@ typedef struct xqhip_step {
  * PAGES_I8: signed 8-bit codes of the fp16 values, with one fp32 scale per page
  * and kv head ([pages][nkv]): scale = max |x| / 127 over the page's positions
  * so far, code = 127 x / max |x| to the nearest (ties to even), value = code *
- * scale.  When a later position raises the maximum the page's codes are taken
- * anew from the fp16 values, which k_open and v_open ([opens][nkv][page]
- * [head_dim]) keep of the page that a sequence's last append ended in; so a
- * page's codes do not depend on the steps that it came in.  A scale never falls
- * while its page is filled.  A sequence may go back (a smaller past[s]) within
- * the page that its last append ended in, or to any page's first position.
+ * scale.  k_open and v_open ([opens][nkv][page][head_dim]) keep the fp16 values
+ * of the page that a sequence's last append ended in: when a later position
+ * raises the maximum, or a step goes on into the next page, the page's codes
+ * are taken anew from them, so they do not depend on the steps that a page came
+ * in.  A scale never falls while its page is filled.  A sequence may go back (a
+ * smaller past[s]) within the page that its last append ended in, or to any
+ * page's first position (so a step that went on into another page is not
+ * repeated from where it began).
  * Infinities and values past fp16's range are held as fp16's largest value,
  * values that are no numbers as 0.
  * One step's appends to one open page must not overlap. */

@@ -189,13 +189,14 @@ def appended(pool_raw, plan, kind, k, v, bad=()):
                 for h in range(vals.shape[1]):
                     was = np.float16(np.float32(new[2 + i][pg, h] * np.float32(127))) if lead else np.float16(0)
                     mx = np.abs(vals[:, h]).max()
-                    if mx > was:
-                        new[2 + i][pg, h] = np.float32(mx.astype(np.float64) / 127)
-                        old = pool_raw[4 + i][plan.open[s], h, :lead].astype(np.float64)
-                        new[i][pg, h, :lead] = np.clip(np.rint(old * 127 / mx.astype(np.float64)), -127, 127)
-                    else:
-                        mx = was
-                        new[2 + i][pg, h] = np.float32(mx.astype(np.float64) / 127)
+                    kept = pool_raw[4 + i][plan.open[s], h, :lead]
+                    leaves = lead and at != last  # the step goes on into another page
+                    if leaves:
+                        mx = max(mx, np.abs(kept).max())
+                    grew, mx = mx > was, max(mx, was)
+                    new[2 + i][pg, h] = np.float32(mx.astype(np.float64) / 127)
+                    if grew or leaves:
+                        new[i][pg, h, :lead] = np.clip(np.rint(kept.astype(np.float64) * 127 / mx.astype(np.float64)), -127, 127)
                     new[i][pg, h, offs] = np.rint(vals[:, h].astype(np.float64) * 127 / float(mx)) if mx > 0 else 0
                 if at == last:
                     new[4 + i][plan.open[s]][:, offs] = vals.transpose(1, 0, 2)

@@ -263,11 +263,12 @@ __device__ __forceinline__ int code_of(_Float16 x, float mx, float inv) {
 }
 
 // One page that the step touches, one kv head, k or v, by a block.  The new rows' fp16 values go to LDS (four rows' loads of a
-// wave at a time), then to the page in 16-byte pieces; 8 bits: their maximum is taken on the way, and where it rose the
-// page's earlier values are fetched and the codes of all of them written.
+// wave at a time), then to the page in 16-byte pieces; 8 bits: their maximum is taken on the way, and where it rose, or the
+// step leaves the page, the page's earlier values are fetched and the codes of all of them written.
 template <int E, bool VEC, bool I8>
 __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int h, bool is_k, _Float16* vals, double* turn) {
     typedef HeadLanes<E, VEC> L;
+    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
     constexpr int kBatch = E == 2 ? 4 : 2;
     __shared__ float wave_mx[kPagedWaves];
     __shared__ uint8_t ok[kPagedMaxPage];
@@ -342,7 +343,20 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     }
     int from = lead;
     float inv = 0.0f;
+    auto earlier = [&] {  // the page's values before the step, in fp16
+        for (int i = threadIdx.x; i < lead * (hd / 8); i += kPagedThreads) {
+            const int t = i / (hd / 8), b = i - t * (hd / 8);
+            const half8 y = *reinterpret_cast<const half8*>(kept + static_cast<size_t>(t) * hd + 8 * b);
+            *reinterpret_cast<half8*>(vals + t * ld + 8 * b) = y;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(static_cast<float>(y[e])));
+        }
+    };
     if constexpr (I8) {
+        if (lead && !last) {  // the step leaves the page: it is written as it will stay
+            earlier();
+            from = 0;
+        }
         mx = wave_max(mx);
         if (lane == 0) wave_mx[wid] = mx;
     }
@@ -354,12 +368,11 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
         const bool grew = mx > before;
         mx = grew ? mx : before;
         inv = mx > 0.0f ? 1.0f / mx : 0.0f;
-        if (grew && lead) {
+        if (grew && lead && last) {
+            const float all = mx;
+            earlier();
+            mx = all;
             from = 0;
-            for (int i = threadIdx.x; i < lead * (hd / 8); i += kPagedThreads) {
-                const int t = i / (hd / 8), b = i - t * (hd / 8);
-                *reinterpret_cast<u32x4*>(vals + t * ld + 8 * b) = *reinterpret_cast<const u32x4*>(kept + static_cast<size_t>(t) * hd + 8 * b);
-            }
             __syncthreads();
         }
         if (threadIdx.x == 0) (is_k ? p.kv.k_scale : p.kv.v_scale)[sat] = mx / 127.0f;
@@ -373,7 +386,6 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     }
     auto writes = [&](int t) { return (t < kWave ? go[0] >> t : go[1] >> (t - kWave)) & 1; };
     constexpr int N = I8 ? 16 : 8;  // values of a piece
-    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
     typedef typename std::conditional<I8, int8_t, _Float16>::type T;
     union Piece {
         T v[N];
