@@ -143,9 +143,13 @@ __global__ void __launch_bounds__(256) paged_attn_row_kernel(PagedAttnLaunch p) 
 // its rows again by attend_paged_row.
 // ---------------------------------------------------------------------------
 template <int HD>
-constexpr int kBlockWaves = HD == 128 ? 8 : 4;  // registers for two waves, or one, per SIMD
-constexpr int kNarrowCols = 16;     // up to 16 columns: paged_narrow_kernel
-constexpr int kNarrowBlocks = 256;  // blocks that share the narrow sequences' tiles
+constexpr int kBlockWaves = HD == 128 ? 8 : 4;  // of a wide block: registers for two waves, or one, per SIMD
+template <int HD, bool I8, int NT>
+constexpr int kNarrowPerSimd = HD == 128 || (I8 && NT == 1) ? 2 : 1;  // narrow waves that a SIMD has registers for
+template <int HD, bool I8, int NT>
+constexpr int kNarrowWaves = 4 * kNarrowPerSimd<HD, I8, NT>;  // of a narrow block
+constexpr int kNarrowCols = 16;      // sequences of up to 8 or 16 columns: narrow_block
+constexpr int kNarrowBlocks = 512;  // blocks that share their tiles, at most
 constexpr int kLeastCols = 64, kMostCols = 128;  // columns of other sequences' blocks: wide_block
 constexpr int kWideBlocks = 256;    // blocks that few row tiles' keys are split over
 constexpr int kMostUnits = 65535 * kPagedMaxGroup / kLeastCols + 1024 + kWideBlocks;  // row tiles and splits of a step
@@ -169,7 +173,8 @@ struct SeqKeys {
     }
 };
 
-__device__ __forceinline__ bool is_narrow(int rows, int group) { return rows > 0 && rows * group <= kNarrowCols; }
+// (cols: 8 or 16, the narrow blocks' of the call)
+__device__ __forceinline__ bool is_narrow(int rows, int group, int cols) { return rows > 0 && rows * group <= cols; }
 __device__ __forceinline__ int tiles_of(int last) { return max(0, last) / kTTile + 1; }
 
 // The narrow kernel's work: sequences of up to 16 columns, their 32-key tiles in units of q, for each kv head, one behind
@@ -183,7 +188,7 @@ struct NarrowItem {
 };
 struct NarrowWork {
     int q, blocks, units, per, rem;  // units: all sequences, one kv head; a block has per, the first rem one more
-    int group, nkv;
+    int group, nkv, cols;
     int before;           // lane c: units of the sequences up to 64 c + 63
     int held, in, tiles;  // sequences 64 held + lane: units up to it, its tiles
 
@@ -191,9 +196,9 @@ struct NarrowWork {
         const int s = c * kWave + static_cast<int>(threadIdx.x & (kWave - 1));
         if (s >= p.step.seqs) return 0;
         const SeqKeys k(p, s);
-        return is_narrow(k.r.rows, group) ? tiles_of(k.last(k.r.rows - 1)) : 0;
+        return is_narrow(k.r.rows, group, cols) ? tiles_of(k.last(k.r.rows - 1)) : 0;
     }
-    __device__ __forceinline__ explicit NarrowWork(const PagedAttnLaunch& p) : group(p.nq / p.kv.nkv), nkv(p.kv.nkv) {
+    __device__ __forceinline__ NarrowWork(const PagedAttnLaunch& p, int cols_, int most) : group(p.nq / p.kv.nkv), nkv(p.kv.nkv), cols(cols_) {
         const int lane = threadIdx.x & (kWave - 1), chunks = (p.step.seqs + kWave - 1) / kWave;
         int active = 0, sum = 0;
         for (int c = 0; c < chunks; ++c) {
@@ -203,7 +208,7 @@ struct NarrowWork {
         }
         const int64_t all = static_cast<int64_t>(__builtin_amdgcn_readlane(wave_scan_int(sum), kWave - 1)) * nkv;
         // the smallest unit with which every unit has a block of its own
-        const int room = kNarrowBlocks - min(active * nkv, kNarrowBlocks);
+        const int room = most - min(active * nkv, most);
         if (room > 0 && all <= kMaxTiles * room)
             q = max((static_cast<int>(all) + room - 1) / room, kMinTiles);
         else
@@ -218,7 +223,7 @@ struct NarrowWork {
         held = chunks - 1;
         units = __builtin_amdgcn_readlane(before, kWave - 1);
         const int total = units * nkv;
-        blocks = min(kNarrowBlocks, total);
+        blocks = min(most, total);
         per = total / max(blocks, 1);
         rem = total - per * blocks;
     }
@@ -261,8 +266,9 @@ struct PagedWs {
     int4* wide_at;    // [wide units][nkv], of those without splits: as above
     int* first;       // [slots]: first unit of the slot's row tile
     WideUnit* units;
-    float* narrow;    // [2 blocks][16][hd + 2]
+    float* narrow;    // [2 blocks][columns][hd + 2]
     float* wide;      // [slots][nkv][columns][hd + 2]
+    int narrow_cols, narrow_blocks;  // of the call
 };
 constexpr size_t kWsHead = 16;
 
@@ -290,38 +296,17 @@ __device__ __forceinline__ bool write_paged_quad(float4 r, float L, const float*
 }
 
 // The key waves of a block's columns joined, then written: a partial output (to part_out: [COLS][HD], then [COLS][2]), or
-// the output, and to *entry whether it has to be computed again.  CT column tiles x KS key waves; HALF: hi and lo columns
-// of one tile.
-template <int HD, int CT, int KS, int COLS, bool HALF, int N>
-__device__ __forceinline__ void finish_paged(const PagedAttnLaunch& p, const SeqRows& sr, int kh, int t0, int ntok, int T, uint32_t inv_t,
-                                             float* part_out, int4* entry, bool live, const floatx16 (&o)[N], float m, float l, void* lds, int* redo) {
-    static_assert(HD == 32 * N, "dim tiles");
+// the output, and to *entry whether it has to be computed again.  The waves' outputs, maxima and sums lie in LDS; the block
+// has passed no barrier since.
+template <int HD, int KS, int COLS, int THREADS>
+__device__ __forceinline__ void join_paged(const PagedAttnLaunch& p, const SeqRows& sr, int kh, int t0, int ntok, int T, uint32_t inv_t,
+                                           float* part_out, int4* entry, void* lds, int* redo) {
     using F = PagedBlock<HD, KS, COLS>;
-    constexpr int kThreads = kWave * CT * KS;
-    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, cl = lane & 31, g = lane >> 5;
     const int group = p.nq / p.kv.nkv;
-    float* Ol = static_cast<float*>(lds);          // [KS][columns][kLdo]
-    float* Ml = Ol + KS * F::kCols * F::kLdo;      // [KS][columns][2]
-    float* Fl = Ml + KS * F::kCols * 2;            // [KS][columns]
-    float* Ll = Fl + KS * F::kCols;                // [columns] the sums
-    l = xor_pair_sum<32>(l);
-    if constexpr (HALF) l = xor_pair_sum<16>(l);
-    const int cw = HALF ? cl & 15 : cl, half = HALF ? cl >> 4 : 0;
-    const int ct = wid % CT, ks = wid / CT;
-    __syncthreads();  // every wave is done with what lay here
-    // (HALF: the hi and lo columns' sums; every lane takes part in them)
-    const int at = ks * F::kCols + ct * 32 + cw;
-    float* oc = Ol + at * F::kLdo + 4 * g + 16 * half;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-#pragma unroll
-        for (int a = 0; a < (HALF ? 2 : 4); ++a) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = HALF ? rows_sum(o[j][4 * a + e], o[j][(8 + 4 * a + e) % 16]) : o[j][4 * a + e];
-            if (live) *reinterpret_cast<float4*>(oc + 32 * j + 8 * a) = make_float4(v[0], v[1], v[2], v[3]);
-        }
-    if (live && g == 0 && half == 0) *reinterpret_cast<float2*>(Ml + at * 2) = make_float2(m, l);
+    const float* Ol = static_cast<float*>(lds);         // [KS][columns][kLdo]
+    const float* Ml = Ol + KS * F::kCols * F::kLdo;     // [KS][columns][2]
+    float* Fl = const_cast<float*>(Ml) + KS * F::kCols * 2;  // [KS][columns]
+    float* Ll = Fl + KS * F::kCols;                     // [columns] the sums
     if (threadIdx.x == 0) *redo = 0;
     __syncthreads();
     auto row_of = [&](int c, int& hc, int& tc) {
@@ -346,7 +331,7 @@ __device__ __forceinline__ void finish_paged(const PagedAttnLaunch& p, const Seq
     }
     __syncthreads();
     bool bad = false;
-    for (int i = threadIdx.x; i < F::kCols * F::kQuads; i += kThreads) {
+    for (int i = threadIdx.x; i < F::kCols * F::kQuads; i += THREADS) {
         const int c = i / F::kQuads, d = 4 * (i % F::kQuads);
         int hc, tc;
         if (!row_of(c, hc, tc)) continue;
@@ -452,7 +437,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
     int mine = 0, keys = 0;                      // rows of this thread's sequence, positions
     if (s < seqs) {
         const SeqRows r = seq_rows(p.step, s);
-        if (r.rows > 0 && !is_narrow(r.rows, group)) mine = r.rows;
+        if (r.rows > 0 && !is_narrow(r.rows, group, ws.narrow_cols)) mine = r.rows;
         rows[s] = mine;
         past[s] = r.past;
         keys = r.past < 0 ? 0 : min(cap, r.past);
@@ -560,7 +545,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
         }
     }
     if (wid == 0) {
-        const NarrowWork w(p);
+        const NarrowWork w(p, ws.narrow_cols, ws.narrow_blocks);
         if (lane == 0) {
             ws.head[0] = units & 0xffff;
             ws.head[1] = units >> 16;
@@ -570,41 +555,44 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
     }
 }
 
-// Up to 16 columns, q's hi parts in the tile's first 16 columns and its lo parts in the others: one MFMA does what two
-// do, a lane and its neighbour 16 lanes on add their scores and take eight keys each, and the weights' hi and lo parts go
-// back into the two halves.  Each wave takes its own 32-key tiles, K and V straight into registers, the next tile's on
-// their way meanwhile; no barrier before the waves join.
-template <int HD, bool I8, int KS>
+// Up to 8 columns, or 16 (NT tiles of 8), in MFMA tiles of 16 columns: q's hi parts in a tile's first eight, its lo parts in
+// the others.  One MFMA then does what two do.  A wave takes 32 keys at a time as two tiles of 16 rows; a lane and its
+// neighbour eight lanes on add their scores and take four keys each, and the weights' hi and lo parts go back into the two
+// halves.  MFMA row i of tile h stands for key 8 (i / 4) + 4 h + i % 4, so that a lane's part of the weights, four keys of
+// each tile, is the eight positions of a piece of V.  K and V go straight into registers, the next keys' on their way
+// meanwhile; no barrier before the waves join.
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ float other_half(float v) { return dpp_f32<0x128>(v); }  // of lane l ^ 8
+
+template <int HD, bool I8, int KS, int NT>
 __device__ __forceinline__ void narrow_block(const PagedAttnLaunch& p, const PagedWs& ws, int block, uint4* paged_lds) {
-    using F = PagedBlock<HD, KS, kNarrowCols>;
+    constexpr int kCols = 8 * NT;
+    using F = PagedBlock<HD, KS, kCols>;
     using Q = QueryStage<F, HD>;
-    constexpr int kSteps = HD / 16, kDimTiles = HD / 32;
-    constexpr int kKPieces = HD / (I8 ? 32 : 16), kVPieces = I8 ? kDimTiles : 2 * kDimTiles;
+    constexpr int kSteps = HD / 32, kDimTiles = HD / 16, kKPieces = HD / (I8 ? 64 : 32);
+    typedef typename std::conditional<I8, u32x2, u32x4>::type VPiece;  // eight positions of a dim
     __shared__ int redo;
-    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kNarrowCols / group;
+    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kCols / group;
     const int lane = threadIdx.x & (kWave - 1), ks = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int cl = lane & 31, g = lane >> 5, col = cl & 15, part = cl >> 4;
+    const int i16 = lane & 15, j = lane >> 4, part = i16 >> 3;
     const uint32_t inv_t = (65535u + T) / T;
-    const int ch = static_cast<int>(col * inv_t >> 16), ctok = col - ch * T;
-    NarrowWork w(p);
+    NarrowWork w(p, kCols, ws.narrow_blocks);
     if (block >= w.blocks) return;
     const int begin = w.begin(block), end = w.begin(block + 1);
-    const uint32_t kat = (static_cast<uint32_t>(g) * p.kv.page + key_of_row<I8>(cl)) * 16u, kstep = 32u * p.kv.page;
-    const uint32_t vat = (static_cast<uint32_t>(g) * HD + cl) * 16u;
-    const int lane_key = I8 ? 16 * g + 8 * part : 16 * part + 8 * g;  // of the lane's eight slots
+    const uint32_t kat = (static_cast<uint32_t>(j) * p.kv.page + 8 * (i16 >> 2) + (i16 & 3)) * 16u, kstep = 64u * p.kv.page;
+    const uint32_t vat = I8 ? (static_cast<uint32_t>(j >> 1) * HD + i16) * 16u + 8u * (j & 1) : (static_cast<uint32_t>(j) * HD + i16) * 16u;
+    const int lane_key = 8 * j + 4 * part;  // of the lane's four slots
     for (int at = begin; at < end;) {
         const NarrowItem it = w.find(p, at);
         const int s = it.s, kh = it.kh, u0 = it.unit, u1 = min(it.units, u0 + (end - at));
         const bool whole = u0 == 0 && u1 == it.units;
         const int slot = at == begin ? 0 : 1;
-        float* part_out = whole ? nullptr : ws.narrow + (2 * static_cast<size_t>(block) + slot) * kNarrowCols * (HD + 2);
+        float* part_out = whole ? nullptr : ws.narrow + (2 * static_cast<size_t>(block) + slot) * kCols * (HD + 2);
         int4* entry = ws.narrow_at + s * nkv + kh;
         if (u0 == 0 && !whole && threadIdx.x == 0) *entry = make_int4(w.block_of(at + it.units - 1) - block + 1, block, slot, 0);
         at += u1 - u0;
         const SeqKeys sk(p, s);
         const int ntok = sk.r.rows, last = sk.last(ntok - 1), sure = sk.last(0);
-        const bool live = ch < group && ctok < ntok;
-        const int qpos = live ? sk.last(ctok) : -1;
         TilePages tp;
         tp.first = u0 * w.q + ks;
         tp.step = KS;
@@ -612,117 +600,161 @@ __device__ __forceinline__ void narrow_block(const PagedAttnLaunch& p, const Pag
         const int n = __builtin_amdgcn_readfirstlane(max(0, (tp.end - tp.first + KS - 1) / KS));
         Q query;
         query.load(p.q + static_cast<size_t>(sk.r.row0) * p.q_stride, p.q_stride, kh, ntok, group, T, inv_t);
-        u32x4 kr[kKPieces], vr[kVPieces];
+        u32x4 kr[2][kKPieces];
+        VPiece vr[kDimTiles];
         TileBase<I8, HD> next = tile_base<I8, HD>(p, tp, s, kh, 0, last);
         auto load_k = [&] {
 #pragma unroll
-            for (int u = 0; u < kKPieces; ++u) kr[u] = __builtin_amdgcn_raw_buffer_load_b128(next.k, kat, u * kstep, 0);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int u = 0; u < kKPieces; ++u) kr[h][u] = __builtin_amdgcn_raw_buffer_load_b128(next.k, kat + 64u * h, u * kstep, 0);
         };
         auto load_v = [&] {
 #pragma unroll
-            for (int h = 0; h < kVPieces / kDimTiles; ++h)
-#pragma unroll
-                for (int j = 0; j < kDimTiles; ++j)
-                    vr[h * kDimTiles + j] = __builtin_amdgcn_raw_buffer_load_b128(next.v, vat + (2u * h * HD + 32u * j) * 16u, 0, 0);
+            for (int d = 0; d < kDimTiles; ++d) {
+                if constexpr (I8)
+                    vr[d] = __builtin_amdgcn_raw_buffer_load_b64(next.v, vat + 256u * d, 0, 0);
+                else
+                    vr[d] = __builtin_amdgcn_raw_buffer_load_b128(next.v, vat + 256u * d, 0, 0);
+            }
         };
         load_k();
         load_v();
         query.store(paged_lds);
         __syncthreads();
-        half8 qf[kSteps];  // the lane's own part, hi or lo
+        half8 qf[NT][kSteps];  // the lane's own part, hi or lo
+        float sscale[NT], m[NT], l[NT];
+        int qpos[NT];
+        floatx4 o[NT][kDimTiles];
 #pragma unroll
-        for (int t = 0; t < kSteps; ++t) qf[t] = Q::part(paged_lds, part, col, I8 ? 32 * (t / 2) + 16 * g + 8 * (t % 2) : 16 * t + 8 * g);
-        const float sscale = Q::scale(paged_lds, col);
-        float m = -1.0e30f, l = 0.0f;  // reference of the exponents, this lane's part of the sum
-        floatx16 o[kDimTiles];
+        for (int t = 0; t < NT; ++t) {
+            const int c = 8 * t + (i16 & 7), hc = static_cast<int>(c * inv_t >> 16), tc = c - hc * T;
 #pragma unroll
-        for (int j = 0; j < kDimTiles; ++j) o[j] = floatx16{};
+            for (int u = 0; u < kSteps; ++u) qf[t][u] = Q::part(paged_lds, part, c, I8 ? 64 * (u / 2) + 16 * j + 8 * (u % 2) : 32 * u + 8 * j);
+            sscale[t] = Q::scale(paged_lds, c);
+            qpos[t] = hc < group && tc < ntok ? sk.last(tc) : -1;
+            m[t] = -1.0e30f;  // reference of the exponents
+            l[t] = 0.0f;      // this lane's part of the sum
+#pragma unroll
+            for (int d = 0; d < kDimTiles; ++d) o[t][d] = floatx4{};
+        }
         for (int i = 0; i < n; ++i) {
             const int key0 = (tp.first + i * KS) * kTTile;
-            const float kscale = I8 ? tile_scale(sscale, readlane_f32(tp.ks, i & 63)) : sscale, vscale = I8 ? readlane_f32(tp.vs, i & 63) : 1.0f;
+            const float pscale = I8 ? readlane_f32(tp.ks, i & 63) : 1.0f, vscale = I8 ? readlane_f32(tp.vs, i & 63) : 1.0f;
             const bool valid = next.valid;
-            floatx16 st = floatx16{};
+            floatx4 st[NT][2];
 #pragma unroll
-            for (int t = 0; t < kSteps; ++t) {
-                half8 a;
-                if constexpr (I8) {
-                    const u32x2 w0 = codes_to_half(kr[t / 2][2 * (t % 2)]), w1 = codes_to_half(kr[t / 2][2 * (t % 2) + 1]);
-                    a = __builtin_bit_cast(half8, u32x4{w0.x, w0.y, w1.x, w1.y});
-                } else {
-                    a = __builtin_bit_cast(half8, kr[t]);
-                }
-                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[t], st, 0, 0, 0);
-            }
-            next = tile_base<I8, HD>(p, tp, s, kh, i + 1, last);
-            load_k();
-            float sc[8];
+            for (int t = 0; t < NT; ++t) st[t][0] = st[t][1] = floatx4{};
 #pragma unroll
-            for (int v = 0; v < 8; ++v) sc[v] = rows_sum(st[v], st[v + 8]);
-            if (key0 + kTTile - 1 > sure || !valid) {  // wave-uniform: keys that some column does not see
-                const int see = valid ? qpos - (key0 + lane_key) : -1;  // slots up to here
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int v = 0; v < 8; ++v) sc[v] = v <= see ? sc[v] : -INFINITY;
-                if constexpr (!I8)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int j = 0; j < kDimTiles; ++j)
-                            vr[h * kDimTiles + j] = first_halves(vr[h * kDimTiles + j], last + 1 - (key0 + 16 * h + 8 * g));
-            }
-            float mc = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
-            mc = pair32_max(xor16_max(mc)) * kscale;
-            if constexpr (I8) mc += scale_exponent(vscale);
-            // the reference moves only when a column's max has outgrown it (rarely after the first tiles)
-            const bool up = mc > m + kSlack;
-            if (__builtin_amdgcn_ballot_w64(up)) {
-                const float to = up ? mc : m, f = __builtin_amdgcn_exp2f(m - to);
-                m = to;
-                l *= f;
-#pragma unroll
-                for (int j = 0; j < kDimTiles; ++j) o[j] *= f;
-            }
-            const float off = kRaise - m;
-            float x[8];
-#pragma unroll
-            for (int v = 0; v < 8; ++v) {
-                x[v] = __builtin_amdgcn_exp2f(fmaf(sc[v], kscale, off));
-                l += x[v];
-                if constexpr (I8) {
-                    x[v] *= vscale;
-                    asm("" : "+v"(x[v]));  // the rounded product: hi and lo would else be taken from two roundings of it
-                }
-            }
-            half8 phi, plo;
-            split8(x, phi, plo);
-            half8 pw[2];  // lanes of the hi columns give their lo for the other 8 keys' hi
-            {
-                const u32x4 hi = __builtin_bit_cast(u32x4, phi), lo = __builtin_bit_cast(u32x4, plo);
-                u32x4 r0, r1;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const auto r = __builtin_amdgcn_permlane16_swap(hi[e], lo[e], false, false);
-                    r0[e] = r[0];
-                    r1[e] = r[1];
-                }
-                pw[0] = __builtin_bit_cast(half8, r0);
-                pw[1] = __builtin_bit_cast(half8, r1);
-            }
-#pragma unroll
-            for (int j = 0; j < kDimTiles; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int u = 0; u < kSteps; ++u) {
                     half8 a;
                     if constexpr (I8) {
-                        const u32x2 w0 = codes_to_half(vr[j][2 * h]), w1 = codes_to_half(vr[j][2 * h + 1]);
+                        const u32x2 w0 = codes_to_half(kr[h][u / 2][2 * (u % 2)]), w1 = codes_to_half(kr[h][u / 2][2 * (u % 2) + 1]);
                         a = __builtin_bit_cast(half8, u32x4{w0.x, w0.y, w1.x, w1.y});
                     } else {
-                        a = __builtin_bit_cast(half8, vr[h * kDimTiles + j]);
+                        a = __builtin_bit_cast(half8, kr[h][u]);
                     }
-                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pw[h], o[j], 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) st[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[t][u], st[t][h], 0, 0, 0);
                 }
+            next = tile_base<I8, HD>(p, tp, s, kh, i + 1, last);
+            load_k();
+            const bool masked = key0 + kTTile - 1 > sure || !valid;  // wave-uniform: keys that some column does not see
+            if (!I8 && masked)
+#pragma unroll
+                for (int d = 0; d < kDimTiles; ++d)
+                    if constexpr (!I8) vr[d] = first_halves(vr[d], last + 1 - (key0 + 8 * j));
+            half8 pw[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float sc[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float mine = part ? st[t][1][e] : st[t][0][e], yours = part ? st[t][0][e] : st[t][1][e];
+                    sc[e] = mine + other_half(yours);
+                }
+                const float kscale = I8 ? tile_scale(sscale[t], pscale) : sscale[t];
+                if (masked) {
+                    const int see = valid ? qpos[t] - (key0 + lane_key) : -1;  // slots up to here
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[e] = e <= see ? sc[e] : -INFINITY;
+                }
+                float mc = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+                mc = fmaxf(mc, other_half(mc));
+                mc = pair32_max(xor16_max(mc)) * kscale;
+                if constexpr (I8) mc += scale_exponent(vscale);
+                // the reference moves only when a column's max has outgrown it (rarely after the first tiles)
+                const bool up = mc > m[t] + kSlack;
+                if (__builtin_amdgcn_ballot_w64(up)) {
+                    const float to = up ? mc : m[t], f = __builtin_amdgcn_exp2f(m[t] - to);
+                    m[t] = to;
+                    l[t] *= f;
+#pragma unroll
+                    for (int d = 0; d < kDimTiles; ++d) o[t][d] *= f;
+                }
+                const float off = kRaise - m[t];
+                typedef float f2 __attribute__((ext_vector_type(2)));
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    float x[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        x[k] = __builtin_amdgcn_exp2f(fmaf(sc[e + k], kscale, off));
+                        l[t] += x[k];
+                        if constexpr (I8) {
+                            x[k] *= vscale;
+                            asm("" : "+v"(x[k]));  // the rounded product: hi and lo would else be taken from two roundings of it
+                        }
+                    }
+                    const h2 a = __builtin_convertvector((f2{x[0], x[1]}), h2);
+                    const h2 b = __builtin_convertvector((f2{x[0] - static_cast<float>(a[0]), x[1] - static_cast<float>(a[1])}), h2);
+                    hi[e / 2] = as_u32(a);
+                    lo[e / 2] = as_u32(b);
+                }
+                // a hi lane takes the other's hi, a lo lane the other's lo
+                u32x4 y;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t own = part ? lo[e] : hi[e], got = static_cast<uint32_t>(dpp_i32<0x128>(static_cast<int>(part ? hi[e] : lo[e])));
+                    y[e] = part ? got : own;
+                    y[2 + e] = part ? own : got;
+                }
+                pw[t] = __builtin_bit_cast(half8, y);
+            }
+#pragma unroll
+            for (int d = 0; d < kDimTiles; ++d) {
+                half8 a;
+                if constexpr (I8) {
+                    const u32x2 w0 = codes_to_half(vr[d].x), w1 = codes_to_half(vr[d].y);
+                    a = __builtin_bit_cast(half8, u32x4{w0.x, w0.y, w1.x, w1.y});
+                } else {
+                    a = __builtin_bit_cast(half8, vr[d]);
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pw[t], o[t][d], 0, 0, 0);
+            }
             load_v();
         }
-        finish_paged<HD, 1, KS, kNarrowCols, true>(p, sk.r, kh, 0, ntok, T, inv_t, part_out, entry, live, o, m, l, paged_lds, &redo);
+        __syncthreads();  // every wave has its q: the outputs take its place
+        float* Ol = reinterpret_cast<float*>(paged_lds);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int col = ks * kCols + 8 * t + (i16 & 7);
+            float sum = l[t] + other_half(l[t]);
+            sum = xor_pair_sum<32>(xor_pair_sum<16>(sum));
+#pragma unroll
+            for (int d = 0; d < kDimTiles; d += 2) {  // the hi and lo columns' sums, a dim tile in each half
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (part ? o[t][d + 1][e] : o[t][d][e]) + other_half(part ? o[t][d][e] : o[t][d + 1][e]);
+                *reinterpret_cast<float4*>(Ol + col * F::kLdo + 16 * (d + part) + 4 * j) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+            if (lane < 8) *reinterpret_cast<float2*>(Ol + KS * kCols * F::kLdo + col * 2) = make_float2(m[t], sum);
+        }
+        join_paged<HD, KS, kCols, F::kThreads>(p, sk.r, kh, 0, ntok, T, inv_t, part_out, entry, paged_lds, &redo);
         __syncthreads();
     }
 }
@@ -734,11 +766,11 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
     __shared__ float fac[kNarrowCols][kNarrowBlocks], total[kNarrowCols];
     __shared__ float4 sums[kMergeThreads];
     __shared__ int redo;
-    constexpr int kQuads = HD / 4, kSlot = kNarrowCols * (HD + 2), kBatch = 4;
-    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kNarrowCols / group;
+    constexpr int kQuads = HD / 4, kBatch = 4;
+    const int nkv = p.kv.nkv, group = p.nq / nkv, all_cols = ws.narrow_cols, T = all_cols / group, kSlot = all_cols * (HD + 2);
     const int4 at = ws.narrow_at[s * nkv + kh];
     const SeqRows sr = seq_rows(p.step, s);
-    if (!is_narrow(sr.rows, group)) return;
+    if (!is_narrow(sr.rows, group, all_cols)) return;
     const int n = at.x;
     if (n == 1) {
         if (__builtin_expect(at.w != 0, 0))
@@ -768,7 +800,7 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
 #pragma unroll
         for (int u = 0; u < kNarrowBlocks / kWave; ++u) {
             const int b = lane + u * kWave;
-            ml[u] = b < n ? *reinterpret_cast<const float2*>(part(b) + kNarrowCols * HD + 2 * c) : make_float2(-INFINITY, 0.0f);
+            ml[u] = b < n ? *reinterpret_cast<const float2*>(part(b) + all_cols * HD + 2 * c) : make_float2(-INFINITY, 0.0f);
             M = fmaxf(M, ml[u].x);
         }
         M = wave_max(M);
@@ -1012,8 +1044,23 @@ __device__ __forceinline__ void wide_block(const PagedAttnLaunch& p, const Paged
     for (; c < end; ++c) chunk(c, std::false_type{}, std::true_type{});
     add_values(end - 1);
     float* part_out = un.splits > 1 ? ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * S::kCols * (HD + 2) : nullptr;
-    finish_paged<HD, CT, KS, S::kCols, false>(p, sk.r, kh, t0, ntok, T, inv_t, part_out, ws.wide_at + unit * nkv + kh, live, o, m, l, paged_lds,
-                                               &redo);
+    l = xor_pair_sum<32>(l);
+    __syncthreads();  // every wave is done with K and V: the outputs take their place
+    {
+        using F = typename S::F;
+        float* Ol = reinterpret_cast<float*>(paged_lds);
+        const int at = ks * F::kCols + ct * kTTile + cl;
+        float* oc = Ol + at * F::kLdo + 4 * g;
+        if (live) {
+#pragma unroll
+            for (int j = 0; j < kDimTiles; ++j)
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+                    *reinterpret_cast<float4*>(oc + 32 * j + 8 * a) = make_float4(o[j][4 * a], o[j][4 * a + 1], o[j][4 * a + 2], o[j][4 * a + 3]);
+            if (g == 0) *reinterpret_cast<float2*>(Ol + KS * F::kCols * F::kLdo + at * 2) = make_float2(m, l);
+        }
+    }
+    join_paged<HD, KS, S::kCols, S::kThreads>(p, sk.r, kh, t0, ntok, T, inv_t, part_out, ws.wide_at + unit * nkv + kh, paged_lds, &redo);
 }
 
 // The splits of a row tile joined, each slot's block a share of the columns; and outputs that have to be computed again.
@@ -1124,10 +1171,10 @@ size_t paged_attn_workspace_bytes(int nq, int nkv, int head_dim) {
 }
 
 // Steps of few rows per sequence.
-template <int HD, bool I8>
-__global__ void __launch_bounds__(kWave* kBlockWaves<HD>, kBlockWaves<HD> / 4) paged_narrow_kernel(PagedAttnLaunch p, PagedWs ws) {
+template <int HD, bool I8, int NT>
+__global__ void __launch_bounds__((kWave * kNarrowWaves<HD, I8, NT>), (kNarrowPerSimd<HD, I8, NT>)) paged_narrow_kernel(PagedAttnLaunch p, PagedWs ws) {
     extern __shared__ uint4 paged_lds[];
-    narrow_block<HD, I8, kBlockWaves<HD>>(p, ws, blockIdx.x, paged_lds);
+    narrow_block<HD, I8, kNarrowWaves<HD, I8, NT>, NT>(p, ws, blockIdx.x, paged_lds);
 }
 // Steps with longer ones.  Among the first blocks every fifth eight (one block on each XCD) are narrow ones, as many as there is
 // work for: those wait for memory, the others for the matrix cores.  (Every fourth eight would all go to the same quarter
@@ -1138,7 +1185,10 @@ __global__ void __launch_bounds__(kWave* kBlockWaves<HD>, kBlockWaves<HD> / 4) p
     const int b = blockIdx.x, all = ws.head[2];
     const int n = b / 40 * 8 + max(0, b % 40 - 32);  // narrow ones before this, if they do not end
     if (b % 40 >= 32 && n < all) {
-        narrow_block<HD, I8, kBlockWaves<HD>>(p, ws, n, paged_lds);
+        if (ws.narrow_cols == 8)
+            narrow_block<HD, I8, kBlockWaves<HD>, 1>(p, ws, n, paged_lds);
+        else
+            narrow_block<HD, I8, kBlockWaves<HD>, 2>(p, ws, n, paged_lds);
     } else if (HD == 128 && ws.head[3] == kMostCols) {
         if constexpr (HD == 128) wide_block<HD, I8, kMostCols / kTTile>(p, ws, b - min(n, all), paged_lds);
     } else {
@@ -1154,31 +1204,41 @@ static hipError_t allow_lds(Kernel kernel, size_t bytes) {
 template <int HD>
 constexpr size_t kWideLds = std::max(WideShape<HD, kLeastCols / kTTile>::kLds, WideShape<HD, (HD == 128 ? kMostCols : kLeastCols) / kTTile>::kLds);
 
+template <int HD, bool I8, int NT>
+static hipError_t launch_narrow(const PagedAttnLaunch& p, PagedWs& ws, hipStream_t s) {
+    using F = PagedBlock<HD, kNarrowWaves<HD, I8, NT>, 8 * NT>;
+    constexpr size_t kLds = std::max(F::kOutBytes, QueryStage<F, HD>::kBytes);
+    ws.narrow_cols = 8 * NT;
+    ws.narrow_blocks = 256 * 4 * kNarrowPerSimd<HD, I8, NT> / kNarrowWaves<HD, I8, NT>;
+    static_assert(256 * 4 * kNarrowPerSimd<HD, I8, NT> / kNarrowWaves<HD, I8, NT> <= kNarrowBlocks, "partial outputs");
+    if (hipError_t e = allow_lds(&paged_narrow_kernel<HD, I8, NT>, kLds); e != hipSuccess) return e;
+    hipLaunchKernelGGL((paged_narrow_kernel<HD, I8, NT>), dim3(ws.narrow_blocks), dim3(F::kThreads), kLds, s, p, ws);
+    return hipGetLastError();
+}
+
 template <int HD, bool I8>
 static hipError_t launch_paged_heads(const PagedAttnLaunch& p, hipStream_t s) {
-    using F = PagedBlock<HD, kBlockWaves<HD>, kNarrowCols>;
-    constexpr size_t kLds = std::max(F::kOutBytes, QueryStage<F, HD>::kBytes);
-    constexpr int kThreads = kWave * kBlockWaves<HD>;
     const int nkv = p.kv.nkv, group = p.nq / nkv;
-    const bool mixed = p.step.max_rows * static_cast<int64_t>(group) > kNarrowCols;
-    const PagedWs ws = paged_ws(p.ws, HD, nkv, nullptr);
+    const int64_t most = p.step.max_rows * static_cast<int64_t>(group);  // columns of a sequence
+    PagedWs ws = paged_ws(p.ws, HD, nkv, nullptr);
     const size_t row_lds = paged_row_lds(group, HD);
     int wide_blocks = 0;
-    if (mixed) {
-        static_assert(kWideLds<HD> >= kLds, "narrow blocks among them");
+    if (most > kNarrowCols) {
+        ws.narrow_cols = group <= 8 ? 8 : 16;
+        ws.narrow_blocks = 256;
+        static_assert(kWideLds<HD> >= PagedBlock<HD, kBlockWaves<HD>, kNarrowCols>::kOutBytes, "narrow blocks among them");
         hipLaunchKernelGGL(paged_plan_kernel<HD>, dim3(1), dim3(kPlanThreads), 0, s, p, ws);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         // row tiles of any division of the rows among the sequences, and the splits on top of them
         const int tiles = p.step.rows / (kLeastCols / group) + std::min(p.step.seqs, p.step.rows);
-        const unsigned wide = static_cast<unsigned>(tiles + kWideBlocks / nkv) * nkv;
+        const unsigned wide = static_cast<unsigned>(tiles + kWideBlocks / nkv) * nkv, narrow = ws.narrow_blocks;
         if (hipError_t e = allow_lds(&paged_mixed_kernel<HD, I8>, kWideLds<HD>); e != hipSuccess) return e;
-        hipLaunchKernelGGL((paged_mixed_kernel<HD, I8>), dim3(std::max(wide, 4u * kNarrowBlocks) + kNarrowBlocks), dim3(kThreads), kWideLds<HD>, s, p, ws);
+        hipLaunchKernelGGL((paged_mixed_kernel<HD, I8>), dim3(std::max(wide, 4u * narrow) + narrow), dim3(kWave * kBlockWaves<HD>), kWideLds<HD>, s, p, ws);
         wide_blocks = std::max(1, kWideBlocks / nkv) * nkv;
-    } else {
-        if (hipError_t e = allow_lds(&paged_narrow_kernel<HD, I8>, kLds); e != hipSuccess) return e;
-        hipLaunchKernelGGL((paged_narrow_kernel<HD, I8>), dim3(kNarrowBlocks), dim3(kThreads), kLds, s, p, ws);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    } else if (hipError_t e = most <= 8 ? launch_narrow<HD, I8, 1>(p, ws, s) : launch_narrow<HD, I8, 2>(p, ws, s); e != hipSuccess) {
+        return e;
     }
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (hipError_t e = allow_lds(&paged_merge_kernel<HD>, row_lds); e != hipSuccess) return e;
     hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3(p.step.seqs * nkv + wide_blocks), dim3(kMergeThreads), row_lds, s, p, ws, p.step.seqs * nkv, wide_blocks);
     return hipGetLastError();
