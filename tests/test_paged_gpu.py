@@ -902,3 +902,195 @@ def test_two_streams_at_once():
         xb.ck(L.xqhip_stream_synchronize(s))
         assert (out.download(np.float32, plan.total * 2048).reshape(alone.shape) == alone).all()
         xb.ck(L.xqhip_stream_destroy(s))
+
+
+# ---- sizes at which other kernels, or other parts of them, run --------------------
+def attend_rows(pool, plan, nq, q, gate, picks):
+    """attend_oracle for many rows at once (every page of the sequences there): {row: [nq][hd]} of the rows in `picks`."""
+    k, v = pool.values()
+    g, hd, out = nq // pool.nkv, pool.hd, {}
+    for s, m in enumerate(plan.rows):
+        js = np.array([j for j in range(m) if int(plan.row0[s]) + j in picks], int)
+        if not len(js):
+            continue
+        n = min(plan.past[s] + m, plan.most * plan.page)
+        kk, vv = plan.seq_values(k, s, n), plan.seq_values(v, s, n)
+        rows = int(plan.row0[s]) + js
+        hidden = np.arange(n)[None] > plan.past[s] + js[:, None]
+        o = np.empty((len(js), nq, hd))
+        for h in range(nq):
+            z = q[rows].reshape(len(js), nq, hd)[:, h].astype(np.float64) @ kk[:, h // g].T / math.sqrt(hd)
+            z[hidden] = -np.inf
+            e = np.exp(z - z.max(-1, keepdims=True))
+            o[:, h] = e @ vv[:, h // g] / e.sum(-1, keepdims=True)
+        if gate is not None:
+            o = o * po.sigmoid(gate[rows].reshape(len(js), nq, hd))
+        out.update(zip(rows.tolist(), o))
+    return out
+
+
+MANY = [
+    # nq, nkv, hd, page, past, rows: blocks of 64 columns with and without splits, and of 128
+    (32, 8, 128, 64, [0, 100, 40], [700, 400, 1]), (16, 1, 128, 128, [40000, 3], [200, 1]), (8, 1, 256, 64, [5000, 0], [600, 1]),
+    (32, 2, 256, 32, [70, 3000, 5], [40, 1, 9]), (10, 2, 128, 32, [1000, 0, 500], [333, 12, 3]), (128, 64, 128, 32, [130, 5, 61], [50, 1, 4]),
+    (256, 256, 128, 32, [33, 90], [21, 1]), (256, 256, 256, 32, [40], [18]), (16, 16, 128, 64, [900] * 3, [129, 128, 127]),
+    (3, 3, 128, 128, [0], [1500]), (64, 4, 128, 64, [250, 1030], [300, 5]),
+]
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+@pytest.mark.parametrize("shape", MANY, ids=[f"{a[0]}_{a[1]}x{a[2]}_{a[4][0]}_{a[5][0]}" for a in MANY])
+def test_attention_of_many_rows(kind, shape):
+    nq, nkv, hd, page, past, rows = shape
+    rng = np.random.default_rng(nq + sum(rows))
+    plan = Plan(rng, page, past, rows, pad=1)
+    pool = filled(rng, kind, nkv, hd, page, plan)
+    q, gate = (rng.normal(0, 1, (plan.total, nq * hd)).astype(np.float32) for _ in range(2))
+    got = attention(pool, plan, nq, q, gate)
+    check(got, attend_rows(pool, plan, nq, q, gate, set(range(plan.n))))
+    assert (got[plan.n:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+@pytest.mark.parametrize("most", [1, 2, 30])
+def test_a_step_of_as_many_sequences_as_there_can_be(kind, most):
+    rng = np.random.default_rng(28)
+    rows = [int(r) for r in rng.choice([0, 1, 1, 1, most], 1024)]
+    plan = Plan(rng, 32, [int(p) for p in rng.integers(0, 90, 1024)], rows, pad=1)
+    pool = Pool(kind, 3, 128, 32, plan.pages, 1024, *(rng.normal(0, 1, (plan.pages, 3, 32, 128)).astype(np.float16) for _ in "kv"))
+    for b in pool.open:
+        xb.ck(xb.hip().xqhip_fill_u8(b.ptr, 0, 1024 * 3 * 32 * 128 * 2, None))
+    was = pool.raw()
+    x, q, g, (qn, kn), cs = prep(rng, pool, plan, 6, 32, cap=200)
+    _, gx, kx, vx = split_heads(x, 6, 3, 128, 1)
+    assert (g[:plan.n] == gx[:plan.n]).all() and (q[plan.n:] == 7).all()
+    assert same(pool.raw(), appended(was, plan, kind, po.prepared(kx, kn, cs[:, None], EPS), vx))
+    flat, gate = q.reshape(plan.total, -1), g.reshape(plan.total, -1)
+    got = attention(pool, plan, 6, flat, gate)
+    check(got, attend_oracle(pool, plan, 6, flat, gate))
+    assert (got[plan.n:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+def test_a_prompt_of_as_many_rows_as_there_can_be(kind):
+    rng = np.random.default_rng(29)
+    plan = Plan(rng, 128, [1], [65535])
+    plan.past[0] = 0
+    plan.upload()
+    pool = Pool(kind, 1, 128, 128, plan.pages)
+    was = pool.raw()
+    x, q, g, (qn, kn), cs = prep(rng, pool, plan, 2, 32)
+    _, _, kx, vx = split_heads(x, 2, 1, 128, 1)
+    assert same(pool.raw(), appended(was, plan, kind, po.prepared(kx, kn, cs[:, None], EPS), vx))
+    flat = q.reshape(plan.total, -1)
+    got = attention(pool, plan, 2, flat, None)
+    assert np.isfinite(got).all()
+    check(got, attend_rows(pool, plan, 2, flat, None, {0, 1, 31, 32, 127, 128, 4000, 32767, 50001, 65534}), 1e-4)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,page,past,rows", [(512, 256, 16, 32, [31, 5], [40, 1]), (300, 100, 128, 64, [0, 63], [3, 2]), (65, 1, 32, 128, [127], [1])])
+@pytest.mark.parametrize("kind", [F16, I8])
+def test_prep_of_many_heads(kind, nq, nkv, hd, page, past, rows):
+    rng = np.random.default_rng(30)
+    plan = Plan(rng, page, past, rows, pad=1)
+    pool = Pool(kind, nkv, hd, page, plan.pages, len(past), *(rng.normal(0, 1, (plan.pages, nkv, page, hd)).astype(np.float16) for _ in "kv"))
+    for b in pool.open:
+        xb.ck(xb.hip().xqhip_fill_u8(b.ptr, 0, len(past) * nkv * page * hd * 2, None))
+    was = pool.raw()
+    x, q, g, (qn, kn), cs = prep(rng, pool, plan, nq, 16, cap=300)
+    qx, gx, kx, vx = split_heads(x, nq, nkv, hd, 1)
+    want = po.prepared(qx, qn, cs[:, None], EPS)
+    assert (np.abs(q[:plan.n] - want[:plan.n]) <= 2**-23 * np.abs(want[:plan.n])).all() and (g[:plan.n] == gx[:plan.n]).all()
+    assert same(pool.raw(), appended(was, plan, kind, po.prepared(kx, kn, cs[:, None], EPS), vx))
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+@pytest.mark.parametrize("rows", [1, 2, 40])
+def test_a_page_stands_twice_in_a_table(kind, rows):
+    rng = np.random.default_rng(31)
+    plan = Plan(rng, 32, [150], [rows])
+    pool = filled(rng, kind, 2, 128, 32, plan)
+    plan.table[0, 1] = plan.table[0, 3] = plan.table[0, 0]
+    plan.upload()
+    q = rng.normal(0, 1, (rows, 8 * 128)).astype(np.float32)
+    check(attention(pool, plan, 8, q, None), attend_oracle(pool, plan, 8, q, None))
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+def test_captured_steps_of_changing_rows(kind):
+    """Prep and attention captured once for steps of up to 100 rows, up to 64 of a sequence, then replayed with other divisions of the
+    rows: prompts' chunks, single tokens, sequences without rows, no rows at all; eager work and synchronizations between."""
+    L, rng = xb.hip(), np.random.default_rng(32)
+    nq, nkv, hd, page, seqs, total = 8, 2, 128, 32, 5, 100
+    steps = [[64, 20, 0, 10, 6], [1, 1, 30, 1, 1], [64, 0, 30, 1, 5], [0, 0, 0, 0, 0], [1, 1, 1, 1, 1], [2, 33, 1, 0, 64]]
+    ends = np.sum(steps, 0)
+    whole = Plan(rng, page, [0] * seqs, [int(n) for n in ends])
+    pool, ref_pool = (Pool(kind, nkv, hd, page, whole.pages, seqs) for _ in range(2))
+    wq, norms = 2 * nq * hd, [rng.normal(1, 0.1, hd).astype(np.float32) for _ in range(2)]
+    row = wq + 2 * nkv * hd
+    rot = xb.rotary(dev(rope(32, 300)).ptr, 300, 32, [16])
+    need = L.xqhip_paged_attention_workspace_bytes(nq, nkv, hd)
+    ws, qn, kn = dev(np.full(need, 0xff, np.uint8)), dev(norms[0]), dev(norms[1])
+
+    def plan_of(past, rows):
+        p = Plan(rng, page, past, rows, pad=total - sum(rows), max_rows=64)
+        p.table, p.most, p.open, p.pages = whole.table, whole.most, whole.open, whole.pages
+        p.upload()
+        return p
+
+    plan = plan_of([0] * seqs, steps[0])
+    src, q, gate, out = (xb.DeviceBuffer(4 * total * n) for n in (row, nq * hd, nq * hd, nq * hd))
+    at = lambda f: ctypes.c_void_p(src.ptr.value + 4 * f)  # noqa: E731
+    stream, g = ctypes.c_void_p(), ctypes.c_void_p()
+    xb.ck(L.xqhip_stream_create(ctypes.byref(stream)))
+    xb.ck(L.xqhip_graph_begin(stream))
+    xb.ck(L.xqhip_attn_prep_paged(at(0), at(wq), at(wq + nkv * hd), 1, nq, qn.ptr, kn.ptr, EPS, ctypes.byref(rot), plan.ref, row, nq * hd,
+                                  q.ptr, gate.ptr, pool.ref, stream))
+    xb.ck(L.xqhip_paged_attention(q.ptr, gate.ptr, pool.ref, nq, plan.ref, nq * hd, out.ptr, nq * hd, ws.ptr, need, stream))
+    xb.ck(L.xqhip_graph_end(stream, ctypes.byref(g)))
+    past = np.zeros(seqs, np.int32)
+    for rows in steps:
+        now = plan_of([int(p) for p in past], rows)
+        x = rng.normal(0, 1, (total, row)).astype(np.float32)
+        filler = np.full(total * nq * hd, 7, np.float32)
+        for buf, a in ((src, x), (plan.bufs[0], now.row0), (plan.bufs[1], past), (out, filler), (q, filler), (gate, filler)):
+            xb.ck(L.xqhip_memcpy_h2d(buf.ptr, xb.ptr(np.ascontiguousarray(a)), a.nbytes, stream))
+        xb.ck(L.xqhip_graph_launch(g, stream))
+        xb.ck(L.xqhip_stream_synchronize(stream))
+        got = out.download(np.float32, total * nq * hd).reshape(total, nq, hd)
+        _, q2, g2, _, _ = prep(rng, ref_pool, now, nq, 32, x=x, norms=norms, cap=300)
+        assert (q.download(np.float32, total * nq * hd).reshape(q2.shape) == q2).all()
+        eager = attention(ref_pool, now, nq, q2.reshape(total, -1), g2.reshape(total, -1))
+        assert (got == eager).all() and (got[now.n:] == 7).all()
+        check(got, attend_oracle(ref_pool, now, nq, q2.reshape(total, -1), g2.reshape(total, -1)))
+        assert same(pool.raw(), ref_pool.raw())
+        past = past + np.array(rows, np.int32)
+    xb.ck(L.xqhip_graph_destroy(g))
+    xb.ck(L.xqhip_stream_destroy(stream))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("rows,vocab,top", [(2, 262145, 20), (2, 300001, 64), (1, 600000, 5), (2, 1048577, 1), (1, 2500003, 64), (1, 1 << 24, 20)])
+def test_logprobs_of_large_vocabularies(rows, vocab, top, f16):
+    """Ranks are exact where a row's largest logits come late, early and equal."""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((rows, vocab), np.float32) * 2
+    x[0, -3:] = x[0].max() + 1
+    x[-1, 7] = 20
+    if f16:
+        x = x.astype(np.float16)
+    tokens = [vocab - 1, vocab // 2][:rows]
+    check_logprobs(run_logprobs(x, tokens, 1.0, top, f16), x, tokens, 1.0, top)
+
+
+def test_logprobs_of_as_many_rows_as_there_can_be():
+    rng = np.random.default_rng(33)
+    x = rng.normal(0, 3, (65535, 33)).astype(np.float32)
+    tokens = [int(t) for t in rng.integers(0, 33, 65535)]
+    lp, en, rank, ids, tops = run_logprobs(x, tokens, 1.0, 2)
+    at = [0, 1, 32767, 40000, 65534]
+    check_logprobs([a[at] for a in (lp, en, rank, ids, tops)], x[at], [tokens[i] for i in at], 1.0, 2)
+    z = x.astype(np.float64) - x.max(-1, keepdims=True)
+    want = z[np.arange(65535), tokens] - np.log(np.exp(z).sum(-1))
+    assert np.abs(lp - want).max() <= 1e-5 and (ids[:, 0] == x.argmax(-1)).all()
+    assert (rank == (x > x[np.arange(65535), tokens][:, None]).sum(-1)).all()
