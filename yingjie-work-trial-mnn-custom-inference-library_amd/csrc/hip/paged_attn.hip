@@ -154,12 +154,10 @@ constexpr int kLeastCols = 64, kMostCols = 128;  // columns of other sequences' 
 constexpr int kWideBlocks = 256;    // blocks that few row tiles' keys are split over
 constexpr int kMostUnits = 65535 * kPagedMaxGroup / kLeastCols + 1024 + kWideBlocks;  // row tiles and splits of a step
 
-// the key of a tile that MFMA row r stands for: a lane's slots are then keys 16 (slot / 8) + 8 (lane / 32) + slot % 8
-// (fp16: pieces of 8 positions), or 16 (lane / 32) + 8 (slot / 8) + slot % 8 (8 bits: pieces of 16)
-template <bool I8>
+// the key of a tile that row r of a 32-row MFMA stands for: a lane's slots are then keys 16 (slot / 8) + 8 (lane / 32) + slot % 8
 __device__ __forceinline__ int key_of_row(int r) {
     const int e = r & 3, g = r >> 2 & 1, a0 = r >> 3 & 1, a1 = r >> 4;
-    return I8 ? 16 * g + 8 * a1 + 4 * a0 + e : 16 * a1 + 8 * g + 4 * a0 + e;
+    return 16 * a1 + 8 * g + 4 * a0 + e;
 }
 
 // Rows and keys of a sequence in an attention call.
@@ -167,6 +165,7 @@ struct SeqKeys {
     SeqRows r;
     int cap;  // positions that the table holds
     __device__ __forceinline__ SeqKeys(const PagedAttnLaunch& p, int s) : r(seq_rows(p.step, s)), cap(table_positions(p.step, p.kv)) {}
+    __device__ __forceinline__ SeqKeys(const PagedAttnLaunch& p, const SeqRows& rows) : r(rows), cap(table_positions(p.step, p.kv)) {}
     // last position that row j sees, -1: none
     __device__ __forceinline__ int last(int j) const {
         return r.past < 0 ? -1 : static_cast<int>(min(static_cast<int64_t>(r.past) + j, static_cast<int64_t>(cap) - 1));
@@ -255,8 +254,10 @@ struct NarrowWork {
 
 // Chunks [begin, end) of the keys of a row tile; its `splits` units lie one behind the other, and of a tile with several
 // so do their partial outputs' slots.
-struct WideUnit {
-    int seq, tile, begin, end, splits, slot;
+struct alignas(16) WideUnit {
+    int seq, tile, begin, end;
+    int splits, split, slot;  // of the row tile: units, which of them this is, the first's slot
+    SeqRows rows;             // the sequence's
 };
 // Workspace: where the merge finds the narrow sequences' parts, the wide kernel's units, partial outputs.
 struct PagedWs {
@@ -264,8 +265,8 @@ struct PagedWs {
     int4* narrow_at;  // [seqs][nkv]: blocks that share the sequence's tiles, the first of them and its slot, whether a single
                       // block's output has to be computed again
     int4* wide_at;    // [wide units][nkv], of those without splits: as above
-    int* first;       // [slots]: first unit of the slot's row tile
     WideUnit* units;
+    WideUnit* split;  // [slots]: their units
     float* narrow;    // [2 blocks][columns][hd + 2]
     float* wide;      // [slots][nkv][columns][hd + 2]
     int narrow_cols, narrow_blocks;  // of the call
@@ -416,21 +417,21 @@ struct WideShape {
     static_assert(QueryStage<Q, HD>::kBytes <= kLds && kLds + 64 <= 160 * 1024, "LDS");
 };
 
-// The units of the sequences that the narrow kernel does not take, by one block (5 us, a launch's and a dozen barriers'
-// latencies).
+// The units of the sequences that the narrow kernel does not take, by one block: of one wave where that has a lane per
+// sequence and few row tiles (4.5 to 6.5 us; by sixteen waves, with their barriers, 5.7 to 8.4).
 //
 // Columns of a block: with 128 each key and value is staged for four column tiles instead of two, but there are half as many
 // row tiles.  128 where those still give every block of a round its own (three chunks of 512 rows after 2300 beside 21 tokens
 // 148 us, with 64 columns 171; 2000 rows after 2000 220, 243), or where a round's blocks have over kLong chunks each, so that
 // splits cost little beside them (512 rows after 16000 292, 312; 64 after 131000 289, 317); elsewhere 64 (500 rows after
 // 3584 85, 91; 64 after 1000 24, 27).
-constexpr int kPlanThreads = 1024;
 constexpr int kLong = 60;
-static_assert(kPlanThreads >= 1024, "a thread per sequence");
-template <int HD>
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunch p, PagedWs ws) {
-    constexpr int kWaves = kPlanThreads / kWave;
-    __shared__ int pre[kPlanThreads], rows[kPlanThreads], past[kPlanThreads], red[3][kWaves], length;
+constexpr int kPlanTiles = 256;  // row tiles, at most, for one wave
+template <int HD, int WAVES>
+__global__ void __launch_bounds__(WAVES* kWave) paged_plan_kernel(PagedAttnLaunch p, PagedWs ws) {
+    constexpr int kWaves = WAVES, kThreads = WAVES * kWave;
+    __shared__ int pre[kThreads], red[3][kWaves], length;
+    __shared__ SeqRows seq[kThreads];
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, s = threadIdx.x;
     const int nkv = p.kv.nkv, group = p.nq / nkv, seqs = p.step.seqs, cap = table_positions(p.step, p.kv);
     const int room = max(1, kWideBlocks / nkv);  // units of a round of blocks
@@ -438,9 +439,12 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
     if (s < seqs) {
         const SeqRows r = seq_rows(p.step, s);
         if (r.rows > 0 && !is_narrow(r.rows, group, ws.narrow_cols)) mine = r.rows;
-        rows[s] = mine;
-        past[s] = r.past;
+        seq[s] = r;
         keys = r.past < 0 ? 0 : min(cap, r.past);
+    }
+    if (wid == kWaves - 1) {
+        const NarrowWork w(p, ws.narrow_cols, ws.narrow_blocks);
+        if (lane == 0) ws.head[2] = w.blocks;
     }
     auto wave_total = [&](int v) { return __builtin_amdgcn_readlane(wave_scan_int(v), kWave - 1); };
     auto tiles_of_rows = [&](int n, int cols) { return n ? (n + cols / group - 1) / (cols / group) : 0; };
@@ -485,7 +489,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
         }
         q = lo;
         tile = f - pre[lo];
-        const int seen = past[lo] < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(past[lo]) + min((tile + 1) * T, rows[lo]), static_cast<int64_t>(cap)));
+        const SeqRows r = seq[lo];
+        const int seen = r.past < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(r.past) + min((tile + 1) * T, r.rows), static_cast<int64_t>(cap)));
         return max(0, seen - 1) / chunk + 1;
     };
     // Splits: the shortest length with which all units fit one round of blocks; none where the tiles alone are more.  (Two
@@ -499,7 +504,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
             for (int i = 0; i < kHeld; ++i) {
                 const int f = i * kWave + lane;
                 int q, tile;
-                c[i] = f < tiles ? tile_at(f, q, tile) : 0;
+                c[i] = 0;
+                if (f < tiles) c[i] = tile_at(f, q, tile);
                 most = max(most, c[i]);
                 sum += c[i];
             }
@@ -509,7 +515,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
                 const int mid = (low + high) / 2;
                 int n = 0;
 #pragma unroll
-                for (int i = 0; i < kHeld; ++i) n += (c[i] + mid - 1) / mid;
+                for (int i = 0; i < kHeld; ++i)
+                    if (i * kWave < tiles) n += (c[i] + mid - 1) / mid;  // wave-uniform
                 if (wave_total(n) <= room)
                     high = mid;
                 else
@@ -522,7 +529,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
     __syncthreads();
     const int per = length;
     int units = 0;  // unit count, slots << 16
-    for (int f0 = 0; f0 < tiles; f0 += kPlanThreads) {
+    for (int f0 = 0; f0 < tiles; f0 += kThreads) {
         const int f = tiles - 1 - (f0 + static_cast<int>(threadIdx.x));  // later rows, which see more, first
         int q = 0, tile = 0, n = 0, c = 0;
         if (f >= 0) {
@@ -539,19 +546,16 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnLaunc
             units += red[0][i];
         }
         for (int i = 0; i < n; ++i) {
-            const int u = (at & 0xffff) + i, slot = (at >> 16) + i;
-            ws.units[u] = WideUnit{q, tile, static_cast<int>(static_cast<int64_t>(c) * i / n), static_cast<int>(static_cast<int64_t>(c) * (i + 1) / n), n, slot};
-            if (n > 1) ws.first[slot] = at & 0xffff;
+            // (c < 2^15 chunks, n <= 2^8)
+            const WideUnit un{q, tile, c * i / n, c * (i + 1) / n, n, i, at >> 16, seq[q]};
+            ws.units[(at & 0xffff) + i] = un;
+            if (n > 1) ws.split[(at >> 16) + i] = un;
         }
     }
-    if (wid == 0) {
-        const NarrowWork w(p, ws.narrow_cols, ws.narrow_blocks);
-        if (lane == 0) {
-            ws.head[0] = units & 0xffff;
-            ws.head[1] = units >> 16;
-            ws.head[2] = w.blocks;
-            ws.head[3] = cols;
-        }
+    if (threadIdx.x == 0) {
+        ws.head[0] = units & 0xffff;
+        ws.head[1] = units >> 16;
+        ws.head[3] = cols;
     }
 }
 
@@ -859,14 +863,14 @@ __device__ __forceinline__ void wide_block(const PagedAttnLaunch& p, const Paged
     __shared__ int redo;
     const int nkv = p.kv.nkv, kh = index % nkv, group = p.nq / nkv, T = S::kCols / group;
     const int unit = index / nkv;
+    const WideUnit un = ws.units[min(unit, kMostUnits - 1)];  // (on its way with the number of them)
     if (unit >= ws.head[0]) return;
-    const WideUnit un = ws.units[unit];
     const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int ct = wid % CT, ks = wid / CT, cl = lane & 31, g = lane >> 5;
     const uint32_t inv_t = (65535u + T) / T;  // c / T = c inv_t >> 16 for c < 128, T <= 128
     const int s = __builtin_amdgcn_readfirstlane(un.seq), t0 = __builtin_amdgcn_readfirstlane(un.tile) * T;
     const int begin = __builtin_amdgcn_readfirstlane(un.begin), end = __builtin_amdgcn_readfirstlane(un.end);
-    const SeqKeys sk(p, s);
+    const SeqKeys sk(p, un.rows);
     const int ntok = min(T, sk.r.rows - t0);
     Q query;
     query.load(p.q + static_cast<size_t>(sk.r.row0 + t0) * p.q_stride, p.q_stride, kh, ntok, group, T, inv_t);
@@ -974,7 +978,7 @@ __device__ __forceinline__ void wide_block(const PagedAttnLaunch& p, const Paged
                 o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, phi[h], o[j], 0, 0, 0);
             }
     };
-    const int krow = (ks * (HD / 8) + g) * 32 + key_of_row<false>(cl);
+    const int krow = (ks * (HD / 8) + g) * 32 + key_of_row(cl);
     // One chunk: its scores, the values of the chunk before (the matrix cores work on them while the softmax runs), the
     // next keys and this chunk's values into LDS.  One barrier: both are double-buffered.
     auto chunk = [&](int c, auto first, auto masked) {
@@ -1043,7 +1047,7 @@ __device__ __forceinline__ void wide_block(const PagedAttnLaunch& p, const Paged
     for (; c < clear; ++c) chunk(c, std::false_type{}, std::false_type{});
     for (; c < end; ++c) chunk(c, std::false_type{}, std::true_type{});
     add_values(end - 1);
-    float* part_out = un.splits > 1 ? ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * S::kCols * (HD + 2) : nullptr;
+    float* part_out = un.splits > 1 ? ws.wide + (static_cast<size_t>(un.slot + un.split) * nkv + kh) * S::kCols * (HD + 2) : nullptr;
     l = xor_pair_sum<32>(l);
     __syncthreads();  // every wave is done with K and V: the outputs take their place
     {
@@ -1063,31 +1067,47 @@ __device__ __forceinline__ void wide_block(const PagedAttnLaunch& p, const Paged
     join_paged<HD, KS, S::kCols, S::kThreads>(p, sk.r, kh, t0, ntok, T, inv_t, part_out, ws.wide_at + unit * nkv + kh, paged_lds, &redo);
 }
 
-// The splits of a row tile joined, each slot's block a share of the columns; and outputs that have to be computed again.
+// The splits of a row tile joined, the blocks of each slot (as many as there are for it) a share of the columns (13 rows'
+// three splits by 12 blocks 10 us, by all 256 5.9); and outputs that have to be computed again.
 template <int HD>
 __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int block, int blocks, float* smem) {
     __shared__ float fac[kMostCols + kWideBlocks], total[kMostCols];  // a block's columns times the splits
+    __shared__ float2 sums[kMostCols + kWideBlocks];
     __shared__ int list[kMergeThreads], count, redo;
+    static_assert(kMergeThreads >= kMostCols + kWideBlocks, "a thread per column and split");
     constexpr int kQuads = HD / 4;
-    const int cols = ws.head[3], slot_size = cols * (HD + 2), nkv = p.kv.nkv, group = p.nq / nkv, T = cols / group;
-    const int units = ws.head[0], slots = ws.head[1], slot = block / nkv, kh = block % nkv;
+    const int nkv = p.kv.nkv, group_of = block / nkv, kh = block - group_of * nkv;
+    WideUnit un = ws.split[group_of];  // (on its way with the number of them: right if each slot has one block)
+    const int cols = ws.head[3], slot_size = cols * (HD + 2), group = p.nq / nkv, T = cols / group;
+    const int units = ws.head[0], slots = ws.head[1];
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+    int each = 1, slot = group_of;
+    if (2 * slots * nkv <= blocks) {
+        each = blocks / nkv / max(slots, 1);
+        slot = group_of / each;
+        if (slot < slots) un = ws.split[slot];
+    }
+    const int which = group_of - slot * each;
     if (slot < slots) {
-        const WideUnit un = ws.units[ws.first[slot]];
-        const SeqRows sr = seq_rows(p.step, un.seq);
-        const int n = un.splits, k = slot - un.slot, t0 = un.tile * T, ntok = min(T, sr.rows - t0);
-        const int c0 = cols * k / n, c1 = cols * (k + 1) / n;
+        const SeqRows sr = un.rows;
+        const int n = un.splits, t0 = un.tile * T, ntok = min(T, sr.rows - t0);
+        const int share = un.split * each + which, c0 = cols * share / (n * each), c1 = cols * (share + 1) / (n * each);
         const size_t stride = static_cast<size_t>(nkv) * slot_size;
         const float* base = ws.wide + (static_cast<size_t>(un.slot) * nkv + kh) * slot_size;
-        for (int c = c0 + wid; c < c1; c += kMergeThreads / kWave) {
+        if (static_cast<int>(threadIdx.x) < (c1 - c0) * n) {  // all splits' maxima and sums at once
+            const int c = c0 + static_cast<int>(threadIdx.x) / n, b = static_cast<int>(threadIdx.x) % n;
+            const bool on = c / T < group && c % T < ntok;  // (others' were not written)
+            sums[threadIdx.x] = on ? *reinterpret_cast<const float2*>(base + b * stride + cols * HD + 2 * c) : make_float2(-INFINITY, 0.0f);
+        }
+        __syncthreads();
+        for (int c = wid; c < c1 - c0; c += kMergeThreads / kWave) {
             float M = -INFINITY, L = 0.0f;
-            const bool on = c / T < group && c % T < ntok;  // (others' sums were not written)
-            for (int b = lane; on && b < n; b += kWave) M = fmaxf(M, base[b * stride + cols * HD + 2 * c]);
+            for (int b = lane; b < n; b += kWave) M = fmaxf(M, sums[c * n + b].x);
             M = wave_max(M);
-            for (int b = lane; on && b < n; b += kWave) {
-                const float2 ml = *reinterpret_cast<const float2*>(base + b * stride + cols * HD + 2 * c);
+            for (int b = lane; b < n; b += kWave) {
+                const float2 ml = sums[c * n + b];
                 const float f = __builtin_amdgcn_exp2f(ml.x - M);
-                fac[(c - c0) * n + b] = f;
+                fac[c * n + b] = f;
                 L += f * ml.y;
             }
             L = wave_sum(L);
@@ -1103,7 +1123,7 @@ __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int bloc
 #pragma unroll 4
             for (int b = 0; b < n; ++b) add_scaled(r, fac[(c - c0) * n + b], *reinterpret_cast<const float4*>(base + b * stride + c * HD + d));
             const size_t row = sr.row0 + t0 + tc, colm = static_cast<size_t>(kh * group + hc) * HD + d;
-            bad |= write_paged_quad(r, total[c], p.gate ? p.gate + row * p.q_stride + colm : nullptr, p.out + row * p.out_stride + colm);
+            bad |= write_paged_quad(r, total[c - c0], p.gate ? p.gate + row * p.q_stride + colm : nullptr, p.out + row * p.out_stride + colm);
         }
         if (bad) redo = 1;
         __syncthreads();
@@ -1126,20 +1146,19 @@ __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int bloc
         const int n = count;
         for (int j = 0; j < n; ++j) {
             const int at = list[j];
-            const WideUnit un = ws.units[at / nkv];
-            const SeqRows sr = seq_rows(p.step, un.seq);
-            for (int t = un.tile * T; t < min((un.tile + 1) * T, sr.rows); ++t) attend_paged_row<kMergeThreads>(p, un.seq, sr, sr.row0 + t, at % nkv, smem);
+            const WideUnit u = ws.units[at / nkv];
+            for (int t = u.tile * T; t < min((u.tile + 1) * T, u.rows.rows); ++t) attend_paged_row<kMergeThreads>(p, u.seq, u.rows, u.rows.row0 + t, at % nkv, smem);
         }
         __syncthreads();
     }
 }
 
-template <int HD>
+template <int HD, bool WIDE>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedAttnLaunch p, PagedWs ws, int narrow_blocks, int wide_blocks) {
     extern __shared__ float smem[];  // attend_paged_row's
     if (static_cast<int>(blockIdx.x) < narrow_blocks)
         merge_narrow<HD>(p, ws, blockIdx.x / p.kv.nkv, blockIdx.x % p.kv.nkv, smem);
-    else
+    else if constexpr (WIDE)
         merge_wide<HD>(p, ws, blockIdx.x - narrow_blocks, wide_blocks, smem);
 }
 
@@ -1154,8 +1173,8 @@ static PagedWs paged_ws(float* base, int hd, int nkv, size_t* bytes) {
     w.head = reinterpret_cast<int*>(take(kWsHead));
     w.narrow_at = reinterpret_cast<int4*>(take(sizeof(int4) * 1024 * nkv));
     w.wide_at = reinterpret_cast<int4*>(take(sizeof(int4) * kMostUnits * nkv));
-    w.first = reinterpret_cast<int*>(take(sizeof(int) * kWideBlocks));
     w.units = reinterpret_cast<WideUnit*>(take(sizeof(WideUnit) * kMostUnits));
+    w.split = reinterpret_cast<WideUnit*>(take(sizeof(WideUnit) * kWideBlocks));
     w.narrow = reinterpret_cast<float*>(take(sizeof(float) * 2 * kNarrowBlocks * kNarrowCols * (hd + 2)));
     w.wide = reinterpret_cast<float*>(take(sizeof(float) * kWideBlocks * (hd == 128 ? kMostCols : kLeastCols) * (hd + 2)));
     if (bytes) *bytes = at - reinterpret_cast<char*>(base);
@@ -1178,13 +1197,14 @@ __global__ void __launch_bounds__((kWave * kNarrowWaves<HD, I8, NT>), (kNarrowPe
 }
 // Steps with longer ones.  Among the first blocks every fifth eight (one block on each XCD) are narrow ones, as many as there is
 // work for: those wait for memory, the others for the matrix cores.  (Every fourth eight would all go to the same quarter
-// of an XCD.)
+// of an XCD.)  Few wide blocks: every third, so that fewer blocks without work are launched (50
+// sequences, one of 9 rows: 11.3 us, with every fifth 13.8; every second 14.6).
 template <int HD, bool I8>
-__global__ void __launch_bounds__(kWave* kBlockWaves<HD>, kBlockWaves<HD> / 4) paged_mixed_kernel(PagedAttnLaunch p, PagedWs ws) {
+__global__ void __launch_bounds__(kWave* kBlockWaves<HD>, kBlockWaves<HD> / 4) paged_mixed_kernel(PagedAttnLaunch p, PagedWs ws, int turn) {
     extern __shared__ uint4 paged_lds[];
     const int b = blockIdx.x, all = ws.head[2];
-    const int n = b / 40 * 8 + max(0, b % 40 - 32);  // narrow ones before this, if they do not end
-    if (b % 40 >= 32 && n < all) {
+    const int at = b % turn - (turn - 8), n = b / turn * 8 + max(0, at);  // narrow ones before this, if they do not end
+    if (at >= 0 && n < all) {
         if (ws.narrow_cols == 8)
             narrow_block<HD, I8, kBlockWaves<HD>, 1>(p, ws, n, paged_lds);
         else
@@ -1227,21 +1247,29 @@ static hipError_t launch_paged_heads(const PagedAttnLaunch& p, hipStream_t s) {
         ws.narrow_cols = group <= 8 ? 8 : 16;
         ws.narrow_blocks = 256;
         static_assert(kWideLds<HD> >= PagedBlock<HD, kBlockWaves<HD>, kNarrowCols>::kOutBytes, "narrow blocks among them");
-        hipLaunchKernelGGL(paged_plan_kernel<HD>, dim3(1), dim3(kPlanThreads), 0, s, p, ws);
-        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         // row tiles of any division of the rows among the sequences, and the splits on top of them
         const int tiles = p.step.rows / (kLeastCols / group) + std::min(p.step.seqs, p.step.rows);
         const unsigned wide = static_cast<unsigned>(tiles + kWideBlocks / nkv) * nkv, narrow = ws.narrow_blocks;
-        if (hipError_t e = allow_lds(&paged_mixed_kernel<HD, I8>, kWideLds<HD>); e != hipSuccess) return e;
-        hipLaunchKernelGGL((paged_mixed_kernel<HD, I8>), dim3(std::max(wide, 4u * narrow) + narrow), dim3(kWave * kBlockWaves<HD>), kWideLds<HD>, s, p, ws);
-        wide_blocks = std::max(1, kWideBlocks / nkv) * nkv;
+        if (p.step.seqs <= kWave && tiles <= kPlanTiles)
+            hipLaunchKernelGGL((paged_plan_kernel<HD, 1>), dim3(1), dim3(kWave), 0, s, p, ws);
+        else
+            hipLaunchKernelGGL((paged_plan_kernel<HD, 16>), dim3(1), dim3(16 * kWave), 0, s, p, ws);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        const unsigned every = wide >= 4 * narrow ? 5 : 3;
+        if (hipError_t e = allow_lds(&paged_mixed_kernel<HD, I8>, kWideLds<HD>); e != hipSuccess) return e;
+        hipLaunchKernelGGL((paged_mixed_kernel<HD, I8>), dim3(std::max(wide, (every - 1) * narrow) + narrow), dim3(kWave * kBlockWaves<HD>), kWideLds<HD>, s, p, ws, 8 * every);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        wide_blocks = std::max(1, kWideBlocks / nkv) * nkv;
     } else if (hipError_t e = most <= 8 ? launch_narrow<HD, I8, 1>(p, ws, s) : launch_narrow<HD, I8, 2>(p, ws, s); e != hipSuccess) {
         return e;
     }
-    if (hipError_t e = allow_lds(&paged_merge_kernel<HD>, row_lds); e != hipSuccess) return e;
-    hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3(p.step.seqs * nkv + wide_blocks), dim3(kMergeThreads), row_lds, s, p, ws, p.step.seqs * nkv, wide_blocks);
-    return hipGetLastError();
+    const int pairs = p.step.seqs * nkv;
+    auto merge = [&](auto kernel) {
+        if (hipError_t e = allow_lds(kernel, row_lds); e != hipSuccess) return e;
+        hipLaunchKernelGGL(kernel, dim3(pairs + wide_blocks), dim3(kMergeThreads), row_lds, s, p, ws, pairs, wide_blocks);
+        return hipGetLastError();
+    };
+    return wide_blocks ? merge(&paged_merge_kernel<HD, true>) : merge(&paged_merge_kernel<HD, false>);
 }
 
 hipError_t launch_paged_attn(const PagedAttnLaunch& p, hipStream_t s) {
