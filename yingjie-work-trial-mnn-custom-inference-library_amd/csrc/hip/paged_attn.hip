@@ -197,7 +197,7 @@ struct NarrowWork {
         const SeqKeys k(p, s);
         return is_narrow(k.r.rows, group, cols) ? tiles_of(k.last(k.r.rows - 1)) : 0;
     }
-    __device__ __forceinline__ NarrowWork(const PagedAttnLaunch& p, int cols_, int most) : group(p.nq / p.kv.nkv), nkv(p.kv.nkv), cols(cols_) {
+    __device__ __forceinline__ NarrowWork(const PagedAttnLaunch& p, int group_, int cols_, int most) : group(group_), nkv(p.kv.nkv), cols(cols_) {
         const int lane = threadIdx.x & (kWave - 1), chunks = (p.step.seqs + kWave - 1) / kWave;
         int active = 0, sum = 0;
         for (int c = 0; c < chunks; ++c) {
@@ -270,7 +270,14 @@ struct PagedWs {
     float* narrow;    // [2 blocks][columns][hd + 2]
     float* wide;      // [slots][nkv][columns][hd + 2]
     int narrow_cols, narrow_blocks;  // of the call
+    int group, narrow_rows, least_rows, most_rows;  // query heads of a kv head; rows whose heads fill a block's columns
 };
+// Kernel arguments that are needed at any rate, all on their way at once: where they are first used, behind branches, each
+// would be waited for alone.
+template <typename... Ts>
+__device__ __forceinline__ void fetch_args(Ts... v) {
+    (..., [](auto x) { asm volatile("" ::"s"(x)); }(v));
+}
 constexpr size_t kWsHead = 16;
 
 template <int HD, int KS, int COLS>
@@ -300,10 +307,9 @@ __device__ __forceinline__ bool write_paged_quad(float4 r, float L, const float*
 // the output, and to *entry whether it has to be computed again.  The waves' outputs, maxima and sums lie in LDS; the block
 // has passed no barrier since.
 template <int HD, int KS, int COLS, int THREADS>
-__device__ __forceinline__ void join_paged(const PagedAttnLaunch& p, const SeqRows& sr, int kh, int t0, int ntok, int T, uint32_t inv_t,
-                                           float* part_out, int4* entry, void* lds, int* redo) {
+__device__ __forceinline__ void join_paged(const PagedAttnLaunch& p, const SeqRows& sr, int kh, int group, int t0, int ntok, int T,
+                                           uint32_t inv_t, float* part_out, int4* entry, void* lds, int* redo) {
     using F = PagedBlock<HD, KS, COLS>;
-    const int group = p.nq / p.kv.nkv;
     const float* Ol = static_cast<float*>(lds);         // [KS][columns][kLdo]
     const float* Ml = Ol + KS * F::kCols * F::kLdo;     // [KS][columns][2]
     float* Fl = const_cast<float*>(Ml) + KS * F::kCols * 2;  // [KS][columns]
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(WAVES* kWave) paged_plan_kernel(PagedAttnLaunc
     __shared__ int pre[kThreads], red[3][kWaves], length;
     __shared__ SeqRows seq[kThreads];
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, s = threadIdx.x;
-    const int nkv = p.kv.nkv, group = p.nq / nkv, seqs = p.step.seqs, cap = table_positions(p.step, p.kv);
+    const int nkv = p.kv.nkv, group = ws.group, seqs = p.step.seqs, cap = table_positions(p.step, p.kv);
     const int room = max(1, kWideBlocks / nkv);  // units of a round of blocks
     int mine = 0, keys = 0;                      // rows of this thread's sequence, positions
     if (s < seqs) {
@@ -443,13 +449,13 @@ __global__ void __launch_bounds__(WAVES* kWave) paged_plan_kernel(PagedAttnLaunc
         keys = r.past < 0 ? 0 : min(cap, r.past);
     }
     if (wid == kWaves - 1) {
-        const NarrowWork w(p, ws.narrow_cols, ws.narrow_blocks);
+        const NarrowWork w(p, ws.group, ws.narrow_cols, ws.narrow_blocks);
         if (lane == 0) ws.head[2] = w.blocks;
     }
     auto wave_total = [&](int v) { return __builtin_amdgcn_readlane(wave_scan_int(v), kWave - 1); };
-    auto tiles_of_rows = [&](int n, int cols) { return n ? (n + cols / group - 1) / (cols / group) : 0; };
+    auto tiles_of_rows = [&](int n, int rows) { return (n + rows - 1) / rows; };
     int cols = kLeastCols;
-    const int n64 = tiles_of_rows(mine, kLeastCols), n128 = tiles_of_rows(mine, kMostCols);
+    const int n64 = tiles_of_rows(mine, ws.least_rows), n128 = tiles_of_rows(mine, ws.most_rows);
     {
         // (chunks of 128 keys, in the order of their number)
         const int chunks = n64 ? min(n64 * ((keys + mine / 2) / 128 + 1), 1 << 20) : 0;
@@ -475,7 +481,7 @@ __global__ void __launch_bounds__(WAVES* kWave) paged_plan_kernel(PagedAttnLaunc
         tiles = tiles128;
         before = before128;
     }
-    const int own = cols == kMostCols ? n128 : n64, T = cols / group, chunk = kBlockWaves<HD> * kTTile * kTTile / cols;
+    const int own = cols == kMostCols ? n128 : n64, T = cols == kMostCols ? ws.most_rows : ws.least_rows, chunk = kBlockWaves<HD> * kTTile * kTTile / cols;
     pre[s] = before + wave_scan_int(own) - own;
     __syncthreads();
     auto tile_at = [&](int f, int& q, int& tile) {  // chunks of row tile f
@@ -576,11 +582,11 @@ __device__ __forceinline__ void narrow_block(const PagedAttnLaunch& p, const Pag
     constexpr int kSteps = HD / 32, kDimTiles = HD / 16, kKPieces = HD / (I8 ? 64 : 32);
     typedef typename std::conditional<I8, u32x2, u32x4>::type VPiece;  // eight positions of a dim
     __shared__ int redo;
-    const int nkv = p.kv.nkv, group = p.nq / nkv, T = kCols / group;
+    const int nkv = p.kv.nkv, group = ws.group, T = ws.narrow_rows;
     const int lane = threadIdx.x & (kWave - 1), ks = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int i16 = lane & 15, j = lane >> 4, part = i16 >> 3;
     const uint32_t inv_t = (65535u + T) / T;
-    NarrowWork w(p, kCols, ws.narrow_blocks);
+    NarrowWork w(p, ws.group, kCols, ws.narrow_blocks);
     if (block >= w.blocks) return;
     const int begin = w.begin(block), end = w.begin(block + 1);
     const uint32_t kat = (static_cast<uint32_t>(j) * p.kv.page + 8 * (i16 >> 2) + (i16 & 3)) * 16u, kstep = 64u * p.kv.page;
@@ -758,7 +764,7 @@ __device__ __forceinline__ void narrow_block(const PagedAttnLaunch& p, const Pag
             }
             if (lane < 8) *reinterpret_cast<float2*>(Ol + KS * kCols * F::kLdo + col * 2) = make_float2(m[t], sum);
         }
-        join_paged<HD, KS, kCols, F::kThreads>(p, sk.r, kh, 0, ntok, T, inv_t, part_out, entry, paged_lds, &redo);
+        join_paged<HD, KS, kCols, F::kThreads>(p, sk.r, kh, group, 0, ntok, T, inv_t, part_out, entry, paged_lds, &redo);
         __syncthreads();
     }
 }
@@ -771,7 +777,8 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
     __shared__ float4 sums[kMergeThreads];
     __shared__ int redo;
     constexpr int kQuads = HD / 4, kBatch = 4;
-    const int nkv = p.kv.nkv, group = p.nq / nkv, all_cols = ws.narrow_cols, T = all_cols / group, kSlot = all_cols * (HD + 2);
+    const int nkv = p.kv.nkv, group = ws.group, all_cols = ws.narrow_cols, T = ws.narrow_rows, kSlot = all_cols * (HD + 2);
+    fetch_args(p.gate, p.q_stride, p.out, p.out_stride, ws.narrow, group, T);
     const int4 at = ws.narrow_at[s * nkv + kh];
     const SeqRows sr = seq_rows(p.step, s);
     if (!is_narrow(sr.rows, group, all_cols)) return;
@@ -861,7 +868,7 @@ __device__ __forceinline__ void wide_block(const PagedAttnLaunch& p, const Paged
     constexpr uint32_t es = I8 ? 1u : 2u;
     constexpr int kKLoads = HD / (I8 ? 32 : 16) / CT, kVLoads = (I8 ? 2 : 4) * HD / 64 / CT;  // of a wave and chunk, 1 KiB each
     __shared__ int redo;
-    const int nkv = p.kv.nkv, kh = index % nkv, group = p.nq / nkv, T = S::kCols / group;
+    const int nkv = p.kv.nkv, kh = index % nkv, group = ws.group, T = S::kCols == kMostCols ? ws.most_rows : ws.least_rows;
     const int unit = index / nkv;
     const WideUnit un = ws.units[min(unit, kMostUnits - 1)];  // (on its way with the number of them)
     if (unit >= ws.head[0]) return;
@@ -1064,26 +1071,26 @@ __device__ __forceinline__ void wide_block(const PagedAttnLaunch& p, const Paged
             if (g == 0) *reinterpret_cast<float2*>(Ol + KS * F::kCols * F::kLdo + at * 2) = make_float2(m, l);
         }
     }
-    join_paged<HD, KS, S::kCols, S::kThreads>(p, sk.r, kh, t0, ntok, T, inv_t, part_out, ws.wide_at + unit * nkv + kh, paged_lds, &redo);
+    join_paged<HD, KS, S::kCols, S::kThreads>(p, sk.r, kh, group, t0, ntok, T, inv_t, part_out, ws.wide_at + unit * nkv + kh, paged_lds, &redo);
 }
 
 // The splits of a row tile joined, the blocks of each slot (as many as there are for it) a share of the columns (13 rows'
 // three splits by 12 blocks 10 us, by all 256 5.9); and outputs that have to be computed again.
 template <int HD>
-__device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int block, int blocks, float* smem) {
+__device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int group_of, int groups, int kh, float* smem) {
     __shared__ float fac[kMostCols + kWideBlocks], total[kMostCols];  // a block's columns times the splits
     __shared__ float2 sums[kMostCols + kWideBlocks];
     __shared__ int list[kMergeThreads], count, redo;
     static_assert(kMergeThreads >= kMostCols + kWideBlocks, "a thread per column and split");
     constexpr int kQuads = HD / 4;
-    const int nkv = p.kv.nkv, group_of = block / nkv, kh = block - group_of * nkv;
+    const int nkv = p.kv.nkv;
     WideUnit un = ws.split[group_of];  // (on its way with the number of them: right if each slot has one block)
-    const int cols = ws.head[3], slot_size = cols * (HD + 2), group = p.nq / nkv, T = cols / group;
+    const int cols = ws.head[3], slot_size = cols * (HD + 2), group = ws.group, T = cols == kMostCols ? ws.most_rows : ws.least_rows;
     const int units = ws.head[0], slots = ws.head[1];
     const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
     int each = 1, slot = group_of;
-    if (2 * slots * nkv <= blocks) {
-        each = blocks / nkv / max(slots, 1);
+    if (2 * slots <= groups) {
+        each = groups / max(slots, 1);
         slot = group_of / each;
         if (slot < slots) un = ws.split[slot];
     }
@@ -1136,7 +1143,7 @@ __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int bloc
         __syncthreads();
     }
     // the units without a split, a share of them by each block
-    const int all = units * nkv, per = (all + blocks - 1) / blocks;
+    const int block = group_of * nkv + kh, blocks = groups * nkv, all = units * nkv, per = (all + blocks - 1) / blocks;
     for (int i0 = block * per; i0 < min(all, (block + 1) * per); i0 += kMergeThreads) {
         const int i = i0 + threadIdx.x;
         if (threadIdx.x == 0) count = 0;
@@ -1153,13 +1160,15 @@ __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int bloc
     }
 }
 
+// Grid: kv heads, then sequences and behind them the groups of a wide block per kv head.
 template <int HD, bool WIDE>
-__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedAttnLaunch p, PagedWs ws, int narrow_blocks, int wide_blocks) {
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(PagedAttnLaunch p, PagedWs ws) {
     extern __shared__ float smem[];  // attend_paged_row's
-    if (static_cast<int>(blockIdx.x) < narrow_blocks)
-        merge_narrow<HD>(p, ws, blockIdx.x / p.kv.nkv, blockIdx.x % p.kv.nkv, smem);
+    const int s = blockIdx.y, kh = blockIdx.x;
+    if (!WIDE || s < p.step.seqs)
+        merge_narrow<HD>(p, ws, s, kh, smem);
     else if constexpr (WIDE)
-        merge_wide<HD>(p, ws, blockIdx.x - narrow_blocks, wide_blocks, smem);
+        merge_wide<HD>(p, ws, s - p.step.seqs, gridDim.y - p.step.seqs, kh, smem);
 }
 
 static PagedWs paged_ws(float* base, int hd, int nkv, size_t* bytes) {
@@ -1229,6 +1238,7 @@ static hipError_t launch_narrow(const PagedAttnLaunch& p, PagedWs& ws, hipStream
     using F = PagedBlock<HD, kNarrowWaves<HD, I8, NT>, 8 * NT>;
     constexpr size_t kLds = std::max(F::kOutBytes, QueryStage<F, HD>::kBytes);
     ws.narrow_cols = 8 * NT;
+    ws.narrow_rows = ws.narrow_cols / ws.group;
     ws.narrow_blocks = 256 * 4 * kNarrowPerSimd<HD, I8, NT> / kNarrowWaves<HD, I8, NT>;
     static_assert(256 * 4 * kNarrowPerSimd<HD, I8, NT> / kNarrowWaves<HD, I8, NT> <= kNarrowBlocks, "partial outputs");
     if (hipError_t e = allow_lds(&paged_narrow_kernel<HD, I8, NT>, kLds); e != hipSuccess) return e;
@@ -1241,10 +1251,14 @@ static hipError_t launch_paged_heads(const PagedAttnLaunch& p, hipStream_t s) {
     const int nkv = p.kv.nkv, group = p.nq / nkv;
     const int64_t most = p.step.max_rows * static_cast<int64_t>(group);  // columns of a sequence
     PagedWs ws = paged_ws(p.ws, HD, nkv, nullptr);
+    ws.group = group;
+    ws.least_rows = kLeastCols / group;
+    ws.most_rows = kMostCols / group;
     const size_t row_lds = paged_row_lds(group, HD);
-    int wide_blocks = 0;
+    int wide_groups = 0;  // of merge blocks, one per kv head
     if (most > kNarrowCols) {
         ws.narrow_cols = group <= 8 ? 8 : 16;
+        ws.narrow_rows = ws.narrow_cols / group;
         ws.narrow_blocks = 256;
         static_assert(kWideLds<HD> >= PagedBlock<HD, kBlockWaves<HD>, kNarrowCols>::kOutBytes, "narrow blocks among them");
         // row tiles of any division of the rows among the sequences, and the splits on top of them
@@ -1259,17 +1273,16 @@ static hipError_t launch_paged_heads(const PagedAttnLaunch& p, hipStream_t s) {
         if (hipError_t e = allow_lds(&paged_mixed_kernel<HD, I8>, kWideLds<HD>); e != hipSuccess) return e;
         hipLaunchKernelGGL((paged_mixed_kernel<HD, I8>), dim3(std::max(wide, (every - 1) * narrow) + narrow), dim3(kWave * kBlockWaves<HD>), kWideLds<HD>, s, p, ws, 8 * every);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-        wide_blocks = std::max(1, kWideBlocks / nkv) * nkv;
+        wide_groups = std::max(1, kWideBlocks / nkv);
     } else if (hipError_t e = most <= 8 ? launch_narrow<HD, I8, 1>(p, ws, s) : launch_narrow<HD, I8, 2>(p, ws, s); e != hipSuccess) {
         return e;
     }
-    const int pairs = p.step.seqs * nkv;
     auto merge = [&](auto kernel) {
         if (hipError_t e = allow_lds(kernel, row_lds); e != hipSuccess) return e;
-        hipLaunchKernelGGL(kernel, dim3(pairs + wide_blocks), dim3(kMergeThreads), row_lds, s, p, ws, pairs, wide_blocks);
+        hipLaunchKernelGGL(kernel, dim3(nkv, p.step.seqs + wide_groups), dim3(kMergeThreads), row_lds, s, p, ws);
         return hipGetLastError();
     };
-    return wide_blocks ? merge(&paged_merge_kernel<HD, true>) : merge(&paged_merge_kernel<HD, false>);
+    return wide_groups ? merge(&paged_merge_kernel<HD, true>) : merge(&paged_merge_kernel<HD, false>);
 }
 
 hipError_t launch_paged_attn(const PagedAttnLaunch& p, hipStream_t s) {
