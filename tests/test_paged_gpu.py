@@ -735,7 +735,7 @@ def test_logprobs_of_any_stride(ld, shift, f16):
     check_logprobs(run_logprobs(x, tokens, 1.0, 10, f16, ld, shift), x, tokens, 1.0, 10)
 
 
-@pytest.mark.parametrize("vocab", [700, 30000])
+@pytest.mark.parametrize("vocab", [700, 1022, 1027, 8190, 8193, 30000])
 def test_logprobs_of_special_rows(vocab):
     """Ties, masked tokens, rows that leave nothing or one token, infinities, NaN, tokens that are none, rows that rise or fall."""
     rng = np.random.default_rng(21)
@@ -1067,6 +1067,23 @@ def test_captured_steps_of_changing_rows(kind):
         past = past + np.array(rows, np.int32)
     xb.ck(L.xqhip_graph_destroy(g))
     xb.ck(L.xqhip_stream_destroy(stream))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("vocab", [1, 3, 7, 8, 9, 1023, 1024, 1025, 1029, 8191, 8192, 8193])
+@pytest.mark.parametrize("masked", [0.0, 0.5, 0.99])
+def test_logprobs_of_few_logits(vocab, masked, f16):
+    """Rows that one block holds and the next sizes, masked tokens asked for too."""
+    rng = np.random.default_rng(vocab)
+    x = rng.normal(0, 3, (8, vocab)).astype(np.float16 if f16 else np.float32)
+    x[rng.random(x.shape) < masked] = -np.inf
+    x[1] = np.round(x[1])
+    tokens = [int(t) for t in rng.integers(0, vocab, 8)]
+    tokens[2], tokens[3] = vocab - 1, max(0, vocab - 2)
+    x[3, tokens[3]] = -np.inf
+    for ld in (vocab, (vocab + 7) // 8 * 8):
+        for top in (0, 1, 20, 64):
+            check_logprobs(run_logprobs(x, tokens, 1.0, top, f16, ld), x, tokens, 1.0, top)
 
 
 @pytest.mark.parametrize("f16", [False, True])

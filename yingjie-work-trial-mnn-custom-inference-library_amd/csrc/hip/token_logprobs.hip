@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "xqhip.h"
 #include "xqhip_common.hpp"
 #include "xqhip_kernels.hpp"
 
@@ -32,10 +33,12 @@ namespace xqhip {
 // ---------------------------------------------------------------------------
 constexpr int kMostSegments = 1024, kFewSegments = 256;
 constexpr int kPartWaves = 4;
+constexpr int kRun = 8;  // logits of a lane
 constexpr int kRowThreads = 512, kFewThreads = 256;
 constexpr int kCandidates = 2048;  // candidates of a row that are held
 constexpr int kMany = 512;         // ... that are put in order as they are
 constexpr int kMostLanes = 1024;   // lanes of a row that are looked at again
+constexpr int kSmallLogits = 16;   // of a thread, where a block holds a row
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 // Segments of a row.
@@ -109,15 +112,21 @@ __global__ void __launch_bounds__(kWave* kPartWaves) logprobs_part_kernel(Logpro
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int i = i0 + element<F16, VEC>(lane, e);
-                x[e] = i < p.vocab ? static_cast<float>(x0[i]) : -INFINITY;
+                const float v = static_cast<float>(x0[min(i, p.vocab - 1)]);  // (no branches: the loads go out together)
+                x[e] = i < p.vocab ? v : -INFINITY;
             }
             if (it == 0 && p.out_rank) t = p.tokens[row];
         }
         const bool has = t >= 0 && t < p.vocab;  // wave-uniform
         if (it == 0 && has) xt = clean(static_cast<float>(x0[t]));
-        float lm = -INFINITY;
+        float lm = -INFINITY, rm[E / kRun];  // of a lane, of its runs
 #pragma unroll
-        for (int e = 0; e < E; ++e) lm = fmaxf(lm, x[e]);
+        for (int r = 0; r < E / kRun; ++r) {
+            rm[r] = x[kRun * r];
+#pragma unroll
+            for (int e = 1; e < kRun; ++e) rm[r] = fmaxf(rm[r], x[kRun * r + e]);
+            lm = fmaxf(lm, rm[r]);
+        }
         mine = fmaxf(mine, lm);
         const float m = wave_max(lm);
         if (has && m >= xt) {  // wave-uniform
@@ -135,13 +144,25 @@ __global__ void __launch_bounds__(kWave* kPartWaves) logprobs_part_kernel(Logpro
             float s = 0.0f, h = 0.0f;
             int same = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float d = gap2(x[e], m, c);
-                const bool top = x[e] == m;
-                same += __popcll(__builtin_amdgcn_ballot_w64(top));
-                const float w = top ? 0.0f : __builtin_amdgcn_exp2f(d);
-                s += w;
-                h = fmaf(w, d, h);
+            for (int r = 0; r < E / kRun; ++r) {
+                if (__builtin_amdgcn_ballot_w64(rm[r] == m)) {  // wave-uniform: only there the maximum is looked for
+#pragma unroll
+                    for (int e = kRun * r; e < kRun * (r + 1); ++e) {
+                        const float d = gap2(x[e], m, c);
+                        const bool top = x[e] == m;
+                        same += __popcll(__builtin_amdgcn_ballot_w64(top));
+                        const float w = top ? 0.0f : __builtin_amdgcn_exp2f(d);
+                        s += w;
+                        h = fmaf(w, d, h);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = kRun * r; e < kRun * (r + 1); ++e) {
+                        const float d = gap2(x[e], m, c), w = __builtin_amdgcn_exp2f(d);
+                        s += w;
+                        h = fmaf(w, d, h);
+                    }
+                }
             }
             s = wave_sum(s) + static_cast<float>(same - 1);
             h = wave_sum(h);
@@ -225,6 +246,24 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[R], int k) {
             high = mid - 1;
     }
     return 0;
+}
+
+// The first of a row's n candidates, by a block of `threads`.
+__device__ __forceinline__ void put_in_order(const LogprobsLaunch& p, int row, const uint64_t* cand, int n, float m, float lz, int threads) {
+    const int k = p.top;
+    auto put = [&](int place, uint64_t v) {
+        const size_t o = static_cast<size_t>(row) * k + place;
+        if (p.out_top) p.out_top[o] = v ? static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(v)) : -1;
+        if (p.out_top_logprob)
+            p.out_top_logprob[o] = v ? logit_gap(float_from_order_key(static_cast<uint32_t>(v >> 32)), m, p.inv_t) - lz : -INFINITY;
+    };
+    for (int i = threadIdx.x; i < n; i += threads) {
+        const uint64_t v = cand[i];
+        int place = 0;
+        for (int j = 0; j < n; ++j) place += cand[j] > v;
+        if (place < k) put(place, v);
+    }
+    for (int i = n + threadIdx.x; i < k; i += threads) put(i, 0);
 }
 
 template <bool F16, bool VEC, bool TOP, int THREADS>
@@ -448,25 +487,135 @@ __global__ void __launch_bounds__(THREADS) logprobs_row_kernel(LogprobsLaunch p,
                 __syncthreads();
             }
         }
-        const int n = counts[2];
-        auto put = [&](int place, uint64_t v) {
-            const size_t o = static_cast<size_t>(row) * k + place;
-            if (p.out_top) p.out_top[o] = v ? static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(v)) : -1;
-            if (p.out_top_logprob)
-                p.out_top_logprob[o] = v ? logit_gap(float_from_order_key(static_cast<uint32_t>(v >> 32)), m, p.inv_t) - lz : -INFINITY;
-        };
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-            const uint64_t v = cand[i];
-            int place = 0;
-            for (int j = 0; j < n; ++j) place += cand[j] > v;
-            if (place < k) put(place, v);
-        }
-        for (int i = n + threadIdx.x; i < k; i += THREADS) put(i, 0);
+        put_in_order(p, row, cand, counts[2], m, lz, THREADS);
     }
+}
+
+// A row of few logits, in a block's registers: one launch and no workspace.  VEC: the threads' pieces, and the logits behind
+// the last whole piece, one for each of the first threads.
+template <bool F16, bool VEC, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS) logprobs_small_kernel(LogprobsLaunch p) {
+    typedef logit_t<F16> L;
+    constexpr int E = kSmallLogits, N = VEC ? 16 / sizeof(L) : 1, kWaves = THREADS / kWave;
+    typedef L piece __attribute__((ext_vector_type(N)));
+    __shared__ float maxima[kWaves];
+    __shared__ float4 sums[kWaves];
+    __shared__ uint64_t cand[kCandidates];
+    __shared__ uint64_t best[THREADS];
+    __shared__ uint32_t keys[THREADS];
+    __shared__ int count;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave, vocab = p.vocab;
+    const L* x0 = logit_row<F16>(p, row);
+    const int t = p.tokens ? p.tokens[row] : -1;
+    const bool has = t >= 0 && t < vocab;
+    const int whole = vocab / N, rest = VEC ? vocab - whole * N : 0;
+    auto index = [&](int e) {  // past the row's end: no token's
+        const int at = e / N * THREADS + tid;
+        return e < E ? (!VEC || at < whole ? at * N : vocab) + e % N : whole * N + tid;
+    };
+    float x[E + 1];
+#pragma unroll
+    for (int u = 0; u < E / N; ++u) {  // (no branches: the loads go out together)
+        const int at = u * THREADS + tid;
+        const piece v = *reinterpret_cast<const piece*>(x0 + min(at, whole - 1) * N);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            float y;
+            if constexpr (VEC)
+                y = static_cast<float>(v[e]);
+            else
+                y = static_cast<float>(v[0]);
+            x[u * N + e] = at < whole ? y : -INFINITY;
+        }
+    }
+    x[E] = static_cast<float>(x0[min(whole * N + tid, vocab - 1)]);
+    if (tid >= rest) x[E] = -INFINITY;
+    const float xt = clean(static_cast<float>(x0[has ? t : 0])), c = p.inv_t * kLog2e;
+    float lm = x[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) lm = fmaxf(lm, x[e]);
+    lm = clean(lm);
+    const float wm = wave_max(lm);
+    if (lane == 0) maxima[wid] = wm;
+    if (TOP) keys[tid] = lm > -INFINITY ? float_order_key(lm) : 0;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    float m = maxima[0];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, maxima[i]);
+    const bool any = m > -INFINITY;
+    float s = 0.0f, h = 0.0f;
+    int same = 0, before = 0;
+#pragma unroll
+    for (int e = 0; e <= E; ++e) {
+        const bool top = x[e] == m;
+        const float d = gap2(x[e], m, c), w = top ? 0.0f : __builtin_amdgcn_exp2f(d), y = clean(x[e]);
+        same += __popcll(__builtin_amdgcn_ballot_w64(top));
+        s += w;
+        h = fmaf(w, d, h);
+        before += __popcll(__builtin_amdgcn_ballot_w64(y > xt || (y == xt && index(e) < t)));
+    }
+    s = wave_sum(s);
+    h = wave_sum(h);
+    if (lane == 0) sums[wid] = make_float4(s, h, static_cast<float>(before), static_cast<float>(same));
+    uint64_t least = 1;
+    if constexpr (TOP) {  // a value that `top` threads' maxima reach, found by every wave for itself
+        uint32_t w[kWaves];
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) w[i] = keys[i * kWave + lane];
+        least = static_cast<uint64_t>(reached_by(w, p.top)) << 32;
+        if (least == 0) {  // block-uniform: fewer threads have any, or ties
+            uint64_t mine = 0;
+#pragma unroll
+            for (int e = 0; e <= E; ++e) mine = clean(x[e]) > -INFINITY ? u64_max(mine, argmax_key(clean(x[e]), index(e))) : mine;
+            best[tid] = mine;
+            __syncthreads();
+            uint64_t v[kWaves];
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) v[i] = best[i * kWave + lane];
+            least = u64_max(kth_largest(v, p.top), 1);
+        }
+        // (of at most 1.25 top + 4 threads, E + 1 each)
+        static_assert((XQHIP_TOP_MAX + XQHIP_TOP_MAX / 4 + 4) * (E + 1) <= kCandidates, "candidates");
+#pragma unroll
+        for (int e = 0; e <= E; ++e) {
+            const float y = clean(x[e]);
+            if (y > -INFINITY && float_order_key(y) >= static_cast<uint32_t>(least >> 32)) {
+                const uint64_t v = argmax_key(y, index(e));
+                if (v >= least) cand[atomicAdd(&count, 1)] = v;
+            }
+        }
+    }
+    __syncthreads();
+    float4 a = sums[0];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) {
+        a.x += sums[i].x;
+        a.y += sums[i].y;
+        a.z += sums[i].z;
+        a.w += sums[i].w;
+    }
+    const float rs = a.x + (a.w - 1.0f), lz = log1pf(rs);
+    if (tid == 0) {
+        if (p.out_rank) p.out_rank[row] = has ? static_cast<int32_t>(a.z) : -1;
+        if (p.out_logprob) p.out_logprob[row] = any && has ? logit_gap(xt, m, p.inv_t) - lz : -INFINITY;
+        if (p.out_entropy) p.out_entropy[row] = any ? lz - kLn2 * a.y / (1.0f + rs) : 0.0f;
+    }
+    if constexpr (TOP) put_in_order(p, row, cand, count, m, lz, THREADS);
+}
+
+template <bool F16, bool VEC, int THREADS>
+static void launch_small(const LogprobsLaunch& p, hipStream_t s) {
+    if (p.top)
+        hipLaunchKernelGGL((logprobs_small_kernel<F16, VEC, true, THREADS>), dim3(p.rows), dim3(THREADS), 0, s, p);
+    else
+        hipLaunchKernelGGL((logprobs_small_kernel<F16, VEC, false, THREADS>), dim3(p.rows), dim3(THREADS), 0, s, p);
 }
 
 template <bool F16, bool VEC>
 static void launch_rows(const LogprobsLaunch& p, hipStream_t s) {
+    if (p.vocab <= kSmallLogits * kWave) return launch_small<F16, VEC, kWave>(p, s);
+    if (p.vocab <= kSmallLogits * kRowThreads) return launch_small<F16, VEC, kRowThreads>(p, s);
     const Segments sg = segments_of(p.vocab, F16);
     hipLaunchKernelGGL((logprobs_part_kernel<F16, VEC>), dim3((sg.count + kPartWaves - 1) / kPartWaves, p.rows), dim3(kWave * kPartWaves), 0, s, p, sg);
     if (hipPeekAtLastError() != hipSuccess) return;
@@ -477,7 +626,8 @@ static void launch_rows(const LogprobsLaunch& p, hipStream_t s) {
 }
 
 hipError_t launch_logprobs(const LogprobsLaunch& p, hipStream_t s) {
-    const bool vec = (reinterpret_cast<uintptr_t>(p.logits) & 15u) == 0 && p.ld % (p.f16 ? 8 : 4) == 0;
+    const int piece = p.f16 ? 8 : 4;
+    const bool vec = (reinterpret_cast<uintptr_t>(p.logits) & 15u) == 0 && p.ld % piece == 0 && p.vocab >= piece;
     if (p.f16)
         vec ? launch_rows<true, true>(p, s) : launch_rows<true, false>(p, s);
     else
