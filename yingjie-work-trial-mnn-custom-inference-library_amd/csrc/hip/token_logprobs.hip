@@ -38,7 +38,6 @@ constexpr int kRowThreads = 512, kFewThreads = 256;
 constexpr int kCandidates = 2048;  // candidates of a row that are held
 constexpr int kMany = 512;         // ... that are put in order as they are
 constexpr int kMostLanes = 1024;   // lanes of a row that are looked at again
-constexpr int kSmallLogits = 16;   // of a thread, where a block holds a row
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 // Segments of a row.
@@ -493,14 +492,14 @@ __global__ void __launch_bounds__(THREADS) logprobs_row_kernel(LogprobsLaunch p,
 
 // A row of few logits, in a block's registers: one launch and no workspace.  VEC: the threads' pieces, and the logits behind
 // the last whole piece, one for each of the first threads.
-template <bool F16, bool VEC, bool TOP, int THREADS>
+template <bool F16, bool VEC, bool TOP, int THREADS, int E>
 __global__ void __launch_bounds__(THREADS) logprobs_small_kernel(LogprobsLaunch p) {
     typedef logit_t<F16> L;
-    constexpr int E = kSmallLogits, N = VEC ? 16 / sizeof(L) : 1, kWaves = THREADS / kWave;
+    constexpr int N = VEC ? 16 / sizeof(L) : 1, kWaves = THREADS / kWave;
     typedef L piece __attribute__((ext_vector_type(N)));
     __shared__ float maxima[kWaves];
     __shared__ float4 sums[kWaves];
-    __shared__ uint64_t cand[kCandidates];
+    __shared__ uint64_t cand[(XQHIP_TOP_MAX + XQHIP_TOP_MAX / 4 + 4) * (E + 1)];  // as many threads, at most, hold any
     __shared__ uint64_t best[THREADS];
     __shared__ uint32_t keys[THREADS];
     __shared__ int count;
@@ -575,8 +574,6 @@ __global__ void __launch_bounds__(THREADS) logprobs_small_kernel(LogprobsLaunch 
             for (int i = 0; i < kWaves; ++i) v[i] = best[i * kWave + lane];
             least = u64_max(kth_largest(v, p.top), 1);
         }
-        // (of at most 1.25 top + 4 threads, E + 1 each)
-        static_assert((XQHIP_TOP_MAX + XQHIP_TOP_MAX / 4 + 4) * (E + 1) <= kCandidates, "candidates");
 #pragma unroll
         for (int e = 0; e <= E; ++e) {
             const float y = clean(x[e]);
@@ -604,18 +601,19 @@ __global__ void __launch_bounds__(THREADS) logprobs_small_kernel(LogprobsLaunch 
     if constexpr (TOP) put_in_order(p, row, cand, count, m, lz, THREADS);
 }
 
-template <bool F16, bool VEC, int THREADS>
+template <bool F16, bool VEC, int THREADS, int E>
 static void launch_small(const LogprobsLaunch& p, hipStream_t s) {
     if (p.top)
-        hipLaunchKernelGGL((logprobs_small_kernel<F16, VEC, true, THREADS>), dim3(p.rows), dim3(THREADS), 0, s, p);
+        hipLaunchKernelGGL((logprobs_small_kernel<F16, VEC, true, THREADS, E>), dim3(p.rows), dim3(THREADS), 0, s, p);
     else
-        hipLaunchKernelGGL((logprobs_small_kernel<F16, VEC, false, THREADS>), dim3(p.rows), dim3(THREADS), 0, s, p);
+        hipLaunchKernelGGL((logprobs_small_kernel<F16, VEC, false, THREADS, E>), dim3(p.rows), dim3(THREADS), 0, s, p);
 }
 
 template <bool F16, bool VEC>
 static void launch_rows(const LogprobsLaunch& p, hipStream_t s) {
-    if (p.vocab <= kSmallLogits * kWave) return launch_small<F16, VEC, kWave>(p, s);
-    if (p.vocab <= kSmallLogits * kRowThreads) return launch_small<F16, VEC, kRowThreads>(p, s);
+    if (p.vocab <= 16 * kWave) return launch_small<F16, VEC, kWave, 16>(p, s);
+    if (p.vocab <= 16 * kRowThreads) return launch_small<F16, VEC, kRowThreads, 16>(p, s);
+    if (p.vocab <= 32 * kRowThreads) return launch_small<F16, VEC, kRowThreads, 32>(p, s);
     const Segments sg = segments_of(p.vocab, F16);
     hipLaunchKernelGGL((logprobs_part_kernel<F16, VEC>), dim3((sg.count + kPartWaves - 1) / kPartWaves, p.rows), dim3(kWave * kPartWaves), 0, s, p, sg);
     if (hipPeekAtLastError() != hipSuccess) return;
