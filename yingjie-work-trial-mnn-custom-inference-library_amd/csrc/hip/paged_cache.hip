@@ -262,21 +262,15 @@ __device__ __forceinline__ int code_of(_Float16 x, float mx, float inv) {
     return static_cast<int>(__builtin_amdgcn_fmed3f(rintf(q), -127.0f, 127.0f));  // (a position never written may pass the maximum)
 }
 
-// One page that the step touches, one kv head, k or v, by a block.  The new rows' fp16 values go to LDS (four rows' loads of a
-// wave at a time), then to the page in 16-byte pieces; 8 bits: their maximum is taken on the way, and where it rose, or the
-// step leaves the page, the page's earlier values are fetched and the codes of all of them written.
-template <int E, bool VEC, bool I8>
-__device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int h, bool is_k, _Float16* vals, double* turn) {
+// A step's rows of one page, one kv head, k or v, as the page holds them, by a block (four rows' loads of a wave at a time):
+// those at [from, end) of the page with the first position `base`; to(t, held, v) takes row t.  before(): what is fetched
+// beside the first ones.
+template <int E, bool VEC, bool I8, typename Before, typename To>
+__device__ __forceinline__ void page_rows(const PagedPrepLaunch& p, const SeqRows& sr, int base, int from, int end, int h, bool is_k, double* turn, Before before,
+                                          To to) {
     typedef HeadLanes<E, VEC> L;
-    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
     constexpr int kBatch = E == 2 ? 4 : 2;
-    __shared__ float wave_mx[kPagedWaves];
-    __shared__ uint8_t ok[kPagedMaxPage];
-    const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
-    const int base = index * P, ld = hd + 8;                                          // position of the page's first
-    const int lead = max(0, sr.past - base), end = min(P, sr.past + sr.rows - base);  // new ones: [lead, end)
-    const bool last = base + P >= sr.past + sr.rows;
+    const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), hd = p.kv.head_dim;
     const LanePairs<E, VEC> pairs(p.rot, lane);
     float x[kBatch][E], w[E];
     RowAxes axes[kBatch];
@@ -288,19 +282,10 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
             axes[b].load(p.rot, p.step.rows, row, base + min(t0 + b * kPagedWaves, end - 1));
         }
     };
-    load(lead + wid);
+    load(from + wid);
     if (is_k) L::load(p.k_norm, lane, hd, w);
-    const Place place(p, s, base);
-    if (place.none()) return;  // block-uniform
-    const int page = place.page;
-    const size_t sat = static_cast<size_t>(page) * nkv + h;
-    _Float16* kept = nullptr;
-    float was = 0.0f, mx = 0.0f;
-    if constexpr (I8) {
-        kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(place.open) * nkv + h) * P * hd;
-        was = lead ? (is_k ? p.kv.k_scale : p.kv.v_scale)[sat] : 0.0f;
-    }
-    for (int t0 = lead + wid; t0 < end; t0 += kBatch * kPagedWaves) {
+    if (!before()) return;  // block-uniform
+    for (int t0 = from + wid; t0 < end; t0 += kBatch * kPagedWaves) {
         float2 cs[kBatch][E];
         bool held[kBatch];
         float y[kBatch][E];
@@ -317,30 +302,68 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
         for (int b = 0; b < kBatch; ++b) {
             const int t = t0 + b * kPagedWaves;
             if (t >= end) break;  // wave-uniform
-            if (lane == 0) ok[t] = held[b];
             _Float16 v[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                v[e] = I8 ? held_value(y[b][e]) : static_cast<_Float16>(y[b][e]);
-                if (I8 && held[b] && L::in(lane, e, hd)) mx = fmaxf(mx, fabsf(static_cast<float>(v[e])));
-            }
-            auto put = [&](_Float16* d) {
-                if constexpr (VEC) {
-                    typedef _Float16 hv __attribute__((ext_vector_type(E)));
-                    hv y;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) y[e] = v[e];
-                    *reinterpret_cast<hv*>(d + lane * E) = y;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (L::in(lane, e, hd)) d[L::dim(lane, e)] = v[e];
-                }
-            };
-            put(vals + t * ld);
-            if (I8 && last && held[b]) put(kept + static_cast<size_t>(t) * hd);
+            for (int e = 0; e < E; ++e) v[e] = I8 ? held_value(y[b][e]) : static_cast<_Float16>(y[b][e]);
+            to(t, held[b], v);
         }
     }
+}
+
+template <int E, bool VEC>
+__device__ __forceinline__ void put_row(const _Float16 (&v)[E], int lane, int hd, _Float16* d) {
+    typedef HeadLanes<E, VEC> L;
+    if constexpr (VEC) {
+        typedef _Float16 hv __attribute__((ext_vector_type(E)));
+        hv y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = v[e];
+        *reinterpret_cast<hv*>(d + lane * E) = y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (L::in(lane, e, hd)) d[L::dim(lane, e)] = v[e];
+    }
+}
+
+// One page that the step touches, one kv head, k or v, by a block.  The new rows' fp16 values go to LDS, then to the page in
+// 16-byte pieces; 8 bits: their maximum is taken on the way, and where it rose, or the step leaves the page, the page's
+// earlier values are fetched and the codes of all of them written.  The last page's rows from keep_from on are kept.
+template <int E, bool VEC, bool I8>
+__device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int keep_from, int h, bool is_k, _Float16* vals, double* turn) {
+    typedef HeadLanes<E, VEC> L;
+    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+    __shared__ float wave_mx[kPagedWaves];
+    __shared__ uint8_t ok[kPagedMaxPage];
+    const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
+    const int base = index * P, ld = hd + 8;                                          // position of the page's first
+    const int lead = max(0, sr.past - base), end = min(P, sr.past + sr.rows - base);  // new ones: [lead, end)
+    const bool last = base + P >= sr.past + sr.rows;
+    int page = -1;
+    size_t sat = 0;
+    _Float16* kept = nullptr;
+    float was = 0.0f, mx = 0.0f;
+    auto before = [&] {
+        const Place place(p, s, base);
+        page = place.page;
+        if (place.none()) return false;  // block-uniform
+        sat = static_cast<size_t>(page) * nkv + h;
+        if constexpr (I8) {
+            kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(place.open) * nkv + h) * P * hd;
+            was = lead ? (is_k ? p.kv.k_scale : p.kv.v_scale)[sat] : 0.0f;
+        }
+        return true;
+    };
+    page_rows<E, VEC, I8>(p, sr, base, lead, end, h, is_k, turn, before, [&](int t, bool held, const _Float16(&v)[E]) {
+        if (lane == 0) ok[t] = held;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (I8 && held && L::in(lane, e, hd)) mx = fmaxf(mx, fabsf(static_cast<float>(v[e])));
+        put_row<E, VEC>(v, lane, hd, vals + t * ld);
+        if (I8 && last && held && t >= keep_from) put_row<E, VEC>(v, lane, hd, kept + static_cast<size_t>(t) * hd);
+    });
+    if (page < 0) return;
     int from = lead;
     float inv = 0.0f;
     auto earlier = [&] {  // the page's values before the step, in fp16
@@ -431,13 +454,13 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     }
 }
 
-// The pages that the step touches, a block per page, kv head and k or v, in the order of the sequences.  Where a sequence's
-// first 8-bit page holds earlier positions, it and the last are one block's: their values lie where the last's are kept.
+// The pages that the step touches, a block per page, kv head and k or v, in the order of the sequences.  The earlier values of
+// an 8-bit page that the step leaves lie where those of its last page are kept: the block of the first has fetched them
+// before it keeps those rows of the last, which it computes too, and the last's block the others.
 __device__ __forceinline__ int hold_blocks_of(const PagedPrepLaunch& p, const SeqRows& r) {
     // (positions past the table have no page: the sums stay in 32 bits)
     if (r.rows == 0 || r.past < 0 || r.past >= table_positions(p.step, p.kv)) return 0;
-    const int pages = (r.past + r.rows - 1) / p.kv.page - r.past / p.kv.page + 1;
-    return pages > 1 && p.kv.i8 && r.past % p.kv.page ? pages - 1 : pages;
+    return (r.past + r.rows - 1) / p.kv.page - r.past / p.kv.page + 1;
 }
 template <int E, bool VEC, bool I8>
 __device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _Float16* vals, double* turn) {
@@ -457,13 +480,22 @@ __device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _F
     }
     if (s < 0) return;  // fewer pages than blocks
     const SeqRows sr = seq_rows(p.step, s);
-    const int first = sr.past / p.kv.page, last = (sr.past + sr.rows - 1) / p.kv.page, at = nth - first_block;
-    const bool both = I8 && at == 0 && sr.past % p.kv.page;
-    for (int index = first + at;; index = last) {
-        hold_page<E, VEC, I8>(p, sr, s, index, h, is_k, vals, turn);
-        if (!both || index == last) return;
-        __syncthreads();
-    }
+    const int P = p.kv.page, lead = sr.past % P, first = sr.past / P, last = (sr.past + sr.rows - 1) / P, index = first + nth - first_block;
+    hold_page<E, VEC, I8>(p, sr, s, index, index == first ? 0 : lead, h, is_k, vals, turn);
+    if constexpr (I8)
+        if (index == first && first < last && lead) {
+            __syncthreads();
+            const int end = min(lead, sr.past + sr.rows - last * P), lane = threadIdx.x & (kWave - 1), hd = p.kv.head_dim;
+            _Float16* kept = nullptr;
+            auto before = [&] {
+                const Place place(p, s, static_cast<int64_t>(last) * P);
+                kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(max(place.open, 0)) * p.kv.nkv + h) * P * hd;
+                return !place.none();
+            };
+            page_rows<E, VEC, I8>(p, sr, last * P, 0, end, h, is_k, turn, before, [&](int t, bool held, const _Float16(&v)[E]) {
+                if (held) put_row<E, VEC>(v, lane, hd, kept + static_cast<size_t>(t) * hd);
+            });
+        }
 }
 
 template <int E, bool VEC, bool I8>
@@ -586,8 +618,8 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
     const int per = p.step.rows >= 128 ? std::min(kQueryHeads, std::max(1, p.nq / kPagedWaves)) : 1;
     const int row_blocks = (p.nq + kPagedWaves * per - 1) / (kPagedWaves * per);
     // pages of any division of the rows among the sequences: n rows reach over n / P page borders, and one more; one more
-    // page than borders (one less block than pages: 8 bits)
-    const int64_t hold = 2 * static_cast<int64_t>(p.kv.nkv) * (p.step.rows / P + (p.kv.i8 ? 1 : 2) * std::min(p.step.seqs, p.step.rows));
+    // page than borders
+    const int64_t hold = 2 * static_cast<int64_t>(p.kv.nkv) * (p.step.rows / P + 2 * std::min(p.step.seqs, p.step.rows));
     const int64_t blocks = hold + static_cast<int64_t>(row_blocks) * p.step.rows;
     if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
     const size_t lds = static_cast<size_t>(P) * (hd + 8) * 2;
