@@ -115,19 +115,21 @@ __global__ void __launch_bounds__(256) paged_attn_row_kernel(PagedAttnLaunch p) 
 }
 
 // ---------------------------------------------------------------------------
-// Matrix-core forms, heads of 128 and 256 dims.  A block takes some columns of
-// one sequence and kv head and a range of its keys, a column being one (row,
-// query head) pair: column c of C is head c / T of the kv head's `group` and row
-// t0 + c % T, T = C / group.  Its waves share the keys in 32-key tiles, each with
-// its own running max, sum and output, joined through LDS at the end.
+// Matrix-core forms, heads of 128 and 256 dims: narrow_block for sequences of up
+// to 8 or 16 columns (single tokens), wide_block for the others (prompt chunks),
+// 64 or 128 columns a block.  A block takes some columns of one sequence and kv
+// head and a range of its keys, a column being one (row, query head) pair: column
+// c of C is head c / T of the kv head's `group` and row t0 + c % T, T = C / group.
+// Its waves share the keys in 32-key tiles, each with its own running max, sum and
+// output, joined through LDS at the end; blocks' parts of the same columns are
+// joined by paged_merge_kernel.
 //
 // Scores are formed transposed, S^T = K Q^T (keys are the MFMA rows).  The pages
 // hold keys and values as the operands are: a lane's eight (or sixteen) values
 // are 16 bytes in a row, 32 lanes' 512 bytes, so K and V go from memory to the
-// matrix cores without a transposition.  An MFMA leaves a lane rows 8 (v / 4) + 4
-// (l >> 5) + v % 4; the order in which a tile's keys are given to the rows is
-// chosen so that those are eight keys in a row, the ones whose values the lane
-// loads (key_of_row).
+// matrix cores without a transposition.  An MFMA leaves a lane some rows of its
+// column; the order in which a tile's keys are given to the rows is chosen so that
+// those are eight keys in a row, the ones whose values the lane loads.
 //
 // An 8-bit page's codes become fp16 integers, exactly; its scales enter as one
 // factor of a tile's scores and of its weights.
@@ -146,8 +148,7 @@ template <int HD>
 constexpr int kBlockWaves = HD == 128 ? 8 : 4;  // of a wide block: registers for two waves, or one, per SIMD
 template <int HD, bool I8, int NT>
 constexpr int kNarrowPerSimd = HD == 128 || (I8 && NT == 1) ? 2 : 1;  // narrow waves that a SIMD has registers for
-template <int HD, bool I8, int NT>
-constexpr int kNarrowWaves = 4 * kNarrowPerSimd<HD, I8, NT>;  // of a narrow block
+constexpr int kNarrowWaves = 4;  // of a narrow block (8, one block on a CU: 45 sequences of 500 27.4 us, not 18.5)
 constexpr int kNarrowCols = 16;      // sequences of up to 8 or 16 columns: narrow_block
 constexpr int kNarrowBlocks = 512;  // blocks that share their tiles, at most
 constexpr int kLeastCols = 64, kMostCols = 128;  // columns of other sequences' blocks: wide_block
@@ -177,11 +178,17 @@ __device__ __forceinline__ bool is_narrow(int rows, int group, int cols) { retur
 __device__ __forceinline__ int tiles_of(int last) { return max(0, last) / kTTile + 1; }
 
 // The narrow kernel's work: sequences of up to 16 columns, their 32-key tiles in units of q, for each kv head, one behind
-// the other; `blocks` blocks take equal ranges of them.  Few tiles: a block has one unit, and a unit lies in one
-// sequence and head.  Many: q = 1, and a block's range may end inside one and go on in the next.
+// the other; `blocks` blocks take equal numbers of units.
+// Units: a unit lies in one sequence and head and has a block of its own: a CU's only one, or where those are too few one
+// of two.  A whole sequence and head where that is not much longer: it needs no joining.
+// Ranges (q = 1): a block's tiles may end inside a sequence and head and go on in the next, where some unit would be over
+// kApart tiles more than its share.  Every sequence a block goes on to costs it some tiles' time (its place, queries, join).
+// (Whole calls, us: 45 sequences of 500 positions in units 18.5, in ranges 23.7; 60 of 1500, 8 bits 28.1, 31.6; 32 of
+// 4000, where a unit of 81 tiles stands against ranges of 41, 83, 70.  32 of 1000 in units of a CU each 20.7, of two 25.1.)
 // Each wave finds its block's place by itself, 64 sequences in its lanes at a time: no barrier, no launch before.
-constexpr int kMinTiles = 2;   // smallest unit of few tiles
-constexpr int kMaxTiles = 16;  // largest
+constexpr int kMinTiles = 4;  // smallest unit, a tile for every wave (one sequence of 700 11.2 us, with 8 11.8)
+constexpr int kApart = 32;    // (24: 60000 positions, 8 bits 30.6 us instead of 28.8; 16: 60 sequences of 1500 32.6, not 28.9)
+constexpr int kCus = 256;
 struct NarrowItem {
     int s, kh, unit, units;  // of the sequence and head: the unit asked for, and how many there are
 };
@@ -199,19 +206,25 @@ struct NarrowWork {
     }
     __device__ __forceinline__ NarrowWork(const PagedAttnLaunch& p, int group_, int cols_, int most) : group(group_), nkv(p.kv.nkv), cols(cols_) {
         const int lane = threadIdx.x & (kWave - 1), chunks = (p.step.seqs + kWave - 1) / kWave;
-        int active = 0, sum = 0;
+        int active = 0, sum = 0, longest = 0;
         for (int c = 0; c < chunks; ++c) {
             tiles = load(p, c);
             sum += tiles;
+            longest = max(longest, tiles);
             active += __popcll(__builtin_amdgcn_ballot_w64(tiles > 0));
         }
         const int64_t all = static_cast<int64_t>(__builtin_amdgcn_readlane(wave_scan_int(sum), kWave - 1)) * nkv;
-        // the smallest unit with which every unit has a block of its own
-        const int room = most - min(active * nkv, most);
-        if (room > 0 && all <= kMaxTiles * room)
-            q = max((static_cast<int>(all) + room - 1) / room, kMinTiles);
-        else
-            q = 1 + static_cast<int>(all >> 30);  // (units are counted in 32 bits)
+        longest = static_cast<int>(wave_max(static_cast<float>(longest)));
+        // a block of its own for every unit: on a CU of its own, else beside another
+        const int pairs = active * nkv, some = static_cast<int>(min(all, int64_t(1) << 30)), share = some / most;
+        q = 0;
+        for (int n = min(kCus, most); q == 0 && n <= most; n *= 2) {
+            if (pairs > n) continue;
+            int u = pairs < n ? max((some + n - pairs - 1) / (n - pairs), kMinTiles) : longest;
+            if (2 * longest <= 3 * u) u = longest;
+            if (min(u, longest) <= share + kApart) q = u;
+        }
+        if (q == 0) q = 1 + static_cast<int>(all >> 30);  // (units are counted in 32 bits)
         before = 0;
         for (int c = 0; c < chunks; ++c) {
             if (chunks > 1) tiles = load(p, c);
@@ -1200,9 +1213,9 @@ size_t paged_attn_workspace_bytes(int nq, int nkv, int head_dim) {
 
 // Steps of few rows per sequence.
 template <int HD, bool I8, int NT>
-__global__ void __launch_bounds__((kWave * kNarrowWaves<HD, I8, NT>), (kNarrowPerSimd<HD, I8, NT>)) paged_narrow_kernel(PagedAttnLaunch p, PagedWs ws) {
+__global__ void __launch_bounds__((kWave * kNarrowWaves), (kNarrowPerSimd<HD, I8, NT>)) paged_narrow_kernel(PagedAttnLaunch p, PagedWs ws) {
     extern __shared__ uint4 paged_lds[];
-    narrow_block<HD, I8, kNarrowWaves<HD, I8, NT>, NT>(p, ws, blockIdx.x, paged_lds);
+    narrow_block<HD, I8, kNarrowWaves, NT>(p, ws, blockIdx.x, paged_lds);
 }
 // Steps with longer ones.  Among the first blocks every fifth eight (one block on each XCD) are narrow ones, as many as there is
 // work for: those wait for memory, the others for the matrix cores.  (Every fourth eight would all go to the same quarter
@@ -1235,12 +1248,12 @@ constexpr size_t kWideLds = std::max(WideShape<HD, kLeastCols / kTTile>::kLds, W
 
 template <int HD, bool I8, int NT>
 static hipError_t launch_narrow(const PagedAttnLaunch& p, PagedWs& ws, hipStream_t s) {
-    using F = PagedBlock<HD, kNarrowWaves<HD, I8, NT>, 8 * NT>;
+    using F = PagedBlock<HD, kNarrowWaves, 8 * NT>;
     constexpr size_t kLds = std::max(F::kOutBytes, QueryStage<F, HD>::kBytes);
     ws.narrow_cols = 8 * NT;
     ws.narrow_rows = ws.narrow_cols / ws.group;
-    ws.narrow_blocks = 256 * 4 * kNarrowPerSimd<HD, I8, NT> / kNarrowWaves<HD, I8, NT>;
-    static_assert(256 * 4 * kNarrowPerSimd<HD, I8, NT> / kNarrowWaves<HD, I8, NT> <= kNarrowBlocks, "partial outputs");
+    ws.narrow_blocks = 256 * 4 * kNarrowPerSimd<HD, I8, NT> / kNarrowWaves;
+    static_assert(256 * 4 * kNarrowPerSimd<HD, I8, NT> / kNarrowWaves <= kNarrowBlocks, "partial outputs");
     if (hipError_t e = allow_lds(&paged_narrow_kernel<HD, I8, NT>, kLds); e != hipSuccess) return e;
     hipLaunchKernelGGL((paged_narrow_kernel<HD, I8, NT>), dim3(ws.narrow_blocks), dim3(F::kThreads), kLds, s, p, ws);
     return hipGetLastError();
