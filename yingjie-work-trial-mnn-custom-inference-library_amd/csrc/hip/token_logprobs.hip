@@ -17,6 +17,11 @@ namespace xqhip {
 //   s' = s1' + (s2' + 1) exp((m2 - m1) / T).
 // Equal infinities differ by 0.
 //
+// logprobs_small_kernel: rows of up to 16384 logits, a block per row, the row in
+//   registers: one launch (one row of 8192 4.5 us, by two launches 6.6; 200 fp16
+//   rows of 16000, 20 alternatives 12.0, 17.2; one of 16384 6.5, 6.6).  One wave
+//   for up to 1024 (5000 rows of 100 14.6 us, by eight waves 63), 16 logits a
+//   thread for up to 8192 (one row of 8000, 5 alternatives 7.2 us; 32 a thread 9.8).
 // logprobs_part_kernel: one pass over the logits.  A wave takes a segment (16
 //   fp32 logits a lane or 32 fp16 ones; more where the row would have over 1024
 //   segments) in registers: its maximum, s', the sum of exp(d) d, how many
@@ -28,8 +33,9 @@ namespace xqhip {
 //   fewer than 8 k segments (of up to 256) the threads' shares of all lanes'
 //   maxima stand in for the segments: one row of 243 segments, 20 alternatives
 //   10.2 us (so 11.4), 64 alternatives 15.3 (13.3).
-// What bounds it: the logits' bytes and, with fp16 logits, 13 operations a
-// logit; for one row a chain of two launches.
+// What bounds it: the logits' bytes (500 fp32 rows of 248320, 497 MB, 83 us, 6.0
+// TB/s) and, with fp16 logits, 11 to 13 operations a logit (48 rows 9.5 us); for
+// one row a chain of two launches, 3.5 and 5.5 us.
 // ---------------------------------------------------------------------------
 constexpr int kMostSegments = 1024, kFewSegments = 256;
 constexpr int kPartWaves = 4;
