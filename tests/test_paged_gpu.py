@@ -381,6 +381,28 @@ def test_read(kind, nkv, hd, page, past, rows, out):
     assert (alone.download(t, n) == bufs[1].download(t, n)).all()
 
 
+@pytest.mark.parametrize("kind", [F16, I8])
+@pytest.mark.parametrize("out", [xb.F32, xb.F16])
+def test_read_to_any_address(kind, out):
+    """Outputs at addresses that are multiples of their values' size only."""
+    rng = np.random.default_rng(34)
+    plan = Plan(rng, 64, [50, 3], [40, 70])
+    pool = Pool(kind, 3, 80, 64, plan.pages, 1, *(rng.normal(0, 2, (plan.pages, 3, 64, 80)).astype(np.float16) for _ in "kv"))
+    t, n = (np.float32 if out == xb.F32 else np.float16), plan.total * 3 * 80
+    got = []
+    for shift in (0, 1, 3):
+        bufs = [dev(np.full(n + 8, 7, t)) for _ in "kv"]
+        xb.ck(xb.hip().xqhip_paged_read(pool.ref, plan.ref, out, *(ctypes.c_void_p(b.ptr.value + shift * t().itemsize) for b in bufs), None))
+        x = [b.download(t, n + 8) for b in bufs]
+        assert all((y[:shift] == 7).all() and (y[shift + n:] == 7).all() for y in x)
+        got.append([y[shift: shift + n] for y in x])
+    assert all((a == b).all() for g in got[1:] for a, b in zip(g, got[0]))
+    k, v = pool.values()
+    want = [np.concatenate([plan.seq_values(x, s, p + m)[p:] for s, (p, m) in enumerate(zip(plan.past, plan.rows))]) for x in (k, v)]
+    for g, w in zip(got[0], want):  # a rounding of code * scale to fp32 and one to the output
+        assert (np.abs(g.reshape(w.shape) - w) <= (2**-10 if out == xb.F16 else 2**-23) * np.abs(w)).all()
+
+
 # ---- attention ------------------------------------------------------------------
 def attention(pool, plan, nq, q, gate, q_stride=None, out_stride=None, shift=0, stream=None, ws=None):
     L, width = xb.hip(), nq * pool.hd
