@@ -302,11 +302,10 @@ struct PagedBlock {
 };
 
 // writes the quad at `out`; whether its row has to be computed again
-__device__ __forceinline__ bool write_paged_quad(float4 r, float L, const float* gate, float* out) {
+__device__ __forceinline__ bool write_gated_quad(float4 r, float L, bool gated, float4 gt, float* out) {
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
     float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
-    if (gate) {
-        const float4 gt = *reinterpret_cast<const float4*>(gate);
+    if (gated) {
         y.x *= sigmoid_dev(gt.x);
         y.y *= sigmoid_dev(gt.y);
         y.z *= sigmoid_dev(gt.z);
@@ -314,6 +313,10 @@ __device__ __forceinline__ bool write_paged_quad(float4 r, float L, const float*
     }
     *reinterpret_cast<float4*>(out) = y;
     return !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
+}
+
+__device__ __forceinline__ bool write_paged_quad(float4 r, float L, const float* gate, float* out) {
+    return write_gated_quad(r, L, gate != nullptr, gate ? *reinterpret_cast<const float4*>(gate) : float4{}, out);
 }
 
 // The key waves of a block's columns joined, then written: a partial output (to part_out: [COLS][HD], then [COLS][2]), or
@@ -441,7 +444,7 @@ struct WideShape {
 //
 // Columns of a block: with 128 each key and value is staged for four column tiles instead of two, but there are half as many
 // row tiles.  128 where those still give every block of a round its own (three chunks of 512 rows after 2300 beside 21 tokens
-// 148 us, with 64 columns 171; 2000 rows after 2000 220, 243), or where a round's blocks have over kLong chunks each, so that
+// 154 us, with 64 columns 173; 2000 rows after 2000 212, 239), or where a round's blocks have over kLong chunks each, so that
 // splits cost little beside them (512 rows after 16000 292, 312; 64 after 131000 289, 317); elsewhere 64 (500 rows after
 // 3584 85, 91; 64 after 1000 24, 27).
 constexpr int kLong = 60;
@@ -820,6 +823,18 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
         }
     };
     load(first, slice);
+    // a quad's row, and its place in it
+    auto place = [&](int item, size_t& row) {
+        const int i = item / kQuads, head = i / sr.rows;
+        row = static_cast<size_t>(sr.row0 + i - head * sr.rows);
+        return static_cast<size_t>(kh * group + head) * HD + 4 * (item % kQuads);
+    };
+    float4 gates = {};  // of the first quad, on their way with its parts
+    if (p.gate && slice == 0 && first < items) {
+        size_t row;
+        const size_t at_col = place(first, row);
+        gates = *reinterpret_cast<const float4*>(p.gate + row * p.q_stride + at_col);
+    }
     for (int i = wid; i < cols; i += kMergeThreads / kWave) {
         const int c = column(i);
         float M = -INFINITY, L = 0.0f;
@@ -844,9 +859,14 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
     __syncthreads();
     bool bad = false;
     for (int item = first; item < items; item += kMergeThreads) {  // (more than one round only without slices)
-        const int i = item / kQuads, d = 4 * (item % kQuads);
+        const int i = item / kQuads;
         float4 r = {};
-        if (item != first) load(item, 0);
+        size_t row;
+        const size_t col = place(item, row);
+        if (item != first) {
+            load(item, 0);
+            if (p.gate) gates = *reinterpret_cast<const float4*>(p.gate + row * p.q_stride + col);
+        }
         if (slice < slices)
             for (int b0 = slice;;) {
 #pragma unroll
@@ -862,10 +882,7 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
             if (slice == 0)
                 for (int k = 1; k < slices; ++k) add_scaled(r, 1.0f, sums[k * items + item]);
         }
-        if (slice == 0) {
-            const size_t row = sr.row0 + i % sr.rows, colm = static_cast<size_t>(kh * group + i / sr.rows) * HD + d;
-            bad |= write_paged_quad(r, total[i], p.gate ? p.gate + row * p.q_stride + colm : nullptr, p.out + row * p.out_stride + colm);
-        }
+        if (slice == 0) bad |= write_gated_quad(r, total[i], p.gate != nullptr, gates, p.out + row * p.out_stride + col);
     }
     if (bad) redo = 1;
     __syncthreads();
