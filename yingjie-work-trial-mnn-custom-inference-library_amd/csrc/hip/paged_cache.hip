@@ -203,7 +203,7 @@ struct Place {
     __device__ __forceinline__ bool none() const { return page < 0; }
 };
 
-// `per` query heads of one row by a wave, h0 and every kPagedWaves-th from there: q and their gates.
+// `per` query heads of one row by a wave, from h0 on: q and their gates.
 constexpr int kQueryHeads = 4;
 template <int E, bool VEC>
 __device__ __forceinline__ void query_unit(const PagedPrepLaunch& p, int h0, int per, int row, double* turn) {
@@ -212,11 +212,11 @@ __device__ __forceinline__ void query_unit(const PagedPrepLaunch& p, int h0, int
     const LanePairs<E, VEC> pairs(p.rot, lane);
     const float* src = p.q_src + static_cast<size_t>(row) * p.src_stride;
     float x[kQueryHeads][E], gate[kQueryHeads][E], w[E];
-    auto on = [&](int i) { return i < per && h0 + i * kPagedWaves < p.nq; };  // wave-uniform
+    auto on = [&](int i) { return i < per && h0 + i < p.nq; };  // wave-uniform
 #pragma unroll
     for (int i = 0; i < kQueryHeads; ++i)
         if (on(i)) {
-            const float* at = src + static_cast<size_t>(h0 + i * kPagedWaves) * (p.gated ? 2 * hd : hd);
+            const float* at = src + static_cast<size_t>(h0 + i) * (p.gated ? 2 * hd : hd);
             L::load(at, lane, hd, x[i]);
             if (p.gated) L::load(at + hd, lane, hd, gate[i]);
         }
@@ -247,7 +247,7 @@ __device__ __forceinline__ void query_unit(const PagedPrepLaunch& p, int h0, int
             y[0][e] = held ? y[0][e] : __builtin_nanf("");
             if (!p.gated) gate[i][e] = 0.0f;
         }
-        const size_t at = o + static_cast<size_t>(h0 + i * kPagedWaves) * hd;
+        const size_t at = o + static_cast<size_t>(h0 + i) * hd;
         L::store(p.q_out + at, lane, hd, y[0]);
         if (p.gate_out) L::store(p.gate_out + at, lane, hd, gate[i]);
     }
@@ -504,7 +504,7 @@ __device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _F
 }
 
 template <int E, bool VEC, bool I8>
-__global__ void __launch_bounds__(kPagedThreads, 4) paged_prep_kernel(PagedPrepLaunch p, int hold_blocks, int row_blocks, int per) {
+__global__ void __launch_bounds__(kPagedThreads, 4) paged_prep_kernel(PagedPrepLaunch p, int hold_blocks, int row_units, int per) {
     extern __shared__ uint4 page_lds[];
     _Float16* page_vals = reinterpret_cast<_Float16*>(page_lds);
     __shared__ double turn[kPagedWaves][kPagedMaxDim];
@@ -513,8 +513,8 @@ __global__ void __launch_bounds__(kPagedThreads, 4) paged_prep_kernel(PagedPrepL
         hold_unit<E, VEC, I8>(p, blockIdx.x, page_vals, turn[wid]);
         return;
     }
-    const int b = blockIdx.x - hold_blocks, row = b / row_blocks, h = (b - row * row_blocks) * kPagedWaves * per + wid;
-    if (h < p.nq) query_unit<E, VEC>(p, h, per, row, turn[wid]);
+    const int unit = (static_cast<int>(blockIdx.x) - hold_blocks) * kPagedWaves + wid, row = unit / row_units;
+    if (row < p.step.rows) query_unit<E, VEC>(p, (unit - row * row_units) * per, per, row, turn[wid]);
 }
 
 // Steps of single tokens: a wave per sequence and head (query heads, then keys, then values), no barrier between them (with
@@ -622,12 +622,12 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
         return p.kv.i8 ? go(paged_token_kernel<E, false, true>) : go(paged_token_kernel<E, false, false>);
     }
     // (512 rows with one head a wave 24.1 us, with four 18.6; 51 rows 19.4 and 20.1)
-    const int per = p.step.rows >= 128 ? std::min(kQueryHeads, std::max(1, p.nq / kPagedWaves)) : 1;
-    const int row_blocks = (p.nq + kPagedWaves * per - 1) / (kPagedWaves * per);
+    const int per = p.step.rows >= 128 ? std::min(kQueryHeads, p.nq) : 1;
+    const int row_units = (p.nq + per - 1) / per;
     // pages of any division of the rows among the sequences: n rows reach over n / P page borders, and one more; one more
     // page than borders
     const int64_t hold = 2 * static_cast<int64_t>(p.kv.nkv) * (p.step.rows / P + 2 * std::min(p.step.seqs, p.step.rows));
-    const int64_t blocks = hold + static_cast<int64_t>(row_blocks) * p.step.rows;
+    const int64_t blocks = hold + (static_cast<int64_t>(row_units) * p.step.rows + kPagedWaves - 1) / kPagedWaves;
     if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
     const size_t lds = static_cast<size_t>(P) * (hd + 8) * 2;
     auto go = [&](auto kernel) {
@@ -635,7 +635,7 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
                                                static_cast<int>(lds));
             e != hipSuccess)
             return e;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPagedThreads), lds, s, p, static_cast<int>(hold), row_blocks, per);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPagedThreads), lds, s, p, static_cast<int>(hold), row_units, per);
         return hipGetLastError();
     };
     if (hd == 128 && al) return p.kv.i8 ? go(paged_prep_kernel<2, true, true>) : go(paged_prep_kernel<2, true, false>);
