@@ -225,7 +225,7 @@ __device__ __forceinline__ void query_unit(const PagedPrepLaunch& p, int h0, int
     if (s >= p.step.seqs) return;
     const SeqRows sr = seq_rows(p.step, s);
     const int j = row - sr.row0;
-    if (j < 0 || j >= sr.rows) return;
+    if (j < 0 || j >= sr.rows || sr.rows == 1) return;  // (token_unit's)
     const int64_t pos = sr.past < 0 ? -1 : static_cast<int64_t>(sr.past) + j;
     RowAxes axes;
     axes.load(p.rot, p.step.rows, row, static_cast<int>(pos));
@@ -464,7 +464,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
 // before it keeps those rows of the last, which it computes too, and the last's block the others.
 __device__ __forceinline__ int hold_blocks_of(const PagedPrepLaunch& p, const SeqRows& r) {
     // (positions past the table have no page: the sums stay in 32 bits)
-    if (r.rows == 0 || r.past < 0 || r.past >= table_positions(p.step, p.kv)) return 0;
+    if (r.rows <= 1 || r.past < 0 || r.past >= table_positions(p.step, p.kv)) return 0;
     return (r.past + r.rows - 1) / p.kv.page - r.past / p.kv.page + 1;
 }
 template <int E, bool VEC, bool I8>
@@ -503,33 +503,13 @@ __device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _F
         }
 }
 
+// A sequence that brings one row: a head by a wave (query heads, then keys, then values).
 template <int E, bool VEC, bool I8>
-__global__ void __launch_bounds__(kPagedThreads, 4) paged_prep_kernel(PagedPrepLaunch p, int hold_blocks, int row_units, int per) {
-    extern __shared__ uint4 page_lds[];
-    _Float16* page_vals = reinterpret_cast<_Float16*>(page_lds);
-    __shared__ double turn[kPagedWaves][kPagedMaxDim];
-    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    if (static_cast<int>(blockIdx.x) < hold_blocks) {
-        hold_unit<E, VEC, I8>(p, blockIdx.x, page_vals, turn[wid]);
-        return;
-    }
-    const int unit = (static_cast<int>(blockIdx.x) - hold_blocks) * kPagedWaves + wid, row = unit / row_units;
-    if (row < p.step.rows) query_unit<E, VEC>(p, (unit - row * row_units) * per, per, row, turn[wid]);
-}
-
-// Steps of single tokens: a wave per sequence and head (query heads, then keys, then values), no barrier between them (with
-// their read-back 32 tokens 10.3 us, by the general kernel 16.1; one token 7.8, 11.1).
-constexpr int kTokenWaves = 4;
-template <int E, bool VEC, bool I8>
-__global__ void __launch_bounds__(kWave* kTokenWaves) paged_token_kernel(PagedPrepLaunch p, int row_blocks) {
+__device__ __forceinline__ void token_unit(const PagedPrepLaunch& p, int s, int unit, double* turn) {
     typedef HeadLanes<E, VEC> L;
-    __shared__ double turn_lds[kTokenWaves][kPagedMaxDim];
-    const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
-    const int s = blockIdx.x / row_blocks, unit = (static_cast<int>(blockIdx.x) - s * row_blocks) * kTokenWaves + wid;
-    if (unit >= p.nq + 2 * nkv) return;
+    const int lane = threadIdx.x & (kWave - 1), hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
     const SeqRows sr = seq_rows(p.step, s);
-    if (sr.rows == 0) return;
+    if (sr.rows != 1) return;
     const int row = sr.row0;
     const bool is_q = unit < p.nq, is_k = !is_q && unit < p.nq + nkv;
     const int h = is_q ? unit : (is_k ? unit - p.nq : unit - p.nq - nkv);
@@ -553,7 +533,7 @@ __global__ void __launch_bounds__(kWave* kTokenWaves) paged_token_kernel(PagedPr
     const size_t sat = static_cast<size_t>(max(place.page, 0)) * nkv + h;
     float* scale = is_k ? p.kv.k_scale : p.kv.v_scale;
     if (I8 && !is_q && held && t) was = scale[sat];
-    if (is_q || is_k) turn_heads<1, E, VEC>(in, w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn_lds[wid]);
+    if (is_q || is_k) turn_heads<1, E, VEC>(in, w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn);
     if (is_q) {
         const size_t o = static_cast<size_t>(row) * p.out_stride + static_cast<size_t>(h) * hd;
 #pragma unroll
@@ -603,6 +583,38 @@ __global__ void __launch_bounds__(kWave* kTokenWaves) paged_token_kernel(PagedPr
     }
 }
 
+// Steps with longer sequences: blocks of pages, then waves of the sequences with one row, then of the others' query heads
+// (with its read-back a step of 59 tokens and 30 rows 22.5 us; the tokens by page and row too 28.6).
+template <int E, bool VEC, bool I8>
+__global__ void __launch_bounds__(kPagedThreads, 4) paged_prep_kernel(PagedPrepLaunch p, int hold_blocks, int token_blocks, int row_units, int per) {
+    extern __shared__ uint4 page_lds[];
+    _Float16* page_vals = reinterpret_cast<_Float16*>(page_lds);
+    __shared__ double turn[kPagedWaves][kPagedMaxDim];
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (static_cast<int>(blockIdx.x) < hold_blocks) {
+        hold_unit<E, VEC, I8>(p, blockIdx.x, page_vals, turn[wid]);
+        return;
+    }
+    if (static_cast<int>(blockIdx.x) < hold_blocks + token_blocks) {
+        const int heads = p.nq + 2 * p.kv.nkv, unit = (static_cast<int>(blockIdx.x) - hold_blocks) * kPagedWaves + wid, s = unit / heads;
+        if (s < p.step.seqs) token_unit<E, VEC, I8>(p, s, unit - s * heads, turn[wid]);
+        return;
+    }
+    const int unit = (static_cast<int>(blockIdx.x) - hold_blocks - token_blocks) * kPagedWaves + wid, row = unit / row_units;
+    if (row < p.step.rows) query_unit<E, VEC>(p, (unit - row * row_units) * per, per, row, turn[wid]);
+}
+
+// Steps of single tokens: no barrier between a block's waves (with their read-back 32 tokens 10.3 us, by page and row 16.1;
+// one token 7.8, 11.1).
+constexpr int kTokenWaves = 4;
+template <int E, bool VEC, bool I8>
+__global__ void __launch_bounds__(kWave* kTokenWaves) paged_token_kernel(PagedPrepLaunch p, int row_blocks) {
+    __shared__ double turn[kTokenWaves][kPagedMaxDim];
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int s = blockIdx.x / row_blocks, unit = (static_cast<int>(blockIdx.x) - s * row_blocks) * kTokenWaves + wid;
+    if (unit < p.nq + 2 * p.kv.nkv) token_unit<E, VEC, I8>(p, s, unit, turn[wid]);
+}
+
 hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
     const int hd = p.kv.head_dim, P = p.kv.page;
     const uintptr_t ptrs = reinterpret_cast<uintptr_t>(p.q_src) | reinterpret_cast<uintptr_t>(p.k_src) |
@@ -627,7 +639,8 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
     // pages of any division of the rows among the sequences: n rows reach over n / P page borders, and one more; one more
     // page than borders
     const int64_t hold = 2 * static_cast<int64_t>(p.kv.nkv) * (p.step.rows / P + 2 * std::min(p.step.seqs, p.step.rows));
-    const int64_t blocks = hold + (static_cast<int64_t>(row_units) * p.step.rows + kPagedWaves - 1) / kPagedWaves;
+    const int64_t tokens = (static_cast<int64_t>(p.step.seqs) * (p.nq + 2 * p.kv.nkv) + kPagedWaves - 1) / kPagedWaves;
+    const int64_t blocks = hold + tokens + (static_cast<int64_t>(row_units) * p.step.rows + kPagedWaves - 1) / kPagedWaves;
     if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
     const size_t lds = static_cast<size_t>(P) * (hd + 8) * 2;
     auto go = [&](auto kernel) {
@@ -635,7 +648,7 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
                                                static_cast<int>(lds));
             e != hipSuccess)
             return e;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPagedThreads), lds, s, p, static_cast<int>(hold), row_units, per);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPagedThreads), lds, s, p, static_cast<int>(hold), static_cast<int>(tokens), row_units, per);
         return hipGetLastError();
     };
     if (hd == 128 && al) return p.kv.i8 ? go(paged_prep_kernel<2, true, true>) : go(paged_prep_kernel<2, true, false>);
