@@ -22,8 +22,6 @@ namespace xqhip {
 // 128 with their read-back take 18.6 us, 509 rows of 16 / 4 heads of 256 into
 // 8-bit pages 15.5 us and 6.6 for the read-back; single tokens 3.7 to 4.5 us.
 // ---------------------------------------------------------------------------
-constexpr int kPagedWaves = 8;
-constexpr int kPagedThreads = kWave * kPagedWaves;
 constexpr int kPagedMaxDim = 256;
 constexpr int kPagedMaxPage = 128;
 
@@ -270,7 +268,7 @@ __device__ __forceinline__ int code_of(_Float16 x, float mx, float inv) {
 // A step's rows of one page, one kv head, k or v, as the page holds them, by a block (four rows' loads of a wave at a time):
 // those at [from, end) of the page with the first position `base`; to(t, held, v) takes row t.  before(): what is fetched
 // beside the first ones.
-template <int E, bool VEC, bool I8, typename Before, typename To>
+template <int W, int E, bool VEC, bool I8, typename Before, typename To>
 __device__ __forceinline__ void page_rows(const PagedPrepLaunch& p, const SeqRows& sr, int base, int from, int end, int h, bool is_k, double* turn, Before before,
                                           To to) {
     typedef HeadLanes<E, VEC> L;
@@ -282,30 +280,30 @@ __device__ __forceinline__ void page_rows(const PagedPrepLaunch& p, const SeqRow
     auto load = [&](int t0) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {  // (rows behind the last: the last again)
-            const int row = sr.row0 + base + min(t0 + b * kPagedWaves, end - 1) - sr.past;
+            const int row = sr.row0 + base + min(t0 + b * W, end - 1) - sr.past;
             L::load((is_k ? p.k_src : p.v_src) + static_cast<size_t>(row) * p.src_stride + static_cast<size_t>(h) * hd, lane, hd, x[b]);
-            axes[b].load(p.rot, p.step.rows, row, base + min(t0 + b * kPagedWaves, end - 1));
+            axes[b].load(p.rot, p.step.rows, row, base + min(t0 + b * W, end - 1));
         }
     };
     load(from + wid);
     if (is_k) L::load(p.k_norm, lane, hd, w);
     if (!before()) return;  // block-uniform
-    for (int t0 = from + wid; t0 < end; t0 += kBatch * kPagedWaves) {
+    for (int t0 = from + wid; t0 < end; t0 += kBatch * W) {
         float2 cs[kBatch][E];
         bool held[kBatch];
         float y[kBatch][E];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            held[b] = t0 + b * kPagedWaves < end && axes[b].fine;
+            held[b] = t0 + b * W < end && axes[b].fine;
             if (is_k) pairs.angles(p.rot, axes[b], cs[b]);
 #pragma unroll
             for (int e = 0; e < E; ++e) y[b][e] = x[b][e];
         }
-        if (t0 + kBatch * kPagedWaves < end) load(t0 + kBatch * kPagedWaves);  // (wave-uniform; they come while these are turned)
+        if (t0 + kBatch * W < end) load(t0 + kBatch * W);  // (wave-uniform; they come while these are turned)
         if (is_k) turn_heads<kBatch, E, VEC>(y, w, cs, hd, p.rot.pairs, p.inv_hd, p.eps, lane, turn);
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const int t = t0 + b * kPagedWaves;
+            const int t = t0 + b * W;
             if (t >= end) break;  // wave-uniform
             _Float16 v[E];
 #pragma unroll
@@ -334,11 +332,12 @@ __device__ __forceinline__ void put_row(const _Float16 (&v)[E], int lane, int hd
 // One page that the step touches, one kv head, k or v, by a block.  The new rows' fp16 values go to LDS, then to the page in
 // 16-byte pieces; 8 bits: their maximum is taken on the way, and where it rose, or the step leaves the page, the page's
 // earlier values are fetched and the codes of all of them written.  The last page's rows from keep_from on are kept.
-template <int E, bool VEC, bool I8>
+template <int W, int E, bool VEC, bool I8>
 __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int keep_from, int h, bool is_k, _Float16* vals, double* turn) {
     typedef HeadLanes<E, VEC> L;
     typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-    __shared__ float wave_mx[kPagedWaves];
+    constexpr int kThreads = kWave * W;
+    __shared__ float wave_mx[W];
     __shared__ uint8_t ok[kPagedMaxPage];
     const int lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int hd = p.kv.head_dim, nkv = p.kv.nkv, P = p.kv.page;
@@ -360,7 +359,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
         }
         return true;
     };
-    page_rows<E, VEC, I8>(p, sr, base, lead, end, h, is_k, turn, before, [&](int t, bool held, const _Float16(&v)[E]) {
+    page_rows<W, E, VEC, I8>(p, sr, base, lead, end, h, is_k, turn, before, [&](int t, bool held, const _Float16(&v)[E]) {
         if (lane == 0) ok[t] = held;
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -372,7 +371,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     int from = lead;
     float inv = 0.0f;
     auto earlier = [&] {  // the page's values before the step, in fp16
-        for (int i = threadIdx.x; i < lead * (hd / 8); i += kPagedThreads) {
+        for (int i = threadIdx.x; i < lead * (hd / 8); i += kThreads) {
             const int t = i / (hd / 8), b = i - t * (hd / 8);
             const half8 y = *reinterpret_cast<const half8*>(kept + static_cast<size_t>(t) * hd + 8 * b);
             *reinterpret_cast<half8*>(vals + t * ld + 8 * b) = y;
@@ -391,7 +390,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     __syncthreads();
     if constexpr (I8) {
 #pragma unroll
-        for (int i = 0; i < kPagedWaves; ++i) mx = fmaxf(mx, wave_mx[i]);
+        for (int i = 0; i < W; ++i) mx = fmaxf(mx, wave_mx[i]);
         const float before = static_cast<float>(static_cast<_Float16>(was * 127.0f));  // the maximum, an fp16 value, exactly
         const bool grew = mx > before;
         mx = grew ? mx : before;
@@ -428,7 +427,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     T* d = static_cast<T*>(is_k ? p.kv.k : p.kv.v) + page_head(p.kv, page, h);
     if (is_k) {  // lanes over positions, then blocks of dims
         const int n = end - from;
-        for (int i = threadIdx.x; i < n * (hd / N); i += kPagedThreads) {
+        for (int i = threadIdx.x; i < n * (hd / N); i += kThreads) {
             const int b = i / n, t = from + i - b * n;
             if (!writes(t)) continue;
             Piece o;
@@ -442,7 +441,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
         }
     } else {  // lanes over dims, then blocks of positions
         const int b0 = from / N, n = (end - 1) / N + 1 - b0;
-        for (int i = threadIdx.x; i < n * hd; i += kPagedThreads) {
+        for (int i = threadIdx.x; i < n * hd; i += kThreads) {
             const int b = b0 + i / hd, dim = i % hd, t0 = b * N;
             const uint32_t on = static_cast<uint32_t>((t0 < kWave ? go[0] >> t0 : go[1] >> (t0 - kWave)) & ((1u << N) - 1));
             T* at = d + (static_cast<size_t>(b) * hd + dim) * N;
@@ -467,7 +466,7 @@ __device__ __forceinline__ int hold_blocks_of(const PagedPrepLaunch& p, const Se
     if (r.rows <= 1 || r.past < 0 || r.past >= table_positions(p.step, p.kv)) return 0;
     return (r.past + r.rows - 1) / p.kv.page - r.past / p.kv.page + 1;
 }
-template <int E, bool VEC, bool I8>
+template <int W, int E, bool VEC, bool I8>
 __device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _Float16* vals, double* turn) {
     const bool is_k = (unit & 1) == 0;
     unit >>= 1;
@@ -486,7 +485,7 @@ __device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _F
     if (s < 0) return;  // fewer pages than blocks
     const SeqRows sr = seq_rows(p.step, s);
     const int P = p.kv.page, lead = sr.past % P, first = sr.past / P, last = (sr.past + sr.rows - 1) / P, index = first + nth - first_block;
-    hold_page<E, VEC, I8>(p, sr, s, index, index == first ? 0 : lead, h, is_k, vals, turn);
+    hold_page<W, E, VEC, I8>(p, sr, s, index, index == first ? 0 : lead, h, is_k, vals, turn);
     if constexpr (I8)
         if (index == first && first < last && lead) {
             __syncthreads();
@@ -497,7 +496,7 @@ __device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _F
                 kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(max(place.open, 0)) * p.kv.nkv + h) * P * hd;
                 return !place.none();
             };
-            page_rows<E, VEC, I8>(p, sr, last * P, 0, end, h, is_k, turn, before, [&](int t, bool held, const _Float16(&v)[E]) {
+            page_rows<W, E, VEC, I8>(p, sr, last * P, 0, end, h, is_k, turn, before, [&](int t, bool held, const _Float16(&v)[E]) {
                 if (held) put_row<E, VEC>(v, lane, hd, kept + static_cast<size_t>(t) * hd);
             });
         }
@@ -585,22 +584,22 @@ __device__ __forceinline__ void token_unit(const PagedPrepLaunch& p, int s, int 
 
 // Steps with longer sequences: blocks of pages, then waves of the sequences with one row, then of the others' query heads
 // (with its read-back a step of 59 tokens and 30 rows 22.5 us; the tokens by page and row too 28.6).
-template <int E, bool VEC, bool I8>
-__global__ void __launch_bounds__(kPagedThreads, 4) paged_prep_kernel(PagedPrepLaunch p, int hold_blocks, int token_blocks, int row_units, int per) {
+template <int W, int E, bool VEC, bool I8>
+__global__ void __launch_bounds__(kWave* W, 4) paged_prep_kernel(PagedPrepLaunch p, int hold_blocks, int token_blocks, int row_units, int per) {
     extern __shared__ uint4 page_lds[];
     _Float16* page_vals = reinterpret_cast<_Float16*>(page_lds);
-    __shared__ double turn[kPagedWaves][kPagedMaxDim];
+    __shared__ double turn[W][kPagedMaxDim];
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (static_cast<int>(blockIdx.x) < hold_blocks) {
-        hold_unit<E, VEC, I8>(p, blockIdx.x, page_vals, turn[wid]);
+        hold_unit<W, E, VEC, I8>(p, blockIdx.x, page_vals, turn[wid]);
         return;
     }
     if (static_cast<int>(blockIdx.x) < hold_blocks + token_blocks) {
-        const int heads = p.nq + 2 * p.kv.nkv, unit = (static_cast<int>(blockIdx.x) - hold_blocks) * kPagedWaves + wid, s = unit / heads;
+        const int heads = p.nq + 2 * p.kv.nkv, unit = (static_cast<int>(blockIdx.x) - hold_blocks) * W + wid, s = unit / heads;
         if (s < p.step.seqs) token_unit<E, VEC, I8>(p, s, unit - s * heads, turn[wid]);
         return;
     }
-    const int unit = (static_cast<int>(blockIdx.x) - hold_blocks - token_blocks) * kPagedWaves + wid, row = unit / row_units;
+    const int unit = (static_cast<int>(blockIdx.x) - hold_blocks - token_blocks) * W + wid, row = unit / row_units;
     if (row < p.step.rows) query_unit<E, VEC>(p, (unit - row * row_units) * per, per, row, turn[wid]);
 }
 
@@ -639,8 +638,13 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
     // pages of any division of the rows among the sequences: n rows reach over n / P page borders, and one more; one more
     // page than borders
     const int64_t hold = 2 * static_cast<int64_t>(p.kv.nkv) * (p.step.rows / P + 2 * std::min(p.step.seqs, p.step.rows));
-    const int64_t tokens = (static_cast<int64_t>(p.step.seqs) * (p.nq + 2 * p.kv.nkv) + kPagedWaves - 1) / kPagedWaves;
-    const int64_t blocks = hold + tokens + (static_cast<int64_t>(row_units) * p.step.rows + kPagedWaves - 1) / kPagedWaves;
+    // Waves of a block: eight; sixteen where pages take many passes of eight and there are few of them (with the read-back: 500
+    // rows, fp16 pages of 128, heads of 128 20.5 us, by eight waves 25.4; 139 rows in 8 bits, heads of 256 31.9, 35.6; four
+    // chunks of 512 49.1, 44.2).
+    const bool long_pages = std::min(P, p.step.max_rows) * (hd > 128 ? 2 : 1) >= 128, few = 2 * p.kv.nkv * p.step.rows <= 128 * P;
+    const int waves = long_pages && few ? 16 : 8;
+    const int64_t tokens = (static_cast<int64_t>(p.step.seqs) * (p.nq + 2 * p.kv.nkv) + waves - 1) / waves;
+    const int64_t blocks = hold + tokens + (static_cast<int64_t>(row_units) * p.step.rows + waves - 1) / waves;
     if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
     const size_t lds = static_cast<size_t>(P) * (hd + 8) * 2;
     auto go = [&](auto kernel) {
@@ -648,13 +652,16 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
                                                static_cast<int>(lds));
             e != hipSuccess)
             return e;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPagedThreads), lds, s, p, static_cast<int>(hold), static_cast<int>(tokens), row_units, per);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kWave * waves), lds, s, p, static_cast<int>(hold), static_cast<int>(tokens), row_units, per);
         return hipGetLastError();
     };
-    if (hd == 128 && al) return p.kv.i8 ? go(paged_prep_kernel<2, true, true>) : go(paged_prep_kernel<2, true, false>);
-    if (hd == 256 && al) return p.kv.i8 ? go(paged_prep_kernel<4, true, true>) : go(paged_prep_kernel<4, true, false>);
-    constexpr int E = kPagedMaxDim / kWave;
-    return p.kv.i8 ? go(paged_prep_kernel<E, false, true>) : go(paged_prep_kernel<E, false, false>);
+    auto by_waves = [&](auto w) {
+        constexpr int W = decltype(w)::value, E = kPagedMaxDim / kWave;
+        if (hd == 128 && al) return p.kv.i8 ? go(paged_prep_kernel<W, 2, true, true>) : go(paged_prep_kernel<W, 2, true, false>);
+        if (hd == 256 && al) return p.kv.i8 ? go(paged_prep_kernel<W, 4, true, true>) : go(paged_prep_kernel<W, 4, true, false>);
+        return p.kv.i8 ? go(paged_prep_kernel<W, E, false, true>) : go(paged_prep_kernel<W, E, false, false>);
+    };
+    return waves == 16 ? by_waves(std::integral_constant<int, 16>{}) : by_waves(std::integral_constant<int, 8>{});
 }
 
 // ---------------------------------------------------------------------------
