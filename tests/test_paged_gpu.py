@@ -218,6 +218,9 @@ SHAPES = [
     (5, 5, 48, 48, None, False, 32, [3, 0, 0], [100, 0, 32], 0, 3, 5),
     (2, 1, 16, 0, None, False, 32, [30], [3], 1, 0, 0),
     (4, 1, 112, 2, None, False, 128, [100] * 70, [1] * 70, 1, 0, 0),
+    (16, 4, 256, 64, [12, 10, 10], True, 128, [23, 0, 200], [139, 70, 1], 1, 0, 2), (16, 4, 256, 64, None, False, 64, [63, 0], [200, 1], 1, 1, 0),
+    (8, 2, 128, 32, None, False, 128, [100, 7], [400, 130], 1, 4, 1), (6, 2, 80, 20, [4, 2, 2, 2], True, 128, [127], [140], 0, 0, 0),
+    (8, 2, 128, 32, None, False, 64, [5] * 9, [1, 30, 1, 0, 1, 2, 1, 64, 1], 1, 0, 4),
 ]
 
 
