@@ -515,10 +515,10 @@ __global__ void __launch_bounds__(WAVES* kWave) paged_plan_kernel(PagedAttnLaunc
         const int seen = r.past < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(r.past) + min((tile + 1) * T, r.rows), static_cast<int64_t>(cap)));
         return max(0, seen - 1) / chunk + 1;
     };
-    // Splits: whole rounds of blocks take whole tiles; the others, no more than half a round, are split to the shortest length
-    // with which their units fit one (two chunks of 600 rows after 1500, heads of 256, 8 bits, 127 us, by whole tiles 159;
-    // more than half a round: 900 rows after 500 60 instead of 57).
-    const int rest = tiles < room ? tiles : 2 * (tiles % room) <= room ? tiles % room : 0;
+    // Splits: whole rounds of blocks take whole tiles; the others, no more than three eighths of a round, are split to the
+    // shortest length with which their units fit one (two chunks of 600 rows after 1500, heads of 256, 8 bits, 128 us, by whole
+    // tiles 159; with half a round the three chunks above 156 instead of 148, with more 900 rows after 500 60 instead of 57).
+    const int rest = tiles < room ? tiles : 8 * (tiles % room) <= 3 * room ? tiles % room : 0;
     constexpr int kHeld = kWideBlocks / kWave;
     if (wid == 0) {
         int per = 1 << 20;  // (no tile has so many chunks)
