@@ -1,0 +1,214 @@
+"""The kernels over paged caches run on the host (host_kernels): their own sources under AddressSanitizer, every buffer of
+exactly the size that the interface asks for, workspaces and outputs full of 0xA5.  So what an index reaches is shown without a
+GPU; the results are compared with the 64-bit ones as on the GPU (the same bounds, test_paged_gpu)."""
+import os
+
+import numpy as np
+import pytest
+
+import host_kernels as hk
+import paged_oracle as po
+import test_paged_gpu as gpu
+import xqbind as xb
+
+pytestmark = pytest.mark.skipif(not os.path.exists(hk.CLANG), reason="the compiler for the host is not there")
+F16, I8 = xb.PAGES_F16, xb.PAGES_I8
+ORDERS = [1, -1]  # of the blocks
+
+
+class Plan(gpu.Plan):
+    def upload(self):
+        pass
+
+    def step(self, run):
+        open_ = run.buf(np.array(self.open, np.int32))
+        run.call("step", len(self.past), self.total, self.max_rows, self.most, run.buf(np.array(self.row0, np.int32)),
+                 run.buf(np.array(self.past, np.int32)), run.buf(self.table), open_)
+
+
+class Pool:
+    """gpu.Pool's arrays, in a run's buffers."""
+
+    def __init__(self, kind, nkv, hd, page, pages, opens=1, k=None, v=None):
+        self.kind, self.nkv, self.hd, self.page, self.pages, self.opens = kind, nkv, hd, page, pages, opens
+        self.e = 16 if kind == I8 else 8
+        self.x = [np.full((pages, nkv, page, hd), 99 if kind == I8 else np.nan, np.int8 if kind == I8 else np.float16) for _ in range(2)]
+        self.scale = np.full((2, pages, nkv), np.nan, np.float32)
+        self.open = np.full((2, opens, nkv, page, hd), np.nan, np.float16)
+        for i, given in enumerate((k, v)):
+            if given is None:
+                continue
+            if kind == F16:
+                self.x[i][:] = given
+                continue
+            for p in range(pages):
+                for h in range(nkv):
+                    on = ~np.isnan(given[p, h].astype(np.float32)).any(-1)
+                    if on.any():
+                        self.x[i][p, h, on], self.scale[i, p, h] = po.codes(given[p, h][on])
+
+    def raw(self):
+        return [a.copy() for a in (*self.x, *self.scale, *self.open)]
+
+    def pages_of(self, run):
+        self.names = [run.buf(po.to_pages_k(self.x[0], self.e)), run.buf(po.to_pages_v(self.x[1], self.e))]
+        extra = [run.buf(a) for a in (*self.scale, *self.open)] if self.kind == I8 else [hk.NONE] * 4
+        self.names += extra
+        run.call("pages", self.kind, self.nkv, self.hd, self.page, self.pages, self.opens, *self.names)
+
+    def save(self, run):
+        t = self.x[0].dtype
+        run.save(self.names[0], t, (self.pages, self.nkv, self.hd // self.e, self.page, self.e))
+        run.save(self.names[1], t, (self.pages, self.nkv, self.page // self.e, self.hd, self.e))
+        if self.kind == I8:
+            for n, a in zip(self.names[2:], (*self.scale, *self.open)):
+                run.save(n, a.dtype, a.shape)
+
+    def take(self, saved):
+        """What the run left."""
+        self.x = [po.from_pages_k(saved[0]), po.from_pages_v(saved[1])]
+        if self.kind == I8:
+            self.scale, self.open = np.stack(saved[2:4]), np.stack(saved[4:6])
+
+    def values(self):
+        if self.kind == F16:
+            return [x.astype(np.float64) for x in self.x]
+        return [x * s[..., None, None].astype(np.float64) for x, s in zip(self.x, self.scale)]
+
+
+def rope(pairs, cap):
+    ang = np.arange(cap)[:, None] * 1e4 ** (-np.arange(pairs) / max(1, pairs))
+    return np.stack([np.cos(ang), np.sin(ang)], -1).astype(np.float32)
+
+
+def prep(tmp, rng, pool, plan, nq, rotary, sections=None, inter=False, axes=None, gated=1, pad=0, x=None, norms=None, cap=None, order=1):
+    """gpu.prep on the host: (projections, q, gate, norms, cos/sin of every row); the pool as it is then."""
+    nkv, hd, T = pool.nkv, pool.hd, plan.total
+    row = nq * hd * (2 if gated else 1) + 2 * nkv * hd + pad
+    x = rng.normal(0, 1, (T, row)).astype(np.float32) if x is None else x
+    qn, kn = norms or (rng.normal(1, 0.1, hd).astype(np.float32) for _ in range(2))
+    cap = cap or max(p + m for p, m in zip(plan.past, plan.rows)) + 1
+    run = hk.Run(tmp)
+    run.call("order", order)
+    pool.pages_of(run)
+    plan.step(run)
+    cs, angles = rope(rotary // 2, cap), np.zeros((T, rotary // 2, 2), np.float32)
+    if rotary:
+        sections = sections or [rotary // 2]
+        run.call("rotary", run.buf(cs), cap, rotary, len(sections), int(inter), run.buf(axes) if axes is not None else hk.NONE, *sections)
+        of = np.array(list(xb.rotary(1 << 20, cap, rotary, sections, inter).axis)[:rotary // 2])
+        for s, j, i, p in plan.each():
+            at = axes[of, i] if axes is not None else np.full(rotary // 2, p)
+            ok = (at >= 0) & (at < cap)
+            angles[i] = np.where(ok[:, None], cs[np.where(ok, at, 0), np.arange(rotary // 2)], np.nan)
+    q, g = run.buf(np.full((T, nq * hd), 7, np.float32)), run.buf(np.full((T, nq * hd), 7, np.float32))
+    run.call("prep", gated, nq, gpu.EPS, row, nq * hd, run.buf(x), run.buf(qn), run.buf(kn), q, g if gated else hk.NONE)
+    run.save(q, np.float32, (T, nq, hd))
+    run.save(g, np.float32, (T, nq, hd))
+    pool.save(run)
+    got = run.result()
+    pool.take(got[2:])
+    return x, got[0], got[1], (qn, kn), angles
+
+
+def attention(tmp, pool, plan, nq, q, gate, order=1, out_rows=None):
+    run = hk.Run(tmp)
+    run.call("order", order)
+    pool.pages_of(run)
+    plan.step(run)
+    out = run.buf(np.full((out_rows or plan.total, nq * pool.hd), 7, np.float32))
+    run.call("attention", nq, nq * pool.hd, nq * pool.hd, run.buf(q), run.buf(gate) if gate is not None else hk.NONE, out)
+    run.save(out, np.float32, (out_rows or plan.total, nq, pool.hd))
+    return run.result()[0]
+
+
+def filled(rng, kind, nkv, hd, page, plan):
+    k, v = (np.full((plan.pages, nkv, page, hd), np.nan, np.float16) for _ in range(2))
+    for s, (p, m) in enumerate(zip(plan.past, plan.rows)):
+        for i in range((p + m + page - 1) // page):
+            n = min(page, p + m - i * page)
+            for x in (k, v):
+                x[plan.table[s, i], :, :n] = rng.normal(0, 1, (nkv, n, hd)) * rng.uniform(0.2, 1.0)
+    return Pool(kind, nkv, hd, page, plan.pages, 1, k, v)
+
+
+# rows, splits and joins of every kind: the planned steps with 64 and 128 columns, several units of a row tile, query heads
+# that do not divide a block's columns; single tokens over many blocks and within one
+ATTEND = [a for a in gpu.ATTEND if max(a[4]) < 1000] + [
+    (16, 4, 256, 64, [33], [64]), (16, 4, 256, 64, [33], [66]), (16, 4, 256, 32, [0], [65]), (16, 4, 256, 128, [200, 33], [33, 65]),
+    (8, 8, 128, 32, [5] * 70, [3] * 70), (32, 2, 256, 64, [40, 500, 9], [17, 2, 30]), (256, 256, 128, 32, [20], [12]),
+    (16, 16, 256, 32, [20, 3], [70, 9]), (8, 2, 128, 32, [700], [70]), (4, 1, 256, 32, [700], [70]), (2, 2, 128, 64, [130] * 3, [150] * 3)]
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+@pytest.mark.parametrize("shape", ATTEND, ids=[f"{a[0]}_{a[1]}x{a[2]}_{a[3]}_{a[4][0]}_{a[5][0]}_{len(a[4])}" for a in ATTEND])
+def test_attention_stays_in_its_buffers(tmp_path, kind, shape):
+    nq, nkv, hd, page, past, rows = shape
+    rng = np.random.default_rng(nq + hd + page + sum(past))
+    plan = Plan(rng, page, past, rows, pad=2)
+    pool = filled(rng, kind, nkv, hd, page, plan)
+    q, gate = (rng.normal(0, 1, (plan.total, nq * hd)).astype(np.float32) for _ in range(2))
+    some = set(rng.permutation(plan.n)[:40])
+    for order in ORDERS[kind != I8:]:
+        got = attention(tmp_path, pool, plan, nq, q, gate, order)
+        gpu.check(got, gpu.attend_oracle(pool, plan, nq, q, gate, rows=some))
+        assert (got[plan.n:] == 7).all() and not (got[:plan.n] == 7).all(-1).any()
+
+
+@pytest.mark.parametrize("rows,hd", [([1, 1], 128), ([65], 256), ([3], 64)])
+def test_a_row_past_the_buffer_is_seen(tmp_path, rows, hd):
+    """An output buffer one row short: the run ends there, for each of the forms."""
+    rng = np.random.default_rng(1)
+    plan = Plan(rng, 64, [33] * len(rows), rows)
+    pool = filled(rng, F16, 4, hd, 64, plan)
+    q = rng.normal(0, 1, (plan.total, 16 * hd)).astype(np.float32)
+    with pytest.raises(AssertionError, match="heap-buffer-overflow"):
+        attention(tmp_path, pool, plan, 16, q, None, out_rows=plan.total - 1)
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+@pytest.mark.parametrize("shape", gpu.SHAPES, ids=[f"{s[0]}_{s[1]}x{s[2]}_{s[6]}_{s[7][0]}_{s[8][0]}" for s in gpu.SHAPES])
+def test_prep_stays_in_its_buffers(tmp_path, kind, shape):
+    nq, nkv, hd, rotary, sections, inter, page, past, rows, gated, pad, behind = shape
+    rng = np.random.default_rng(hd + page + len(past))
+    plan = Plan(rng, page, past, rows, pad=behind)
+    pool = Pool(kind, nkv, hd, page, plan.pages, len(past))
+    if kind == I8:
+        before = Plan(rng, page, [p // page * page for p in past], [p % page for p in past])
+        if before.n:
+            before.table, before.most, before.open = plan.table, plan.most, plan.open
+            prep(tmp_path, rng, pool, before, nq, rotary, gated=gated, cap=4000)
+    cap = max(past) + max(rows) + 40
+    axes = rng.integers(0, cap, (len(sections), plan.total)).astype(np.int32) if sections else None
+    was = pool.raw()
+    x, norms = None, [rng.normal(1, 0.1, hd).astype(np.float32) for _ in range(2)]
+    for order in ORDERS[kind != I8:]:
+        pool.x, pool.scale, pool.open = was[:2], np.stack(was[2:4]), np.stack(was[4:])
+        x, q, g, (qn, kn), cs = prep(tmp_path, rng, pool, plan, nq, rotary, sections, inter, axes, gated, pad, x=x, norms=norms, cap=cap, order=order)
+        qx, gx, kx, vx = gpu.split_heads(x, nq, nkv, hd, gated)
+        want, live = po.prepared(qx, qn, cs[:, None], gpu.EPS), plan.n
+        assert (np.abs(q[:live] - want[:live]) <= 2**-23 * np.abs(want[:live])).all()
+        assert (q[live:] == 7).all() and (g[live:] == 7).all()
+        assert gpu.same(pool.raw(), gpu.appended(was, plan, kind, po.prepared(kx, kn, cs[:, None], gpu.EPS), vx))
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+@pytest.mark.parametrize("out", [np.float32, np.float16])
+@pytest.mark.parametrize("hd,page,past,rows", [(128, 64, [0, 63, 100], [1, 70, 0]), (48, 32, [17], [50]), (256, 128, [1], [300])])
+def test_read_stays_in_its_buffers(tmp_path, kind, out, hd, page, past, rows):
+    rng = np.random.default_rng(hd)
+    plan = Plan(rng, page, past, rows)
+    pool = filled(rng, kind, 3, hd, page, plan)
+    run = hk.Run(tmp_path)
+    pool.pages_of(run)
+    plan.step(run)
+    shape = (plan.n, 3, hd)
+    k, v = (run.buf(np.full(shape, 7, out)) for _ in range(2))
+    run.call("read", xb.F32 if out == np.float32 else xb.F16, k, v)
+    run.save(k, out, shape)
+    run.save(v, out, shape)
+    for got, values in zip(run.result(), pool.values()):
+        values = values.astype(np.float32) if kind == I8 else values  # (codes times their scale: one fp32 product)
+        for s, j, i, p in plan.each():
+            want = values[plan.table[s, p // page], :, p % page].astype(np.float32).astype(out)
+            assert np.array_equal(got[i], want)
