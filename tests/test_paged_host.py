@@ -212,3 +212,67 @@ def test_read_stays_in_its_buffers(tmp_path, kind, out, hd, page, past, rows):
         for s, j, i, p in plan.each():
             want = values[plan.table[s, p // page], :, p % page].astype(np.float32).astype(out)
             assert np.array_equal(got[i], want)
+
+
+# ---- rows of an 8-bit page that are not held --------------------------------------
+def steps_with_holes(tmp, rng, pool, whole, sizes, bad, nq=2, on=None):
+    """Appends whole's rows to `pool` in steps of the given sizes; rows in `bad` have rotary positions outside the table.  The
+    rows' keys and values [rows][nkv][hd] as an 8-bit page takes them."""
+    n, cap = sum(sizes), 500
+    x = (rng.normal(0, 1, (n, 2 * nq * pool.hd + 2 * pool.nkv * pool.hd)) * rng.uniform(0.1, 3, (n, 1))).astype(np.float32)
+    norms, done, keys = [rng.normal(1, 0.1, pool.hd).astype(np.float32) for _ in range(2)], 0, []
+    for m in sizes:
+        plan = (on.Plan if on else Plan)(rng, pool.page, [whole.past[0] + done], [m])
+        plan.table, plan.most, plan.open = whole.table, whole.most, whole.open
+        plan.upload()
+        axes = (plan.past[0] + np.arange(m, dtype=np.int32))[None].copy()
+        for i, r in enumerate(range(done, done + m)):
+            if r in bad:
+                axes[0, i] = [-1, cap][r % 2]
+        call = on.prep if on else lambda *a, **o: prep(tmp, *a, **o)
+        _, q, _, (_, kn), cs = call(rng, pool, plan, nq, 32, axes=axes, x=x[done: done + m], norms=norms, cap=cap)
+        _, _, kx, vx = gpu.split_heads(x[done: done + m], nq, pool.nkv, pool.hd, 1)
+        assert (np.isnan(q).all((1, 2)) == [r in bad for r in range(done, done + m)]).all()
+        keys.append((po.held(po.prepared(kx, kn, cs[:, None], gpu.EPS)), po.held(vx)))
+        done += m
+    return [np.concatenate(z) for z in zip(*keys)]
+
+
+def check_holes(pool, was, whole, values, bad):
+    """Codes of the rows that are held, each page's scale: the largest of its held rows, and what the page's scale said before
+    where its first position was not written."""
+    now = pool.raw()
+    for i, x in enumerate(values):
+        for at in range(whole.past[0] // pool.page, (whole.past[0] + len(x) - 1) // pool.page + 1):
+            pg = whole.table[0, at]
+            rows = [r for r in range(len(x)) if (whole.past[0] + r) // pool.page == at and r not in bad]
+            offs = [(whole.past[0] + r) % pool.page for r in rows]
+            for h in range(pool.nkv):
+                if not rows:
+                    assert np.array_equal(now[i][pg, h], was[i][pg, h]) and now[2 + i][pg, h] == was[2 + i][pg, h]
+                    continue
+                mx = np.abs(x[rows][:, h].astype(np.float64)).max()
+                if 0 not in offs:
+                    mx = max(mx, float(np.float16(was[2 + i][pg, h] * np.float32(127))))
+                assert now[2 + i][pg, h] == np.float32(mx / 127), (i, at, h)
+                assert np.array_equal(now[i][pg, h, offs], np.rint(x[rows][:, h].astype(np.float64) * 127 / mx)), (i, at, h)
+
+
+HOLES = [  # positions before, rows of the steps, rows without a rotary position
+    (0, [20], set(range(20))),                                 # a chunk over a page that holds codes: all as it was
+    (32, [40], set(range(40))), (0, [1], {0}),                 # over two pages; one row
+    (0, [10, 30], {4}), (0, [1] * 10 + [40], {4, 5, 9}),       # a hole, then a step that leaves the page
+    (0, [6, 6, 6], {2, 7, 8}), (0, [10, 1, 1, 25, 1], {3, 11}), (0, [3, 70], {1, 33, 34}),
+    (0, [12], {0}), (0, [1] * 12, {0}), (0, [3, 40], {0, 1, 2}), (0, [1, 1, 1, 40], {0, 1, 32})]  # the page's first position
+
+
+@pytest.mark.parametrize("stale,old", [(6e4, 0.5), (np.inf, 30), (np.nan, 0.5)])
+@pytest.mark.parametrize("past,sizes,bad", HOLES, ids=[f"{p}_{'_'.join(map(str, s))}_{len(b)}" for p, s, b in HOLES])
+def test_rows_that_are_not_held_do_not_count(tmp_path, past, sizes, bad, stale, old):
+    """Open pages hold what a sequence before left there, pages values of another size."""
+    rng = np.random.default_rng(len(bad) + past)
+    whole = Plan(rng, 32, [past], [sum(sizes)])
+    pool = Pool(I8, 2, 128, 32, whole.pages, 1, *(rng.normal(0, old, (2, whole.pages, 2, 32, 128)).astype(np.float16)))
+    pool.open[:] = stale
+    was = pool.raw()
+    check_holes(pool, was, whole, steps_with_holes(tmp_path, rng, pool, whole, sizes, bad), bad)

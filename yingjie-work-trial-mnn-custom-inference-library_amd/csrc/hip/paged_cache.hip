@@ -329,9 +329,16 @@ __device__ __forceinline__ void put_row(const _Float16 (&v)[E], int lane, int hd
     }
 }
 
+// The largest magnitude that a page's scale stands for: an fp16 value, exactly.  (A page that no row began may have any scale.)
+__device__ __forceinline__ float recorded_max(float scale) {
+    return static_cast<float>(static_cast<_Float16>(fminf(fmaxf(scale * 127.0f, 0.0f), 65504.0f)));
+}
+
 // One page that the step touches, one kv head, k or v, by a block.  The new rows' fp16 values go to LDS, then to the page in
 // 16-byte pieces; 8 bits: their maximum is taken on the way, and where it rose, or the step leaves the page, the page's
-// earlier values are fetched and the codes of all of them written.  The last page's rows from keep_from on are kept.
+// earlier values are fetched and the codes of all of them written.  The earlier values' maximum is the recorded one: where a
+// row was not held, the open page has what another sequence left.  A page of which no row is held stays as it is, and only a
+// row that is held at its first position begins it anew.  The last page's rows from keep_from on are kept.
 template <int W, int E, bool VEC, bool I8>
 __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int keep_from, int h, bool is_k, _Float16* vals, double* turn) {
     typedef HeadLanes<E, VEC> L;
@@ -355,7 +362,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
         sat = static_cast<size_t>(page) * nkv + h;
         if constexpr (I8) {
             kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(place.open) * nkv + h) * P * hd;
-            was = lead ? (is_k ? p.kv.k_scale : p.kv.v_scale)[sat] : 0.0f;
+            was = (is_k ? p.kv.k_scale : p.kv.v_scale)[sat];
         }
         return true;
     };
@@ -373,10 +380,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     auto earlier = [&] {  // the page's values before the step, in fp16
         for (int i = threadIdx.x; i < lead * (hd / 8); i += kThreads) {
             const int t = i / (hd / 8), b = i - t * (hd / 8);
-            const half8 y = *reinterpret_cast<const half8*>(kept + static_cast<size_t>(t) * hd + 8 * b);
-            *reinterpret_cast<half8*>(vals + t * ld + 8 * b) = y;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(static_cast<float>(y[e])));
+            *reinterpret_cast<half8*>(vals + t * ld + 8 * b) = *reinterpret_cast<const half8*>(kept + static_cast<size_t>(t) * hd + 8 * b);
         }
     };
     if constexpr (I8) {
@@ -388,17 +392,22 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
         if (lane == 0) wave_mx[wid] = mx;
     }
     __syncthreads();
+    uint64_t on[2];  // new positions that are held
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = i * kWave + lane;
+        on[i] = __builtin_amdgcn_ballot_w64(t >= lead && t < end && ok[t] != 0);
+    }
+    if ((on[0] | on[1]) == 0) return;  // block-uniform
     if constexpr (I8) {
 #pragma unroll
         for (int i = 0; i < W; ++i) mx = fmaxf(mx, wave_mx[i]);
-        const float before = static_cast<float>(static_cast<_Float16>(was * 127.0f));  // the maximum, an fp16 value, exactly
+        const float before = on[0] & 1 ? 0.0f : recorded_max(was);
         const bool grew = mx > before;
         mx = grew ? mx : before;
         inv = mx > 0.0f ? 1.0f / mx : 0.0f;
         if (grew && lead && last) {
-            const float all = mx;
             earlier();
-            mx = all;
             from = 0;
             __syncthreads();
         }
@@ -409,7 +418,7 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int t = i * kWave + lane;
-        go[i] = __builtin_amdgcn_ballot_w64(t >= from && t < end && (t < lead || ok[t] != 0));
+        go[i] = on[i] | __builtin_amdgcn_ballot_w64(t >= from && t < lead);
     }
     auto writes = [&](int t) { return (t < kWave ? go[0] >> t : go[1] >> (t - kWave)) & 1; };
     constexpr int N = I8 ? 16 : 8;  // values of a piece
@@ -563,7 +572,7 @@ __device__ __forceinline__ void token_unit(const PagedPrepLaunch& p, int s, int 
             kept[static_cast<size_t>(t) * hd + L::dim(lane, e)] = v[e];
         }
         mx = wave_max(mx);
-        const float before = static_cast<float>(static_cast<_Float16>(was * 127.0f));  // the maximum, an fp16 value, exactly
+        const float before = recorded_max(was);
         const bool grew = mx > before;
         mx = grew ? mx : before;
         const float inv = mx > 0.0f ? 1.0f / mx : 0.0f;
