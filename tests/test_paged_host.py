@@ -276,3 +276,23 @@ def test_rows_that_are_not_held_do_not_count(tmp_path, past, sizes, bad, stale, 
     pool.open[:] = stale
     was = pool.raw()
     check_holes(pool, was, whole, steps_with_holes(tmp_path, rng, pool, whole, sizes, bad), bad)
+
+
+@pytest.mark.parametrize("hd,seqs,rows", [(256, 1024, 512), (128, 1024, 1024), (256, 60, 40)])
+def test_rows_in_no_order_stay_in_the_workspace(tmp_path, hd, seqs, rows):
+    """Every second sequence claims every row (row0 falls): some 65536 row tiles where a step of so many rows has 896 at most.
+    What all sequences agree on comes out."""
+    rng = np.random.default_rng(hd)
+    plan = Plan(rng, 32, [0], [rows])
+    pool = Pool(F16, 1, hd, 32, 3, 1, *rng.normal(0, 1, (2, 3, 1, 32, hd)).astype(np.float16))
+    plan.table, plan.most, plan.pages, plan.open = np.full((seqs, 1), 1, np.int32), 1, 3, np.zeros(seqs, np.int32)
+    run = hk.Run(tmp_path)
+    pool.pages_of(run)
+    run.call("step", seqs, rows, rows, 1, run.buf(np.array([[0, rows][i % 2] for i in range(seqs + 1)], np.int32)),
+             run.buf(np.zeros(seqs, np.int32)), run.buf(plan.table), hk.NONE)
+    q = rng.normal(0, 1, (rows, 16 * hd)).astype(np.float32)
+    out = run.buf(np.full((rows, 16 * hd), 7, np.float32))
+    run.call("attention", 16, 16 * hd, 16 * hd, run.buf(q), hk.NONE, out)
+    run.save(out, np.float32, (rows, 16, hd))
+    some = set(rng.permutation(rows)[:40])
+    gpu.check(run.result()[0], gpu.attend_oracle(pool, plan, 16, q, None, rows=some))

@@ -498,6 +498,9 @@ __global__ void __launch_bounds__(WAVES* kWave) paged_plan_kernel(PagedAttnLaunc
         before = before128;
     }
     const int own = cols == kMostCols ? n128 : n64, T = cols == kMostCols ? ws.most_rows : ws.least_rows, chunk = kBlockWaves<HD> * kTTile * kTTile / cols;
+    // any division of the rows has no more; sequences that claim the same rows (row0 falls) have as many, and units and slots
+    // stay within the workspace
+    tiles = min(tiles, p.step.rows / T + min(seqs, p.step.rows));
     pre[s] = before + wave_scan_int(own) - own;
     __syncthreads();
     auto tile_at = [&](int f, int& q, int& tile) {  // chunks of row tile f
