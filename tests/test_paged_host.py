@@ -296,3 +296,35 @@ def test_rows_in_no_order_stay_in_the_workspace(tmp_path, hd, seqs, rows):
     run.save(out, np.float32, (rows, 16, hd))
     some = set(rng.permutation(rows)[:40])
     gpu.check(run.result()[0], gpu.attend_oracle(pool, plan, 16, q, None, rows=some))
+
+
+BIG, LOW = 2**31 - 1, -2**31
+
+
+@pytest.mark.parametrize("kind,hd", [(F16, 64), (I8, 128), (F16, 256)])
+@pytest.mark.parametrize("max_rows", [1, 100])
+@pytest.mark.parametrize("row0,past", [([0, 100] * 20, 5), ([100, 0, 50, -7, 200, 3, 3, 2], 5), ([BIG, LOW, 60, 0, 99], 5),
+                                       ([LOW, BIG, 0, LOW, BIG], 31), ([0, 3, 4, 40, 100], BIG), ([0, 3, 4, 40, 100], BIG - 50),
+                                       ([0, 3, 4, 40, 100], LOW), ([0, 3, 4, 40, 100], 2**20 - 20)])
+def test_numbers_of_any_size(tmp_path, kind, hd, max_rows, row0, past):
+    """Rows of several sequences or of none, numbers outside the step, pages and open pages that are none: nothing outside the
+    buffers."""
+    rng = np.random.default_rng(9)
+    seqs, rows = len(row0) - 1, 100
+    plan = Plan(rng, 32, [5] * seqs, [rows] * seqs)
+    plan.row0, plan.total, plan.max_rows, plan.past = row0, rows, max_rows, [past] * seqs
+    plan.table[0, 0], plan.table[1, 1], plan.table[2, 0] = BIG, LOW, plan.pages
+    pool = Pool(kind, 2, hd, 32, plan.pages, seqs, *rng.normal(0, 1, (2, plan.pages, 2, 32, hd)).astype(np.float16))
+    plan.open = np.array([BIG, LOW] + list(range(seqs - 2)), np.int64).astype(np.int32)
+    x = rng.normal(0, 1, (rows, 8 * hd)).astype(np.float32)
+    run = hk.Run(tmp_path)
+    pool.pages_of(run)
+    plan.step(run)
+    ones, q = run.buf(np.ones(hd, np.float32)), run.buf(np.full((rows, 4 * hd), 7, np.float32))
+    axes = rng.choice([0, 3, 39, 40, BIG, LOW, -1], (2, rows)).astype(np.int32)
+    run.call("rotary", run.buf(rope(8, 40)), 40, 16, 2, 1, run.buf(axes), 4, 4)
+    run.call("prep", 0, 4, gpu.EPS, 8 * hd, 4 * hd, run.buf(x), ones, ones, q, hk.NONE)
+    k, v = (run.buf(np.full((rows, 2, hd), 7, np.float32)) for _ in range(2))
+    run.call("read", xb.F32, k, v)
+    run.call("attention", 4, 4 * hd, 4 * hd, run.buf(x[:, :4 * hd]), hk.NONE, run.buf(x[:, :4 * hd]))
+    run.result()

@@ -18,7 +18,7 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedStep& st, int s) {
     const int a = st.row0[s], b = st.row0[s + 1], past = st.past[s];
     SeqRows r;
     r.row0 = max(0, min(a, st.rows));
-    r.rows = min(max(0, min(b, st.rows) - r.row0), st.max_rows);
+    r.rows = min(max(0, max(0, min(b, st.rows)) - r.row0), st.max_rows);  // (b bounded by itself: any int32 less row0 may wrap)
     r.past = past;
     return r;
 }
