@@ -89,10 +89,11 @@ struct RowAxes {
         auto in = [&](int a, int p) { return !(r.used >> a & 1) || (p >= 0 && p < r.positions); };
         const int p0 = at(0), p1 = at(1), p2 = at(2), p3 = at(3);
         fine = in(0, p0) && in(1, p1) && in(2, p2) && in(3, p3);
+        auto less = [](int a, int b) { return static_cast<int>(static_cast<uint32_t>(a) - static_cast<uint32_t>(b)); };  // (of an axis without pairs it may wrap)
         a0 = fine ? p0 : 0;  // (the angles of a row that is not: those of position 0)
-        d1 = fine ? p1 - p0 : 0;
-        d2 = fine ? p2 - p0 : 0;
-        d3 = fine ? p3 - p0 : 0;
+        d1 = fine ? less(p1, p0) : 0;
+        d2 = fine ? less(p2, p0) : 0;
+        d3 = fine ? less(p3, p0) : 0;
     }
     __device__ __forceinline__ int of(int axis) const { return a0 + (axis == 1 ? d1 : 0) + (axis == 2 ? d2 : 0) + (axis == 3 ? d3 : 0); }
 };
