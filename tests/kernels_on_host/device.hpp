@@ -88,7 +88,7 @@ inline int order = 1;  // of the blocks: 1, or -1
 extern "C" void host_switch(void** save, void* to);
 asm(R"(
 .text
-.globl host_switch
+.weak host_switch
 .type host_switch, @function
 host_switch:
     pushq %rbp
@@ -399,7 +399,7 @@ inline uint32_t __shfl_xor(uint32_t v, int mask, int) { return static_cast<uint3
 #define __builtin_amdgcn_raw_buffer_load_b64(r, at, skip, aux) host::buffer_load<host::u2>(r, at, skip)
 #define __builtin_amdgcn_raw_buffer_load_b32(r, at, skip, aux) host::buffer_load<uint32_t>(r, at, skip)
 #define __builtin_amdgcn_raw_buffer_load_b16(r, at, skip, aux) host::buffer_load<uint16_t>(r, at, skip)
-#define __builtin_amdgcn_ballot_w64(v) host::ballot(v)
+#define __builtin_amdgcn_ballot_w64(...) host::ballot(__VA_ARGS__)
 #define __builtin_amdgcn_readfirstlane(v) host::readfirstlane(v)
 #define __builtin_amdgcn_readlane(v, l) static_cast<int>(host::from_lane(static_cast<uint32_t>(v), l))
 #define __builtin_amdgcn_ds_bpermute(at, v) static_cast<int>(host::from_lane(static_cast<uint32_t>(v), (at) / 4))

@@ -9,7 +9,8 @@
 //   prep GATED NQ EPS SRC_STRIDE OUT_STRIDE src q_norm k_norm q gate     (k and v behind q in a row of src)
 //   read OUT_TYPE k v
 //   attention NQ Q_STRIDE OUT_STRIDE q gate out
-//   codes FILE               of every fp16 value up to every fp16 maximum: values whose code is not the nearest
+//   logprobs TYPE LD ROWS VOCAB INV_TEMPERATURE TOP logits tokens logprob entropy rank top top_logprob
+//   codes FILE               of fp16 values up to fp16 maxima: how many have a code that is not the nearest
 // Names of nothing are 0.
 #include "device.hpp"
 
@@ -31,8 +32,6 @@
 
 namespace xqhip {
 void set_last_error(const std::string& msg) { std::cerr << msg << "\n"; }
-size_t logprobs_workspace_bytes(int, int, int) { return 0; }
-hipError_t launch_logprobs(const LogprobsLaunch&, hipStream_t) { return hipErrorInvalidConfiguration; }
 }  // namespace xqhip
 
 namespace {
@@ -163,6 +162,20 @@ int main() {
             float* out = as<float>(next());
             Buffer ws = allocate(xqhip_paged_attention_workspace_bytes(nq, kv.nkv, kv.head_dim));
             rc = xqhip_paged_attention(q, gate, &kv, nq, &step, q_stride, out, out_stride, ws.at, ws.bytes, nullptr);
+            std::free(ws.at);
+        } else if (what == "logprobs") {
+            const int type = number(), ld = number(), rows = number(), vocab = number();
+            const float inv_t = std::stof(next());
+            const int top = number();
+            const void* x = at(next());
+            const int32_t* tokens = as<int32_t>(next());
+            float* logprob = as<float>(next());
+            float* entropy = as<float>(next());
+            int32_t* rank = as<int32_t>(next());
+            int32_t* ids = as<int32_t>(next());
+            float* top_logprob = as<float>(next());
+            Buffer ws = allocate(xqhip_token_logprobs_workspace_bytes(rows, vocab, top));
+            rc = xqhip_token_logprobs(x, type, ld, rows, vocab, inv_t, tokens, top, logprob, entropy, rank, ids, top_logprob, ws.at, ws.bytes, nullptr);
             std::free(ws.at);
         } else if (what == "codes") {
             std::ofstream(next()) << wrong_codes();

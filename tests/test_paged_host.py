@@ -328,3 +328,44 @@ def test_numbers_of_any_size(tmp_path, kind, hd, max_rows, row0, past):
     run.call("read", xb.F32, k, v)
     run.call("attention", 4, 4 * hd, 4 * hd, run.buf(x[:, :4 * hd]), hk.NONE, run.buf(x[:, :4 * hd]))
     run.result()
+
+
+# ---- log probabilities ----------------------------------------------------------
+def logprobs(tmp, x, tokens, inv_t, top, ld):
+    rows, vocab = x.shape
+    run = hk.Run(tmp)
+    y = np.full(rows * ld, np.nan, x.dtype)  # (nothing behind the last row's logits)
+    y.reshape(rows, ld)[:, :vocab] = x
+    shapes = [(np.float32, rows), (np.float32, rows), (np.int32, rows), (np.int32, rows * top), (np.float32, rows * top)]
+    outs = [run.buf(np.full(n, 7, t)) if n else hk.NONE for t, n in shapes]
+    run.call("logprobs", xb.F16 if x.dtype == np.float16 else xb.F32, ld, rows, vocab, inv_t, top, run.buf(y[:(rows - 1) * ld + vocab]),
+             run.buf(np.array(tokens, np.int32)), *outs)
+    for name, (t, n) in zip(outs, shapes):
+        if n:
+            run.save(name, t, (n,))
+    got = run.result()
+    return got[:3] + [a.reshape(rows, top) for a in got[3:]]
+
+
+@pytest.mark.parametrize("t", [np.float32, np.float16])
+@pytest.mark.parametrize("vocab", [1, 5, 33, 1022, 1025, 8193, 16384, 16385, 40007])
+def test_logprobs_stay_in_their_buffers(tmp_path, vocab, t):
+    rng = np.random.default_rng(vocab)
+    x = rng.normal(0, 3, (6, vocab)).astype(t)
+    x[1] = np.round(x[1])
+    x[2] = 1.5
+    x[3, rng.random(vocab) < 0.99] = -np.inf
+    x[4, :] = np.nan
+    tokens = [0, vocab - 1, vocab // 2, vocab, -1, 2**31 - 1]
+    for ld, top in ((vocab, 0), (vocab, 64), ((vocab + 7) // 8 * 8, 5)):
+        got = logprobs(tmp_path, x, tokens, 1.0, top, ld)
+        gpu.check_logprobs(got + [np.zeros((6, 0), np.int32), np.zeros((6, 0), np.float32)][:5 - len(got)], x, tokens, 1.0, top)
+
+
+def test_codes_are_the_nearest(tmp_path):
+    """code_of against the quotient in 64 bits, ties to even: every fp16 value up to every maximum of two exponents and the
+    subnormal ones, and to some of the other maxima."""
+    run = hk.Run(tmp_path)
+    run.call("codes", tmp_path / "wrong")
+    run.result()
+    assert (tmp_path / "wrong").read_text() == "0"
