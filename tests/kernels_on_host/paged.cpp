@@ -141,7 +141,7 @@ int main() {
             turned = true;
         } else if (what == "prep") {
             const int gated = number(), nq = number();
-            const float eps = std::stof(next());
+            const float eps = std::strtof(next().c_str(), nullptr);
             const int src_stride = number(), out_stride = number(), q_width = nq * kv.head_dim * (gated ? 2 : 1);
             const float* src = as<float>(next());
             const float* qn = as<float>(next());
@@ -165,7 +165,7 @@ int main() {
             std::free(ws.at);
         } else if (what == "logprobs") {
             const int type = number(), ld = number(), rows = number(), vocab = number();
-            const float inv_t = std::stof(next());
+            const float inv_t = std::strtof(next().c_str(), nullptr);
             const int top = number();
             const void* x = at(next());
             const int32_t* tokens = as<int32_t>(next());

@@ -369,3 +369,23 @@ def test_codes_are_the_nearest(tmp_path):
     run.call("codes", tmp_path / "wrong")
     run.result()
     assert (tmp_path / "wrong").read_text() == "0"
+
+
+def far_rows(vocab):
+    """Logits whose differences pass fp32's range, at temperatures that bring them back."""
+    rng = np.random.default_rng(vocab)
+    x = rng.uniform(-3.4e38, 3.4e38, (5, vocab)).astype(np.float32)
+    x[1, :] = -3.4e38
+    x[1, vocab // 2] = 3.4e38                # one against all
+    x[2] = np.where(np.arange(vocab) % 3, -2e38, 2e38)
+    x[3] = rng.normal(0, 1, vocab)           # ordinary ones beside the range's ends
+    x[3, 0], x[3, vocab - 1] = np.finfo(np.float32).max, -np.finfo(np.float32).max
+    x[4] = rng.normal(0, 1e-38, vocab)
+    return x, [0, vocab - 1, 1, vocab - 1, 3]
+
+
+@pytest.mark.parametrize("vocab", [33, 1100, 20011])
+@pytest.mark.parametrize("inv_t", [1e-38, 3e-39, 2e-38, 1e-30, 0.4])
+def test_logprobs_of_logits_far_apart(tmp_path, vocab, inv_t):
+    x, tokens = far_rows(vocab)
+    gpu.check_logprobs(logprobs(tmp_path, x, tokens, inv_t, 7, vocab + 3), x, tokens, inv_t, 7)

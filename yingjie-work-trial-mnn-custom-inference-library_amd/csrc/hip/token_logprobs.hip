@@ -44,7 +44,7 @@ constexpr int kRowThreads = 512, kFewThreads = 256;
 constexpr int kCandidates = 2048;  // candidates of a row that are held
 constexpr int kMany = 512;         // ... that are put in order as they are
 constexpr int kMostLanes = 1024;   // lanes of a row that are looked at again
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kTwoLog2e = 2 * 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 // Segments of a row.
 struct Segments {
@@ -70,9 +70,11 @@ size_t logprobs_workspace_bytes(int rows, int vocab, int top) {
     return n * (sizeof(LogPart) + (top ? kWave * sizeof(float) : 0));
 }
 
-// (x - m) / T in units of ln 2, 2^-200 and less is nothing (minus infinity, no number, and infinity less infinity too)
-__device__ __forceinline__ float gap2(float x, float m, float c) { return fmaxf((x - m) * c, -200.0f); }
-__device__ __forceinline__ float logit_gap(float x, float m, float inv_t) { return x == m ? 0.0f : (x - m) * inv_t; }
+// (x - m) / T in units of ln 2 (c: 2 / (T ln 2)), 2^-200 and less is nothing (minus infinity, no number, and infinity less infinity too).
+// Half the difference: of two logits it is in fp32's range, and rounded as the whole one.
+__device__ __forceinline__ float half_gap(float x, float m) { return fmaf(x, 0.5f, -0.5f * m); }
+__device__ __forceinline__ float gap2(float x, float m, float c) { return fmaxf(half_gap(x, m) * c, -200.0f); }
+__device__ __forceinline__ float logit_gap(float x, float m, float inv_t) { return x == m ? 0.0f : 2.0f * (half_gap(x, m) * inv_t); }
 template <bool F16>
 using logit_t = typename std::conditional<F16, _Float16, float>::type;
 template <bool F16>
@@ -98,7 +100,7 @@ __global__ void __launch_bounds__(kWave* kPartWaves) logprobs_part_kernel(Logpro
     const int seg = __builtin_amdgcn_readfirstlane(blockIdx.x * kPartWaves + wid);
     if (seg >= sg.count) return;
     const L* x0 = logit_row<F16>(p, row);
-    const float c = p.inv_t * kLog2e;
+    const float c = p.inv_t * kTwoLog2e;
     float M = -INFINITY, S = 0.0f, H = 0.0f, mine = -INFINITY;  // the segment so far, this lane's maximum
     int before = 0, t = -1;
     float xt = 0.0f;
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_row_kernel(LogprobsLaunch p,
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) best = u64_max(best, red[i]);
     const bool any = best != 0;
-    const float m = any ? float_from_order_key(static_cast<uint32_t>(best >> 32)) : -INFINITY, c = p.inv_t * kLog2e;
+    const float m = any ? float_from_order_key(static_cast<uint32_t>(best >> 32)) : -INFINITY, c = p.inv_t * kTwoLog2e;
     float s = 0.0f, h = 0.0f;
     int before = 0;
 #pragma unroll
@@ -535,7 +537,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_small_kernel(LogprobsLaunch 
     }
     x[E] = static_cast<float>(x0[min(whole * N + tid, vocab - 1)]);
     if (tid >= rest) x[E] = -INFINITY;
-    const float xt = clean(static_cast<float>(x0[has ? t : 0])), c = p.inv_t * kLog2e;
+    const float xt = clean(static_cast<float>(x0[has ? t : 0])), c = p.inv_t * kTwoLog2e;
     float lm = x[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) lm = fmaxf(lm, x[e]);
