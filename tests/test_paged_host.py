@@ -389,3 +389,25 @@ def far_rows(vocab):
 def test_logprobs_of_logits_far_apart(tmp_path, vocab, inv_t):
     x, tokens = far_rows(vocab)
     gpu.check_logprobs(logprobs(tmp_path, x, tokens, inv_t, 7, vocab + 3), x, tokens, inv_t, 7)
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+@pytest.mark.parametrize("rows", [[1, 1, 1], [3, 40, 2]])
+def test_heads_with_an_infinity(tmp_path, kind, rows):
+    """x / sqrt(mean x^2 + eps) of a head with an infinity: 0, not a number where the infinity and its partner are.
+    A page that no row began has no scale: any that is not a number counts as 0."""
+    rng = np.random.default_rng(2)
+    plan = Plan(rng, 32, [0, 31, 5], rows)
+    pool = Pool(kind, 2, 128, 32, plan.pages, 3)
+    pool.open[:] = 0
+    was = pool.raw()
+    x = rng.normal(0, 1, (plan.total, 2 * 4 * 128 + 4 * 128)).astype(np.float32)
+    x[:, 3], x[1, 256 + 70], x[:, 1024 + 7] = np.inf, -np.inf, np.inf  # of query heads, of a key's
+    with np.errstate(invalid="ignore"):
+        x, q, _, (qn, kn), cs = prep(tmp_path, rng, pool, plan, 4, 32, x=x)
+        qx, _, kx, vx = gpu.split_heads(x, 4, 2, 128, 1)
+        want, k = po.prepared(qx, qn, cs[:, None], gpu.EPS), po.prepared(kx, kn, cs[:, None], gpu.EPS)
+    assert np.array_equal(np.isnan(q), np.isnan(want))
+    assert (np.abs(q - want) <= 2**-23 * np.abs(want))[~np.isnan(want)].all()
+    numbers = lambda raw: raw[:2] + [np.nan_to_num(s) for s in raw[2:4]] + raw[4:]  # noqa: E731
+    assert gpu.same(numbers(pool.raw()), gpu.appended(numbers(was), plan, kind, k, vx))

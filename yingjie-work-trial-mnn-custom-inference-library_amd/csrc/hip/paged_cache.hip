@@ -127,7 +127,7 @@ __device__ __forceinline__ double inverse_sqrt(double v) {
     double y = __builtin_amdgcn_rsq(v);
 #pragma unroll
     for (int i = 0; i < 2; ++i) y = fma(0.5 * y, fma(-v * y, y, 1.0), y);
-    return y;
+    return v == static_cast<double>(INFINITY) ? 0.0 : y;  // (Newton's step has 0 times infinity there)
 }
 
 __device__ __forceinline__ double lane_value(double v, int from) {
