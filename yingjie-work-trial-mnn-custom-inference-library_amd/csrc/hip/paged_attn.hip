@@ -301,22 +301,8 @@ struct PagedBlock {
     static constexpr size_t kOutBytes = static_cast<size_t>(kCols) * (KS * (kLdo + 3) + 1) * 4;
 };
 
-// writes the quad at `out`; whether its row has to be computed again
-__device__ __forceinline__ bool write_gated_quad(float4 r, float L, bool gated, float4 gt, float* out) {
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    float4 y = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
-    if (gated) {
-        y.x *= sigmoid_dev(gt.x);
-        y.y *= sigmoid_dev(gt.y);
-        y.z *= sigmoid_dev(gt.z);
-        y.w *= sigmoid_dev(gt.w);
-    }
-    *reinterpret_cast<float4*>(out) = y;
-    return !(L > 0.0f && fabsf(r.x) + fabsf(r.y) + fabsf(r.z) + fabsf(r.w) < INFINITY);
-}
-
 __device__ __forceinline__ bool write_paged_quad(float4 r, float L, const float* gate, float* out) {
-    return write_gated_quad(r, L, gate != nullptr, gate ? *reinterpret_cast<const float4*>(gate) : float4{}, out);
+    return write_quad(r, L, gate != nullptr, gate ? *reinterpret_cast<const float4*>(gate) : float4{}, out);
 }
 
 // The key waves of a block's columns joined, then written: a partial output (to part_out: [COLS][HD], then [COLS][2]), or
@@ -885,7 +871,7 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
             if (slice == 0)
                 for (int k = 1; k < slices; ++k) add_scaled(r, 1.0f, sums[k * items + item]);
         }
-        if (slice == 0) bad |= write_gated_quad(r, total[i], p.gate != nullptr, gates, p.out + row * p.out_stride + col);
+        if (slice == 0) bad |= write_quad(r, total[i], p.gate != nullptr, gates, p.out + row * p.out_stride + col);
     }
     if (bad) redo = 1;
     __syncthreads();
