@@ -278,6 +278,24 @@ def test_rows_that_are_not_held_do_not_count(tmp_path, past, sizes, bad, stale, 
     check_holes(pool, was, whole, steps_with_holes(tmp_path, rng, pool, whole, sizes, bad), bad)
 
 
+@pytest.mark.parametrize("first,stale", [(10, 6e4), (1, np.inf), (40, np.nan)])
+def test_rows_before_their_page_is_there_do_not_count(tmp_path, first, stale):
+    """A sequence's first rows find no page (one, a chunk, a chunk over two pages); the page that is there later takes the rest."""
+    rng = np.random.default_rng(first)
+    at = first // 32
+    whole = Plan(rng, 32, [0], [first + 3 + 40])
+    pool = Pool(I8, 2, 128, 32, whole.pages, 1, *(rng.normal(0, 0.5, (2, whole.pages, 2, 32, 128)).astype(np.float16)))
+    pool.open[:] = stale
+    was, table = pool.raw(), whole.table.copy()
+    whole.table[0, :at + 1] = [-1, whole.pages][first % 2]
+    pages = Plan(rng, 32, [0], [first])
+    pages.table, pages.most, pages.open = whole.table, whole.most, whole.open
+    prep(tmp_path, rng, pool, pages, 2, 32, cap=500)
+    assert gpu.same(pool.raw()[:4], was[:4])
+    whole.table, whole.past = table, [first]
+    check_holes(pool, was, whole, steps_with_holes(tmp_path, rng, pool, whole, [3, 40], set()), set())
+
+
 @pytest.mark.parametrize("hd,seqs,rows", [(256, 1024, 512), (128, 1024, 1024), (256, 60, 40)])
 def test_rows_in_no_order_stay_in_the_workspace(tmp_path, hd, seqs, rows):
     """Every second sequence claims every row (row0 falls): some 65536 row tiles where a step of so many rows has 896 at most.

@@ -122,12 +122,14 @@ struct LanePairs {
     }
 };
 
-// 1 / sqrt(v): the hardware's estimate and two steps of Newton's, within 2^-50 (what is kept of it has 24 bits)
+// 1 / sqrt(v): the hardware's estimate and two steps of Newton's, within 2^-50 (what is kept of it has 24 bits).  Of infinity
+// 0, the estimate, which the steps leave with a number in its place (chosen behind them 0.3 us more in a step of 16 rows).
 __device__ __forceinline__ double inverse_sqrt(double v) {
     double y = __builtin_amdgcn_rsq(v);
+    v = fmin(v, 1.0e300);
 #pragma unroll
     for (int i = 0; i < 2; ++i) y = fma(0.5 * y, fma(-v * y, y, 1.0), y);
-    return v == static_cast<double>(INFINITY) ? 0.0 : y;  // (Newton's step has 0 times infinity there)
+    return y;
 }
 
 __device__ __forceinline__ double lane_value(double v, int from) {
@@ -190,14 +192,16 @@ __device__ __forceinline__ void turn_heads(float (&x)[B][E], const float (&w)[E]
     }
 }
 
-// Where a sequence's position goes.  (Both loads go out at once, from places that exist.)
+// Where a sequence's position goes: its page, and its open page (-1: none).  (Both loads go out at once, from places that
+// exist.)
 struct Place {
     int page, open;
     __device__ __forceinline__ Place(const PagedPrepLaunch& p, int s, int64_t pos) {
         const int at = static_cast<int>(max(int64_t(0), min(pos, static_cast<int64_t>(table_positions(p.step, p.kv)) - 1))) / p.kv.page;
         page = p.step.table[static_cast<size_t>(s) * p.step.max_pages + at];
         open = p.kv.i8 ? p.step.open[s] : 0;
-        if (pos != at * static_cast<int64_t>(p.kv.page) + (pos & (p.kv.page - 1)) || page >= p.kv.pages || open < 0 || (p.kv.i8 && open >= p.kv.opens)) page = -1;
+        if (pos != at * static_cast<int64_t>(p.kv.page) + (pos & (p.kv.page - 1)) || (p.kv.i8 && open >= p.kv.opens)) open = -1;
+        if (page >= p.kv.pages || open < 0) page = -1;
     }
     __device__ __forceinline__ bool none() const { return page < 0; }
 };
@@ -330,6 +334,26 @@ __device__ __forceinline__ void put_row(const _Float16 (&v)[E], int lane, int hd
     }
 }
 
+// a row's fp16 values for the open page, zeros where it is not held
+template <int E, bool VEC>
+__device__ __forceinline__ void keep_row(const _Float16 (&v)[E], bool held, int lane, int hd, _Float16* d) {
+    _Float16 y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = held ? v[e] : static_cast<_Float16>(0.0f);
+    put_row<E, VEC>(y, lane, hd, d);
+}
+// rows [from, end) of an open page, by a block
+template <int THREADS>
+__device__ __forceinline__ void keep_zeros(_Float16* kept, int from, int end, int hd) {
+    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+    for (int i = from * (hd / 8) + threadIdx.x; i < end * (hd / 8); i += THREADS) reinterpret_cast<half8*>(kept)[i] = half8{};
+}
+// a head's rows in the open page, nullptr: none
+__device__ __forceinline__ _Float16* open_rows(const PagedPrepLaunch& p, const Place& place, int h, bool is_k) {
+    if (place.open < 0) return nullptr;
+    return (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(place.open) * p.kv.nkv + h) * p.kv.page * p.kv.head_dim;
+}
+
 // The largest magnitude that a page's scale stands for: an fp16 value, exactly.  (A page that no row began may have any scale.)
 __device__ __forceinline__ float recorded_max(float scale) {
     return static_cast<float>(static_cast<_Float16>(fminf(fmaxf(scale * 127.0f, 0.0f), 65504.0f)));
@@ -337,9 +361,9 @@ __device__ __forceinline__ float recorded_max(float scale) {
 
 // One page that the step touches, one kv head, k or v, by a block.  The new rows' fp16 values go to LDS, then to the page in
 // 16-byte pieces; 8 bits: their maximum is taken on the way, and where it rose, or the step leaves the page, the page's
-// earlier values are fetched and the codes of all of them written.  The earlier values' maximum is the recorded one: where a
-// row was not held, the open page has what another sequence left.  A page of which no row is held stays as it is, and only a
-// row that is held at its first position begins it anew.  The last page's rows from keep_from on are kept.
+// earlier values are fetched and the codes of all of them written.  A page of which no row is held stays as it is, and only a
+// row that is held at its first position begins it anew.  The last page's rows from keep_from on are kept, as zeros where they
+// are not held: what another sequence left there would count in the page's maximum.
 template <int W, int E, bool VEC, bool I8>
 __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRows& sr, int s, int index, int keep_from, int h, bool is_k, _Float16* vals, double* turn) {
     typedef HeadLanes<E, VEC> L;
@@ -359,12 +383,10 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     auto before = [&] {
         const Place place(p, s, base);
         page = place.page;
+        if constexpr (I8) kept = open_rows(p, place, h, is_k);
         if (place.none()) return false;  // block-uniform
         sat = static_cast<size_t>(page) * nkv + h;
-        if constexpr (I8) {
-            kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(place.open) * nkv + h) * P * hd;
-            was = (is_k ? p.kv.k_scale : p.kv.v_scale)[sat];
-        }
+        if (I8 && lead) was = (is_k ? p.kv.k_scale : p.kv.v_scale)[sat];
         return true;
     };
     page_rows<W, E, VEC, I8>(p, sr, base, lead, end, h, is_k, turn, before, [&](int t, bool held, const _Float16(&v)[E]) {
@@ -373,15 +395,21 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
         for (int e = 0; e < E; ++e)
             if (I8 && held && L::in(lane, e, hd)) mx = fmaxf(mx, fabsf(static_cast<float>(v[e])));
         put_row<E, VEC>(v, lane, hd, vals + t * ld);
-        if (I8 && last && held && t >= keep_from) put_row<E, VEC>(v, lane, hd, kept + static_cast<size_t>(t) * hd);
+        if (I8 && last && t >= keep_from) keep_row<E, VEC>(v, held, lane, hd, kept + static_cast<size_t>(t) * hd);
     });
-    if (page < 0) return;
+    if (page < 0) {
+        if (I8 && last && kept) keep_zeros<kThreads>(kept, max(lead, keep_from), end, hd);
+        return;
+    }
     int from = lead;
     float inv = 0.0f;
     auto earlier = [&] {  // the page's values before the step, in fp16
         for (int i = threadIdx.x; i < lead * (hd / 8); i += kThreads) {
             const int t = i / (hd / 8), b = i - t * (hd / 8);
-            *reinterpret_cast<half8*>(vals + t * ld + 8 * b) = *reinterpret_cast<const half8*>(kept + static_cast<size_t>(t) * hd + 8 * b);
+            const half8 y = *reinterpret_cast<const half8*>(kept + static_cast<size_t>(t) * hd + 8 * b);
+            *reinterpret_cast<half8*>(vals + t * ld + 8 * b) = y;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(static_cast<float>(y[e])));
         }
     };
     if constexpr (I8) {
@@ -403,12 +431,15 @@ __device__ __forceinline__ void hold_page(const PagedPrepLaunch& p, const SeqRow
     if constexpr (I8) {
 #pragma unroll
         for (int i = 0; i < W; ++i) mx = fmaxf(mx, wave_mx[i]);
-        const float before = on[0] & 1 ? 0.0f : recorded_max(was);
+        if (!lead && !(on[0] & 1)) was = (is_k ? p.kv.k_scale : p.kv.v_scale)[sat];  // block-uniform
+        const float before = recorded_max(was);
         const bool grew = mx > before;
         mx = grew ? mx : before;
         inv = mx > 0.0f ? 1.0f / mx : 0.0f;
         if (grew && lead && last) {
+            const float all = mx;
             earlier();
+            mx = all;
             from = 0;
             __syncthreads();
         }
@@ -501,14 +532,16 @@ __device__ __forceinline__ void hold_unit(const PagedPrepLaunch& p, int unit, _F
             __syncthreads();
             const int end = min(lead, sr.past + sr.rows - last * P), lane = threadIdx.x & (kWave - 1), hd = p.kv.head_dim;
             _Float16* kept = nullptr;
+            bool none = true;
             auto before = [&] {
                 const Place place(p, s, static_cast<int64_t>(last) * P);
-                kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(max(place.open, 0)) * p.kv.nkv + h) * P * hd;
-                return !place.none();
+                kept = open_rows(p, place, h, is_k);
+                none = place.none();
+                return !none;
             };
-            page_rows<W, E, VEC, I8>(p, sr, last * P, 0, end, h, is_k, turn, before, [&](int t, bool held, const _Float16(&v)[E]) {
-                if (held) put_row<E, VEC>(v, lane, hd, kept + static_cast<size_t>(t) * hd);
-            });
+            page_rows<W, E, VEC, I8>(p, sr, last * P, 0, end, h, is_k, turn, before,
+                                     [&](int t, bool held, const _Float16(&v)[E]) { keep_row<E, VEC>(v, held, lane, hd, kept + static_cast<size_t>(t) * hd); });
+            if (none && kept) keep_zeros<kWave * W>(kept, 0, end, hd);
         }
 }
 
@@ -551,7 +584,13 @@ __device__ __forceinline__ void token_unit(const PagedPrepLaunch& p, int s, int 
         if (p.gate_out) L::store(p.gate_out + o, lane, hd, gate);
         return;
     }
-    if (!held) return;
+    if (!held) {
+        if (I8 && place.open >= 0) {
+            const _Float16 zeros[E] = {};
+            put_row<E, VEC>(zeros, lane, hd, open_rows(p, place, h, is_k) + static_cast<size_t>(t) * hd);
+        }
+        return;
+    }
     constexpr int N = I8 ? 16 : 8;
     auto offset = [&](int pos_in, int dim) { return is_k ? k_offset<N>(p.kv, pos_in, dim) : v_offset<N>(p.kv, pos_in, dim); };
     const size_t head = page_head(p.kv, place.page, h);
@@ -562,7 +601,7 @@ __device__ __forceinline__ void token_unit(const PagedPrepLaunch& p, int s, int 
             if (L::in(lane, e, hd)) d[offset(t, L::dim(lane, e))] = static_cast<_Float16>(x[e]);
     } else {
         int8_t* d = static_cast<int8_t*>(is_k ? p.kv.k : p.kv.v) + head;
-        _Float16* kept = (is_k ? p.kv.k_open : p.kv.v_open) + (static_cast<size_t>(place.open) * nkv + h) * P * hd;
+        _Float16* kept = open_rows(p, place, h, is_k);
         _Float16 v[E];
         float mx = 0.0f;
 #pragma unroll
