@@ -183,11 +183,12 @@ __device__ __forceinline__ int tiles_of(int last) { return max(0, last) / kTTile
 // of two.  A whole sequence and head where that is not much longer: it needs no joining.
 // Ranges (q = 1): a block's tiles may end inside a sequence and head and go on in the next, where some unit would be over
 // kApart tiles more than its share.  Every sequence a block goes on to costs it some tiles' time (its place, queries, join).
-// (Whole calls, us: 45 sequences of 500 positions in units 18.5, in ranges 23.7; 60 of 1500, 8 bits 28.1, 31.6; 32 of
-// 4000, where a unit of 81 tiles stands against ranges of 41, 83, 70.  32 of 1000 in units of a CU each 20.7, of two 25.1.)
+// (Whole calls, us: 45 sequences of 500 positions in units 17.9, in ranges 22.6; 60 of 1500, 8 bits 27.5, 30.8; 32 of
+// 4000, where a unit of 81 tiles stands against ranges of 41, 83, 69.  32 of 1000, 16 / 4 heads, in units of a CU each 14.6,
+// of two 16.1; 32 / 8 heads 20.1 either way.)
 // Each wave finds its block's place by itself, 64 sequences in its lanes at a time: no barrier, no launch before.
-constexpr int kMinTiles = 4;  // smallest unit, a tile for every wave (one sequence of 700 11.2 us, with 8 11.8)
-constexpr int kApart = 32;    // (24: 60000 positions, 8 bits 30.6 us instead of 28.8; 16: 60 sequences of 1500 32.6, not 28.9)
+constexpr int kMinTiles = 4;  // smallest unit, a tile for every wave (one sequence of 700 11.1 us, with 8 11.7)
+constexpr int kApart = 32;    // (24: one of 60000, 8 bits 30.0 us instead of 27.9; 16: 60 sequences of 1500 31.7, not 27.4)
 constexpr int kCus = 256;
 struct NarrowItem {
     int s, kh, unit, units;  // of the sequence and head: the unit asked for, and how many there are
@@ -426,13 +427,13 @@ struct WideShape {
 };
 
 // The units of the sequences that the narrow kernel does not take, by one block: of one wave where that has a lane per
-// sequence and few row tiles (4.5 to 6.5 us; by sixteen waves, with their barriers, 5.7 to 8.4).
+// sequence and few row tiles (13 rows beside 13 tokens 22.9 us; by sixteen waves, with their barriers, 24.5).
 //
 // Columns of a block: with 128 each key and value is staged for four column tiles instead of two, but there are half as many
-// row tiles.  128 where those still give every block of a round its own (three chunks of 512 rows after 2300 beside 21 tokens
-// 154 us, with 64 columns 173; 2000 rows after 2000 212, 239), or where a round's blocks have over kLong chunks each, so that
-// splits cost little beside them (512 rows after 16000 292, 312; 64 after 131000 289, 317); elsewhere 64 (500 rows after
-// 3584 85, 91; 64 after 1000 24, 27).
+// row tiles.  128 where those still give every block of a round its own (calls one after the other on the same data: three
+// chunks of 512 rows after 2300 beside 21 tokens 139 us, with 64 columns 162; 2000 rows after 2000 208, 233), or where a
+// round's blocks have over kLong chunks each, so that splits cost little beside them (512 rows after 16000 268, 283; 64 after
+// 131000 267, 291); elsewhere 64 (500 rows after 3584 81, with 128 columns 85; 64 after 1000 23, 26).
 constexpr int kLong = 60;
 constexpr int kPlanTiles = 256;  // row tiles, at most, for one wave
 template <int HD, int WAVES>
@@ -505,8 +506,8 @@ __global__ void __launch_bounds__(WAVES* kWave) paged_plan_kernel(PagedAttnLaunc
         return max(0, seen - 1) / chunk + 1;
     };
     // Splits: whole rounds of blocks take whole tiles; the others, no more than three eighths of a round, are split to the
-    // shortest length with which their units fit one (two chunks of 600 rows after 1500, heads of 256, 8 bits, 128 us, by whole
-    // tiles 159; with half a round the three chunks above 156 instead of 148, with more 900 rows after 500 60 instead of 57).
+    // shortest length with which their units fit one (two chunks of 600 rows after 1500, heads of 256, 8 bits, 127 us, by whole
+    // tiles 154; with half a round the three chunks above 144 instead of 138, with more 900 rows after 500 59 instead of 54).
     const int rest = tiles < room ? tiles : 8 * (tiles % room) <= 3 * room ? tiles % room : 0;
     constexpr int kHeld = kWideBlocks / kWave;
     if (wid == 0) {
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(WAVES* kWave) paged_plan_kernel(PagedAttnLaunc
 }
 
 // Up to 8 columns, or 16 (NT tiles of 8): bounded by memory, with short contexts by the chain of loads from the step's
-// tables to the values (one sequence of 700 positions 7 us; 32 of 4000, 336 MB, 66, 5.1 TB/s).  MFMA tiles of 16 columns: q's hi parts in a tile's first eight, its lo parts in
+// tables to the values (one sequence of 700 positions 6.9 us; 32 of 4000, 336 MB, 64, 5.3 TB/s).  MFMA tiles of 16 columns: q's hi parts in a tile's first eight, its lo parts in
 // the others.  One MFMA then does what two do.  A wave takes 32 keys at a time as two tiles of 16 rows; a lane and its
 // neighbour eight lanes on add their scores and take four keys each, and the weights' hi and lo parts go back into the two
 // halves.  MFMA row i of tile h stands for key 8 (i / 4) + 4 h + i % 4, so that a lane's part of the weights, four keys of
@@ -879,8 +880,9 @@ __device__ void merge_narrow(const PagedAttnLaunch& p, const PagedWs& ws, int s,
     for (int t = 0; t < sr.rows; ++t) attend_paged_row<kMergeThreads>(p, s, sr, sr.row0 + t, kh, smem);
 }
 
-// 64 or 128 columns: CT column tiles x KS key waves.  Bounded by the matrix cores and the vector units in turn (500 rows
-// after 3584, 8-bit pages: 35 % and 47 % of the 81 us, 0.77 PFLOP/s of fp16 hi + lo passes).  K and V are staged chunk by chunk (32 KS keys, shared by the column tiles) in
+// 64 or 128 columns: CT column tiles x KS key waves.  500 rows after 3584, 8-bit pages: 81 to 85 us, 0.75 PFLOP/s of fp16 hi +
+// lo passes; the matrix cores are busy for 34 % of the cycles, the vector units for 45 %: neither is full, but the waves of a
+// SIMD pass each chunk's barrier together, so products and softmax alternate, and blocks differ in length.  K and V are staged chunk by chunk (32 KS keys, shared by the column tiles) in
 // LDS as the pages hold them (8-bit codes as fp16), twice each: one barrier a chunk, the next chunk's loads over a whole
 // chunk ahead, and a chunk's products with V beside the next one's softmax.
 template <int HD, bool I8, int CT>
@@ -1097,8 +1099,8 @@ __device__ __forceinline__ void wide_block(const PagedAttnLaunch& p, const Paged
     join_paged<HD, KS, S::kCols, S::kThreads>(p, sk.r, kh, group, t0, ntok, T, inv_t, part_out, ws.wide_at + unit * nkv + kh, paged_lds, &redo);
 }
 
-// The splits of a row tile joined, the blocks of each slot (as many as there are for it) a share of the columns (13 rows'
-// three splits by 12 blocks 10 us, by all 256 5.9); and outputs that have to be computed again.
+// The splits of a row tile joined, the blocks of each slot (as many as there are for it) a share of the columns (13 rows after
+// 200 18.8 us, by one block for each slot 20.7); and outputs that have to be computed again.
 template <int HD>
 __device__ void merge_wide(const PagedAttnLaunch& p, const PagedWs& ws, int group_of, int groups, int kh, float* smem) {
     __shared__ float fac[kMostCols + kWideBlocks], total[kMostCols];  // a block's columns times the splits
@@ -1230,7 +1232,7 @@ __global__ void __launch_bounds__((kWave * kNarrowWaves), (kNarrowPerSimd<HD, I8
 // Steps with longer ones.  Among the first blocks every fifth eight (one block on each XCD) are narrow ones, as many as there is
 // work for: those wait for memory, the others for the matrix cores.  (Every fourth eight would all go to the same quarter
 // of an XCD.)  Few wide blocks: every third, so that fewer blocks without work are launched (50
-// sequences, one of 9 rows: 11.3 us, with every fifth 13.8; every second 14.6).
+// sequences of up to 200 positions, one of 9 rows: 35 us, with every fifth 37; every second 42).
 template <int HD, bool I8>
 __global__ void __launch_bounds__(kWave* kBlockWaves<HD>, kBlockWaves<HD> / 4) paged_mixed_kernel(PagedAttnLaunch p, PagedWs ws, int turn) {
     extern __shared__ uint4 paged_lds[];

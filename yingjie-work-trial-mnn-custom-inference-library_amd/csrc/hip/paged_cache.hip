@@ -17,10 +17,13 @@ namespace xqhip {
 // A head's values lie in a wave's lanes: lane l has the dims E l .. E l + E - 1
 // (VEC, one load) or l, l + 64, .. (other sizes).
 //
-// What bounds it: 64-bit operations and, in small steps, the chain of loads (the
-// step's tables, the rotary positions, the angles).  512 rows of 32 / 8 heads of
-// 128 with their read-back take 18.6 us, 509 rows of 16 / 4 heads of 256 into
-// 8-bit pages 15.5 us and 6.6 for the read-back; single tokens 3.7 to 4.5 us.
+// What bounds it: loads that wait for each other (the step's tables, the rotary
+// positions, the angles, the rows) and the barrier before the codes.  All blocks are
+// on the card at once, so a step takes as long as one block's chain: 509 rows of 16 /
+// 4 heads of 256 into 8-bit pages 15.7 us, in which the vector units are busy for a
+// third of the cycles (13 % of their instructions are 64-bit ones) and the waves wait
+// for half of them; 5.6 for the read-back.  512 rows of 32 / 8 heads of 128 with their
+// read-back 17.3 us; single tokens 3.8 to 4.7 us.
 // ---------------------------------------------------------------------------
 constexpr int kPagedMaxDim = 256;
 constexpr int kPagedMaxPage = 128;
@@ -652,8 +655,8 @@ __global__ void __launch_bounds__(kWave* W, 4) paged_prep_kernel(PagedPrepLaunch
     if (row < p.step.rows) query_unit<E, VEC>(p, (unit - row * row_units) * per, per, row, turn[wid]);
 }
 
-// Steps of single tokens: no barrier between a block's waves (with their read-back 32 tokens 10.3 us, by page and row 16.1;
-// one token 7.8, 11.1).
+// Steps of single tokens: no barrier between a block's waves (with the read-back of that time 32 tokens 10.3 us, by page and
+// row 16.1; one token 7.8, 11.1; with today's 9.4 and 8.3).
 constexpr int kTokenWaves = 4;
 template <int E, bool VEC, bool I8>
 __global__ void __launch_bounds__(kWave* kTokenWaves) paged_token_kernel(PagedPrepLaunch p, int row_blocks) {
@@ -681,15 +684,15 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
         if (hd == 256 && al) return p.kv.i8 ? go(paged_token_kernel<4, true, true>) : go(paged_token_kernel<4, true, false>);
         return p.kv.i8 ? go(paged_token_kernel<E, false, true>) : go(paged_token_kernel<E, false, false>);
     }
-    // (512 rows with one head a wave 24.1 us, with four 18.6; 51 rows 19.4 and 20.1)
+    // (with the read-back: 512 rows with one head a wave 23.2 us, with four 17.3; 51 rows 13.4 either way)
     const int per = p.step.rows >= 128 ? std::min(kQueryHeads, p.nq) : 1;
     const int row_units = (p.nq + per - 1) / per;
     // pages of any division of the rows among the sequences: n rows reach over n / P page borders, and one more; one more
     // page than borders
     const int64_t hold = 2 * static_cast<int64_t>(p.kv.nkv) * (p.step.rows / P + 2 * std::min(p.step.seqs, p.step.rows));
     // Waves of a block: eight; sixteen where pages take many passes of eight and there are few of them (with the read-back: 500
-    // rows, fp16 pages of 128, heads of 128 20.5 us, by eight waves 25.4; 139 rows in 8 bits, heads of 256 31.9, 35.6; four
-    // chunks of 512 49.1, 44.2).
+    // rows, fp16 pages of 128, heads of 128 20.2 us, by eight waves 25.0; 139 rows in 8 bits, heads of 256 29.2, 32.8; four
+    // chunks of 512, 8-bit pages of 64, 45.3, 42.2, fp16 pages of 128 47.8, 42.9).
     const bool long_pages = std::min(P, p.step.max_rows) * (hd > 128 ? 2 : 1) >= 128, few = 2 * p.kv.nkv * p.step.rows <= 128 * P;
     const int waves = long_pages && few ? 16 : 8;
     const int64_t tokens = (static_cast<int64_t>(p.step.seqs) * (p.nq + 2 * p.kv.nkv) + waves - 1) / waves;
@@ -715,7 +718,7 @@ hipError_t launch_paged_prep(const PagedPrepLaunch& p, hipStream_t s) {
 
 // ---------------------------------------------------------------------------
 // Positions read back, a block per sequence, 16 positions in a row of a page, kv
-// head, and k or v: four 16-byte pieces in flight in a thread (3.8 to 5.6 us: a launch
+// head, and k or v: four 16-byte pieces in flight in a thread (3.9 to 5.8 us: a launch
 // and three loads that wait for each other).
 // ---------------------------------------------------------------------------
 constexpr int kReadRows = 16, kReadThreads = 128;

@@ -18,10 +18,10 @@ namespace xqhip {
 // Equal infinities differ by 0.
 //
 // logprobs_small_kernel: rows of up to 16384 logits, a block per row, the row in
-//   registers: one launch (one row of 8192 4.5 us, by two launches 6.6; 200 fp16
-//   rows of 16000, 20 alternatives 12.0, 17.2; one of 16384 6.5, 6.6).  One wave
-//   for up to 1024 (5000 rows of 100 14.6 us, by eight waves 63), 16 logits a
-//   thread for up to 8192 (one row of 8000, 5 alternatives 7.2 us; 32 a thread 9.8).
+//   registers: one launch (one row of 8192 4.1 us, by two launches 6.0; 200 fp16
+//   rows of 16000, 20 alternatives 11.9, 14.5; one of 16384 6.4, 6.1).  One wave
+//   for up to 1024 (5000 rows of 100 7.5 us, by eight waves 31), 16 logits a
+//   thread for up to 8192 (one row of 8000, 5 alternatives 6.9 us; 32 a thread 9.8).
 // logprobs_part_kernel: one pass over the logits.  A wave takes a segment (16
 //   fp32 logits a lane or 32 fp16 ones; more where the row would have over 1024
 //   segments) in registers: its maximum, s', the sum of exp(d) d, how many
@@ -31,11 +31,15 @@ namespace xqhip {
 //   segments' maxima reach is reached by the k first tokens: the lanes whose
 //   maxima reach it, in those segments, are all that is looked at again.  With
 //   fewer than 8 k segments (of up to 256) the threads' shares of all lanes'
-//   maxima stand in for the segments: one row of 243 segments, 20 alternatives
-//   10.2 us (so 11.4), 64 alternatives 15.3 (13.3).
+//   maxima stand in for the segments: 200 rows of 25 segments, 20 alternatives
+//   19.5 us (by segments 28.8); one row of 243 segments, 20 alternatives, by
+//   segments 9.8 (so 11.2).  Between them the sides are close: 48 rows of 122
+//   segments with 64 alternatives 22.3 (by segments 23.9), with 20 19.2 (17.7).
 // What bounds it: the logits' bytes (500 fp32 rows of 248320, 497 MB, 83 us, 6.0
-// TB/s) and, with fp16 logits, 11 to 13 operations a logit (48 rows 9.5 us); for
-// one row a chain of two launches, 3.5 and 5.5 us.
+// TB/s); with fp16 logits the vector units are busy for half of the time (48 rows
+// 9 to 10 us; 15 instructions a logit, 4.7 us of them) and the waves, which are all on
+// the card at once, wait for their loads in the other; for one row a chain of two
+// launches, 3.7 and 5.5 us.
 // ---------------------------------------------------------------------------
 constexpr int kMostSegments = 1024, kFewSegments = 256;
 constexpr int kPartWaves = 4;
