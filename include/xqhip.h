@@ -667,9 +667,10 @@ typedef struct xqhip_step {
  * repeated from where it began).
  * A row that is not held (xqhip_attn_prep_paged) changes neither codes nor
  * scale; its place in the open page becomes 0, and its position holds no value
- * that may be read once a later row of its page is held.  A row held at a page's
- * first position begins the page; where that one is not held, the maximum that
- * the page's scale records counts on.
+ * that may be read once a later row of its page is held.  Such rows count among
+ * a step's: it ends in the page of its last row.  A row held at a page's first
+ * position begins the page; where that one is not held, the maximum that the
+ * page's scale records counts on.
  * Infinities and values past fp16's range are held as fp16's largest value,
  * values that are no numbers as 0.
  * One step's appends to one open page must not overlap. */

@@ -429,3 +429,25 @@ def test_heads_with_an_infinity(tmp_path, kind, rows):
     assert (np.abs(q - want) <= 2**-23 * np.abs(want))[~np.isnan(want)].all()
     numbers = lambda raw: raw[:2] + [np.nan_to_num(s) for s in raw[2:4]] + raw[4:]  # noqa: E731
     assert gpu.same(numbers(pool.raw()), gpu.appended(numbers(was), plan, kind, k, vx))
+
+
+@pytest.mark.parametrize("steps", [[(0, 10, 6), (10, 30, 0)], [(0, 10, 6), (10, 1, 3), (11, 1, 0), (12, 20, 9), (32, 5, 2)], [(0, 20, 0), (20, 12, 5), (32, 7, 2), (39, 1, 0)],
+                                   [(0, 32, 40), (32, 40, 0)], [(0, 1, 31), (1, 1, 1), (2, 60, 2), (62, 2, 3), (64, 1, 0)]])
+def test_padded_steps(tmp_path, steps):
+    """Steps whose last rows are padding (no rotary position), in the page where the next one goes on or past a page that is full:
+    the rows' codes as of one append."""
+    rng = np.random.default_rng(len(steps))
+    n = max(p + m + pad for p, m, pad in steps)
+    whole = Plan(rng, 32, [0], [n])
+    pool = Pool(I8, 2, 128, 32, whole.pages, 1, *(rng.normal(0, 20, (2, whole.pages, 2, 32, 128)).astype(np.float16)))
+    pool.open[:] = 6e4
+    was, norms, keys = pool.raw(), [rng.normal(1, 0.1, 128).astype(np.float32) for _ in range(2)], []
+    for past, m, pad in steps:
+        plan = Plan(rng, 32, [past], [m + pad])
+        plan.table, plan.most, plan.open = whole.table, whole.most, whole.open
+        x = (rng.normal(0, 1, (m + pad, 8 * 128)) * rng.uniform(0.1, 3, (m + pad, 1))).astype(np.float32)
+        axes = np.where(np.arange(m + pad) < m, past + np.arange(m + pad), -1)[None].astype(np.int32)
+        _, _, _, (_, kn), cs = prep(tmp_path, rng, pool, plan, 2, 32, axes=axes, x=x, norms=norms, cap=500)
+        _, _, kx, vx = gpu.split_heads(x, 2, 2, 128, 1)
+        keys.append((po.held(po.prepared(kx, kn, cs[:, None], gpu.EPS))[:m], po.held(vx)[:m]))
+    check_holes(pool, was, whole, [np.concatenate(z) for z in zip(*keys)], set())
