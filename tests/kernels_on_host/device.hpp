@@ -5,8 +5,11 @@
 // A block's threads are fibers of one host thread.  A lane operation (a read of
 // another lane, a ballot, a matrix product) waits until every lane of the wave
 // that has not ended waits in one, which has to be the same: lanes that part are
-// an error here.  Blocks run one after the other.  Static LDS arrays are static
-// arrays, dynamic LDS is an allocation of the launch's size.
+// an error here.  Blocks run one after the other, a block's waves each as far as it
+// comes without a barrier; or, backwards, the last wave first and all of them in turn
+// by one lane operation, so that what a missing barrier leaves to chance comes out in
+// two ways.  Static LDS arrays are static arrays, dynamic LDS is an allocation of the
+// launch's size.
 #pragma once
 
 #include <math.h>
@@ -72,7 +75,6 @@ struct Thread {
     char* stack;
     State state;
     LaneOp op;
-    const void* key;  // operations with other constants differ
     void* operand;
 };
 
@@ -83,7 +85,7 @@ inline dim3 thread_idx, block_idx, grid_dim, block_dim;
 inline char* dynamic_lds;
 inline size_t dynamic_bytes;
 inline std::function<void()>* body;
-inline int order = 1;  // of the blocks: 1, or -1
+inline int order = 1;  // of blocks and waves: 1, or -1
 
 extern "C" void host_switch(void** save, void* to);
 asm(R"(
@@ -136,9 +138,11 @@ inline void run_block(int n) {
     }
     for (;;) {
         int ended = 0, at_barrier = 0;
-        for (int w = 0; w < n; w += kLanes) {
-            const int lanes = std::min(kLanes, n - w);
-            for (;;) {
+        const int waves = (n + kLanes - 1) / kLanes;
+        for (int wave = 0; wave < waves; ++wave) {
+            const int w = (order > 0 ? wave : waves - 1 - wave) * kLanes, lanes = std::min(kLanes, n - w);
+            for (bool again = true; again;) {
+                again = order > 0;
                 for (int i = w; i < w + lanes; ++i)
                     if (threads[i].state == kReady) {
                         now = &threads[i];
@@ -152,7 +156,7 @@ inline void run_block(int n) {
                     Thread& t = threads[w + i];
                     if (t.state != kLaneOp) continue;
                     if (!first) first = &t;
-                    parted |= t.op != first->op || t.key != first->key;
+                    parted |= t.op != first->op;
                     operands[i] = t.operand;
                 }
                 if (!first) break;
@@ -201,16 +205,10 @@ void launch(Kernel kernel, dim3 grid, dim3 block, size_t lds, hipStream_t, const
 
 // `op` over the lanes' operands T, in each lane
 template <typename T>
-inline void together(LaneOp op, T& operand, const void* key = nullptr) {
+inline void together(LaneOp op, T& operand) {
     now->op = op;
-    now->key = key;
     now->operand = &operand;
     wait_as(kLaneOp);
-}
-template <int N>
-inline const void* constant() {
-    static const char c = 0;
-    return &c;
 }
 
 struct FromLane {

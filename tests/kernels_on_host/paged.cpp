@@ -2,7 +2,7 @@
 // each; buffers are allocations of their own of exactly the given size:
 //   buf NAME BYTES FILE      (FILE -: every byte 0xA5)
 //   save NAME FILE
-//   order 1|-1               blocks in the order of their number, or backwards
+//   order 1|-1               blocks and waves in the order of their number, or backwards and in turn
 //   pages TYPE NKV HD PAGE PAGES OPENS k v k_scale v_scale k_open v_open
 //   step SEQS ROWS MAX_ROWS MAX_PAGES row0 past table open
 //   rotary cs POSITIONS ROTARY_DIM AXES INTERLEAVED pos SECTION ..

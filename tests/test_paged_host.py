@@ -13,7 +13,7 @@ import xqbind as xb
 
 pytestmark = pytest.mark.skipif(not os.path.exists(hk.CLANG), reason="the compiler for the host is not there")
 F16, I8 = xb.PAGES_F16, xb.PAGES_I8
-ORDERS = [1, -1]  # of the blocks
+ORDERS = [1, -1]  # of blocks and waves
 
 
 class Plan(gpu.Plan):
